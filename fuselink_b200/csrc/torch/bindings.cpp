@@ -14,6 +14,8 @@
 #include "../kernels/kv_pack.cuh"
 #include "../kernels/decoder.cuh"
 #include "../kernels/thin_gemm.cuh"
+#include "../kernels/kv8.cuh"
+#include "../kernels/sampling.cuh"
 #include "../kernels/moe_dispatch.cuh"
 #include "../kernels/moe_route.cuh"
 #include "../kernels/fp8_gemm.cuh"
@@ -421,6 +423,121 @@ static void dec_advance(torch::Tensor next, torch::Tensor tokens, torch::Tensor 
                           const_cast<long long*>(dec_i64(step, 1, "step: int64")), (int)B, (int)history.size(0), cur_stream()), "fl_dec_advance");
 }
 
+// ------------------------------------------------------------------------------------------------ cache in 8 bits
+// k, v: [layers, blocks, heads, block_size, dim] e4m3; scales: [layers, blocks, heads] fp32; table: [batch, pages] int32
+static FlKv8 kv8_of(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& k_scale, const torch::Tensor& v_scale, const torch::Tensor& table,
+                    int64_t layer, int64_t batch, int64_t status_addr) {
+  for (const auto* t : {&k, &v})
+    TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kFloat8_e4m3fn && t->dim() == 5 && t->is_contiguous() && t->sizes() == k.sizes() && t->device() == k.device(),
+                "kv8: codes [layers, blocks, heads, block_size, dim] e4m3, contiguous, keys and values alike");
+  for (const auto* t : {&k_scale, &v_scale})
+    TORCH_CHECK(t->device() == k.device() && t->scalar_type() == torch::kFloat32 && t->is_contiguous() && t->dim() == 3 && t->size(0) == k.size(0) &&
+                t->size(1) == k.size(1) && t->size(2) == k.size(2), "kv8: scales [layers, blocks, heads] fp32, contiguous");
+  TORCH_CHECK(table.device() == k.device() && table.scalar_type() == torch::kInt32 && table.is_contiguous() && table.dim() == 2 && table.size(0) == batch,
+              "kv8: block_table [batch, pages] int32, contiguous");
+  TORCH_CHECK(layer >= 0 && layer < k.size(0), "kv8: layer out of range");
+  TORCH_CHECK(k.size(1) <= INT32_MAX && k.size(3) <= INT32_MAX && table.size(1) <= INT32_MAX, "kv8: too large");
+  FlKv8 kv;
+  kv.k = k.data_ptr(); kv.v = v.data_ptr(); kv.k_scale = k_scale.data_ptr<float>(); kv.v_scale = v_scale.data_ptr<float>();
+  kv.block_table = table.data_ptr<int>(); kv.table_stride = (int)table.size(1);
+  kv.layer = (int)layer; kv.layers = (int)k.size(0); kv.num_blocks = (int)k.size(1); kv.heads = (int)k.size(2); kv.block_size = (int)k.size(3);
+  kv.dim = (int)k.size(4); kv.status = reinterpret_cast<int*>(status_addr);
+  return kv;
+}
+static const long long* kv8_i64(const c10::optional<torch::Tensor>& t, const torch::Tensor& as, int64_t numel, const char* what) {
+  TORCH_CHECK(!t.has_value() || t->device() == as.device(), what);
+  return dec_i64(t, numel, what);
+}
+static void kv8_write(torch::Tensor k, torch::Tensor v, torch::Tensor k_scale, torch::Tensor v_scale, torch::Tensor table, int64_t layer, torch::Tensor qkv,
+                      torch::Tensor out, c10::optional<torch::Tensor> bias, c10::optional<torch::Tensor> rope, torch::Tensor start,
+                      c10::optional<torch::Tensor> pos, c10::optional<torch::Tensor> counts, int64_t status_addr) {
+  const int dt = dec_dtype(qkv);
+  TORCH_CHECK(qkv.dim() == 4 && qkv.is_contiguous() && qkv.device() == k.device(), "kv8: qkv [batch, tokens, heads + 2 kv_heads, dim], contiguous");
+  const int64_t B = qkv.size(0), T = qkv.size(1), all = qkv.size(2), D = qkv.size(3);
+  TORCH_CHECK(k.dim() == 5 && D == k.size(4) && all >= 2 * k.size(2) && B <= INT32_MAX && T <= INT32_MAX && all * D <= INT32_MAX, "kv8: qkv of another layout than the cache");
+  TORCH_CHECK(out.device() == k.device() && out.scalar_type() == qkv.scalar_type() && out.is_contiguous() && out.sizes() == qkv.sizes(), "kv8: out like qkv");
+  dec_like(bias, qkv, all * D, "kv8: bias [(heads + 2 kv_heads) * dim]");
+  TORCH_CHECK(!bias.has_value() || bias->device() == k.device(), "kv8: bias on the cache's device");
+  TORCH_CHECK(!rope.has_value() || (rope->device() == k.device() && rope->scalar_type() == torch::kFloat32 && rope->is_contiguous() && rope->dim() == 2 && rope->size(1) == D),
+              "kv8: rope [positions, dim] fp32");
+  c10::cuda::CUDAGuard guard(k.device());
+  const FlKv8 kv = kv8_of(k, v, k_scale, v_scale, table, layer, B, status_addr);
+  check_rc(fl_kv8_write(dt, qkv.data_ptr(), out.data_ptr(), opt_ptr(bias), rope.has_value() ? rope->data_ptr<float>() : nullptr, rope.has_value() ? rope->size(0) : 0,
+                        kv8_i64(start, k, B, "kv8: start [batch] int64"), kv8_i64(pos, k, B, "kv8: positions [batch] int64"),
+                        kv8_i64(counts, k, B, "kv8: counts [batch] int64"), (int)B, (int)T, (int)(all - 2 * kv.heads), &kv, cur_stream()), "fl_kv8_write");
+}
+static void kv8_pack(torch::Tensor k, torch::Tensor v, torch::Tensor k_scale, torch::Tensor v_scale, torch::Tensor table, torch::Tensor k_pool, torch::Tensor v_pool,
+                     int64_t src_blocks, torch::Tensor src_table, torch::Tensor lengths, int64_t status_addr) {
+  const int dt = dec_dtype(k_pool);
+  c10::cuda::CUDAGuard guard(k.device());
+  const FlKv8 kv = kv8_of(k, v, k_scale, v_scale, table, 0, table.dim() == 2 ? table.size(0) : -1, status_addr);
+  const int64_t need = src_blocks * kv.layers * kv.block_size * kv.heads * kv.dim;
+  for (const auto* t : {&k_pool, &v_pool})
+    TORCH_CHECK(t->device() == k.device() && t->scalar_type() == k_pool.scalar_type() && t->is_contiguous() && t->numel() >= need, "kv8: pools of src_blocks pages");
+  TORCH_CHECK(src_blocks >= 0 && src_blocks <= INT32_MAX && src_table.device() == k.device() && src_table.scalar_type() == torch::kInt32 && src_table.is_contiguous() &&
+              src_table.dim() == 2 && src_table.size(0) == table.size(0) && src_table.size(1) <= INT32_MAX, "kv8: src_table [batch, pages] int32");
+  check_rc(fl_kv8_pack(dt, k_pool.data_ptr(), v_pool.data_ptr(), (int)src_blocks, src_table.data_ptr<int>(), (int)src_table.size(1),
+                       kv8_i64(lengths, k, table.size(0), "kv8: lengths [batch] int64"), (int)table.size(0), &kv, cur_stream()), "fl_kv8_pack");
+}
+static void kv8_attention(torch::Tensor k, torch::Tensor v, torch::Tensor k_scale, torch::Tensor v_scale, torch::Tensor table, int64_t layer, torch::Tensor q,
+                          torch::Tensor start, c10::optional<torch::Tensor> counts, double scale, torch::Tensor out, c10::optional<torch::Tensor> mass, int64_t status_addr) {
+  const int dt = dec_dtype(q);
+  TORCH_CHECK(q.dim() == 4 && q.device() == k.device() && k.dim() == 5 && q.size(3) == k.size(4) && q.stride(3) == 1, "kv8: q [batch, tokens, heads, dim] with contiguous heads");
+  const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3);
+  TORCH_CHECK(B <= INT32_MAX && T <= INT32_MAX && H <= INT32_MAX && H % std::max<int64_t>(k.size(2), 1) == 0, "kv8: heads in groups that share a KV head");
+  TORCH_CHECK(out.device() == k.device() && out.scalar_type() == q.scalar_type() && out.is_contiguous() && out.numel() == B * T * H * D, "kv8: out [batch, tokens, heads * dim] like q");
+  TORCH_CHECK(!mass.has_value() || (mass->device() == k.device() && mass->scalar_type() == torch::kFloat32 && mass->is_contiguous() && mass->sizes() == table.sizes()),
+              "kv8: mass [batch, pages] fp32");
+  c10::cuda::CUDAGuard guard(k.device());
+  const FlKv8 kv = kv8_of(k, v, k_scale, v_scale, table, layer, B, status_addr);
+  const long long bytes = fl_kv8_attention_scratch((int)B, (int)T, (int)H, &kv, mass.has_value());
+  auto scratch = torch::empty({bytes}, q.options().dtype(torch::kUInt8));
+  check_rc(fl_kv8_attention(dt, q.data_ptr(), B > 1 ? q.stride(0) : 0, T > 1 ? q.stride(1) : 0, H > 1 ? q.stride(2) : 0, kv8_i64(start, k, B, "kv8: start [batch] int64"),
+                            kv8_i64(counts, k, B, "kv8: counts [batch] int64"), (int)B, (int)T, (int)H, (float)scale, &kv, out.data_ptr(),
+                            mass.has_value() ? mass->data_ptr<float>() : nullptr, bytes ? scratch.data_ptr() : nullptr, cur_stream()), "fl_kv8_attention");
+}
+static std::vector<torch::Tensor> kv8_evict(torch::Tensor mass, torch::Tensor table, torch::Tensor lengths, int64_t block_size, int64_t keep, int64_t recent, int64_t sinks) {
+  TORCH_CHECK(mass.is_cuda() && mass.scalar_type() == torch::kFloat32 && mass.is_contiguous() && mass.dim() == 2, "kv8: mass [batch, pages] fp32");
+  TORCH_CHECK(table.device() == mass.device() && table.scalar_type() == torch::kInt32 && table.is_contiguous() && table.sizes() == mass.sizes(), "kv8: block_table [batch, pages] int32");
+  const int64_t B = mass.size(0), M = mass.size(1);
+  TORCH_CHECK(B <= INT32_MAX && M <= INT32_MAX && block_size >= 1 && block_size <= INT32_MAX && keep <= INT32_MAX && recent >= 1 && sinks >= 0 && recent <= keep && sinks <= keep - recent,
+              "kv8: keep at least recent + sinks pages, recent at least one");
+  c10::cuda::CUDAGuard guard(mass.device());
+  auto mass_out = torch::empty_like(mass), table_out = torch::empty_like(table), lengths_out = torch::empty_like(lengths), gone = torch::empty({B}, table.options());
+  check_rc(fl_kv8_evict(mass.data_ptr<float>(), table.data_ptr<int>(), kv8_i64(lengths, mass, B, "kv8: lengths [batch] int64"), (int)B, (int)M, (int)block_size, (int)keep,
+                        (int)recent, (int)sinks, mass_out.data_ptr<float>(), table_out.data_ptr<int>(), reinterpret_cast<long long*>(lengths_out.data_ptr<int64_t>()),
+                        gone.data_ptr<int>(), cur_stream()), "fl_kv8_evict");
+  return {table_out, lengths_out, mass_out, gone};
+}
+// each of the limits: a tensor with an entry per row, or one value
+static std::pair<torch::Tensor, torch::Tensor> sample(torch::Tensor logits, torch::Tensor u, c10::optional<torch::Tensor> temperature, double temperature_all,
+                                                      c10::optional<torch::Tensor> top_k, int64_t top_k_all, c10::optional<torch::Tensor> top_p, double top_p_all,
+                                                      c10::optional<torch::Tensor> min_p, double min_p_all) {
+  const int dt = dec_dtype(logits);
+  TORCH_CHECK(logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1), "sample: logits [rows, vocab] with contiguous rows");
+  const int64_t rows = logits.size(0);
+  TORCH_CHECK(rows <= INT32_MAX, "sample: too many rows");
+  auto per_row = [&](const c10::optional<torch::Tensor>& t, torch::ScalarType type, const char* what) {
+    TORCH_CHECK(!t.has_value() || (t->device() == logits.device() && t->scalar_type() == type && t->is_contiguous() && t->numel() == rows), what);
+    return t.has_value() ? t->data_ptr() : nullptr;
+  };
+  FlSampleArgs a;
+  memset(&a, 0, sizeof a);
+  a.logits = logits.data_ptr(); a.row_stride = rows > 1 ? logits.stride(0) : logits.size(1); a.rows = (int)rows; a.vocab = logits.size(1);
+  TORCH_CHECK(u.device() == logits.device() && u.is_contiguous() && u.numel() == rows && (u.scalar_type() == torch::kFloat32 || u.scalar_type() == torch::kFloat64),
+              "sample: u [rows] fp32 or fp64");
+  if (u.scalar_type() == torch::kFloat64) a.u64 = u.data_ptr<double>(); else a.u32 = u.data_ptr<float>();
+  a.temperature = (const float*)per_row(temperature, torch::kFloat32, "sample: temperature [rows] fp32"); a.temperature_all = (float)temperature_all;
+  a.top_k = (const int*)per_row(top_k, torch::kInt32, "sample: top_k [rows] int32"); a.top_k_all = (int)std::min<int64_t>(std::max<int64_t>(top_k_all, 0), INT32_MAX);
+  a.top_p = (const float*)per_row(top_p, torch::kFloat32, "sample: top_p [rows] fp32"); a.top_p_all = (float)top_p_all;
+  a.min_p = (const float*)per_row(min_p, torch::kFloat32, "sample: min_p [rows] fp32"); a.min_p_all = (float)min_p_all;
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto tokens = torch::empty({rows}, logits.options().dtype(torch::kInt64)), logprobs = torch::empty({rows}, logits.options().dtype(torch::kFloat32));
+  a.tokens = reinterpret_cast<long long*>(tokens.data_ptr<int64_t>()); a.logprobs = logprobs.data_ptr<float>();
+  if (rows > 0) check_rc(fl_sample(dt, &a, cur_stream()), "fl_sample");
+  return {tokens, logprobs};
+}
+
 // ------------------------------------------------------------------------------------------------ MoE
 static void moe_dispatch(torch::Tensor x, torch::Tensor topk_idx, c10::optional<torch::Tensor> row_scale,
                          int64_t num_experts, int64_t experts_per_rank, int64_t cap, int64_t rank, int64_t world,
@@ -679,6 +796,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("THIN_MAX_ROWS") = FL_THIN_MAX_ROWS;
   m.def("dec_argmax", &dec_argmax);
   m.def("dec_advance", &dec_advance);
+  m.def("kv8_write", &kv8_write);
+  m.def("kv8_pack", &kv8_pack);
+  m.def("kv8_attention", &kv8_attention);
+  m.def("kv8_evict", &kv8_evict);
+  m.def("sample", &sample);
+  m.attr("SAMPLE_MAX_VOCAB") = FL_SAMPLE_MAX_VOCAB;
   m.def("moe_dispatch", &moe_dispatch);
   m.def("moe_zero_tail", &moe_zero_tail);
   m.def("moe_combine", &moe_combine);

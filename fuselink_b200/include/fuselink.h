@@ -14,12 +14,14 @@
 #include "../csrc/kernels/fp8_gemm.cuh"
 #include "../csrc/kernels/grouped_gemm.cuh"
 #include "../csrc/kernels/interact.cuh"
+#include "../csrc/kernels/kv8.cuh"
 #include "../csrc/kernels/kv_pack.cuh"
 #include "../csrc/kernels/decoder.cuh"
 #include "../csrc/kernels/mlp_bwd.cuh"
 #include "../csrc/kernels/moe_dispatch.cuh"
 #include "../csrc/kernels/moe_dispatch_noalloc.cuh"
 #include "../csrc/kernels/moe_route.cuh"
+#include "../csrc/kernels/sampling.cuh"
 #include "../csrc/kernels/shadow_reduce.cuh"
 #include "../csrc/kernels/thin_gemm.cuh"
 #include "../csrc/mem/vmm.h"
