@@ -34,10 +34,11 @@ def main():
     ap.add_argument("--emulate", action="store_true")
     ap.add_argument("--device", default="cuda", choices=["cuda", "cpu"], help="cpu: host tensors and a host-memory heap (only under a model of "
                                                                               "the device entry points, as the tests run it)")
-    args = ap.parse_args()
     from fuselink_b200.models.llama import MODEL_ZOO, LlamaShard, load_checkpoint_file
     from fuselink_b200.parallel.symm import SymmetricHeap
-    from fuselink_b200.serving.disagg import DecodeStage, KVLink, PrefillStage, ServeParams, make_prompts
+    from fuselink_b200.serving.disagg import DecodeStage, KVLink, PrefillStage, ServeParams, decoding_flags, decoding_options, make_prompts
+    decoding_flags(ap)
+    args = ap.parse_args()
 
     rank = int(os.environ.get("RANK", 0)); local = int(os.environ.get("LOCAL_RANK", 0)); world = int(os.environ.get("WORLD_SIZE", 1))
     cpu = args.device == "cpu"
@@ -54,7 +55,7 @@ def main():
     cfg = MODEL_ZOO[args.model]
     dtype = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}[args.precision]
     if args.emulate or world == 1:
-        p = ServeParams(cfg, args.batch, args.input_len, args.decode_steps, 1, dtype)
+        p = ServeParams(cfg, args.batch, args.input_len, args.decode_steps, 1, dtype, **decoding_options(args))
         net = LlamaShard(cfg, device=dev, dtype=dtype, max_positions=args.input_len + args.decode_steps)
         if args.model_path != "dummy":
             net.load_hf_state_dict(load_checkpoint_file(args.model_path))
@@ -84,7 +85,7 @@ def main():
     groups = [dist.new_group(list(range(0, tp))), dist.new_group(list(range(tp, world)))]
     tp_group = groups[0] if is_prefill else groups[1]
     tp_rank = rank % tp
-    p = ServeParams(cfg, args.batch, args.input_len, args.decode_steps, tp, dtype)
+    p = ServeParams(cfg, args.batch, args.input_len, args.decode_steps, tp, dtype, **decoding_options(args))
     net = LlamaShard(cfg, tp_rank, tp, tp_group if tp > 1 else None, device=dev, dtype=dtype, max_positions=args.input_len + args.decode_steps)
     if args.model_path != "dummy":
         net.load_hf_state_dict(load_checkpoint_file(args.model_path))      # every shard cuts its part out of the full checkpoint
@@ -146,7 +147,7 @@ def _nccl_iteration(p, net, link, pre, dec, prompts, peer, is_prefill, t0):
     if is_prefill:
         e0, e1, e2 = (torch.cuda.Event(enable_timing=True) for _ in range(3))
         e0.record()
-        first = net.prefill(prompts, pre.k_pool, pre.v_pool, pre.src_bt, None)
+        first = pre.first_tokens(prompts)
         e1.record()
         ops = [dist.P2POp(dist.isend, t, peer) for t in (first, pre.k_pool, pre.v_pool, pre.src_bt, pre.nblocks)]
         for r in dist.batch_isend_irecv(ops):

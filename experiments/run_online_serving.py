@@ -34,13 +34,14 @@ def main():
                                                                               "the device entry points, as the tests run it)")
     ap.add_argument("--policy", default="fcfs", choices=["fcfs", "sjf", "aged"], help="order in which waiting requests are batched (fcfs: the reference)")
     ap.add_argument("--max-batch-tokens", type=int, default=0, help="limit on the active prompt tokens of one batch (0: none)")
-    args = ap.parse_args()
     from fuselink_b200.models.llama import MODEL_ZOO, LlamaShard
     from fuselink_b200.parallel.symm import SymmetricHeap
-    from fuselink_b200.serving.disagg import KVLink, ServeParams
+    from fuselink_b200.serving.disagg import KVLink, ServeParams, decoding_flags, decoding_options
+    decoding_flags(ap)
+    args = ap.parse_args()
     from fuselink_b200.serving.online import MAX_BATCH, OnlineDecode, OnlinePrefill, TraceReader, parse_trace
     cfg = MODEL_ZOO[args.model]
-    p = ServeParams(cfg, MAX_BATCH, args.input_len, args.decode_steps)
+    p = ServeParams(cfg, MAX_BATCH, args.input_len, args.decode_steps, **decoding_options(args))
     if args.trace:
         reqs = parse_trace(open(args.trace))
     else:
@@ -81,7 +82,7 @@ def multi_process(args, cfg, p, reqs):
     import torch.distributed as dist
     from fuselink_b200.models.llama import LlamaShard
     from fuselink_b200.parallel.symm import SymmetricHeap
-    from fuselink_b200.serving.disagg import KVLink, ServeParams
+    from fuselink_b200.serving.disagg import KVLink, ServeParams, decoding_options
     from fuselink_b200.serving.online import MAX_BATCH, OnlineDecode, OnlinePrefill, TraceReader
     rank, local, world = int(os.environ["RANK"]), int(os.environ.get("LOCAL_RANK", 0)), int(os.environ["WORLD_SIZE"])
     assert world % 2 == 0, "half of the ranks prefill, half decode"
@@ -97,7 +98,7 @@ def multi_process(args, cfg, p, reqs):
     is_prefill = rank < tp
     groups = [dist.new_group(list(range(0, tp))), dist.new_group(list(range(tp, world)))]
     group = groups[0] if is_prefill else groups[1]
-    p = ServeParams(cfg, MAX_BATCH, args.input_len, args.decode_steps, tp)
+    p = ServeParams(cfg, MAX_BATCH, args.input_len, args.decode_steps, tp, **decoding_options(args))
     net = LlamaShard(cfg, rank % tp, tp, group if tp > 1 else None, device=dev, max_positions=args.input_len + args.decode_steps)
     pool = 2 * p.batch_size * p.max_blocks_per_req * cfg.layers * net.kvh_local * cfg.block_size * cfg.head_dim * 2
     heap = SymmetricHeap.create(2 * pool + (64 << 20), device=-1 if cpu else local)

@@ -15,6 +15,8 @@ computation, rounded at the same places; it serves the CPU, fp32 and head sizes 
 Paged KV layouts (block = `block_size` tokens):
   prefill pool  [block][layer][head][slot][dim]   (FL_KV_BLHSD)
   decode pool   [layer][block][slot][head][dim]   (FL_KV_LBSHD)
+A cache in 8 bits (ops/kv8.py) takes the pools' place in ``prefill`` and is what ``extend`` works on.  Next tokens are the greedy choice, or
+what ``choose`` makes of the logits (ops/sampling.py).
 """
 from __future__ import annotations
 
@@ -25,6 +27,8 @@ import torch
 import torch.nn.functional as F
 
 from .._ext import require_native
+from ..ops import kv8
+from ..ops.kv8 import Kv8Cache
 
 KV_BLHSD, KV_LBSHD = 0, 1
 _OPERATIONS = ("_embed", "_norm", "_qkv", "_attn_out", "_mlp", "_logits")      # what the fused route does by itself
@@ -204,12 +208,19 @@ class LlamaShard(torch.nn.Module):
     def _logits(self, x):
         return (self._norm(x, self.final_norm, self.final_norm_b) @ self.lm_head.t()).float()
 
+    def _choose(self, x, choose):
+        """The next tokens at [..., hidden] positions of the residual stream."""
+        logits = self._logits(x)
+        if choose is None:
+            return logits.argmax(-1)
+        return choose(logits.flatten(0, -2).to(self.embed.dtype)).view(x.shape[:-1])      # the type that they were rounded to
+
     # ------------------------------------------------------------------------------------------- fused passes
-    def _fused(self, pool: torch.Tensor) -> bool:
+    def _fused(self, pool: Optional[torch.Tensor]) -> bool:
         """Whether csrc/kernels/decoder.cu takes this shard: not under autocast, which changes the types between the operations."""
         return self.embed.is_cuda and not torch.is_autocast_enabled("cuda") and self._fits(pool)
 
-    def _fits(self, pool: torch.Tensor) -> bool:
+    def _fits(self, pool: Optional[torch.Tensor]) -> bool:
         """16-bit weights and pools, rows and heads in whole 16-byte vectors (a rotated head in two halves of them), heads of at
         most 128; what the kernels read themselves (everything but the matrices) plain tensors of one type on one device,
         contiguous, from a multiple of 16 bytes on; and the operations of this class, not of a subclass or replaced on the object.
@@ -295,12 +306,13 @@ class LlamaShard(torch.nn.Module):
         C = require_native()
         return 0 < rows <= C.THIN_MAX_ROWS and all(C.dec_takes(list(ws), like, shape) for ws, *shape in matrices)
 
-    def _layers_fused(self, x, pos, seq, k_pool, v_pool, table, layout, num_blocks, attend, on_layer_done=None):
-        """Every layer on x [rows, hidden]; ``attend(l, qkv)`` returns the attention output [rows, h_local * D].  Returns
-        (x, y, bias): the residual stream without the last branch, the branch and its bias (final_norm adds them up)."""
+    def _layers_fused(self, x, pos, seq, k_pool, v_pool, table, layout, num_blocks, attend, on_layer_done=None, write=None):
+        """Every layer on x [rows, hidden]; ``attend(l, qkv)`` returns the attention output [rows, h_local * D]; ``write(l, qkv)``, where it is given, takes
+        the place of the pass that turns queries and keys and writes pages.  Returns (x, y, bias): the residual stream without the last
+        branch, the branch and its bias (final_norm adds them up)."""
         C, cfg = require_native(), self.cfg
         rows, kind, status = x.shape[0], _ACT[cfg.arch], self._status_addr()
-        rope = self._rope_table(table.shape[1] * cfg.block_size)
+        rope = None if write is not None else self._rope_table(table.shape[1] * cfg.block_size)
         h = torch.empty_like(x)
         H, q, F2 = cfg.hidden, self.h_local * cfg.head_dim, self.f_local
         thin = self._thin(rows, x, (self.wqkv, q + 2 * self.kvh_local * cfg.head_dim, H), (self.wo, H, q),
@@ -318,7 +330,10 @@ class LlamaShard(torch.nn.Module):
         for l in range(cfg.layers):
             C.dec_add_norm(x, y, bias, self.n1[l], self.n1b[l], h, cfg.eps)
             where = (k_pool, v_pool, table, layout, l, cfg.layers, num_blocks, cfg.block_size, self.h_local, self.kvh_local, cfg.head_dim)
-            if pages_in_product:
+            if write is not None:
+                qkv = product(h, self.wqkv[l])
+                write(l, qkv)
+            elif pages_in_product:
                 qkv = C.dec_qkv_product(h, self.wqkv[l], self.bqkv[l], rope, pos, *where, True, status)
             else:
                 qkv = product(h, self.wqkv[l])
@@ -334,7 +349,7 @@ class LlamaShard(torch.nn.Module):
             y, bias = self._allreduce(product(act, self.w2[l])), self.b2[l]
         return x, y, bias
 
-    def _choose_fused(self, x, y, bias):
+    def _choose_fused(self, x, y, bias, choose=None):
         """The tokens chosen at [..., hidden] positions of the residual stream; ``x`` is overwritten."""
         C = require_native()
         h = torch.empty_like(x)
@@ -344,9 +359,9 @@ class LlamaShard(torch.nn.Module):
             logits = C.dec_product(rows, self.lm_head, None, _STORE, True, self._status_addr())
         else:
             logits = rows @ self.lm_head.t()
-        return C.dec_argmax(logits).view(h.shape[:-1])
+        return (C.dec_argmax(logits) if choose is None else choose(logits)).view(h.shape[:-1])
 
-    def _prefill_fused(self, tokens, k_pool, v_pool, block_table, on_layer_done, last_pos):
+    def _prefill_fused(self, tokens, k_pool, v_pool, block_table, on_layer_done, last_pos, choose):
         self.check_status()
         C, cfg = require_native(), self.cfg
         B, S = tokens.shape
@@ -356,7 +371,8 @@ class LlamaShard(torch.nn.Module):
             raise RuntimeError(f"block table of {tuple(block_table.shape)} for {B} prompts of {S // cfg.block_size} pages")
         if self.pos_embed is not None and S + cfg.pos_offset > self.pos_embed.shape[0]:
             raise IndexError(f"prompts of {S} tokens, {self.pos_embed.shape[0] - cfg.pos_offset} positions")
-        num_blocks = k_pool.view(-1, cfg.layers, kl, cfg.block_size, D).shape[0]
+        cache = k_pool if isinstance(k_pool, Kv8Cache) else None
+        num_blocks = 0 if cache is not None else k_pool.view(-1, cfg.layers, kl, cfg.block_size, D).shape[0]
         x = torch.empty(B * S, cfg.hidden, dtype=self.embed.dtype, device=tokens.device)
         C.dec_embed(tokens, None, self.embed, self.pos_embed, x, S, cfg.pos_offset, self._status_addr())
 
@@ -365,13 +381,56 @@ class LlamaShard(torch.nn.Module):
             o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True, enable_gqa=hl != kl)
             return o.transpose(1, 2).reshape(B * S, hl * D)
 
-        x, y, bias = self._layers_fused(x, None, S, k_pool, v_pool, table, KV_BLHSD, num_blocks, attend, on_layer_done)
+        write = None if cache is None else self._writer(cache, table, B, S, *self._prompts(tokens, last_pos), S)
+        x, y, bias = self._layers_fused(x, None, S, k_pool, v_pool, table, KV_BLHSD, num_blocks, attend, on_layer_done, write)
         # indexed per request, so that a position counts from the request's own end or is out of its range
         at = (slice(None), -1) if last_pos is None else (torch.arange(B, device=x.device), last_pos)
         x, y = (t.view(B, S, cfg.hidden)[at] for t in (x, y))
-        return self._choose_fused(x.contiguous(), y.contiguous(), bias)
+        return self._choose_fused(x.contiguous(), y.contiguous(), bias, choose)
 
-    def _decode_fused(self, tokens, positions, k_pool, v_pool, block_table, num_blocks):
+    def _writer(self, cache, table, B, T, start, counts, positions, max_positions):
+        """What ``_layers_fused`` does with the rows of its products, for a cache in 8 bits."""
+        A, D, status = self.h_local + 2 * self.kvh_local, self.cfg.head_dim, self._status_addr()
+        rope = self._rope_table(max_positions)
+
+        def write(l, qkv):
+            rows = qkv.view(B, T, A, D)
+            kv8.write(cache, l, rows, table, start, counts=counts, positions=positions, rope=rope, bias=self.bqkv[l], out=rows, status=status)
+
+        return write
+
+    @staticmethod
+    def _prompts(tokens, last_pos):
+        """(start, counts, positions) of prompts that begin a cache; where last_pos says which token of each is the last, no more are written, since
+        what follows in its page would share its scale."""
+        B, S = tokens.shape
+        start = torch.zeros(B, dtype=torch.long, device=tokens.device)
+        if not torch.is_tensor(last_pos) or last_pos.shape != (B,):
+            return start, None, None
+        last = last_pos.to(tokens.device).long()
+        return start, torch.where(last < 0, last + S, last) + 1, None
+
+    def _extend_fused(self, tokens, positions, cache, block_table, slots, counts, mass, max_positions, choose):
+        self.check_status()
+        C, cfg, status = require_native(), self.cfg, self._status_addr()
+        (B, T), D, hl, kl, dev = tokens.shape, cfg.head_dim, self.h_local, self.kvh_local, self.embed.device
+        tokens, positions, slots, table = self._indices(tokens), self._indices(positions), self._indices(slots), self._pages(block_table)
+        counts = None if counts is None else self._indices(counts)
+        x = torch.empty(B * T, cfg.hidden, dtype=self.embed.dtype, device=dev)
+        each = positions if T == 1 else (positions.unsqueeze(1) + torch.arange(T, device=dev)).flatten()
+        if T > 1 and self.pos_embed is not None and counts is not None:      # padding has no position
+            each = torch.where((torch.arange(T, device=dev) < counts.unsqueeze(1)).flatten(), each, torch.zeros_like(each))
+        C.dec_embed(tokens, each, self.embed, self.pos_embed, x, 1, cfg.pos_offset, status)
+        out = torch.empty(B, T, hl * D, dtype=x.dtype, device=dev)
+
+        def attend(l, qkv):
+            kv8.attention(cache, l, qkv.view(B, T, hl + 2 * kl, D)[:, :, :hl], table, slots, counts=counts, mass=mass, out=out, status=status)
+            return out.view(B * T, hl * D)
+
+        write = self._writer(cache, table, B, T, slots, counts, positions, max_positions)
+        return self._choose_fused(*self._layers_fused(x, None, 1, None, None, table, KV_LBSHD, 0, attend, write=write), choose).view(B, T)
+
+    def _decode_fused(self, tokens, positions, k_pool, v_pool, block_table, num_blocks, choose):
         self.check_status()
         C, cfg, status = require_native(), self.cfg, self._status_addr()
         B, D, hl, kl, dev = tokens.shape[0], cfg.head_dim, self.h_local, self.kvh_local, self.embed.device
@@ -388,31 +447,43 @@ class LlamaShard(torch.nn.Module):
             C.dec_attention(qkv, positions, k_pool, v_pool, table, l, cfg.layers, num_blocks, cfg.block_size, hl, kl, D, out, status)
             return out
 
-        return self._choose_fused(*self._layers_fused(x, positions, 1, k_pool, v_pool, table, KV_LBSHD, num_blocks, attend))
+        return self._choose_fused(*self._layers_fused(x, positions, 1, k_pool, v_pool, table, KV_LBSHD, num_blocks, attend), choose)
 
     # ------------------------------------------------------------------------------------------- prefill
     @torch.no_grad()
     def prefill(self, tokens: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
-                on_layer_done: Optional[Callable[[int], None]] = None, last_pos: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """tokens: [B, S] (S a multiple of block_size); pools: flat bf16 in the BLHSD layout; block_table: [B, >=S/bs]
-        int32.  Fills the pools, returns the greedy first token of every sequence [B] (int64)."""
+                on_layer_done: Optional[Callable[[int], None]] = None, last_pos: Optional[torch.Tensor] = None,
+                choose: Optional[Callable[[torch.Tensor], torch.Tensor]] = None) -> torch.Tensor:
+        """tokens: [B, S] (S a multiple of block_size); pools: flat bf16 in the BLHSD layout, or a Kv8Cache and None; block_table: [B, >=S/bs]
+        int32.  Fills the pools, returns the first token of every sequence [B] (int64): the greedy one, or what ``choose`` makes of
+        the logits [B, vocab] (of the model's type)."""
         cfg = self.cfg
         B, S = tokens.shape
         bs, D, L = cfg.block_size, cfg.head_dim, cfg.layers
         assert S % bs == 0
-        if self._fused(k_pool) and self._same_kind(v_pool, k_pool):
-            return self._prefill_fused(tokens, k_pool, v_pool, block_table, on_layer_done, last_pos)
+        cache = k_pool if isinstance(k_pool, Kv8Cache) else None
+        if cache is not None:
+            self._check_cache(cache)
+        if self._fused(None) if cache is not None else self._fused(k_pool) and self._same_kind(v_pool, k_pool):
+            return self._prefill_fused(tokens, k_pool, v_pool, block_table, on_layer_done, last_pos, choose)
         nblk = S // bs
-        kp = k_pool.view(-1, L, self.kvh_local, bs, D)
-        vp = v_pool.view(-1, L, self.kvh_local, bs, D)
+        if cache is not None:
+            start, counts, _ = self._prompts(tokens, last_pos)
+            table = self._pages(block_table[:, :nblk])
+        else:
+            kp = k_pool.view(-1, L, self.kvh_local, bs, D)
+            vp = v_pool.view(-1, L, self.kvh_local, bs, D)
         blocks = block_table[:, :nblk].long().reshape(-1)                       # [B*nblk]
         pos = torch.arange(S, device=tokens.device).unsqueeze(0).expand(B, S)
         x = self._embed(tokens, pos)                                            # [B, S, H]
         for l in range(L):
             q, k, v = self._qkv(l, self._norm(x, self.n1[l], self.n1b[l]), pos)
             # page write: [B, S, h, D] -> [B*nblk, h, bs, D]
-            kp[blocks, l] = k.reshape(B * nblk, bs, self.kvh_local, D).permute(0, 2, 1, 3)
-            vp[blocks, l] = v.reshape(B * nblk, bs, self.kvh_local, D).permute(0, 2, 1, 3)
+            if cache is not None:
+                kv8.write(cache, l, torch.cat([q, k, v], -2), table, start, counts=counts, status=self._status_or_0())
+            else:
+                kp[blocks, l] = k.reshape(B * nblk, bs, self.kvh_local, D).permute(0, 2, 1, 3)
+                vp[blocks, l] = v.reshape(B * nblk, bs, self.kvh_local, D).permute(0, 2, 1, 3)
             if on_layer_done is not None:
                 on_layer_done(l)                                                # KV of this layer may leave now
             o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True,
@@ -420,19 +491,20 @@ class LlamaShard(torch.nn.Module):
             x = x + self._attn_out(l, o.transpose(1, 2).reshape(B, S, self.h_local * D))
             x = x + self._mlp(l, self._norm(x, self.n2[l], self.n2b[l]))
         xl = x[:, -1] if last_pos is None else x[torch.arange(B, device=x.device), last_pos]
-        return self._logits(xl).argmax(-1)
+        return self._choose(xl, choose)
 
     # ------------------------------------------------------------------------------------------- decode
     @torch.no_grad()
     def decode_step(self, tokens: torch.Tensor, positions: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
-                    block_table: torch.Tensor, num_pool_blocks: int) -> torch.Tensor:
-        """One greedy step for B sequences.  tokens, positions: [B]; pools: flat bf16 in the LBSHD layout;
-        block_table: [B, max_blocks] int32 covering position + 1 tokens.  Returns next tokens [B]."""
+                    block_table: torch.Tensor, num_pool_blocks: int, choose: Optional[Callable[[torch.Tensor], torch.Tensor]] = None) -> torch.Tensor:
+        """One step for B sequences.  tokens, positions: [B]; pools: flat bf16 in the LBSHD layout;
+        block_table: [B, max_blocks] int32 covering position + 1 tokens.  Returns next tokens [B]: the greedy ones, or what ``choose``
+        makes of the logits [B, vocab]."""
         cfg = self.cfg
         B = tokens.shape[0]
         bs, D, L = cfg.block_size, cfg.head_dim, cfg.layers
         if 0 < B <= 65535 and self._fused(k_pool) and self._same_kind(v_pool, k_pool):
-            return self._decode_fused(tokens, positions, k_pool, v_pool, block_table, num_pool_blocks)
+            return self._decode_fused(tokens, positions, k_pool, v_pool, block_table, num_pool_blocks, choose)
         kp = k_pool.view(L, num_pool_blocks, bs, self.kvh_local, D)
         vp = v_pool.view(L, num_pool_blocks, bs, self.kvh_local, D)
         bt = block_table.long()
@@ -454,7 +526,53 @@ class LlamaShard(torch.nn.Module):
                                                enable_gqa=self.h_local != self.kvh_local)
             x = x + self._attn_out(l, o.transpose(1, 2).reshape(B, self.h_local * D))
             x = x + self._mlp(l, self._norm(x, self.n2[l], self.n2b[l]))
-        return self._logits(x).argmax(-1)
+        return self._choose(x, choose)
+
+    # ------------------------------------------------------------------------------------------- new tokens over a cache in 8 bits
+    def _check_cache(self, cache: Kv8Cache) -> None:
+        cfg = self.cfg
+        want = (cfg.layers, self.kvh_local, cfg.block_size, cfg.head_dim)
+        if tuple(cache.k.shape[i] for i in (0, 2, 3, 4)) != want:
+            raise RuntimeError(f"cache of {tuple(cache.k.shape)} for {want[0]} layers, {want[1]} KV heads, pages of {want[2]}, heads of {want[3]}")
+
+    def _status_or_0(self) -> int:
+        return self._status_addr() if self.embed.is_cuda else 0
+
+    @torch.no_grad()
+    def extend(self, tokens: torch.Tensor, positions: torch.Tensor, cache: Kv8Cache, block_table: torch.Tensor, *, slots: Optional[torch.Tensor] = None,
+               counts: Optional[torch.Tensor] = None, mass: Optional[torch.Tensor] = None, max_positions: Optional[int] = None,
+               choose: Optional[Callable[[torch.Tensor], torch.Tensor]] = None) -> torch.Tensor:
+        """The next tokens behind every one of B sequences' new ones: tokens [B] (a decoding step) or [B, T] (a further piece of a prompt, a guess to
+        be verified), at positions ``positions[b] + t`` and in slots ``slots[b] + t`` (positions, unless pages have been evicted) of the cache's pages
+        ``block_table[b]``; counts ([B]): how many of a padded row's T are tokens.  Returns tokens of the same shape; what stands behind counts
+        says nothing.
+        mass ([B, pages] fp32): this shard's heads' attention weights are added to it, all layers, page by page (ops/kv8.py, ``evict``).
+        max_positions: positions there may be (the table's slots, if not given); one beyond is an IndexError from the next call on."""
+        self._check_cache(cache)
+        cfg, shape = self.cfg, tokens.shape
+        tokens = tokens.unsqueeze(1) if tokens.dim() == 1 else tokens
+        B, T = tokens.shape
+        if block_table.shape[0] != B:
+            raise RuntimeError(f"block table of {tuple(block_table.shape)} for {B} sequences")
+        slots = positions if slots is None else slots
+        most = block_table.shape[1] * cfg.block_size if max_positions is None else max_positions
+        if B == 0 or T == 0:
+            return torch.zeros(shape, dtype=torch.long, device=tokens.device)
+        if B <= 65535 and self._fused(None):
+            return self._extend_fused(tokens, positions, cache, block_table, slots, counts, mass, most, choose).view(shape)
+        table, hl, status = self._pages(block_table), self.h_local, self._status_or_0()
+        slots = slots.long()
+        pos = positions.long().unsqueeze(1) + torch.arange(T, device=tokens.device)
+        if counts is not None:
+            counts = counts.long()
+            pos = torch.where(torch.arange(T, device=tokens.device) < counts.unsqueeze(1), pos, torch.zeros_like(pos))
+        x = self._embed(tokens, pos)                                             # [B, T, H]
+        for l in range(cfg.layers):
+            q, k, v = self._qkv(l, self._norm(x, self.n1[l], self.n1b[l]), pos)
+            kv8.write(cache, l, torch.cat([q, k, v], -2), table, slots, counts=counts, status=status)
+            x = x + self._attn_out(l, kv8.attention(cache, l, q, table, slots, counts=counts, mass=mass, status=status))
+            x = x + self._mlp(l, self._norm(x, self.n2[l], self.n2b[l]))
+        return self._choose(x, choose).view(shape)
 
     # reference path for tests: full-sequence forward without paging, returns logits of the last position
     @torch.no_grad()

@@ -30,23 +30,26 @@ def main():
     ap.add_argument("--tracepath", default="")
     ap.add_argument("--kv", default="fuselink", choices=["fuselink", "fuselink-nopipe", "nccl"])
     ap.add_argument("--device", default="cuda", choices=["cuda", "cpu"], help="cpu: only under a model of the device entry points (tests)")
-    a = ap.parse_args()
     from fuselink_b200.models.llama import MODEL_ZOO
+    from fuselink_b200.serving.disagg import decoding_flags, decoding_options
+    decoding_flags(ap)
+    a = ap.parse_args()
 
     if a.model_name not in MODEL_ZOO:
         raise SystemExit(f"unknown model {a.model_name}; known: {', '.join(MODEL_ZOO)}")
     MODEL_ZOO[a.model_name].block_size = a.block_size
     root = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     world = int(os.environ.get("WORLD_SIZE", "1"))
+    more = [x for k, v in decoding_options(a).items() for x in ("--" + k, str(v))]
     if a.tp_size and world > 1 and a.tp_size != world // 2:
         raise SystemExit(f"--tp_size {a.tp_size} needs {2 * a.tp_size} ranks (got {world})")
     if a.tracepath:
         sys.argv = ["run_online_serving.py", "--trace", a.tracepath, "--model", a.model_name, "--input-len", str(a.input_len),
-                    "--decode-steps", str(a.num_decoding_step), "--device", a.device]
+                    "--decode-steps", str(a.num_decoding_step), "--device", a.device, *more]
         runpy.run_path(os.path.join(root, "experiments", "run_online_serving.py"), run_name="__main__")
     else:
         sys.argv = ["serving_bench.py", "--model", a.model_name, "--kv", a.kv, "--batch", str(a.batch_size), "--input-len",
-                    str(a.input_len), "--decode-steps", str(a.num_decoding_step), "--model-path", a.model_path, "--precision", a.precision, "--device", a.device] + (["--emulate"] if world == 1 else [])
+                    str(a.input_len), "--decode-steps", str(a.num_decoding_step), "--model-path", a.model_path, "--precision", a.precision, "--device", a.device, *more] + (["--emulate"] if world == 1 else [])
         runpy.run_path(os.path.join(root, "bench", "serving_bench.py"), run_name="__main__")
 
 

@@ -24,6 +24,8 @@ import torch
 
 from .._ext import require_native
 from ..models.llama import KV_BLHSD, KV_LBSHD, LlamaConfig, LlamaShard
+from ..ops import kv8
+from ..ops.sampling import Sampler
 from ..parallel.symm import SymmetricHeap
 from ..utils.timing import device_sync, timing_event
 
@@ -39,6 +41,27 @@ def check_model(model) -> None:
         check()
 
 
+def choice(choose) -> dict:
+    """How a model is told of a choice other than the greedy one."""
+    return {} if choose is None else {"choose": choose}
+
+
+def decoding_flags(ap) -> None:
+    """Command line of ServeParams' decoding options."""
+    ap.add_argument("--kv-bits", "--kv_bits", type=int, default=16, choices=[8, 16], help="bits of a cached key or value on the decode side")
+    ap.add_argument("--keep-blocks", "--keep_blocks", type=int, default=0, help="pages that a request may keep, of a cache in 8 bits; the least attended ones go (0: all stay)")
+    ap.add_argument("--temperature", type=float, default=0.0, help="0: greedy")
+    ap.add_argument("--top-k", "--top_k", type=int, default=0)
+    ap.add_argument("--top-p", "--top_p", type=float, default=1.0)
+    ap.add_argument("--min-p", "--min_p", type=float, default=0.0)
+    ap.add_argument("--seed", type=int, default=0)
+
+
+def decoding_options(args) -> dict:
+    """What the flags say, as keyword arguments of ServeParams."""
+    return {k: getattr(args, k) for k in ("kv_bits", "keep_blocks", "temperature", "top_k", "top_p", "min_p", "seed")}
+
+
 @dataclass
 class ServeParams:
     """The experiment's knobs (TestParams of the reference, experiments/serving/model.hh:31-49)."""
@@ -48,6 +71,33 @@ class ServeParams:
     num_decoding_step: int = 256
     tp_size: int = 1
     dtype: torch.dtype = torch.bfloat16     # --precision of the reference's binaries (fp16 / fp32 there); KV pools use it too
+    # Decoding beyond the reference's: a cache in 8 bits (ops/kv8.py), at most so many pages per request (0: all of them; the lightest go, but not the
+    # first and the last two), and tokens drawn by chance (ops/sampling.py; temperature 0: the greedy ones)
+    kv_bits: int = 16
+    keep_blocks: int = 0
+    temperature: float = 0.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: int = 0
+
+    EVICT_SINKS, EVICT_RECENT = 1, 2        # pages that are never given back
+
+    def check(self) -> None:
+        if self.kv_bits not in (8, 16):
+            raise ValueError(f"kv_bits {self.kv_bits}: 8 or 16")
+        if self.keep_blocks and (self.kv_bits != 8 or self.keep_blocks < self.EVICT_SINKS + self.EVICT_RECENT):
+            raise ValueError(f"keep_blocks {self.keep_blocks}: at least {self.EVICT_SINKS + self.EVICT_RECENT}, of a cache in 8 bits")
+
+    def sampler(self, batch: int, device) -> Optional[Sampler]:
+        """What chooses the tokens of a batch; None: the greedy choice."""
+        if not self.temperature > 0:
+            return None
+        return Sampler(torch.zeros(batch, device=device), self.temperature, self.top_k, self.top_p, self.min_p)
+
+    def numbers(self, device) -> torch.Generator:
+        """The source of a stage's uniform numbers, the same one on every shard."""
+        return torch.Generator(device=device).manual_seed(self.seed)
 
     @property
     def elem_bytes(self) -> int:
@@ -114,6 +164,53 @@ class KVLink:
         self.C.wait_flags([(self.heap.sig_addr(self.layer_flags + l), self.seq)], self.heap.status_addr)
 
 
+class SmallCache:
+    """A decode stage's cache in 8 bits: filled from the pages that the hand-off left, extended by every step, and cut to ``p.keep_blocks`` pages per
+    request after every ``block_size`` steps."""
+
+    def __init__(self, p: ServeParams, model: LlamaShard, link: KVLink):
+        self.p, self.model, m = p, model, p.model
+        dev, B = model.embed.device, p.batch_size
+        self.cache = kv8.Kv8Cache.empty(m.layers, link.pool_blocks, model.kvh_local, m.block_size, m.head_dim, device=dev)
+        # buffers that a captured step may hold
+        self._table = torch.zeros(B, p.max_blocks_per_req, dtype=torch.int32, device=dev)
+        self._slots = torch.zeros(B, dtype=torch.long, device=dev)
+        self._seen, self._mass = (torch.zeros(B, p.max_blocks_per_req, device=dev) for _ in range(2))     # since the last eviction, and before
+        self.begin_empty(B)
+
+    def begin_empty(self, batch: int) -> None:
+        self.table, self.slots, self.seen, self.mass = (t[:batch] for t in (self._table, self._slots, self._seen, self._mass))
+        self.steps = 0
+
+    def begin(self, link: KVLink, table: torch.Tensor, lengths: torch.Tensor) -> None:
+        """A batch whose first ``lengths`` tokens are in ``link``'s pages ``table``."""
+        self.begin_empty(table.shape[0])
+        self.table.copy_(table)
+        self.slots.copy_(lengths)
+        self.seen.zero_()
+        self.mass.zero_()
+        status = self.model._status_or_0()
+        kv8.pack(self.cache, link.k_pool.local, link.v_pool.local, link.pool_blocks, table, self.table, self.slots, status=status)
+
+    def step(self, tokens: torch.Tensor, pos: torch.Tensor, choose=None) -> torch.Tensor:
+        return self.model.extend(tokens, pos, self.cache, self.table, slots=self.slots, mass=self.seen if self.p.keep_blocks else None, choose=choose,
+                                 max_positions=self.p.input_len + self.p.num_decoding_step + self.p.block_size)
+
+    def advance(self) -> None:
+        """The step's tokens are in the cache (part of a captured step)."""
+        self.slots.add_(1)
+
+    def after_step(self) -> None:
+        self.steps += 1
+        if self.p.keep_blocks and self.steps % self.p.block_size == 0:
+            self.mass += self.model._allreduce(self.seen)                   # every shard's heads
+            self.seen.zero_()
+            table, slots, mass, _ = kv8.evict(self.mass, self.table, self.slots, self.p.block_size, self.p.keep_blocks,
+                                              recent=self.p.EVICT_RECENT, sinks=self.p.EVICT_SINKS)
+            for t, new in ((self.table, table), (self.slots, slots), (self.mass, mass)):
+                t.copy_(new)
+
+
 @dataclass
 class StageReport:
     role: str
@@ -145,6 +242,14 @@ class PrefillStage:
         self.side = torch.cuda.Stream(device=dev) if dev.type == "cuda" else None
         self.dev = dev
         self.hdr = torch.zeros(HDR_INTS, dtype=torch.int64, device=dev)
+        p.check()
+        self.choose, self.numbers = p.sampler(B, dev), p.numbers(dev)
+
+    def first_tokens(self, tokens: torch.Tensor, on_layer_done=None) -> torch.Tensor:
+        """The prompts through the model, into the stage's own pools."""
+        if self.choose is not None:
+            self.choose.u.copy_(torch.rand(len(self.choose.u), generator=self.numbers, device=self.dev))
+        return self.model.prefill(tokens, self.k_pool, self.v_pool, self.src_bt, on_layer_done, **choice(self.choose))
 
     def run(self, tokens: torch.Tensor) -> StageReport:
         p, link = self.p, self.link
@@ -172,7 +277,7 @@ class PrefillStage:
                 link.send_layers(self.dst, self.k_pool, self.v_pool, self.ctx_blocks, self.src_bt, self.dst_bt, self.nblocks, l, l + 1)
 
         e0.record(main)
-        first = self.model.prefill(tokens, self.k_pool, self.v_pool, self.src_bt, on_layer)
+        first = self.first_tokens(tokens, on_layer)
         e1.record(main)
         self.hdr[0], self.hdr[1], self.hdr[2] = p.batch_size, p.input_len, p.max_blocks_per_req
         self.hdr[4:4 + p.batch_size] = first
@@ -196,8 +301,9 @@ class PrefillStage:
 
 
 class DecodeStage:
-    """Greedy decoding over the paged pool.  The per-token step is launch-bound (hundreds of small kernels), so it
-    is captured once in a CUDA graph and replayed; ``use_graph=False`` keeps the eager loop."""
+    """Decoding over the paged pool, or over a cache in 8 bits made from it (``p.kv_bits``); greedy, or by chance (``p.temperature``).  The
+    per-token step is launch-bound (hundreds of small kernels), so it is captured once in a CUDA graph and replayed;
+    ``use_graph=False`` keeps the eager loop."""
 
     def __init__(self, p: ServeParams, model: LlamaShard, link: KVLink, use_graph: bool = True):
         self.p, self.model, self.link = p, model, link
@@ -215,10 +321,20 @@ class DecodeStage:
         # lengths a caller may change; longer runs than the history has rows for are read out in between.
         self.g_hist = torch.zeros(max(1, p.num_decoding_step), B, dtype=torch.long, device=dev)
         self.g_step = torch.zeros(1, dtype=torch.long, device=dev)
+        p.check()
+        self.small = SmallCache(p, model, link) if p.kv_bits == 8 else None
+        self.choose, self.numbers = p.sampler(B, dev), p.numbers(dev)
+        self.g_u = None if self.choose is None else torch.zeros_like(self.g_hist, dtype=torch.float32)      # what every step draws by
 
     def _step(self, tokens, pos):
         link = self.link
-        return self.model.decode_step(tokens, pos, link.k_pool.local, link.v_pool.local, self.bt, link.pool_blocks)
+        if self.small is not None:
+            return self.small.step(tokens, pos, self.choose)
+        return self.model.decode_step(tokens, pos, link.k_pool.local, link.v_pool.local, self.bt, link.pool_blocks, **choice(self.choose))
+
+    def _draw(self, n: int) -> None:
+        if self.choose is not None:
+            self.g_u[:n].copy_(torch.rand(n, self.p.batch_size, generator=self.numbers, device=self.dev))
 
     def _capture(self):
         """Capture one decode step on static buffers.  The step writes K/V at g_pos, so the capture (which runs the
@@ -232,8 +348,12 @@ class DecodeStage:
             torch.cuda.current_stream().wait_stream(side)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
+                if self.choose is not None:
+                    self.choose.u.copy_(self.g_u.index_select(0, self.g_step)[0])
                 out = self._step(self.g_tokens, self.g_pos)
                 self.link.C.dec_advance(out, self.g_tokens, self.g_pos, self.g_hist, self.g_step)
+                if self.small is not None:
+                    self.small.advance()
             self.graph = g
         except Exception as e:  # noqa: BLE001 - capture is an optimisation; the eager loop is always valid
             self.graph = None
@@ -250,8 +370,12 @@ class DecodeStage:
         if self.use_graph and self.graph is None:
             self.g_tokens.copy_(tokens)
             self.g_pos.copy_(pos)
+            if self.small is not None:
+                self.small.begin(self.link, self.bt, pos)
             self._capture()                     # one-off set-up, outside the timed loop
         d0.record()
+        if self.small is not None:
+            self.small.begin(self.link, self.bt, pos)
         if self.graph is not None:
             self.g_tokens.copy_(tokens)
             self.g_pos.copy_(pos)
@@ -259,13 +383,24 @@ class DecodeStage:
             for first in range(0, p.num_decoding_step, rows):
                 n = min(rows, p.num_decoding_step - first)
                 self.g_step.zero_()
+                self._draw(n)
                 for _ in range(n):
                     self.graph.replay()
+                    if self.small is not None:
+                        self.small.after_step()
                 out.append(self.g_hist[:n].clone() if first + n < p.num_decoding_step else self.g_hist[:n])
             gen = torch.cat([tokens.unsqueeze(1), *(h.t() for h in out[1:])], 1)
         else:
-            for _ in range(p.num_decoding_step):
+            rows = self.g_hist.shape[0]
+            for i in range(p.num_decoding_step):
+                if i % rows == 0:
+                    self._draw(min(rows, p.num_decoding_step - i))
+                if self.choose is not None:
+                    self.choose.u.copy_(self.g_u[i % rows])
                 tokens = self._step(tokens, pos)
+                if self.small is not None:
+                    self.small.advance()
+                    self.small.after_step()
                 out.append(tokens)
                 pos = pos + 1
             gen = torch.stack(out, 1)

@@ -24,7 +24,7 @@ from typing import Callable, Iterable, List, Optional
 
 import torch
 
-from .disagg import HDR_INTS, HDR_LENS, HDR_OUTS, KVLink, ServeParams, check_model
+from .disagg import HDR_INTS, HDR_LENS, HDR_OUTS, KVLink, ServeParams, SmallCache, check_model, choice
 from ..models.llama import LlamaShard
 from ..utils.timing import device_sync, timing_event
 
@@ -120,6 +120,8 @@ class OnlinePrefill:
         self.credit_pad = links[0].heap.alloc_tensor([16], torch.uint8)     # landing zone of the decoder's credit write
         self.batches = 0
         self.stats: List[BatchStats] = []
+        p.check()
+        self.numbers = p.numbers(dev)
 
     def serve_batch(self, reqs: List[Request]) -> BatchStats:
         p, m = self.p, self.p.model
@@ -143,7 +145,10 @@ class OnlinePrefill:
         e0.record()
         # prefill computes on the padded batch; the last real position of each request gives its first token
         last_pos = torch.tensor([l - 1 for l in lens], dtype=torch.long, device=self.dev)
-        first = self.model.prefill(tokens, self.k_pool, self.v_pool, src_bt, None, last_pos=last_pos)
+        choose = p.sampler(B, self.dev)
+        if choose is not None:
+            choose.u.copy_(torch.rand(B, generator=self.numbers, device=self.dev))
+        first = self.model.prefill(tokens, self.k_pool, self.v_pool, src_bt, None, last_pos=last_pos, **choice(choose))
         e1.record()
         if use > 0:   # wait until the decoder has released this pool (credit = number of batches it finished on it)
             self._wait_credit(use)
@@ -201,6 +206,9 @@ class OnlineDecode:
         self.credit_pad = links[0].heap.alloc_tensor([16], torch.uint8)
         self.batches = 0
         self.done_on = [0] * len(links)
+        p.check()
+        self.small = SmallCache(p, model, links[0]) if p.kv_bits == 8 and model is not None else None
+        self.numbers = p.numbers(links[0].k_pool.local.device)
 
     def serve_batch(self, max_steps: int) -> dict:
         p = self.p
@@ -224,11 +232,21 @@ class OnlineDecode:
         bt = (torch.arange(B, dtype=torch.int32, device=dev).unsqueeze(1) * mb + torch.arange(mb, dtype=torch.int32, device=dev).unsqueeze(0)).contiguous()
         steps = min(max_steps, p.num_decoding_step)
         gen = [tokens]
+        choose = p.sampler(B, dev)
+        if self.small is not None:
+            self.small.begin(link, bt, pos)
         for _ in range(steps):
             if self.model is None or self.sleep_ms > 0:
                 time.sleep(self.sleep_ms / 1e3)
             else:
-                tokens = self.model.decode_step(tokens, pos, link.k_pool.local, link.v_pool.local, bt, link.pool_blocks)
+                if choose is not None:
+                    choose.u.copy_(torch.rand(B, generator=self.numbers, device=dev))
+                if self.small is not None:
+                    tokens = self.small.step(tokens, pos, choose)
+                    self.small.advance()
+                    self.small.after_step()
+                else:
+                    tokens = self.model.decode_step(tokens, pos, link.k_pool.local, link.v_pool.local, bt, link.pool_blocks, **choice(choose))
                 pos = pos + 1
                 gen.append(tokens)
         device_sync(dev)

@@ -246,3 +246,78 @@ def test_kv_hand_off_through_the_copy_engine(layout, ctas, hdr_bytes, shift):
         else:
             want[:, di] = s[si].permute(1, 0, 3, 2, 4)
         assert torch.equal(d.view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.parametrize("options", [dict(), dict(keep_blocks=4), dict(temperature=0.7, top_k=20, top_p=0.9), dict(keep_blocks=3, temperature=1.0, min_p=0.05)])
+def test_decode_stage_over_a_small_cache(options):
+    """Captured and eager stages give the same tokens, twice in a row; without limits they are those of the 16-bit cache, whose winners win by a margin."""
+    from fuselink_b200.models.llama import MODEL_ZOO, LlamaShard
+    from fuselink_b200.parallel.symm import SymmetricHeap
+    from fuselink_b200.serving.disagg import DecodeStage, KVLink, ServeParams
+    p = ServeParams(model=MODEL_ZOO["tiny"], batch_size=3, input_len=70, num_decoding_step=40, kv_bits=8, **options)
+    heap, = SymmetricHeap.emulated(1, 32 << 20)
+    try:
+        net = LlamaShard(p.model, device="cuda", seed=1)
+        net.lm_head = net.embed.roll(1, 0).clone()
+        net.embed.mul_(50)
+        link = KVLink(heap, p, net.kvh_local)
+        for pool in (link.k_pool.local, link.v_pool.local):
+            pool.normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+        stages = [DecodeStage(p, net, link, use_graph=g) for g in (True, False)]
+        first = torch.tensor([5, 900, 31], device="cuda")
+        for _ in range(2):
+            got, want = (s.decode(first)[0] for s in stages)
+            assert got.shape == (3, 41) and torch.equal(got, want)
+        assert stages[0].graph is not None and stages[0].small.slots.tolist() == stages[1].small.slots.tolist()
+        pages = (stages[0].small.slots + 15) // 16
+        assert (pages <= (options["keep_blocks"] + 1 if "keep_blocks" in options else 7)).all()
+        if not options:
+            full = ServeParams(model=MODEL_ZOO["tiny"], batch_size=3, input_len=70, num_decoding_step=40)
+            assert torch.equal(DecodeStage(full, net, link).decode(first)[0], got)
+    finally:
+        heap.close()
+
+
+@pytest.mark.parametrize("model", ["tiny", "tiny_opt"])
+def test_fused_layers_over_a_small_cache_match_the_operations(model, monkeypatch):
+    """Prompt, single tokens, a piece of several: pages, weights and tokens with the decoder's kernels and with its operations."""
+    from fuselink_b200.models.llama import MODEL_ZOO, LlamaShard
+    from fuselink_b200.ops import kv8
+    net = LlamaShard(MODEL_ZOO[model], device="cuda", seed=2)
+    net.lm_head = net.embed.roll(1, 0).clone()
+    net.embed.mul_(50)
+    cfg, res = net.cfg, []
+    toks = torch.randint(0, cfg.vocab, (3, 48), generator=torch.Generator().manual_seed(2)).cuda()
+    table = torch.randperm(18, generator=torch.Generator().manual_seed(1)).view(3, 6).int().cuda()
+    for fused in (True, False):
+        if not fused:
+            monkeypatch.setattr(LlamaShard, "_fused", lambda self, pool: False)
+        cache = kv8.Kv8Cache.empty(cfg.layers, 18, cfg.kv_heads, cfg.block_size, cfg.head_dim)
+        mass, pos = torch.zeros(3, 6, device="cuda"), torch.tensor([48, 21, 48], device="cuda")
+        got = [net.prefill(toks, cache, None, table, last_pos=torch.tensor([47, 20, -1], device="cuda"))]
+        for _ in range(2):
+            got.append(net.extend(got[-1], pos, cache, table, mass=mass))
+            pos = pos + 1
+        got.append(net.extend(toks[:, :5], pos, cache, table, counts=torch.tensor([5, 1, 3], device="cuda"), mass=mass))
+        torch.cuda.synchronize()
+        net.check_status()
+        res.append((torch.cat([*got[:3], got[3][0], got[3][1, :1], got[3][2, :3]]), cache, mass))
+    (a, ca, ma), (b, cb, mb) = res
+    assert torch.equal(a, b) and torch.allclose(ma.sum(1), torch.tensor([7.0, 3.0, 5.0], device="cuda") * cfg.layers * cfg.heads, rtol=1e-4)
+    # roundings to bf16 at the same places, of sums in another order: a value next to the middle goes the other way, and attention with it
+    assert (ma - mb).abs().max() <= 0.02 * ma.max()
+
+
+def test_a_position_outside_a_small_cache_is_an_error():
+    from fuselink_b200.models.llama import MODEL_ZOO, LlamaShard
+    from fuselink_b200.ops import kv8
+    net = LlamaShard(MODEL_ZOO["tiny"], device="cuda", seed=2)
+    cfg = net.cfg
+    cache = kv8.Kv8Cache.empty(cfg.layers, 4, cfg.kv_heads, cfg.block_size, cfg.head_dim)
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    one = torch.tensor([1], device="cuda")
+    for pos, slots, table_, what in ((32, None, table, "position"), (5000, 3, table, "position"), (3, None, table + 9, "page")):
+        net.extend(one, torch.tensor([pos], device="cuda"), cache, table_, slots=None if slots is None else torch.tensor([slots], device="cuda"))
+        torch.cuda.synchronize()
+        with pytest.raises(IndexError, match=what):
+            net.check_status()
