@@ -43,10 +43,10 @@ __device__ __forceinline__ uint4 packed(const float (&v)[8]) {
   return make_uint4(Typed<T>::pack(v[0], v[1]), Typed<T>::pack(v[2], v[3]), Typed<T>::pack(v[4], v[5]), Typed<T>::pack(v[6], v[7]));
 }
 
-// two codes as halves, which hold every e4m3 value; the low byte becomes the low half
-__device__ __forceinline__ uint32_t halves(uint32_t codes) {
-  uint32_t h;
-  asm("{.reg .b16 c, d; mov.b32 {c, d}, %1; cvt.rn.f16x2.e4m3x2 %0, c;}" : "=r"(h) : "r"(codes));
+// four codes as halves, which hold every e4m3 value: the first two, the last two
+__device__ __forceinline__ uint2 halves(uint32_t codes) {
+  uint2 h;
+  asm("{.reg .b16 c, d; mov.b32 {c, d}, %2; cvt.rn.f16x2.e4m3x2 %0, c; cvt.rn.f16x2.e4m3x2 %1, d;}" : "=r"(h.x), "=r"(h.y) : "r"(codes));
   return h;
 }
 // the code of a in the low byte, of b in the next; |a|, |b| within 448, or NaN
@@ -175,8 +175,8 @@ __device__ __forceinline__ void write_page(uint8_t* page, float* scale, bool the
         uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t h0 = halves(w[j]), h1 = halves(w[j] >> 16);
-          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+          const uint2 h = halves(w[j]);
+          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
           w[j] = codes4(a.x * f, a.y * f, b.x * f, b.y * f);
         }
         st_v4(page + i, make_uint4(w[0], w[1], w[2], w[3]));
@@ -329,24 +329,36 @@ __global__ void __launch_bounds__(128) pack_kernel(const WriteArgs a, const FlKv
 // times weights), the query rows that share the KV head (heads of the group, and new tokens) the 8 NT columns of both, so that no product
 // is spent on padding of a group of 8.  As in decoder.cu the orders that the products do not fix are chosen for 16-byte loads: lane t of a quad takes
 // columns 16 t .. 16 t + 15 of each 64 of a key, lane group g columns DP / 8 g .. of a value.  Codes become halves exactly; queries are
-// brought into their range by a power of two per row, which loses nothing that counts beside the row's largest (2^-40 of it); weights, at
-// most 1, are rounded to 11 bits for the second product, their sum is not.  The page's scale meets the products' fp32 sums.
-// A request's context is cut into chunks, a CTA each; where there is more than one, finish_kernel joins their (max, sum, output).
+// brought into their range by a power of two per row, which loses nothing that counts beside the row's largest (2^-40 of it); weights
+// are rounded to 11 bits for the second product, their sum is not.
+//
+// What a step of 16 tokens costs beside its 16 products and 64 conversions is kept out of the loop: the maximum that the weights refer to only
+// follows when a score is 2^8 beyond it (a vote, not a reduction, per step), and the sums of the second product stay in units of the largest
+// value scale seen, which a page's weights are brought to where its own is smaller (scales are powers of two).  With a maximum per step and a
+// multiplication of every sum by the page's scale, and the codes on their way through registers, 16 x 2048 tokens of 8 KV heads of 128 took
+// 25.6 us, now 18.7 (10.3 of bytes).  Codes are on their way through a ring in shared memory, two steps ahead of their use.
+//
+// A request's context is dealt out evenly over the warps of the CTAs in the grid's third dimension: a cluster of up to 8, which joins their (max, sum,
+// output) through distributed shared memory, or more, whose parts finish_kernel joins.
 constexpr int WARPS = 4;
+constexpr int FEWEST = 2 * WARPS;          // steps that make a CTA worth having
+constexpr int LONGEST = 64 * WARPS;        // steps beyond which a context is cut even where there are CTAs enough: ragged batches end together
+constexpr int MOST_PARTS = 64;             // two for a lane of the kernel that joins them
 constexpr int PART = 2;                    // floats of a part besides its output: maximum, sum
+constexpr float LOWEST = -3e38f;           // a maximum of nothing: masked scores are -inf, which is below it
+constexpr float SLACK = 8.f;               // log2 of the largest weight; halves hold 2^15
 
 struct AttArgs {
   const void* q; long long sb, st, sh;
   const long long* start; const long long* counts;
   int batch, tokens, heads, group, row_parts;
-  int chunk;                               // units of 16 tokens per CTA
-  int per_page;                            // units of a page
-  int chunks;                              // parts that scratch holds per row
+  int per_page;                            // steps of a page
+  int splits, clustered;                   // CTAs per request, KV head and rows; whether they are a cluster
   float scale;                             // times log2 e
   void* out;
-  float* part_o; float* part_s;            // [batch][heads * tokens][chunks][dim] and [..][PART]
-  float* unit_s;                           // [batch][units][heads * tokens]: log2 of the unit's weights' sum; null: not asked for
-  int units;                               // of a full table
+  float* part_o; float* part_s;            // [batch][heads * tokens][parts][dim] and [..][PART]; parts: splits, or 1 if they are a cluster
+  float* unit_s;                           // [batch][steps of a full table][heads * tokens]: log2 of the weights' sum; null: not asked for
+  int units;                               // steps of a full table
 };
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -363,6 +375,11 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) {
   __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
 }
+__device__ __forceinline__ float exp2_fast(float x) {                     // the hardware's: 2^-22 off, relatively; 0 below 2^-126
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 // over the lane groups (the rows of a product), for every quad lane
 __device__ __forceinline__ float max_rows(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
@@ -374,13 +391,38 @@ __device__ __forceinline__ float sum_rows(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 8);
   return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
 
-template <int DP> struct Unit {               // 16 tokens on their way
-  uint4 k[2][DP / 64];
-  uint32_t v[4][DP / 32];
-  float ks, vs;
-  int live;                                   // tokens of it that the request has; 0: its page is not there
+// A warp's ring in shared memory.  Rows are 16 bytes further apart than they are long, so that the 16-byte (values of heads up to 64: 8-byte) reads of
+// a product's rows meet different banks.
+template <int DP> struct Ring {
+  static constexpr int STAGES = DP == 128 ? 3 : 6;
+  static constexpr int PITCH = DP + 16, KEYS = 16 * PITCH, SCALES = 2 * KEYS;
+  static constexpr int STAGE = SCALES + 16;                    // 16 keys, 16 values, their scales
+  static constexpr int BYTES = WARPS * STAGES * STAGE;
 };
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {        // zeros where it is not there
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds_v2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 
 __device__ __forceinline__ int tokens_of(const long long* counts, int b, int tokens) {
   return counts ? (int)min(max(counts[b], 0ll), (long long)tokens) : tokens;
@@ -390,77 +432,83 @@ __device__ __forceinline__ int seen_by_last(const AttArgs& a, const FlKv8& kv, i
   const int n = tokens_of(a.counts, b, a.tokens);
   return n == 0 ? 0 : (int)min(max(a.start[b] + n, 0ll), (long long)kv.table_stride * kv.block_size);
 }
+// CTAs that a context of so many steps is dealt out to
+__device__ __forceinline__ int parts_of(const AttArgs& a, int units) { return min(max((units + FEWEST - 1) / FEWEST, 1), a.splits); }
 
-template <typename T, int DP, int NT, bool MASS>
-__global__ void __launch_bounds__(WARPS * 32) attention_kernel(const AttArgs a, const FlKv8 kv) {
+// parts' outputs are means (divided by their sums), so that joining them overflows nowhere
+__device__ __forceinline__ float share(float m, float l, float mm) { return l == 0.f ? 0.f : exp2f(m - mm) * l; }      // 0: a part without weight; not one whose sum is NaN
+
+template <typename T, int DP, int NT, bool FULL, bool MASS>   // DP: head dimension rounded up to 64 or 128; FULL: it is that
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(const AttArgs a, const FlKv8 kv) {
+  using R = Ring<DP>;
   constexpr int KJ = DP / 64, MT = DP / 16, VB = DP / 8, ROWS = 8 * NT, LD = DP + 4;
-  __shared__ __align__(16) float s_o[WARPS][ROWS][LD];
-  __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
+  static_assert(WARPS * ROWS * LD * 4 <= R::BYTES, "the warps' parts take the rings' place");
+  extern __shared__ __align__(16) uint8_t s_ring[];
+  auto s_o = reinterpret_cast<float(*)[ROWS][LD]>(s_ring);
+  __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_cm[ROWS], s_cl[ROWS];
   grid_dep_launch();
   grid_dep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int kh = blockIdx.x / a.row_parts, rp = blockIdx.x - kh * a.row_parts, b = blockIdx.y, z = blockIdx.z;
-  const int D = kv.dim, bs = kv.block_size, all_rows = a.group * a.tokens, r0 = rp * ROWS;
+  const int D = FULL ? DP : kv.dim, bs = kv.block_size, all_rows = a.group * a.tokens, r0 = rp * ROWS;
   const int n_rows = min(ROWS, all_rows - r0), n_new = tokens_of(a.counts, b, a.tokens);
   const int len = seen_by_last(a, kv, b);
-  const int pages = (len + bs - 1) / bs, units = pages * a.per_page;
-  const int lo = z * a.chunk, hi = min(lo + a.chunk, units);
-  if (z > 0 && lo >= units) return;
+  const int units = (len + bs - 1) / bs * a.per_page, parts = parts_of(a, units);
+  if (!a.clustered && z >= parts) return;
   // the warp's units
-  const int mine = hi - lo, per = mine / WARPS, extra = mine % WARPS;
-  const int first = lo + warp * per + min(warp, extra), last = first + per + (warp < extra ? 1 : 0);
+  const int nw = parts * WARPS, w0 = z * WARPS + warp, per = units / nw, extra = units % nw;
+  const int first = z < parts ? w0 * per + min(w0, extra) : 0, last = z < parts ? first + per + (w0 < extra ? 1 : 0) : 0;
 
-  const uint8_t* kp = reinterpret_cast<const uint8_t*>(kv.k);
-  const uint8_t* vp = reinterpret_cast<const uint8_t*>(kv.v);
+  // this lane's 16 bytes of a row, in every PASS-th row
+  constexpr int PIECES = DP / 16, PASS = 32 / PIECES;
+  const int row0 = lane / PIECES, piece = lane % PIECES;
+  const uint8_t* kp = reinterpret_cast<const uint8_t*>(kv.k) + row0 * D + 16 * piece;
+  const uint8_t* vp = reinterpret_cast<const uint8_t*>(kv.v) + row0 * D + 16 * piece;
+  const uint32_t ring = smem_u32(s_ring) + warp * R::STAGES * R::STAGE, mine = ring + row0 * R::PITCH + 16 * piece;
+  const long long pool0 = (long long)kv.layer * kv.num_blocks;
   int ids = -1, ids_at = 0;                    // lane i: the page of unit ids_at + i
   auto look_up = [&](int u0) {
     ids_at = u0;
     ids = u0 + lane < last ? page_id(kv, b, (u0 + lane) / a.per_page) : -1;
   };
-  auto load = [&](int u, Unit<DP>& x) {
-    if (u >= ids_at + 32) look_up(u);
-    const int id = __shfl_sync(0xffffffffu, ids, u - ids_at);
-    const int page = u / a.per_page, s0 = (u - page * a.per_page) * 16;
-    const int live = id < 0 ? 0 : min(min(bs - s0, len - page * bs - s0), 16);
-    if (id < 0 && lane == 0) note(kv.status, FL_DEC_BAD_PAGE);
-    x.live = live;
-    const long long cell = ((long long)kv.layer * kv.num_blocks + max(id, 0)) * kv.heads + kh;
-    const uint8_t* k = kp + (cell * bs + s0) * D;
-    const uint8_t* v = vp + (cell * bs + s0) * D;
-    x.ks = live > 0 ? __ldg(kv.k_scale + cell) : 0.f;
-    x.vs = live > 0 ? __ldg(kv.v_scale + cell) : 0.f;
+  // where a unit begins, and tokens of it that the request has
+  auto place = [&](int u, int& base, int& live) {
+    int page = u, s0 = 0;
+    if (a.per_page > 1) { page = u / a.per_page; s0 = (u - page * a.per_page) * 16; }
+    base = page * bs + s0;
+    live = min(min(bs - s0, len - base), 16);
+    return s0;
+  };
+  auto fetch = [&](int u, int stage) {         // every lane calls it; an empty group behind the last
+    if (u < last) {
+      if (u >= ids_at + 32) look_up(u);
+      const int id = __shfl_sync(0xffffffffu, ids, u - ids_at);
+      int base, live;
+      const int s0 = place(u, base, live);
+      if (id < 0 && lane == 0) note(kv.status, FL_DEC_BAD_PAGE);
+      if (id < 0) live = 0;
+      const long long cell = (pool0 + max(id, 0)) * kv.heads + kh, at = (cell * bs + s0) * D;
+      const uint32_t to = mine + stage * R::STAGE;
+      const bool column = FULL || 16 * piece < D;
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) {
-        const int d = 64 * j + 16 * t;
-        x.k[p][j] = make_uint4(0, 0, 0, 0);
-        if (8 * p + g < live && d < D) x.k[p][j] = ld_stream_v4(k + (8 * p + g) * D + d);
+      for (int i = 0; i < 16; i += PASS) {
+        const bool there = column && i + row0 < live;           // the addresses of others may be anything
+        copy16(to + i * R::PITCH, there ? kp + at + i * D : reinterpret_cast<const uint8_t*>(kv.k), there);
+        copy16(to + R::KEYS + i * R::PITCH, there ? vp + at + i * D : reinterpret_cast<const uint8_t*>(kv.v), there);
       }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int tok = 2 * t + (i & 1) + 8 * (i >> 1);
-#pragma unroll
-      for (int w = 0; w < DP / 32; ++w) x.v[i][w] = 0;
-      if (tok < live && VB * g < D) {
-        if constexpr (DP == 128) {
-          const uint4 w4 = ld_stream_v4(v + tok * D + VB * g);
-          x.v[i][0] = w4.x; x.v[i][1] = w4.y; x.v[i][2] = w4.z; x.v[i][3] = w4.w;
-        } else {
-          asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(x.v[i][0]), "=r"(x.v[i][1]) : "l"(v + tok * D + VB * g));
-        }
-      }
+      if (lane < 2) copy4(ring + stage * R::STAGE + R::SCALES + 4 * lane, (lane ? kv.v_scale : kv.k_scale) + cell, id >= 0);
     }
+    copies_commit();
   };
 
   look_up(first);
-  Unit<DP> now;
-  if (first < last) load(first, now);
+#pragma unroll
+  for (int s = 0; s < R::STAGES - 1; ++s) fetch(first + s, s);
 
   // queries, as the second operand; a row's power of two is undone on its scores
   uint32_t qb[NT][KJ][8];
   float factor[NT][2];                         // of columns 2 t and 2 t + 1
-  int sees[NT][2];                             // slots that the column's token sees
+  int sees[NT][2], fewest = len;               // slots that the column's token sees; the fewest of any that sees some
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = r0 + 8 * nt + g, tok = r / a.group, h = r - tok * a.group;
@@ -470,7 +518,7 @@ __global__ void __launch_bounds__(WARPS * 32) attention_kernel(const AttArgs a, 
     float m = 0.f;
 #pragma unroll
     for (int j = 0; j < KJ; ++j) {
-      const int d = 64 * j + 16 * t;
+      const int d = DP == 128 ? 32 * t + 16 * j : 16 * t;
       uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
       if (in && d < D) {
         u0 = ld_v4(q + d);
@@ -490,7 +538,7 @@ __global__ void __launch_bounds__(WARPS * 32) attention_kernel(const AttArgs a, 
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     // largest magnitude to 2^14 .. 2^15; a row of magnitudes below 2^-100 stays below
-    const int e = max((int)(__float_as_uint(m) >> 23), 27);           // 127 + exponent
+    const int e = max((int)(__float_as_uint(m) >> 23), 27);                     // 127 + exponent
     const float to = __uint_as_float((uint32_t)(268 - e) << 23), back = __uint_as_float((uint32_t)(e - 14) << 23);       // 2^(14 - exponent) and its inverse
 #pragma unroll
     for (int j = 0; j < KJ; ++j)
@@ -500,11 +548,13 @@ __global__ void __launch_bounds__(WARPS * 32) attention_kernel(const AttArgs a, 
     for (int c = 0; c < 2; ++c) {
       factor[nt][c] = __shfl_sync(0xffffffffu, back, (2 * t + c) * 4) * a.scale;
       const int rc = r0 + 8 * nt + 2 * t + c, tc = rc / a.group;
-      sees[nt][c] = rc < all_rows && tc < n_new ? max(min(len, (int)min(a.start[b] + tc + 1, (long long)len)), 0) : 0;
+      sees[nt][c] = rc < all_rows && tc < n_new ? max((int)min(a.start[b] + tc + 1, (long long)len), 0) : 0;
+      if (sees[nt][c] > 0) fewest = min(fewest, sees[nt][c]);
     }
   }
+  fewest = __reduce_min_sync(0xffffffffu, fewest);
 
-  float o[NT][MT][4], m[NT][2], l[NT][2];
+  float o[NT][MT][4], m[NT][2], l[NT][2], unit = -200.f;       // unit: log2 of what the sums o are in
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -512,144 +562,287 @@ __global__ void __launch_bounds__(WARPS * 32) attention_kernel(const AttArgs a, 
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) { m[nt][c] = -INFINITY; l[nt][c] = 0.f; }
+    for (int c = 0; c < 2; ++c) { m[nt][c] = LOWEST; l[nt][c] = 0.f; }
   }
 
+  int stage = 0;
 #pragma unroll 1
   for (int u = first; u < last; ++u) {
-    Unit<DP> x = now;
-    if (u + 1 < last) load(u + 1, now);
-    const int page = u / a.per_page, base = page * bs + (u - page * a.per_page) * 16;
-    float s[NT][4];
+    copies_wait<R::STAGES - 2>();
+    __syncwarp();                                // every lane's copies of this unit are there, and the last unit has been read
+    const uint32_t at = ring + stage * R::STAGE;
+    fetch(u + R::STAGES - 1, stage == 0 ? R::STAGES - 1 : stage - 1);
+    stage = stage + 1 == R::STAGES ? 0 : stage + 1;
+    int base, live;
+    place(u, base, live);
+    const uint2 scales = lds_v2(at + R::SCALES);
+    const float ks = __uint_as_float(scales.x), vs = __uint_as_float(scales.y);
+    if (ks == 0.f) live = 0;                     // a page that is not there
+    float s[NT][4], s2[NT][4];                   // two chains of products
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+      for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.f;
 #pragma unroll
     for (int j = 0; j < KJ; ++j) {
-      const uint32_t w0[4] = {x.k[0][j].x, x.k[0][j].y, x.k[0][j].z, x.k[0][j].w};
-      const uint32_t w1[4] = {x.k[1][j].x, x.k[1][j].y, x.k[1][j].z, x.k[1][j].w};
+      const uint32_t from = at + g * R::PITCH + (DP == 128 ? 32 * t + 16 * j : 16 * t);
+      const uint4 u0 = lds_v4(from), u1 = lds_v4(from + 8 * R::PITCH);
+      const uint32_t k0[4] = {u0.x, u0.y, u0.z, u0.w}, k1[4] = {u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t a0 = halves(w0[i]), a2 = halves(w0[i] >> 16), a1 = halves(w1[i]), a3 = halves(w1[i] >> 16);
+        const uint2 h0 = halves(k0[i]), h1 = halves(k1[i]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma(s[nt], a0, a1, a2, a3, qb[nt][j][2 * i], qb[nt][j][2 * i + 1]);
+        for (int nt = 0; nt < NT; ++nt) mma(i & 1 ? s2[nt] : s[nt], h0.x, h1.x, h0.y, h1.y, qb[nt][j][2 * i], qb[nt][j][2 * i + 1]);
       }
     }
-    uint32_t p0[NT], p1[NT];
-    bool split = false;                        // some column sees part of the live tokens, another more
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float f[2], mn[2], add[2];
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[nt][i] += s2[nt][i];
+    uint32_t v[4][DP / 32];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t from = at + R::KEYS + (2 * t + (i & 1) + 8 * (i >> 1)) * R::PITCH + VB * g;
+      if constexpr (DP == 128) {
+        const uint4 w = lds_v4(from);
+        v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w;
+      } else {
+        const uint2 w = lds_v2(from);
+        v[i][0] = w.x; v[i][1] = w.y;
+      }
+    }
+    const bool cut = live < 16 || base + 16 > fewest;          // some column does not see some of the 16
+    if (cut) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int ends = min(sees[nt][c] - base, live);
+          s[nt][c] = g < ends ? s[nt][c] : -INFINITY;
+          s[nt][2 + c] = g + 8 < ends ? s[nt][2 + c] : -INFINITY;
+        }
+    }
+    const float page_unit = (float)((int)(__float_as_uint(vs) >> 23) - 127);
+    bool beyond = page_unit > unit && live > 0;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float k = factor[nt][c] * x.ks;
-        const int ends = min(sees[nt][c] - base, x.live);
-        split |= sees[nt][c] > 0 && ends < x.live;
-        s[nt][c] = g < ends ? s[nt][c] * k : -INFINITY;
-        s[nt][2 + c] = g + 8 < ends ? s[nt][2 + c] * k : -INFINITY;
-        // 0 stands in for a maximum of -inf: a step of nothing else adds nothing.  A score that is NaN or +inf makes the sums NaN.
-        const float before = m[nt][c];
-        m[nt][c] = fmaxf(before, max_rows(fmaxf(s[nt][c], s[nt][2 + c])));
-        mn[c] = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
-        f[c] = exp2f(before - mn[c]);
-        s[nt][c] = exp2f(s[nt][c] - mn[c]);
-        s[nt][2 + c] = exp2f(s[nt][2 + c] - mn[c]);
-        add[c] = s[nt][c] + s[nt][2 + c];
-        l[nt][c] = l[nt][c] * f[c] + add[c];
+        // -inf stays -inf whatever it meets: a factor of 0 (an underflow, or no page) would make it NaN
+        const float k = fmaxf(factor[nt][c] * ks, 0x1p-126f), top = m[nt][c] + SLACK;
+        s[nt][c] *= k;
+        s[nt][2 + c] *= k;
+        beyond |= s[nt][c] > top || s[nt][2 + c] > top;
       }
-      if (MASS) {
-        const float s0 = sum_rows(add[0]), s1 = sum_rows(add[1]);
-        if (g == 0) {
-          float* w = a.unit_s + ((long long)b * a.units + u) * a.heads * a.tokens + kh * all_rows + r0 + 8 * nt + 2 * t;
-          if (8 * nt + 2 * t < n_rows) w[0] = mn[0] + log2f(s0);
-          if (8 * nt + 2 * t + 1 < n_rows) w[1] = mn[1] + log2f(s1);
+    if (__any_sync(0xffffffffu, beyond)) {
+      const float unit_now = live > 0 ? fmaxf(unit, page_unit) : unit, shrink = exp2_fast(unit - unit_now);
+      unit = unit_now;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float before = m[nt][c];
+          m[nt][c] = fmaxf(before, max_rows(fmaxf(s[nt][c], s[nt][2 + c])));
+          const float e = exp2_fast(before - m[nt][c]);
+          l[nt][c] *= e;
+          f[c] = e * shrink;
         }
-      }
-      if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           o[nt][i][0] *= f[0]; o[nt][i][1] *= f[1];
           o[nt][i][2] *= f[0]; o[nt][i][3] *= f[1];
         }
       }
+    }
+    uint32_t p0[NT], p1[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float add[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        s[nt][c] = exp2_fast(s[nt][c] - m[nt][c]);
+        s[nt][2 + c] = exp2_fast(s[nt][2 + c] - m[nt][c]);
+        add[c] = s[nt][c] + s[nt][2 + c];
+        l[nt][c] += add[c];
+      }
+      if (MASS) {
+        const float s0 = sum_rows(add[0]), s1 = sum_rows(add[1]);
+        if (g == 0) {
+          float* w = a.unit_s + ((long long)b * a.units + u) * a.heads * a.tokens + kh * all_rows + r0 + 8 * nt + 2 * t;
+          if (8 * nt + 2 * t < n_rows) w[0] = m[nt][0] + log2f(s0);
+          if (8 * nt + 2 * t + 1 < n_rows) w[1] = m[nt][1] + log2f(s1);
+        }
+      }
+    }
+    if (page_unit < unit) {                                      // a page of smaller values than the largest
+      const float w = exp2_fast(page_unit - unit);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[nt][i] *= w;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
       p0[nt] = transposed(half2_of(s[nt][0], s[nt][1]));
       p1[nt] = transposed(half2_of(s[nt][2], s[nt][3]));
     }
-    auto values = [&](auto takes) {
+    auto values = [&](auto each) {
 #pragma unroll
       for (int w = 0; w < DP / 32; ++w)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t sel = h ? 0x7362u : 0x5140u;
-          const uint32_t u0 = __byte_perm(x.v[0][w], x.v[1][w], sel), u1 = __byte_perm(x.v[2][w], x.v[3][w], sel);
-          const uint32_t a0 = halves(u0), a1 = halves(u0 >> 16), a2 = halves(u1), a3 = halves(u1 >> 16);
+          const uint32_t u0 = __byte_perm(v[0][w], v[1][w], sel), u1 = __byte_perm(v[2][w], v[3][w], sel);
+          const uint2 h0 = halves(u0), h1 = halves(u1);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            mma(c, a0, a1, a2, a3, p0[nt], p1[nt]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (takes(nt, i & 1)) o[nt][2 * w + h][i] += c[i] * x.vs;
-          }
+          for (int nt = 0; nt < NT; ++nt) each(nt, 2 * w + h, h0.x, h0.y, h1.x, h1.y);
         }
     };
-    if (a.tokens == 1 || !__any_sync(0xffffffffu, split)) {
-      values([](int, int) { return true; });
+    if (a.tokens == 1 || base + 16 <= fewest) {
+      values([&](int nt, int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) { mma(o[nt][i], a0, a1, a2, a3, p0[nt], p1[nt]); });
     } else {
       // Among the last tokens a column's weight of 0 must not meet a value of a later token, which may be NaN: one new token at a time, with
-      // the values behind it left out, and only its own columns take the sums.
-      const Unit<DP> whole = x;
+      // the values behind it left out (the last one first, so that each leaves out more), and only its own columns take the sums.
       const int t0 = r0 / a.group, t1 = min((r0 + n_rows - 1) / a.group, n_new - 1);
-      for (int tok = t0; tok <= t1; ++tok) {
+      for (int tok = t1; tok >= t0; --tok) {
         const int ends = (int)min(a.start[b] + tok + 1, (long long)len) - base;
-        if (ends <= 0) continue;
+        if (ends <= 0) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int w = 0; w < DP / 32; ++w) x.v[i][w] = 2 * t + (i & 1) + 8 * (i >> 1) < ends ? whole.v[i][w] : 0;
-        values([&](int nt, int c) { return (r0 + 8 * nt + 2 * t + c) / a.group == tok; });
+          for (int w = 0; w < DP / 32; ++w)
+            if (2 * t + (i & 1) + 8 * (i >> 1) >= ends) v[i][w] = 0;
+        values([&](int nt, int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+          mma(c, a0, a1, a2, a3, p0[nt], p1[nt]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if ((r0 + 8 * nt + 2 * t + (j & 1)) / a.group == tok) o[nt][i][j] += c[j];
+        });
       }
     }
   }
+  copies_wait<0>();
+  __syncthreads();                               // the rings' memory is free
 
   // the warps' parts become one
+  const float scale_o = exp2f(unit);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int row = 8 * nt + 2 * t + c;
-      const float sum = sum_rows(l[nt][c]);
+      const float sum = sum_rows(l[nt][c]), f = sum == 0.f ? 0.f : 1.f / sum;
       if (g == 0) { s_m[warp][row] = m[nt][c]; s_l[warp][row] = sum; }
+      auto mean = [&](float v) { return v * f * scale_o; };
 #pragma unroll
       for (int i = 0; i < MT; i += 2)
-        *reinterpret_cast<float4*>(&s_o[warp][row][VB * g + 2 * i]) = make_float4(o[nt][i][c], o[nt][i][2 + c], o[nt][i + 1][c], o[nt][i + 1][2 + c]);
+        *reinterpret_cast<float4*>(&s_o[warp][row][VB * g + 2 * i]) = make_float4(mean(o[nt][i][c]), mean(o[nt][i][2 + c]), mean(o[nt][i + 1][c]), mean(o[nt][i + 1][2 + c]));
     }
   __syncthreads();
-  const bool whole = units <= a.chunk;                       // of this request's context
-  for (int i = threadIdx.x; i < n_rows * D; i += WARPS * 32) {
-    const int row = i / D, d = i - row * D;
-    float mm = -INFINITY, acc = 0.f, ll = 0.f;
+  // what the warps' means count for in the CTA's
+  if (threadIdx.x < ROWS) {
+    const int row = threadIdx.x;
+    float mm = LOWEST, ll = 0.f, w[WARPS];
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, s_m[w][row]);
+    for (int i = 0; i < WARPS; ++i) mm = fmaxf(mm, s_m[i][row]);
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float e = s_l[w][row] == 0.f ? 0.f : exp2f(s_m[w][row] - mm);       // a part without weight; not one whose sum is NaN
-      acc += e * s_o[w][row][d];
-      ll += e * s_l[w][row];
-    }
-    const int r = r0 + row, tok = r / a.group, h = kh * a.group + r - tok * a.group;
+    for (int i = 0; i < WARPS; ++i) { w[i] = share(s_m[i][row], s_l[i][row], mm); ll += w[i]; }
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) s_l[i][row] = ll == 0.f ? 0.f : w[i] / ll;
+    s_cm[row] = mm;
+    s_cl[row] = ll;
+  }
+  __syncthreads();
+  const long long row_at = (long long)b * a.heads * a.tokens + kh * all_rows + r0;
+  auto result = [&](int row, int d, float mm, float ll, float acc) {
+    const int r = r0 + row, tok = a.tokens == 1 ? 0 : r / a.group, h = kh * a.group + r - tok * a.group;
     const bool none = tok >= n_new || a.start[b] + tok < 0 || len == 0;
-    if (whole) reinterpret_cast<T*>(a.out)[(((long long)b * a.tokens + tok) * a.heads + h) * D + d] = T(none ? 0.f : acc / ll);
-    if (!whole || MASS) {
-      const long long part = ((long long)b * a.heads * a.tokens + kh * all_rows + r) * a.chunks + z;
-      if (!whole) a.part_o[part * D + d] = acc;
-      if (d == 0) { a.part_s[part * PART] = mm; a.part_s[part * PART + 1] = ll; }
+    reinterpret_cast<T*>(a.out)[(((long long)b * a.tokens + tok) * a.heads + h) * D + d] = T(none ? 0.f : ll == 0.f ? NAN : acc);
+    if (MASS && d == 0) {
+      float* p = a.part_s + (row_at + row) * (a.clustered ? 1 : a.splits) * PART;
+      p[0] = mm;
+      p[1] = ll;
+    }
+  };
+  constexpr int AT_ONCE = WARPS * 32 / DP;                     // rows
+  const int d = threadIdx.x % DP, row1 = threadIdx.x / DP;
+  if (!a.clustered || a.splits == 1) {
+    if (FULL || d < D) {
+      for (int row = row1; row < n_rows; row += AT_ONCE) {
+        float acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) acc += s_l[w][row] * s_o[w][row][d];
+        if (parts == 1) {
+          result(row, d, s_cm[row], s_cl[row], acc);
+        } else {
+          const long long part = (row_at + row) * a.splits + z;
+          a.part_o[part * D + d] = acc;
+          if (d == 0) { a.part_s[part * PART] = s_cm[row]; a.part_s[part * PART + 1] = s_cl[row]; }
+        }
+      }
+    }
+    return;
+  }
+  if (FULL || d < D) {
+    for (int row = row1; row < n_rows; row += AT_ONCE) {
+      float acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) acc += s_l[w][row] * s_o[w][row][d];
+      s_o[0][row][d] = acc;                                    // read and written by this thread alone
     }
   }
+  cluster_sync_all();
+  if (FULL || d < D) {
+    for (int row = z * AT_ONCE + row1; row < n_rows; row += a.splits * AT_ONCE) {
+      const uint32_t am = smem_u32(&s_cm[row]), al = smem_u32(&s_cl[row]), ao = smem_u32(&s_o[0][row][d]);
+      float pm[8], pl[8], po[8], mm = LOWEST, ll = 0.f, acc = 0.f;
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (x < a.splits) {
+          pm[x] = ld_cluster_f32(map_to_cta(am, x));
+          pl[x] = ld_cluster_f32(map_to_cta(al, x));
+          po[x] = ld_cluster_f32(map_to_cta(ao, x));
+        }
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (x < a.splits) mm = fmaxf(mm, pm[x]);
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (x < a.splits) { pl[x] = share(pm[x], pl[x], mm); ll += pl[x]; }
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (x < a.splits) acc += ll == 0.f ? 0.f : pl[x] / ll * po[x];
+      result(row, d, mm, ll, acc);
+    }
+  }
+  cluster_sync_all();                            // nobody leaves while its part is being read
 }
 
-// Joins the chunks' parts: a CTA per row and request.  The first row_ctas CTAs of a request have its rows; the others, if weights are asked
+struct Joined { float m, sum, w0, w1; };       // of a row's parts: their maximum and sum; what parts `lane` and `lane` + 32 count for in it
+__device__ __forceinline__ Joined joined(const AttArgs& a, long long at, int parts, int lane) {
+  Joined j;
+  float m[2] = {LOWEST, LOWEST}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + 32 * i < parts) {
+      const float2 p = *reinterpret_cast<const float2*>(a.part_s + (at + lane + 32 * i) * PART);
+      m[i] = p.x;
+      l[i] = p.y;
+    }
+  j.m = fmaxf(m[0], m[1]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) j.m = fmaxf(j.m, __shfl_xor_sync(0xffffffffu, j.m, o));
+  j.w0 = share(m[0], l[0], j.m);
+  j.w1 = share(m[1], l[1], j.m);
+  j.sum = j.w0 + j.w1;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) j.sum += __shfl_xor_sync(0xffffffffu, j.sum, o);
+  return j;
+}
+
+// Joins parts that are no cluster's: a CTA per row and request.  The first row_ctas CTAs of a request have its rows; the others, if weights are asked
 // for, its pages, a warp each, whose lanes add up the rows' shares in an order that is always the same.
 template <typename T>
 __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv8 kv, float* mass, int row_ctas, int page_ctas) {
@@ -657,43 +850,47 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
   grid_dep_wait();
   const int b = blockIdx.y, D = kv.dim, bs = kv.block_size, rows = a.heads * a.tokens, all_rows = a.group * a.tokens;
   const int len = seen_by_last(a, kv, b), units = (len + bs - 1) / bs * a.per_page;
-  const int parts = (units + a.chunk - 1) / a.chunk;
+  const int parts = a.clustered ? 1 : parts_of(a, units), room = a.clustered ? 1 : a.splits, lane = threadIdx.x & 31;
   if ((int)blockIdx.x < row_ctas) {
     if (parts < 2) return;
     const int row = blockIdx.x, kh = row / all_rows, r = row - kh * all_rows, tok = r / a.group, h = kh * a.group + r - tok * a.group;
-    const long long at = ((long long)b * rows + row) * a.chunks;
-    float mm = -INFINITY;
-    for (int z = 0; z < parts; ++z) mm = fmaxf(mm, a.part_s[(at + z) * PART]);
-    for (int d = threadIdx.x; d < D; d += 128) {
-      float acc = 0.f, ll = 0.f;
-#pragma unroll 4
-      for (int z = 0; z < parts; ++z) {
-        const float pm = a.part_s[(at + z) * PART], pl = a.part_s[(at + z) * PART + 1], po = a.part_o[(at + z) * D + d];
-        const float e = pl == 0.f ? 0.f : exp2f(pm - mm);
-        acc += e * po;
-        ll += e * pl;
-      }
-      const bool none = tok >= tokens_of(a.counts, b, a.tokens) || a.start[b] + tok < 0;
-      reinterpret_cast<T*>(a.out)[(((long long)b * a.tokens + tok) * a.heads + h) * D + d] = T(none ? 0.f : acc / ll);
+    const long long at = ((long long)b * rows + row) * room;
+    const Joined j = joined(a, at, parts, lane);
+    const float f = j.sum == 0.f ? 0.f : 1.f / j.sum;
+    const bool none = tok >= tokens_of(a.counts, b, a.tokens) || a.start[b] + tok < 0;
+    const int d = threadIdx.x;
+    const float* part = a.part_o + at * D + min(d, D - 1);
+    float acc = 0.f;
+    for (int z0 = 0; z0 < parts; z0 += 16) {                   // sixteen on their way at a time
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = z0 + i < parts ? part[(z0 + i) * D] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc += __shfl_sync(0xffffffffu, z0 < 32 ? j.w0 : j.w1, (z0 + i) & 31) * f * v[i];
     }
+    if (d < D) reinterpret_cast<T*>(a.out)[(((long long)b * a.tokens + tok) * a.heads + h) * D + d] = T(none ? 0.f : j.sum == 0.f ? NAN : acc);
     return;
   }
   if (mass == nullptr || len == 0) return;
   extern __shared__ float s_lse[];                           // log2 of every row's sum of weights; inf: a row that sees nothing
-  for (int r = threadIdx.x; r < rows; r += 128) {
-    const long long at = ((long long)b * rows + r) * a.chunks;
+  const int n_new = tokens_of(a.counts, b, a.tokens);
+  auto keep = [&](int r, float m, float sum) {
     const int tok = (r % all_rows) / a.group;
-    float mm = -INFINITY, ll = 0.f;
-    for (int z = 0; z < parts; ++z) mm = fmaxf(mm, a.part_s[(at + z) * PART]);
-    for (int z = 0; z < parts; ++z) {
-      const float pm = a.part_s[(at + z) * PART], pl = a.part_s[(at + z) * PART + 1];
-      ll += pl == 0.f ? 0.f : exp2f(pm - mm) * pl;
+    s_lse[r] = tok >= n_new || a.start[b] + tok < 0 ? INFINITY : sum == 0.f ? NAN : m + log2f(sum);
+  };
+  if (room == 1) {
+    for (int r = threadIdx.x; r < rows; r += 128) {
+      const float* p = a.part_s + ((long long)b * rows + r) * PART;
+      keep(r, p[0], p[1]);
     }
-    const bool none = tok >= tokens_of(a.counts, b, a.tokens) || a.start[b] + tok < 0;
-    s_lse[r] = none ? INFINITY : mm + log2f(ll);
+  } else {
+    for (int r = threadIdx.x >> 5; r < rows; r += 4) {
+      const Joined j = joined(a, ((long long)b * rows + r) * room, parts, lane);
+      if (lane == 0) keep(r, j.m, j.sum);
+    }
   }
   __syncthreads();
-  const int pages = units / a.per_page, lane = threadIdx.x & 31;
+  const int pages = units / a.per_page;
   for (int p = (blockIdx.x - row_ctas) * 4 + (threadIdx.x >> 5); p < pages; p += page_ctas * 4) {
     float sum = 0.f;
     for (int i = 0; i < a.per_page; ++i) {
@@ -876,11 +1073,9 @@ extern "C" int fl_kv8_pack(int dtype, const void* k_pool, const void* v_pool, in
   return (int)cudaGetLastError();
 }
 
-// How a call is cut up: `chunk` units of 16 tokens per CTA, so that a full table gives every SM `resident` CTAs but a warp no fewer than two
-// units; a table may be much longer than its contexts, so a chunk is never more than MOST units.
+// How a call is cut up: enough CTAs for the SMs (four of NT = 1, two of NT = 2 each), as a cluster where 8 per request and KV head are enough.
 namespace {
-constexpr int FEWEST = 2 * fl::kv8::WARPS, MOST = 64 * fl::kv8::WARPS;
-struct Cut { int nt, row_parts, per_page, units, chunk, chunks; };
+struct Cut { int nt, row_parts, per_page, units, splits; bool clustered; };
 Cut cut_of(int batch, int tokens, int heads, const FlKv8* kv) {
   Cut c;
   const long long rows = (long long)heads / kv->heads * tokens;
@@ -888,42 +1083,63 @@ Cut cut_of(int batch, int tokens, int heads, const FlKv8* kv) {
   c.row_parts = (int)((rows + 8 * c.nt - 1) / (8 * c.nt));
   c.per_page = (kv->block_size + 15) / 16;
   c.units = kv->table_stride * c.per_page;
-  const long long ctas = (long long)batch * kv->heads * c.row_parts, want = 148ll * (c.nt == 1 ? 3 : 2);
-  long long parts = want / (ctas < 1 ? 1 : ctas);
-  if (parts < 1) parts = 1;
-  long long chunk = (c.units + parts - 1) / parts;
-  if (chunk > MOST) chunk = MOST;
-  if (chunk < FEWEST) chunk = FEWEST;
-  while ((c.units + chunk - 1) / chunk > 65535) chunk *= 2;
-  c.chunk = (int)chunk;
-  c.chunks = (int)((c.units + chunk - 1) / chunk);
-  if (c.chunks < 1) c.chunks = 1;
+  const long long ctas = (long long)batch * kv->heads * c.row_parts, want = 148ll * (c.nt == 1 ? 4 : 2);
+  const long long most = (c.units + fl::kv8::FEWEST - 1) / fl::kv8::FEWEST;
+  long long splits = want / (ctas < 1 ? 1 : ctas);
+  const long long even = (c.units + fl::kv8::LONGEST - 1) / fl::kv8::LONGEST;
+  if (splits < even) splits = even;
+  if (splits > most) splits = most;
+  if (splits > fl::kv8::MOST_PARTS) splits = fl::kv8::MOST_PARTS;
+  if (splits < 1) splits = 1;
+  c.splits = (int)splits;
+  c.clustered = splits <= 8;
   return c;
 }
 long long up16(long long bytes) { return (bytes + 15) / 16 * 16; }
 
-template <typename T, int DP, int NT>
-int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, bool mass, dim3 grid, bool early, cudaStream_t stream) {
+template <typename T, int DP, int NT, bool FULL, bool MASS>
+int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, dim3 grid, bool early, cudaStream_t stream) {
+  constexpr int smem = fl::kv8::Ring<DP>::BYTES;
+  static bool set_on[64];                          // per device: a process may drive several GPUs
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (dev < 0 || dev >= 64) return -3;
+  if (!set_on[dev]) {
+    e = cudaFuncSetAttribute(fl::kv8::attention_kernel<T, DP, NT, FULL, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    set_on[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = smem;
   cfg.gridDim = grid;
   cfg.blockDim = dim3(fl::kv8::WARPS * 32, 1, 1);
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 1; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = a.clustered ? a.splits : 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = early ? 1 : 0;
-  return (int)cudaLaunchKernelEx(&cfg, mass ? fl::kv8::attention_kernel<T, DP, NT, true> : fl::kv8::attention_kernel<T, DP, NT, false>, a, kv);
+  cfg.numAttrs = early ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, fl::kv8::attention_kernel<T, DP, NT, FULL, MASS>, a, kv);
+}
+template <typename T, int DP>
+int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, int nt, bool mass, dim3 grid, bool early, cudaStream_t stream) {
+#define FL_ATT(N, F) return mass ? launch_attention<T, DP, N, F, true>(a, kv, grid, early, stream) : launch_attention<T, DP, N, F, false>(a, kv, grid, early, stream)
+  if (kv.dim == DP) { if (nt == 1) FL_ATT(1, true); else FL_ATT(2, true); }
+  if (nt == 1) FL_ATT(1, false); else FL_ATT(2, false);
+#undef FL_ATT
 }
 }  // namespace
 
 extern "C" long long fl_kv8_attention_scratch(int batch, int tokens, int heads, const FlKv8* kv, int mass) {
   if (!sizes_fit(kv) || batch < 1 || tokens < 1 || heads < 1 || heads % kv->heads) return 0;
   const Cut c = cut_of(batch, tokens, heads, kv);
-  const long long rows = (long long)batch * heads * tokens;
+  const long long rows = (long long)batch * heads * tokens, parts = c.clustered ? 1 : c.splits;
   long long bytes = 0;
-  if (c.chunks > 1) bytes += up16(rows * c.chunks * kv->dim * 4);
-  if (c.chunks > 1 || mass) bytes += up16(rows * c.chunks * fl::kv8::PART * 4);
+  if (!c.clustered) bytes += up16(rows * parts * kv->dim * 4);
+  if (!c.clustered || mass) bytes += up16(rows * parts * fl::kv8::PART * 4);
   if (mass) bytes += up16(rows * c.units * 4);
   return bytes;
 }
@@ -938,31 +1154,25 @@ extern "C" int fl_kv8_attention(int dtype, const void* q, long long stride_b, lo
   if (!aligned({q, out, scratch, kv->k, kv->v})) return -4;
   if (batch == 0 || tokens == 0) return 0;
   const Cut c = cut_of(batch, tokens, heads, kv);
-  const long long rows = (long long)batch * heads * tokens;
-  if ((long long)kv->heads * c.row_parts > 0x7fffffffll || (c.chunks > 1 && (long long)heads * tokens > 0x7fffffffll)) return -2;
+  const long long rows = (long long)batch * heads * tokens, parts = c.clustered ? 1 : c.splits;
   fl::kv8::AttArgs a = {};
   a.q = q; a.sb = stride_b; a.st = stride_t; a.sh = stride_h;
   a.start = start; a.counts = counts; a.batch = batch; a.tokens = tokens; a.heads = heads; a.group = heads / kv->heads;
-  a.row_parts = c.row_parts; a.chunk = c.chunk; a.per_page = c.per_page; a.chunks = c.chunks; a.units = c.units;
+  a.row_parts = c.row_parts; a.per_page = c.per_page; a.splits = c.splits; a.clustered = c.clustered; a.units = c.units;
   a.scale = scale * 1.4426950408889634f;
   a.out = out;
   uint8_t* s = reinterpret_cast<uint8_t*>(scratch);
-  if (c.chunks > 1) { a.part_o = reinterpret_cast<float*>(s); s += up16(rows * c.chunks * kv->dim * 4); }
-  if (c.chunks > 1 || mass) { a.part_s = reinterpret_cast<float*>(s); s += up16(rows * c.chunks * fl::kv8::PART * 4); }
+  if (!c.clustered) { a.part_o = reinterpret_cast<float*>(s); s += up16(rows * parts * kv->dim * 4); }
+  if (!c.clustered || mass) { a.part_s = reinterpret_cast<float*>(s); s += up16(rows * parts * fl::kv8::PART * 4); }
   if (mass) a.unit_s = reinterpret_cast<float*>(s);
-  const dim3 grid(kv->heads * c.row_parts, batch, c.chunks);
+  const dim3 grid(kv->heads * c.row_parts, batch, c.splits);
   const bool early = (long long)batch * tokens <= FL_THIN_MAX_ROWS;
   int rc = 0;
-#define FL_ATT(D, N) rc = launch_attention<T, D, N>(a, *kv, mass != nullptr, grid, early, stream)
-  FL_KV8_TYPES(dtype, {
-    if (kv->dim <= 64) { if (c.nt == 1) FL_ATT(64, 1); else FL_ATT(64, 2); }
-    else { if (c.nt == 1) FL_ATT(128, 1); else FL_ATT(128, 2); }
-  });
-#undef FL_ATT
-  if (rc != 0 || (c.chunks == 1 && mass == nullptr)) return rc;
-  const int row_ctas = c.chunks > 1 ? heads * tokens : 0;
+  FL_KV8_TYPES(dtype, rc = kv->dim <= 64 ? launch_attention<T, 64>(a, *kv, c.nt, mass != nullptr, grid, early, stream)
+                                         : launch_attention<T, 128>(a, *kv, c.nt, mass != nullptr, grid, early, stream));
+  if (rc != 0 || (c.clustered && mass == nullptr)) return rc;
+  const int row_ctas = c.clustered ? 0 : heads * tokens;
   const int pages = kv->table_stride, page_ctas = mass == nullptr ? 0 : pages < 4 ? 1 : pages / 4 > 64 ? 64 : pages / 4;
-  if (row_ctas + page_ctas == 0) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(row_ctas + page_ctas, batch, 1);
   cfg.blockDim = dim3(128, 1, 1);
