@@ -85,14 +85,29 @@ struct WriteArgs {
   const void* src; void* out; const void* bias; const float* rope; long long rope_rows;
   const long long* start; const long long* pos; const long long* counts;
   int batch, tokens, heads, reach;            // reach: pages that a request's tokens can lie in
+  int parts;                                  // warps that share a token's queries
   // pack: pages of 16 bits in place of rows
   const void* src_v; const int* src_table; int src_stride, src_blocks;
+};
+
+struct Angles {                               // of a lane's columns
+  float co[8], si[8];
+  __device__ __forceinline__ void load(const float* rope, int dim, int c) {
+    const float4* a = reinterpret_cast<const float4*>(rope + 8 * c);
+    const float4* b = reinterpret_cast<const float4*>(rope + dim / 2 + 8 * c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 u = __ldg(a + i), v = __ldg(b + i);
+      co[4 * i] = u.x; co[4 * i + 1] = u.y; co[4 * i + 2] = u.z; co[4 * i + 3] = u.w;
+      si[4 * i] = v.x; si[4 * i + 1] = v.y; si[4 * i + 2] = v.z; si[4 * i + 3] = v.w;
+    }
+  }
 };
 
 template <typename T>
 struct Columns {                              // of one token: the two vectors that a lane takes
   uint4 lo, hi;
-  __device__ __forceinline__ void turn(const T* bias, const float* cs, int half) {
+  __device__ __forceinline__ void turn(const T* bias, const Angles* cs, int half) {
     if (bias == nullptr && cs == nullptr) return;
     float a[8], b[8];
     unpack<T>(lo, a);
@@ -109,7 +124,7 @@ struct Columns {                              // of one token: the two vectors t
     if (cs != nullptr) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {             // each product rounded, as separate operations would
-        const float co = cs[j], si = cs[half + j], x = a[j], y = b[j];
+        const float co = cs->co[j], si = cs->si[j], x = a[j], y = b[j];
         a[j] = __fsub_rn(__fmul_rn(x, co), __fmul_rn(y, si));
         b[j] = __fadd_rn(__fmul_rn(y, co), __fmul_rn(x, si));
       }
@@ -201,7 +216,7 @@ __device__ __forceinline__ void write_page(uint8_t* page, float* scale, bool the
 }
 
 template <typename T>
-__global__ void __launch_bounds__(128) write_kernel(const WriteArgs a, const FlKv8 kv, long long page_units, long long units) {
+__global__ void __launch_bounds__(128, 4) write_kernel(const WriteArgs a, const FlKv8 kv, unsigned page_units, unsigned units) {
   grid_dep_launch();
   grid_dep_wait();
   const int lane = threadIdx.x & 31, D = kv.dim, half = D / 2, chunks = D / 16, all = a.heads + 2 * kv.heads, bs = kv.block_size;
@@ -209,11 +224,11 @@ __global__ void __launch_bounds__(128) write_kernel(const WriteArgs a, const FlK
   const T* src = reinterpret_cast<const T*>(a.src);
   T* out = reinterpret_cast<T*>(a.out);
   const T* bias = reinterpret_cast<const T*>(a.bias);
-  for (long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 5); u < units; u += (long long)gridDim.x * 4) {
+  for (unsigned u = blockIdx.x * 4 + (threadIdx.x >> 5); u < units; u += gridDim.x * 4) {
     if (u < page_units) {
       const bool is_v = u & 1;
-      const long long r = u >> 1;
-      const int kh = (int)(r % kv.heads), rest = (int)(r / kv.heads), pi = rest % a.reach, b = rest / a.reach;
+      const unsigned r = u >> 1, rest = r / kv.heads;
+      const int kh = (int)(r - rest * kv.heads), b = (int)(rest / a.reach), pi = (int)(rest - (unsigned)b * a.reach);
       const long long st = a.start[b];
       const int n = a.counts ? (int)min(max(a.counts[b], 0ll), (long long)a.tokens) : a.tokens;
       // tokens [from, to) of the request's are in this page
@@ -247,12 +262,16 @@ __global__ void __launch_bounds__(128) write_kernel(const WriteArgs a, const FlK
             return Columns<T>{ld_v4(p), ld_v4(p + half)};
           },
           [&](int i, int c, Columns<T>& col) {
-            const float* cs = nullptr;
-            if (rotate) {
-              if (turn + i >= 0 && turn + i < a.rope_rows) cs = a.rope + (turn + i) * D + 8 * c;
-              else note(kv.status, FL_DEC_BAD_POSITION);
+            const T* bias_c = bias_h ? bias_h + 8 * c : nullptr;
+            const bool there = rotate && turn + i >= 0 && turn + i < a.rope_rows;
+            if (there) {
+              Angles cs;
+              cs.load(a.rope + (turn + i) * D, D, c);
+              col.turn(bias_c, &cs, half);
+            } else {
+              if (rotate) note(kv.status, FL_DEC_BAD_POSITION);
+              col.turn(bias_c, nullptr, half);
             }
-            col.turn(bias_h ? bias_h + 8 * c : nullptr, cs, half);
             T* p = out + (first + (long long)i * all) * D + 8 * c;
             st_v4(p, col.lo);
             st_v4(p + half, col.hi);
@@ -263,29 +282,37 @@ __global__ void __launch_bounds__(128) write_kernel(const WriteArgs a, const FlK
           });
       continue;
     }
-    // queries; and, where rows may be left out, those rows as they came
-    const int per_row = (a.counts ? all : a.heads) * chunks;
-    const long long item = (u - page_units) * 32 + lane;
-    const long long n = item / per_row;
-    if (n >= (long long)a.batch * a.tokens) continue;
-    const int r = (int)(item - n * per_row), head = r / chunks, c = r - head * chunks;
-    const int b = (int)(n / a.tokens), t = (int)(n - (long long)b * a.tokens);
+    // A token's queries, STEPS heads at a time for each lane, which has the same columns of all of them and so the same angles; of a row that is none of
+    // the request's, everything as it came.
+    const unsigned q = u - page_units, n = q / a.parts;
+    const int part = (int)(q - n * a.parts), b = (int)(n / a.tokens), t = (int)(n - (unsigned)b * a.tokens);
     const bool in = a.counts == nullptr || t < a.counts[b];
-    if (in && head >= a.heads) continue;
     if ((!in || (bias == nullptr && a.rope == nullptr)) && src == out) continue;
-    const long long at = (n * all + head) * D + 8 * c;
-    Columns<T> col{ld_v4(src + at), ld_v4(src + at + half)};
-    if (in) {
-      const long long turn = (a.pos ? a.pos[b] : a.start[b]) + t;
-      const float* cs = nullptr;
-      if (a.rope != nullptr) {
-        if (turn >= 0 && turn < a.rope_rows) cs = a.rope + turn * D + 8 * c;
-        else note(kv.status, FL_DEC_BAD_POSITION);
-      }
-      col.turn(bias ? bias + head * D + 8 * c : nullptr, cs, half);
+    const int at_once = 32 / chunks, tk = lane / chunks, c = lane - tk * chunks, heads = in ? a.heads : all;
+    if (tk >= at_once) continue;
+    const long long turn = (a.pos ? a.pos[b] : a.start[b]) + t;
+    const bool there = in && a.rope != nullptr && turn >= 0 && turn < a.rope_rows;
+    if (in && a.rope != nullptr && !there) note(kv.status, FL_DEC_BAD_POSITION);
+    Angles cs;
+    if (there) cs.load(a.rope + turn * D, D, c);
+    for (int h0 = part * STEPS * at_once + tk; h0 < heads; h0 += a.parts * STEPS * at_once) {
+      Columns<T> col[STEPS];
+      const long long at = ((long long)n * all + h0) * D + 8 * c;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (h0 + s * at_once < heads) {
+          const T* p = src + at + (long long)s * at_once * D;
+          col[s] = Columns<T>{ld_v4(p), ld_v4(p + half)};
+        }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (h0 + s * at_once < heads) {
+          if (in) col[s].turn(bias ? bias + (h0 + s * at_once) * D + 8 * c : nullptr, there ? &cs : nullptr, half);
+          T* p = out + at + (long long)s * at_once * D;
+          st_v4(p, col[s].lo);
+          st_v4(p + half, col[s].hi);
+        }
     }
-    st_v4(out + at, col.lo);
-    st_v4(out + at + half, col.hi);
   }
 }
 
@@ -904,9 +931,11 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
 }
 
 // ---- eviction ---------------------------------------------------------------------------------------------------------------
-// Bound by the latency of one CTA per request: the number of pages that go is known, the weight up to which they go is found digit by
-// digit (four histograms of 256), and one pass deals the row out in its order.
-constexpr int EVICT_THREADS = 512;
+// Bound by the latency of one CTA per request.  How many pages go is known; the weight up to which they go is found digit by digit (four
+// histograms of 256), and the row is dealt out in its order.  Threads keep their weights in registers, so that memory is read once: one each of
+// up to 1024 pages (16 rows of 145: 12.5 us with eight each, 4.4 with one), eight each of more (64 rows of 8192: 28 us with one page per thread and
+// pass, now 17); rows of more than 8192 go by in pieces of that, once for every digit.
+constexpr int EVICT_THREADS = 1024, EVICT_WARPS = EVICT_THREADS / 32, EVICT_EACH = 8;
 
 // weights in an order that whole numbers have: NaN last, -0 as 0
 __device__ __forceinline__ uint32_t evict_key(float m) {
@@ -915,14 +944,68 @@ __device__ __forceinline__ uint32_t evict_key(float m) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+template <int EACH> struct EvictShared {
+  int hist[256];
+  int before[EACH * EVICT_WARPS];        // by pass and warp: how many, then how many before
+  int all, digit, left;
+};
+// How many of the piece's flagged ones come before each of the thread's (bit k of `flags`: the one at k * threads + thread), in `rank`;
+// returns how many there are.
+template <int EACH>
+__device__ __forceinline__ int evict_ranks(EvictShared<EACH>& s, unsigned flags, int (&rank)[EACH]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const unsigned v = __ballot_sync(0xffffffffu, flags >> k & 1);
+    rank[k] = __popc(v & ((1u << lane) - 1));
+    if (lane == 0) s.before[k * EVICT_WARPS + warp] = __popc(v);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int n[EACH], sum = 0;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int at = lane * EACH + j;
+      n[j] = (at % EVICT_WARPS) * 32 < (int)blockDim.x ? s.before[at] : 0;
+      sum += n[j];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) s.all = upto;
+    upto -= sum;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      s.before[lane * EACH + j] = upto;
+      upto += n[j];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) rank[k] += s.before[k * EVICT_WARPS + warp];
+  return s.all;
+}
+
+template <int EACH>
 __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass, const int* table, const long long* lengths, int pages, int bs, int keep,
                                                               int recent, int sinks, float* mass_out, int* table_out, long long* lengths_out, int* gone) {
-  __shared__ int hist[256];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_left, s_sum[2][EVICT_THREADS / 32];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ EvictShared<EACH> s;
+  const int b = blockIdx.x, threads = blockDim.x, piece_size = threads * EACH, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   mass += (long long)b * pages; table += (long long)b * pages;
   mass_out += (long long)b * pages; table_out += (long long)b * pages;
+  float m[EACH];
+  auto load = [&](int piece) {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const long long i = (long long)piece + k * threads + tid;
+      m[k] = i < pages ? mass[i] : 0.f;
+    }
+  };
+  load(0);
   const long long len = max(lengths[b], 0ll);
   const int used = (int)min(len / bs + (len % bs != 0), (long long)pages), extra = max(used - keep, 0);
   if (tid == 0) {
@@ -934,21 +1017,32 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass,
   int left = extra;                                            // of those that go, among the weights that begin with the digits found
   if (extra > 0) {
     for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += EVICT_THREADS) hist[i] = 0;
+      for (int i = tid; i < 256; i += threads) s.hist[i] = 0;
       __syncthreads();
-      for (int i0 = lo; i0 < hi; i0 += EVICT_THREADS) {
-        const int i = i0 + tid;
-        const uint32_t key = i < hi ? evict_key(mass[i]) : 0;
-        const bool in = i < hi && (shift == 24 || key >> (shift + 8) == prefix);
-        const int digit = in ? (int)(key >> shift & 255) : 256;
-        const unsigned same = __match_any_sync(0xffffffffu, digit);          // weights that no token ever saw are all alike
-        if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+      for (int piece = 0; piece < pages; piece += piece_size) {
+        if (pages > piece_size) load(piece);
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+          const long long i = (long long)piece + k * threads + tid;
+          const uint32_t key = evict_key(m[k]);
+          const bool in = i >= lo && i < hi && (shift == 24 || key >> (shift + 8) == prefix);
+          // weights that no token ever saw are all alike: those that agree with the first of the warp are added at once
+          const int digit = (int)(key >> shift & 255);
+          const unsigned some = __ballot_sync(0xffffffffu, in);
+          if (some == 0) continue;
+          const int leader = __ffs(some) - 1, first = __shfl_sync(0xffffffffu, digit, leader);
+          const bool like = in && digit == first;
+          const unsigned alike = __ballot_sync(0xffffffffu, like);
+          if (lane == leader) atomicAdd(&s.hist[digit], __popc(alike));
+          else if (in && !like) atomicAdd(&s.hist[digit], 1);
+        }
+        if (piece > 0x7fffffff - piece_size) break;
       }
       __syncthreads();
       if (warp == 0) {
         int n[8], sum = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { n[j] = hist[lane * 8 + j]; sum += n[j]; }
+        for (int j = 0; j < 8; ++j) { n[j] = s.hist[lane * 8 + j]; sum += n[j]; }
         int before = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -958,52 +1052,55 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass,
         before -= sum;
         if (before < left && before + sum >= left) {
           int j = 0;
-          while (j < 7 && before + n[j] < left) before += n[j++];
-          s_prefix = prefix << 8 | (lane * 8 + j);
-          s_left = left - before;
+#pragma unroll
+          for (int q = 0; q < 7; ++q)
+            if (j == q && before + n[q] < left) { before += n[q]; ++j; }
+          s.digit = lane * 8 + j;
+          s.left = left - before;
         }
       }
       __syncthreads();
-      prefix = s_prefix;
-      left = s_left;
+      prefix = prefix << 8 | (uint32_t)s.digit;
+      left = s.left;
     }
   }
-  // positions below: kept pages from 0, those that go from used - extra
+  // kept pages go to the front, those that go to used - extra and on
   int equal_before = 0, gone_before = 0;
-  for (int i0 = 0; i0 < pages; i0 += EVICT_THREADS) {
-    const int i = i0 + tid;
-    float m = 0.f;
-    int id = 0;
-    if (i < pages) { m = mass[i]; id = table[i]; }
-    const bool free = extra > 0 && i >= lo && i < hi;
-    const uint32_t key = evict_key(m);
-    const bool equal = free && key == prefix;
-    const unsigned eq = __ballot_sync(0xffffffffu, equal);
-    if (lane == 0) s_sum[0][warp] = __popc(eq);
-    __syncthreads();
-    int rank = equal_before + __popc(eq & ((1u << lane) - 1)), all_eq = 0;
+  for (int piece = 0; piece < pages; piece += piece_size) {
+    if (pages > piece_size) load(piece);
+    int id[EACH], rank[EACH] = {};
+    unsigned below = 0, equal = 0;
 #pragma unroll
-    for (int w = 0; w < EVICT_THREADS / 32; ++w) {
-      if (w < warp) rank += s_sum[0][w];
-      all_eq += s_sum[0][w];
+    for (int k = 0; k < EACH; ++k) {
+      const long long i = (long long)piece + k * threads + tid;
+      id[k] = i < pages ? table[i] : 0;
+      const bool free = extra > 0 && i >= lo && i < hi;
+      const uint32_t key = evict_key(m[k]);
+      below |= (free && key < prefix ? 1u : 0u) << k;
+      equal |= (free && key == prefix ? 1u : 0u) << k;
     }
-    const bool goes = free && (key < prefix || (equal && rank < left));
-    const unsigned go = __ballot_sync(0xffffffffu, goes);
-    if (lane == 0) s_sum[1][warp] = __popc(go);
-    __syncthreads();
-    int out = gone_before + __popc(go & ((1u << lane) - 1)), all_go = 0;
+    unsigned goes = below;
+    if (extra > 0) {
+      const int equals = evict_ranks(s, equal, rank);
 #pragma unroll
-    for (int w = 0; w < EVICT_THREADS / 32; ++w) {
-      if (w < warp) out += s_sum[1][w];
-      all_go += s_sum[1][w];
+      for (int k = 0; k < EACH; ++k)
+        if ((equal >> k & 1) && equal_before + rank[k] < left) goes |= 1u << k;
+      equal_before += equals;
+      const int going = evict_ranks(s, goes, rank);
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) rank[k] += gone_before;
+      gone_before += going;
     }
-    if (i < pages) {
-      const int to = i >= used ? i : goes ? used - extra + out : i - out;
-      table_out[to] = id;
-      mass_out[to] = goes ? 0.f : m;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const long long i = (long long)piece + k * threads + tid;
+      if (i >= pages) continue;
+      const bool out = goes >> k & 1;
+      const int to = (int)i >= used ? (int)i : out ? used - extra + rank[k] : (int)i - rank[k];
+      table_out[to] = id[k];
+      mass_out[to] = out ? 0.f : m[k];
     }
-    equal_before += all_eq;
-    gone_before += all_go;
+    if (piece > 0x7fffffff - piece_size) break;
   }
 }
 
@@ -1044,10 +1141,11 @@ extern "C" int fl_kv8_write(int dtype, const void* qkv, void* out, const void* b
   a.start = start; a.pos = pos; a.counts = counts; a.batch = batch; a.tokens = tokens; a.heads = heads;
   a.reach = (tokens + kv->block_size - 2) / kv->block_size + 1;
   const long long page_units = 2ll * batch * a.reach * kv->heads, rows = (long long)batch * tokens;
-  if ((long long)batch * a.reach > 0x7fffffffll) return -2;
-  const bool copy = qkv != out, q = copy || bias != nullptr || rope != nullptr;
-  const long long items = q ? rows * (counts ? heads + 2 * kv->heads : heads) * (kv->dim / 16) : 0;
-  const long long units = page_units + (items + 31) / 32;
+  const bool q = qkv != out || bias != nullptr || rope != nullptr;
+  const int per_warp = fl::kv8::STEPS * (32 / (kv->dim / 16));       // heads
+  a.parts = heads <= per_warp ? 1 : (heads + per_warp - 1) / per_warp;
+  const long long units = page_units + (q ? rows * a.parts : 0);
+  if (units > 0x7fffffffll || (long long)(heads + 2 * kv->heads) * kv->dim > 0x7fffffffll) return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid_of(units), 1, 1);
   cfg.blockDim = dim3(128, 1, 1);
@@ -1057,7 +1155,7 @@ extern "C" int fl_kv8_write(int dtype, const void* qkv, void* out, const void* b
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = rows <= FL_THIN_MAX_ROWS ? 1 : 0;      // as the decoder's other passes
-  FL_KV8_TYPES(dtype, return (int)cudaLaunchKernelEx(&cfg, fl::kv8::write_kernel<T>, a, *kv, page_units, units));
+  FL_KV8_TYPES(dtype, return (int)cudaLaunchKernelEx(&cfg, fl::kv8::write_kernel<T>, a, *kv, (unsigned)page_units, (unsigned)units));
 }
 
 extern "C" int fl_kv8_pack(int dtype, const void* k_pool, const void* v_pool, int src_blocks, const int* src_table, int src_stride,
@@ -1190,7 +1288,10 @@ extern "C" int fl_kv8_evict(const float* mass, const int* table, const long long
                             int sinks, float* mass_out, int* table_out, long long* lengths_out, int* gone, cudaStream_t stream) {
   if (batch < 0 || pages < 0 || block_size < 1 || recent < 1 || sinks < 0 || (long long)recent + sinks > keep) return -2;
   if (batch == 0) return 0;
-  fl::kv8::evict_kernel<<<batch, fl::kv8::EVICT_THREADS, 0, stream>>>(mass, table, lengths, pages, block_size, keep, recent, sinks, mass_out, table_out,
-                                                                      lengths_out, gone);
+  const int each = pages <= fl::kv8::EVICT_THREADS ? 1 : fl::kv8::EVICT_EACH;
+  const long long wanted = ((long long)pages + each - 1) / each;
+  const int threads = wanted > fl::kv8::EVICT_THREADS ? fl::kv8::EVICT_THREADS : wanted < 32 ? 32 : (int)(wanted + 31) / 32 * 32;
+  if (each == 1) fl::kv8::evict_kernel<1><<<batch, threads, 0, stream>>>(mass, table, lengths, pages, block_size, keep, recent, sinks, mass_out, table_out, lengths_out, gone);
+  else fl::kv8::evict_kernel<fl::kv8::EVICT_EACH><<<batch, threads, 0, stream>>>(mass, table, lengths, pages, block_size, keep, recent, sinks, mass_out, table_out, lengths_out, gone);
   return (int)cudaGetLastError();
 }
