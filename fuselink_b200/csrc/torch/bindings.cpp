@@ -448,10 +448,13 @@ static const long long* kv8_i64(const c10::optional<torch::Tensor>& t, const tor
   TORCH_CHECK(!t.has_value() || t->device() == as.device(), what);
   return dec_i64(t, numel, what);
 }
-static void kv8_write(torch::Tensor k, torch::Tensor v, torch::Tensor k_scale, torch::Tensor v_scale, torch::Tensor table, int64_t layer, torch::Tensor qkv,
-                      torch::Tensor out, c10::optional<torch::Tensor> bias, c10::optional<torch::Tensor> rope, torch::Tensor start,
-                      c10::optional<torch::Tensor> pos, c10::optional<torch::Tensor> counts, int64_t status_addr) {
+static torch::Tensor kv8_write(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& k_scale, const torch::Tensor& v_scale, const torch::Tensor& table, int64_t layer,
+                               torch::Tensor qkv, c10::optional<torch::Tensor> into, const c10::optional<torch::Tensor>& bias, const c10::optional<torch::Tensor>& rope,
+                               const torch::Tensor& start, const c10::optional<torch::Tensor>& pos, const c10::optional<torch::Tensor>& counts, int64_t status_addr) {
   const int dt = dec_dtype(qkv);
+  c10::cuda::CUDAGuard guard(qkv.device());
+  if (!into.has_value()) qkv = qkv.contiguous();
+  const torch::Tensor out = into.has_value() ? *into : torch::empty_like(qkv);
   TORCH_CHECK(qkv.dim() == 4 && qkv.is_contiguous() && qkv.device() == k.device(), "kv8: qkv [batch, tokens, heads + 2 kv_heads, dim], contiguous");
   const int64_t B = qkv.size(0), T = qkv.size(1), all = qkv.size(2), D = qkv.size(3);
   TORCH_CHECK(k.dim() == 5 && D == k.size(4) && all >= 2 * k.size(2) && B <= INT32_MAX && T <= INT32_MAX && all * D <= INT32_MAX, "kv8: qkv of another layout than the cache");
@@ -460,11 +463,11 @@ static void kv8_write(torch::Tensor k, torch::Tensor v, torch::Tensor k_scale, t
   TORCH_CHECK(!bias.has_value() || bias->device() == k.device(), "kv8: bias on the cache's device");
   TORCH_CHECK(!rope.has_value() || (rope->device() == k.device() && rope->scalar_type() == torch::kFloat32 && rope->is_contiguous() && rope->dim() == 2 && rope->size(1) == D),
               "kv8: rope [positions, dim] fp32");
-  c10::cuda::CUDAGuard guard(k.device());
   const FlKv8 kv = kv8_of(k, v, k_scale, v_scale, table, layer, B, status_addr);
   check_rc(fl_kv8_write(dt, qkv.data_ptr(), out.data_ptr(), opt_ptr(bias), rope.has_value() ? rope->data_ptr<float>() : nullptr, rope.has_value() ? rope->size(0) : 0,
                         kv8_i64(start, k, B, "kv8: start [batch] int64"), kv8_i64(pos, k, B, "kv8: positions [batch] int64"),
                         kv8_i64(counts, k, B, "kv8: counts [batch] int64"), (int)B, (int)T, (int)(all - 2 * kv.heads), &kv, cur_stream()), "fl_kv8_write");
+  return out;
 }
 static void kv8_pack(torch::Tensor k, torch::Tensor v, torch::Tensor k_scale, torch::Tensor v_scale, torch::Tensor table, torch::Tensor k_pool, torch::Tensor v_pool,
                      int64_t src_blocks, torch::Tensor src_table, torch::Tensor lengths, int64_t status_addr) {
@@ -479,24 +482,28 @@ static void kv8_pack(torch::Tensor k, torch::Tensor v, torch::Tensor k_scale, to
   check_rc(fl_kv8_pack(dt, k_pool.data_ptr(), v_pool.data_ptr(), (int)src_blocks, src_table.data_ptr<int>(), (int)src_table.size(1),
                        kv8_i64(lengths, k, table.size(0), "kv8: lengths [batch] int64"), (int)table.size(0), &kv, cur_stream()), "fl_kv8_pack");
 }
-static void kv8_attention(torch::Tensor k, torch::Tensor v, torch::Tensor k_scale, torch::Tensor v_scale, torch::Tensor table, int64_t layer, torch::Tensor q,
-                          torch::Tensor start, c10::optional<torch::Tensor> counts, double scale, torch::Tensor out, c10::optional<torch::Tensor> mass, int64_t status_addr) {
+static torch::Tensor kv8_attention(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& k_scale, const torch::Tensor& v_scale, const torch::Tensor& table, int64_t layer,
+                                   const torch::Tensor& q, const torch::Tensor& start, const c10::optional<torch::Tensor>& counts, double scale,
+                                   c10::optional<torch::Tensor> into, const c10::optional<torch::Tensor>& mass, int64_t status_addr) {
   const int dt = dec_dtype(q);
   TORCH_CHECK(q.dim() == 4 && q.device() == k.device() && k.dim() == 5 && q.size(3) == k.size(4) && q.stride(3) == 1, "kv8: q [batch, tokens, heads, dim] with contiguous heads");
   const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3);
   TORCH_CHECK(B <= INT32_MAX && T <= INT32_MAX && H <= INT32_MAX && H % std::max<int64_t>(k.size(2), 1) == 0, "kv8: heads in groups that share a KV head");
+  c10::cuda::CUDAGuard guard(k.device());
+  const torch::Tensor out = into.has_value() ? *into : torch::empty({B, T, H * D}, q.options());
   TORCH_CHECK(out.device() == k.device() && out.scalar_type() == q.scalar_type() && out.is_contiguous() && out.numel() == B * T * H * D, "kv8: out [batch, tokens, heads * dim] like q");
   TORCH_CHECK(!mass.has_value() || (mass->device() == k.device() && mass->scalar_type() == torch::kFloat32 && mass->is_contiguous() && mass->sizes() == table.sizes()),
               "kv8: mass [batch, pages] fp32");
-  c10::cuda::CUDAGuard guard(k.device());
   const FlKv8 kv = kv8_of(k, v, k_scale, v_scale, table, layer, B, status_addr);
   const long long bytes = fl_kv8_attention_scratch((int)B, (int)T, (int)H, &kv, mass.has_value());
-  auto scratch = torch::empty({bytes}, q.options().dtype(torch::kUInt8));
+  torch::Tensor scratch;
+  if (bytes > 0) scratch = torch::empty({bytes}, q.options().dtype(torch::kUInt8));
   check_rc(fl_kv8_attention(dt, q.data_ptr(), B > 1 ? q.stride(0) : 0, T > 1 ? q.stride(1) : 0, H > 1 ? q.stride(2) : 0, kv8_i64(start, k, B, "kv8: start [batch] int64"),
                             kv8_i64(counts, k, B, "kv8: counts [batch] int64"), (int)B, (int)T, (int)H, (float)scale, &kv, out.data_ptr(),
-                            mass.has_value() ? mass->data_ptr<float>() : nullptr, bytes ? scratch.data_ptr() : nullptr, cur_stream()), "fl_kv8_attention");
+                            mass.has_value() ? mass->data_ptr<float>() : nullptr, bytes > 0 ? scratch.data_ptr() : nullptr, cur_stream()), "fl_kv8_attention");
+  return out;
 }
-static std::vector<torch::Tensor> kv8_evict(torch::Tensor mass, torch::Tensor table, torch::Tensor lengths, int64_t block_size, int64_t keep, int64_t recent, int64_t sinks) {
+static std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> kv8_evict(const torch::Tensor& mass, const torch::Tensor& table, const torch::Tensor& lengths, int64_t block_size, int64_t keep, int64_t recent, int64_t sinks) {
   TORCH_CHECK(mass.is_cuda() && mass.scalar_type() == torch::kFloat32 && mass.is_contiguous() && mass.dim() == 2, "kv8: mass [batch, pages] fp32");
   TORCH_CHECK(table.device() == mass.device() && table.scalar_type() == torch::kInt32 && table.is_contiguous() && table.sizes() == mass.sizes(), "kv8: block_table [batch, pages] int32");
   const int64_t B = mass.size(0), M = mass.size(1);

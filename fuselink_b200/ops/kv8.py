@@ -68,24 +68,20 @@ def write(cache: Kv8Cache, layer: int, qkv: torch.Tensor, block_table: torch.Ten
     that a request has, of a padded batch; rows behind them stay as they are.  rope ([positions, dim] fp32): cosines, then sines;
     positions ([batch] int64): what the first token is rotated by, where that is not its slot.  bias: [(heads + 2 kv_heads) * dim].  Returns the rows as the
     attention takes them: ``out``, which may be qkv, or a new tensor."""
-    _check_like(cache, qkv, "rows")
-    if out is None:
-        qkv = qkv.contiguous()
-        out = torch.empty_like(qkv)
     if qkv.is_cuda:
-        require_native().kv8_write(*cache.tensors(), block_table, layer, qkv, out, bias, rope, start, positions, counts, status)
-        return out
-    return _plain_write(cache, layer, qkv, out, block_table, start, counts, positions, rope, bias)
+        return require_native().kv8_write(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, layer, qkv, out, bias, rope, start, positions, counts, status)
+    _check_like(cache, qkv, "rows")
+    return _plain_write(cache, layer, qkv, torch.empty_like(qkv) if out is None else out, block_table, start, counts, positions, rope, bias)
 
 
 def pack(cache: Kv8Cache, k_pool: torch.Tensor, v_pool: torch.Tensor, src_blocks: int, src_table: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, *,
          status: int = 0) -> None:
     """The first ``lengths[b]`` tokens ([batch] int64) of every request, all layers, from 16-bit pages [layers, src_blocks, block_size, kv_heads, dim] (what
     the KV hand-off leaves on the decode side) at ``src_table`` to the cache's at ``block_table``."""
-    _check_like(cache, k_pool, "pages")
     if k_pool.is_cuda:
-        require_native().kv8_pack(*cache.tensors(), block_table, k_pool, v_pool, src_blocks, src_table, lengths, status)
+        require_native().kv8_pack(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, k_pool, v_pool, src_blocks, src_table, lengths, status)
         return
+    _check_like(cache, k_pool, "pages")
     L, _, KH, bs, D = cache.k.shape
     k, v = (p.view(L, src_blocks, bs, KH, D) for p in (k_pool, v_pool))
     for b, n in enumerate(lengths.tolist()):
@@ -106,15 +102,13 @@ def attention(cache: Kv8Cache, layer: int, q: torch.Tensor, block_table: torch.T
     are multiples of 8 elements; token t of request b sees slots 0 .. start[b] + t.  Returns [batch, tokens, heads * dim]; zeros for tokens behind
     ``counts`` and for those that see nothing.  scale: 1 / sqrt(dim) by default.
     mass ([batch, pages] fp32) has the weights' sum over this call's tokens and heads added, page by page of ``block_table``."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if q.is_cuda:
+        return require_native().kv8_attention(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, layer, q, start, counts, scale, out, mass, status)
     _check_like(cache, q, "queries")
     B, T, H, D = q.shape
-    if out is None:
-        out = torch.empty(B, T, H * D, dtype=q.dtype, device=q.device)
-    scale = 1.0 / math.sqrt(D) if scale is None else scale
-    if q.is_cuda:
-        require_native().kv8_attention(*cache.tensors(), block_table, layer, q, start, counts, scale, out, mass, status)
-        return out
-    return _plain_attention(cache, layer, q, block_table, start, counts, scale, mass, out)
+    return _plain_attention(cache, layer, q, block_table, start, counts, scale, mass, torch.empty(B, T, H * D, dtype=q.dtype) if out is None else out)
 
 
 def evict(mass: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, block_size: int, keep: int, *, recent: int = 1,
@@ -127,7 +121,7 @@ def evict(mass: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, 
     if keep < recent + sinks or recent < 1 or sinks < 0 or block_size < 1:
         raise ValueError(f"kv8: keep ({keep}) at least recent ({recent}) + sinks ({sinks}) pages, recent at least one")
     if mass.is_cuda:
-        return tuple(require_native().kv8_evict(mass, block_table, lengths, block_size, keep, recent, sinks))
+        return require_native().kv8_evict(mass, block_table, lengths, block_size, keep, recent, sinks)
     table, mass, lens, gone = block_table.clone(), mass.clone(), lengths.clone(), torch.zeros(len(lengths), dtype=torch.int32)
     for b, n in enumerate(lengths.tolist()):
         used = min(-(-max(n, 0) // block_size), mass.shape[1])

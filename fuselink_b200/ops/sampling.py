@@ -23,8 +23,10 @@ Limit = Union[float, int, torch.Tensor]
 
 def _limit(value: Limit, dtype, rows: int, device, name: str):
     """(tensor or None, value for all rows) as the kernel takes it."""
-    if not torch.is_tensor(value):
+    if not isinstance(value, torch.Tensor):
         return None, value
+    if value.dtype == dtype and value.shape == (rows,) and value.is_contiguous():      # the kernel sees to the device
+        return value, 0
     if value.dim() == 0:
         value = value.expand(rows)
     if value.shape != (rows,):
@@ -48,12 +50,13 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Limit = 1.0, top_
         raise ValueError(f"sample: u [{rows}] of fp32 or fp64 expected, not {tuple(u.shape)} of {u.dtype}")
     if u.device != dev:
         raise RuntimeError(f"sample: u on {dev} expected, not on {u.device}")
-    given = [_limit(v, t, rows, dev, n) for v, t, n in ((temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"),
-                                                      (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p"))]
+    given = (_limit(temperature, torch.float32, rows, dev, "temperature"), _limit(top_k, torch.int32, rows, dev, "top_k"),
+             _limit(top_p, torch.float32, rows, dev, "top_p"), _limit(min_p, torch.float32, rows, dev, "min_p"))
     if logits.is_cuda:
-        if logits.shape[1] > 1 and logits.stride(1) != 1:
+        if logits.stride(1) != 1:
             logits = logits.contiguous()
-        return require_native().sample(logits, u.contiguous(), *(x for g in given for x in g))
+        (t, t_all), (k, k_all), (p, p_all), (m, m_all) = given
+        return require_native().sample(logits, u.contiguous(), t, t_all, k, k_all, p, p_all, m, m_all)
     return _plain_sample(logits, u, *(torch.full((rows,), all_, dtype=torch.float64) if t is None else t.double() for t, all_ in given))
 
 
