@@ -407,6 +407,11 @@ __device__ __forceinline__ float exp2_fast(float x) {                     // the
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float log2_fast(float x) {                     // the hardware's: 2^-22 off; -inf of 0
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 // over the lane groups (the rows of a product), for every quad lane
 __device__ __forceinline__ float max_rows(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
@@ -435,6 +440,7 @@ template <int DP> struct Ring {
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {        // zeros where it is not there
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
@@ -517,6 +523,14 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
       const long long cell = (pool0 + max(id, 0)) * kv.heads + kh, at = (cell * bs + s0) * D;
       const uint32_t to = mine + stage * R::STAGE;
       const bool column = FULL || 16 * piece < D;
+      if (FULL && live == 16) {
+        const uint8_t *k = kp + at, *v = vp + at;
+#pragma unroll
+        for (int i = 0; i < 16; i += PASS) {
+          copy16(to + i * R::PITCH, k + i * DP);
+          copy16(to + R::KEYS + i * R::PITCH, v + i * DP);
+        }
+      } else
 #pragma unroll
       for (int i = 0; i < 16; i += PASS) {
         const bool there = column && i + row0 < live;           // the addresses of others may be anything
@@ -697,8 +711,8 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
         const float s0 = sum_rows(add[0]), s1 = sum_rows(add[1]);
         if (g == 0) {
           float* w = a.unit_s + ((long long)b * a.units + u) * a.heads * a.tokens + kh * all_rows + r0 + 8 * nt + 2 * t;
-          if (8 * nt + 2 * t < n_rows) w[0] = m[nt][0] + log2f(s0);
-          if (8 * nt + 2 * t + 1 < n_rows) w[1] = m[nt][1] + log2f(s1);
+          if (8 * nt + 2 * t < n_rows) w[0] = m[nt][0] + log2_fast(s0);
+          if (8 * nt + 2 * t + 1 < n_rows) w[1] = m[nt][1] + log2_fast(s1);
         }
       }
     }
@@ -922,7 +936,7 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
     float sum = 0.f;
     for (int i = 0; i < a.per_page; ++i) {
       const float* w = a.unit_s + ((long long)b * a.units + p * a.per_page + i) * rows;
-      for (int r = lane; r < rows; r += 32) sum += s_lse[r] == INFINITY ? 0.f : exp2f(w[r] - s_lse[r]);
+      for (int r = lane; r < rows; r += 32) sum += exp2_fast(w[r] - s_lse[r]);          // 0 where the row sees nothing
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -1270,7 +1284,8 @@ extern "C" int fl_kv8_attention(int dtype, const void* q, long long stride_b, lo
                                          : launch_attention<T, 128>(a, *kv, c.nt, mass != nullptr, grid, early, stream));
   if (rc != 0 || (c.clustered && mass == nullptr)) return rc;
   const int row_ctas = c.clustered ? 0 : heads * tokens;
-  const int pages = kv->table_stride, page_ctas = mass == nullptr ? 0 : pages < 4 ? 1 : pages / 4 > 64 ? 64 : pages / 4;
+  const int pages = kv->table_stride, most = 8 * 148 / batch;                 // eight CTAs per SM, if there is a page for each warp of theirs
+  const int page_ctas = mass == nullptr ? 0 : pages < 4 || most < 1 ? 1 : pages / 4 > most ? most : pages / 4;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(row_ctas + page_ctas, batch, 1);
   cfg.blockDim = dim3(128, 1, 1);
