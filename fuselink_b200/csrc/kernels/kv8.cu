@@ -431,6 +431,11 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 
 // A warp's ring in shared memory.  Rows are 16 bytes further apart than they are long, so that the 16-byte (values of heads up to 64: 8-byte) reads of
 // a product's rows meet different banks.
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
 template <int DP> struct Ring {
   static constexpr int STAGES = DP == 128 ? 3 : 6;
   static constexpr int PITCH = DP + 16, KEYS = 16 * PITCH, SCALES = 2 * KEYS;
@@ -465,8 +470,6 @@ __device__ __forceinline__ int seen_by_last(const AttArgs& a, const FlKv8& kv, i
   const int n = tokens_of(a.counts, b, a.tokens);
   return n == 0 ? 0 : (int)min(max(a.start[b] + n, 0ll), (long long)kv.table_stride * kv.block_size);
 }
-// CTAs that a context of so many steps is dealt out to
-__device__ __forceinline__ int parts_of(const AttArgs& a, int units) { return min(max((units + FEWEST - 1) / FEWEST, 1), a.splits); }
 
 // parts' outputs are means (divided by their sums), so that joining them overflows nowhere
 __device__ __forceinline__ float share(float m, float l, float mm) { return l == 0.f ? 0.f : exp2f(m - mm) * l; }      // 0: a part without weight; not one whose sum is NaN
@@ -484,26 +487,43 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int kh = blockIdx.x / a.row_parts, rp = blockIdx.x - kh * a.row_parts, b = blockIdx.y, z = blockIdx.z;
   const int D = FULL ? DP : kv.dim, bs = kv.block_size, all_rows = a.group * a.tokens, r0 = rp * ROWS;
-  const int n_rows = min(ROWS, all_rows - r0), n_new = tokens_of(a.counts, b, a.tokens);
-  const int len = seen_by_last(a, kv, b);
-  const int units = (len + bs - 1) / bs * a.per_page, parts = parts_of(a, units);
-  if (!a.clustered && z >= parts) return;
-  // the warp's units
-  const int nw = parts * WARPS, w0 = z * WARPS + warp, per = units / nw, extra = units % nw;
-  const int first = z < parts ? w0 * per + min(w0, extra) : 0, last = z < parts ? first + per + (w0 < extra ? 1 : 0) : 0;
+  const int n_rows = min(ROWS, all_rows - r0);
+  // The warp's units: every nw-th.  Which pages these are does not depend on the context's length, nor do the queries, so that all three are on
+  // their way side by side.
+  const int nw = a.splits * WARPS, first = z * WARPS + warp;
+  auto look_up = [&](int u0) {                 // lane i: the page of unit u0 + i nw
+    const int u = u0 + lane * nw;
+    return u < a.units ? page_id(kv, b, a.per_page == 1 ? u : u / a.per_page) : -1;
+  };
+  int ids = look_up(first);
+  const long long start = a.start[b];
+  const int n_new = tokens_of(a.counts, b, a.tokens);
+  uint4 q_raw[NT][KJ][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = r0 + 8 * nt + g, tok = a.tokens == 1 ? 0 : r / a.group, h = r - tok * a.group;
+    const T* q = reinterpret_cast<const T*>(a.q) + b * a.sb + tok * a.st + (long long)(kh * a.group + h) * a.sh;
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) {
+      const int d = DP == 128 ? 32 * t + 16 * j : 16 * t;
+      q_raw[nt][j][0] = q_raw[nt][j][1] = make_uint4(0, 0, 0, 0);
+      if (r < all_rows && d < D) {
+        q_raw[nt][j][0] = ld_v4(q + d);
+        q_raw[nt][j][1] = ld_v4(q + d + 8);
+      }
+    }
+  }
+  const int len = n_new == 0 ? 0 : (int)min(max(start + n_new, 0ll), (long long)kv.table_stride * bs);
+  const int units = (len + bs - 1) / bs * a.per_page;
+  const int mine = first < units ? (units - first + nw - 1) / nw : 0;
 
   // this lane's 16 bytes of a row, in every PASS-th row
   constexpr int PIECES = DP / 16, PASS = 32 / PIECES;
   const int row0 = lane / PIECES, piece = lane % PIECES;
   const uint8_t* kp = reinterpret_cast<const uint8_t*>(kv.k) + row0 * D + 16 * piece;
   const uint8_t* vp = reinterpret_cast<const uint8_t*>(kv.v) + row0 * D + 16 * piece;
-  const uint32_t ring = smem_u32(s_ring) + warp * R::STAGES * R::STAGE, mine = ring + row0 * R::PITCH + 16 * piece;
+  const uint32_t ring = smem_u32(s_ring) + warp * R::STAGES * R::STAGE, cell0 = ring + row0 * R::PITCH + 16 * piece;
   const long long pool0 = (long long)kv.layer * kv.num_blocks;
-  int ids = -1, ids_at = 0;                    // lane i: the page of unit ids_at + i
-  auto look_up = [&](int u0) {
-    ids_at = u0;
-    ids = u0 + lane < last ? page_id(kv, b, (u0 + lane) / a.per_page) : -1;
-  };
   // where a unit begins, and tokens of it that the request has
   auto place = [&](int u, int& base, int& live) {
     int page = u, s0 = 0;
@@ -512,16 +532,17 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
     live = min(min(bs - s0, len - base), 16);
     return s0;
   };
-  auto fetch = [&](int u, int stage) {         // every lane calls it; an empty group behind the last
-    if (u < last) {
-      if (u >= ids_at + 32) look_up(u);
-      const int id = __shfl_sync(0xffffffffu, ids, u - ids_at);
+  auto fetch = [&](int i, int stage) {         // the warp's i-th unit; every lane calls it, i by i; an empty group behind the last
+    if (i < mine) {
+      const int u = first + i * nw;
+      if (i > 0 && i % 32 == 0) ids = look_up(u);
+      const int id = __shfl_sync(0xffffffffu, ids, i % 32);
       int base, live;
       const int s0 = place(u, base, live);
       if (id < 0 && lane == 0) note(kv.status, FL_DEC_BAD_PAGE);
       if (id < 0) live = 0;
       const long long cell = (pool0 + max(id, 0)) * kv.heads + kh, at = (cell * bs + s0) * D;
-      const uint32_t to = mine + stage * R::STAGE;
+      const uint32_t to = cell0 + stage * R::STAGE;
       const bool column = FULL || 16 * piece < D;
       if (FULL && live == 16) {
         const uint8_t *k = kp + at, *v = vp + at;
@@ -542,9 +563,8 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
     copies_commit();
   };
 
-  look_up(first);
 #pragma unroll
-  for (int s = 0; s < R::STAGES - 1; ++s) fetch(first + s, s);
+  for (int s = 0; s < R::STAGES - 1; ++s) fetch(s, s);
 
   // queries, as the second operand; a row's power of two is undone on its scores
   uint32_t qb[NT][KJ][8];
@@ -552,22 +572,13 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   int sees[NT][2], fewest = len;               // slots that the column's token sees; the fewest of any that sees some
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int r = r0 + 8 * nt + g, tok = r / a.group, h = r - tok * a.group;
-    const bool in = r < all_rows && tok < n_new;
-    const T* q = reinterpret_cast<const T*>(a.q) + b * a.sb + tok * a.st + (long long)(kh * a.group + h) * a.sh;
     float f[KJ][16];
     float m = 0.f;
 #pragma unroll
     for (int j = 0; j < KJ; ++j) {
-      const int d = DP == 128 ? 32 * t + 16 * j : 16 * t;
-      uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
-      if (in && d < D) {
-        u0 = ld_v4(q + d);
-        u1 = ld_v4(q + d + 8);
-      }
       float v0[8], v1[8];
-      unpack<T>(u0, v0);
-      unpack<T>(u1, v1);
+      unpack<T>(q_raw[nt][j][0], v0);
+      unpack<T>(q_raw[nt][j][1], v1);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         f[j][i] = v0[i];
@@ -588,8 +599,8 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       factor[nt][c] = __shfl_sync(0xffffffffu, back, (2 * t + c) * 4) * a.scale;
-      const int rc = r0 + 8 * nt + 2 * t + c, tc = rc / a.group;
-      sees[nt][c] = rc < all_rows && tc < n_new ? max((int)min(a.start[b] + tc + 1, (long long)len), 0) : 0;
+      const int rc = r0 + 8 * nt + 2 * t + c, tc = a.tokens == 1 ? 0 : rc / a.group;
+      sees[nt][c] = rc < all_rows && tc < n_new ? max((int)min(start + tc + 1, (long long)len), 0) : 0;
       if (sees[nt][c] > 0) fewest = min(fewest, sees[nt][c]);
     }
   }
@@ -608,11 +619,12 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
 
   int stage = 0;
 #pragma unroll 1
-  for (int u = first; u < last; ++u) {
+  for (int i = 0; i < mine; ++i) {
     copies_wait<R::STAGES - 2>();
     __syncwarp();                                // every lane's copies of this unit are there, and the last unit has been read
     const uint32_t at = ring + stage * R::STAGE;
-    fetch(u + R::STAGES - 1, stage == 0 ? R::STAGES - 1 : stage - 1);
+    const int u = first + i * nw;
+    fetch(i + R::STAGES - 1, stage == 0 ? R::STAGES - 1 : stage - 1);
     stage = stage + 1 == R::STAGES ? 0 : stage + 1;
     int base, live;
     place(u, base, live);
@@ -747,7 +759,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
       // the values behind it left out (the last one first, so that each leaves out more), and only its own columns take the sums.
       const int t0 = r0 / a.group, t1 = min((r0 + n_rows - 1) / a.group, n_new - 1);
       for (int tok = t1; tok >= t0; --tok) {
-        const int ends = (int)min(a.start[b] + tok + 1, (long long)len) - base;
+        const int ends = (int)min(start + tok + 1, (long long)len) - base;
         if (ends <= 0) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -782,81 +794,89 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
         *reinterpret_cast<float4*>(&s_o[warp][row][VB * g + 2 * i]) = make_float4(mean(o[nt][i][c]), mean(o[nt][i][2 + c]), mean(o[nt][i + 1][c]), mean(o[nt][i + 1][2 + c]));
     }
   __syncthreads();
-  // what the warps' means count for in the CTA's
-  if (threadIdx.x < ROWS) {
-    const int row = threadIdx.x;
-    float mm = LOWEST, ll = 0.f, w[WARPS];
+  // Four columns of a row per thread.  `joined4` adds up the warps' means by what they count for in the CTA's.
+  const long long row_at = (long long)b * a.heads * a.tokens + kh * all_rows + r0;
+  const int pieces = D / 4;
+  auto joined4 = [&](int row, int d, float& mm, float& ll) {
+    float w[WARPS];
+    mm = LOWEST;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) mm = fmaxf(mm, s_m[i][row]);
+    ll = 0.f;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) { w[i] = share(s_m[i][row], s_l[i][row], mm); ll += w[i]; }
+    const float f = ll == 0.f ? 0.f : 1.f / ll;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) s_l[i][row] = ll == 0.f ? 0.f : w[i] / ll;
-    s_cm[row] = mm;
-    s_cl[row] = ll;
-  }
-  __syncthreads();
-  const long long row_at = (long long)b * a.heads * a.tokens + kh * all_rows + r0;
-  auto result = [&](int row, int d, float mm, float ll, float acc) {
+    for (int i = 0; i < WARPS; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(&s_o[i][row][d]);
+      const float k = w[i] * f;
+      acc.x += k * v.x; acc.y += k * v.y; acc.z += k * v.z; acc.w += k * v.w;
+    }
+    return acc;
+  };
+  auto result = [&](int row, int d, float mm, float ll, float4 acc) {
     const int r = r0 + row, tok = a.tokens == 1 ? 0 : r / a.group, h = kh * a.group + r - tok * a.group;
-    const bool none = tok >= n_new || a.start[b] + tok < 0 || len == 0;
-    reinterpret_cast<T*>(a.out)[(((long long)b * a.tokens + tok) * a.heads + h) * D + d] = T(none ? 0.f : ll == 0.f ? NAN : acc);
+    const bool none = tok >= n_new || start + tok < 0 || len == 0;
+    if (none) acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    else if (ll == 0.f) acc = make_float4(NAN, NAN, NAN, NAN);
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (((long long)b * a.tokens + tok) * a.heads + h) * D + d) =
+        make_uint2(Typed<T>::pack(acc.x, acc.y), Typed<T>::pack(acc.z, acc.w));
     if (MASS && d == 0) {
       float* p = a.part_s + (row_at + row) * (a.clustered ? 1 : a.splits) * PART;
       p[0] = mm;
       p[1] = ll;
     }
   };
-  constexpr int AT_ONCE = WARPS * 32 / DP;                     // rows
-  const int d = threadIdx.x % DP, row1 = threadIdx.x / DP;
   if (!a.clustered || a.splits == 1) {
-    if (FULL || d < D) {
-      for (int row = row1; row < n_rows; row += AT_ONCE) {
-        float acc = 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) acc += s_l[w][row] * s_o[w][row][d];
-        if (parts == 1) {
-          result(row, d, s_cm[row], s_cl[row], acc);
-        } else {
-          const long long part = (row_at + row) * a.splits + z;
-          a.part_o[part * D + d] = acc;
-          if (d == 0) { a.part_s[part * PART] = s_cm[row]; a.part_s[part * PART + 1] = s_cl[row]; }
-        }
+    for (int i = threadIdx.x; i < n_rows * pieces; i += WARPS * 32) {
+      const int row = i / pieces, d = 4 * (i - row * pieces);
+      float mm, ll;
+      const float4 acc = joined4(row, d, mm, ll);
+      if (a.splits == 1) {
+        result(row, d, mm, ll, acc);
+      } else {
+        const long long part = (row_at + row) * a.splits + z;
+        *reinterpret_cast<float4*>(a.part_o + part * D + d) = acc;
+        if (d == 0) { a.part_s[part * PART] = mm; a.part_s[part * PART + 1] = ll; }
       }
     }
     return;
   }
-  if (FULL || d < D) {
-    for (int row = row1; row < n_rows; row += AT_ONCE) {
-      float acc = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) acc += s_l[w][row] * s_o[w][row][d];
-      s_o[0][row][d] = acc;                                    // read and written by this thread alone
-    }
+  for (int i = threadIdx.x; i < n_rows * pieces; i += WARPS * 32) {
+    const int row = i / pieces, d = 4 * (i - row * pieces);
+    float mm, ll;
+    const float4 acc = joined4(row, d, mm, ll);
+    *reinterpret_cast<float4*>(&s_o[0][row][d]) = acc;         // read and written by this thread alone
+    if (d == 0) { s_cm[row] = mm; s_cl[row] = ll; }
   }
   cluster_sync_all();
-  if (FULL || d < D) {
-    for (int row = z * AT_ONCE + row1; row < n_rows; row += a.splits * AT_ONCE) {
-      const uint32_t am = smem_u32(&s_cm[row]), al = smem_u32(&s_cl[row]), ao = smem_u32(&s_o[0][row][d]);
-      float pm[8], pl[8], po[8], mm = LOWEST, ll = 0.f, acc = 0.f;
+  for (int i = z * WARPS * 32 + threadIdx.x; i < n_rows * pieces; i += a.splits * WARPS * 32) {
+    const int row = i / pieces, d = 4 * (i - row * pieces);
+    const uint32_t am = smem_u32(&s_cm[row]), al = smem_u32(&s_cl[row]), ao = smem_u32(&s_o[0][row][d]);
+    float pm[8], pl[8], mm = LOWEST, ll = 0.f;
+    float4 po[8], acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (x < a.splits) {
-          pm[x] = ld_cluster_f32(map_to_cta(am, x));
-          pl[x] = ld_cluster_f32(map_to_cta(al, x));
-          po[x] = ld_cluster_f32(map_to_cta(ao, x));
-        }
+    for (int x = 0; x < 8; ++x)
+      if (x < a.splits) {
+        pm[x] = ld_cluster_f32(map_to_cta(am, x));
+        pl[x] = ld_cluster_f32(map_to_cta(al, x));
+        po[x] = ld_cluster_f32x4(map_to_cta(ao, x));
+      }
 #pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (x < a.splits) mm = fmaxf(mm, pm[x]);
+    for (int x = 0; x < 8; ++x)
+      if (x < a.splits) mm = fmaxf(mm, pm[x]);
 #pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (x < a.splits) { pl[x] = share(pm[x], pl[x], mm); ll += pl[x]; }
+    for (int x = 0; x < 8; ++x)
+      if (x < a.splits) { pl[x] = share(pm[x], pl[x], mm); ll += pl[x]; }
+    const float f = ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (x < a.splits) acc += ll == 0.f ? 0.f : pl[x] / ll * po[x];
-      result(row, d, mm, ll, acc);
-    }
+    for (int x = 0; x < 8; ++x)
+      if (x < a.splits) {
+        const float k = pl[x] * f;
+        acc.x += k * po[x].x; acc.y += k * po[x].y; acc.z += k * po[x].z; acc.w += k * po[x].w;
+      }
+    result(row, d, mm, ll, acc);
   }
   cluster_sync_all();                            // nobody leaves while its part is being read
 }
@@ -891,11 +911,10 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
   grid_dep_wait();
   const int b = blockIdx.y, D = kv.dim, bs = kv.block_size, rows = a.heads * a.tokens, all_rows = a.group * a.tokens;
   const int len = seen_by_last(a, kv, b), units = (len + bs - 1) / bs * a.per_page;
-  const int parts = a.clustered ? 1 : parts_of(a, units), room = a.clustered ? 1 : a.splits, lane = threadIdx.x & 31;
+  const int parts = a.clustered ? 1 : a.splits, lane = threadIdx.x & 31;
   if ((int)blockIdx.x < row_ctas) {
-    if (parts < 2) return;
     const int row = blockIdx.x, kh = row / all_rows, r = row - kh * all_rows, tok = r / a.group, h = kh * a.group + r - tok * a.group;
-    const long long at = ((long long)b * rows + row) * room;
+    const long long at = ((long long)b * rows + row) * parts;
     const Joined j = joined(a, at, parts, lane);
     const float f = j.sum == 0.f ? 0.f : 1.f / j.sum;
     const bool none = tok >= tokens_of(a.counts, b, a.tokens) || a.start[b] + tok < 0;
@@ -919,14 +938,14 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
     const int tok = (r % all_rows) / a.group;
     s_lse[r] = tok >= n_new || a.start[b] + tok < 0 ? INFINITY : sum == 0.f ? NAN : m + log2f(sum);
   };
-  if (room == 1) {
+  if (parts == 1) {
     for (int r = threadIdx.x; r < rows; r += 128) {
       const float* p = a.part_s + ((long long)b * rows + r) * PART;
       keep(r, p[0], p[1]);
     }
   } else {
     for (int r = threadIdx.x >> 5; r < rows; r += 4) {
-      const Joined j = joined(a, ((long long)b * rows + r) * room, parts, lane);
+      const Joined j = joined(a, ((long long)b * rows + r) * parts, parts, lane);
       if (lane == 0) keep(r, j.m, j.sum);
     }
   }
