@@ -69,7 +69,7 @@ __device__ __forceinline__ void note(int* status, int what) {
 
 // the page at position `page` of request b's row, or -1
 __device__ __forceinline__ int page_id(const FlKv8& kv, int b, int page) {
-  int id = __ldg(kv.block_table + (long long)b * kv.table_stride + page);
+  int id = __ldcg(kv.block_table + (long long)b * kv.table_stride + page);
   if (id < 0) id += kv.num_blocks;
   return id >= 0 && id < kv.num_blocks ? id : -1;
 }
@@ -381,6 +381,7 @@ struct AttArgs {
   int batch, tokens, heads, group, row_parts;
   int per_page;                            // steps of a page
   int splits, clustered;                   // CTAs per request, KV head and rows; whether they are a cluster
+  int early;                               // launched while the kernel before may still run
   float scale;                             // times log2 e
   void* out;
   float* part_o; float* part_s;            // [batch][heads * tokens][parts][dim] and [..][PART]; parts: splits, or 1 if they are a cluster
@@ -483,7 +484,6 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   auto s_o = reinterpret_cast<float(*)[ROWS][LD]>(s_ring);
   __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_cm[ROWS], s_cl[ROWS];
   grid_dep_launch();
-  grid_dep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int kh = blockIdx.x / a.row_parts, rp = blockIdx.x - kh * a.row_parts, b = blockIdx.y, z = blockIdx.z;
   const int D = FULL ? DP : kv.dim, bs = kv.block_size, all_rows = a.group * a.tokens, r0 = rp * ROWS;
@@ -495,6 +495,25 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
     const int u = u0 + lane * nw;
     return u < a.units ? page_id(kv, b, a.per_page == 1 ? u : u / a.per_page) : -1;
   };
+  if (a.early) {
+    // a look ahead, before the wait for the kernel that writes queries and the new tokens' pages: the first units asked into L2, a line per
+    // lane.  Whatever it finds only says what is worth having there; all of it is read again behind the wait.
+    const long long n = __ldcg(a.start + b) + a.tokens, bytes = (long long)16 * D;
+    const int id = look_up(first);
+#pragma unroll
+    for (int i = 0; i < R::STAGES - 1; ++i) {
+      const int u = first + i * nw, at = __shfl_sync(0xffffffffu, id, i);
+      const int page = a.per_page == 1 ? u : u / a.per_page, s0 = (u - page * a.per_page) * 16;
+      const long long byte = (lane & 15) * 128;
+      if (at >= 0 && (long long)page * bs + s0 < n && byte < bytes && s0 * D + byte < (long long)bs * D)
+      {
+        const long long cell = ((long long)kv.layer * kv.num_blocks + at) * kv.heads + kh;
+        prefetch_l2(reinterpret_cast<const uint8_t*>(lane < 16 ? kv.k : kv.v) + (cell * bs + s0) * D + byte);
+        if ((lane & 15) == 0) prefetch_l2((lane ? kv.v_scale : kv.k_scale) + cell);
+      }
+    }
+  }
+  grid_dep_wait();
   int ids = look_up(first);
   const long long start = a.start[b];
   const int n_new = tokens_of(a.counts, b, a.tokens);
@@ -524,6 +543,12 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   const uint8_t* vp = reinterpret_cast<const uint8_t*>(kv.v) + row0 * D + 16 * piece;
   const uint32_t ring = smem_u32(s_ring) + warp * R::STAGES * R::STAGE, cell0 = ring + row0 * R::PITCH + 16 * piece;
   const long long pool0 = (long long)kv.layer * kv.num_blocks;
+  const bool column = FULL || 16 * piece < D;
+  if (!column) {                               // columns that there are not: zeros, once
+    for (int s = 0; s < R::STAGES; ++s)
+      for (int i = 0; i < 32; i += PASS)
+        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(cell0 + s * R::STAGE + i * R::PITCH), "r"(0u) : "memory");
+  }
   // where a unit begins, and tokens of it that the request has
   auto place = [&](int u, int& base, int& live) {
     int page = u, s0 = 0;
@@ -543,20 +568,22 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
       if (id < 0) live = 0;
       const long long cell = (pool0 + max(id, 0)) * kv.heads + kh, at = (cell * bs + s0) * D;
       const uint32_t to = cell0 + stage * R::STAGE;
-      const bool column = FULL || 16 * piece < D;
-      if (FULL && live == 16) {
+      if (column) {
         const uint8_t *k = kp + at, *v = vp + at;
+        if (live == 16) {
 #pragma unroll
-        for (int i = 0; i < 16; i += PASS) {
-          copy16(to + i * R::PITCH, k + i * DP);
-          copy16(to + R::KEYS + i * R::PITCH, v + i * DP);
+          for (int i = 0; i < 16; i += PASS) {
+            copy16(to + i * R::PITCH, k + i * D);
+            copy16(to + R::KEYS + i * R::PITCH, v + i * D);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; i += PASS) {
+            const bool there = i + row0 < live;                  // the addresses of others may be anything
+            copy16(to + i * R::PITCH, there ? k + i * D : reinterpret_cast<const uint8_t*>(kv.k), there);
+            copy16(to + R::KEYS + i * R::PITCH, there ? v + i * D : reinterpret_cast<const uint8_t*>(kv.v), there);
+          }
         }
-      } else
-#pragma unroll
-      for (int i = 0; i < 16; i += PASS) {
-        const bool there = column && i + row0 < live;           // the addresses of others may be anything
-        copy16(to + i * R::PITCH, there ? kp + at + i * D : reinterpret_cast<const uint8_t*>(kv.k), there);
-        copy16(to + R::KEYS + i * R::PITCH, there ? vp + at + i * D : reinterpret_cast<const uint8_t*>(kv.v), there);
       }
       if (lane < 2) copy4(ring + stage * R::STAGE + R::SCALES + 4 * lane, (lane ? kv.v_scale : kv.k_scale) + cell, id >= 0);
     }
@@ -1298,6 +1325,7 @@ extern "C" int fl_kv8_attention(int dtype, const void* q, long long stride_b, lo
   if (mass) a.unit_s = reinterpret_cast<float*>(s);
   const dim3 grid(kv->heads * c.row_parts, batch, c.splits);
   const bool early = (long long)batch * tokens <= FL_THIN_MAX_ROWS;
+  a.early = early;
   int rc = 0;
   FL_KV8_TYPES(dtype, rc = kv->dim <= 64 ? launch_attention<T, 64>(a, *kv, c.nt, mass != nullptr, grid, early, stream)
                                          : launch_attention<T, 128>(a, *kv, c.nt, mass != nullptr, grid, early, stream));
