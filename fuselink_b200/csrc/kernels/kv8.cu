@@ -385,7 +385,7 @@ struct AttArgs {
   float scale;                             // times log2 e
   void* out;
   float* part_o; float* part_s;            // [batch][heads * tokens][parts][dim] and [..][PART]; parts: splits, or 1 if they are a cluster
-  float* unit_s;                           // [batch][steps of a full table][heads * tokens]: log2 of the weights' sum; null: not asked for
+  float2* unit_s;                          // [batch][steps of a full table][heads * tokens]: the weights' sum, and the maximum that they refer to; null: not asked for
   int units;                               // steps of a full table
 };
 
@@ -406,11 +406,6 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) {
 __device__ __forceinline__ float exp2_fast(float x) {                     // the hardware's: 2^-22 off, relatively; 0 below 2^-126
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float log2_fast(float x) {                     // the hardware's: 2^-22 off; -inf of 0
-  float r;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 // over the lane groups (the rows of a product), for every quad lane
@@ -749,9 +744,9 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
       if (MASS) {
         const float s0 = sum_rows(add[0]), s1 = sum_rows(add[1]);
         if (g == 0) {
-          float* w = a.unit_s + ((long long)b * a.units + u) * a.heads * a.tokens + kh * all_rows + r0 + 8 * nt + 2 * t;
-          if (8 * nt + 2 * t < n_rows) w[0] = m[nt][0] + log2_fast(s0);
-          if (8 * nt + 2 * t + 1 < n_rows) w[1] = m[nt][1] + log2_fast(s1);
+          float2* w = a.unit_s + ((long long)b * a.units + u) * a.heads * a.tokens + kh * all_rows + r0 + 8 * nt + 2 * t;
+          if (8 * nt + 2 * t < n_rows) w[0] = make_float2(s0, m[nt][0]);
+          if (8 * nt + 2 * t + 1 < n_rows) w[1] = make_float2(s1, m[nt][1]);
         }
       }
     }
@@ -959,11 +954,11 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
     return;
   }
   if (mass == nullptr || len == 0) return;
-  extern __shared__ float s_lse[];                           // log2 of every row's sum of weights; inf: a row that sees nothing
+  extern __shared__ float2 s_row[];                          // of every row: the maximum, and 1 / its sum of weights (0: a row that sees nothing)
   const int n_new = tokens_of(a.counts, b, a.tokens);
   auto keep = [&](int r, float m, float sum) {
     const int tok = (r % all_rows) / a.group;
-    s_lse[r] = tok >= n_new || a.start[b] + tok < 0 ? INFINITY : sum == 0.f ? NAN : m + log2f(sum);
+    s_row[r] = make_float2(m, tok >= n_new || a.start[b] + tok < 0 ? 0.f : sum == 0.f ? NAN : 1.f / sum);
   };
   if (parts == 1) {
     for (int r = threadIdx.x; r < rows; r += 128) {
@@ -981,8 +976,8 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
   for (int p = (blockIdx.x - row_ctas) * 4 + (threadIdx.x >> 5); p < pages; p += page_ctas * 4) {
     float sum = 0.f;
     for (int i = 0; i < a.per_page; ++i) {
-      const float* w = a.unit_s + ((long long)b * a.units + p * a.per_page + i) * rows;
-      for (int r = lane; r < rows; r += 32) sum += exp2_fast(w[r] - s_lse[r]);          // 0 where the row sees nothing
+      const float2* w = a.unit_s + ((long long)b * a.units + p * a.per_page + i) * rows;
+      for (int r = lane; r < rows; r += 32) sum += w[r].x * exp2_fast(w[r].y - s_row[r].x) * s_row[r].y;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -1291,26 +1286,46 @@ int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, int nt, bool ma
 }
 }  // namespace
 
+// More requests than a grid's second dimension takes go in several launches, which use the same scratch one after the other.
+constexpr int MOST_REQUESTS = 65535;
+
 extern "C" long long fl_kv8_attention_scratch(int batch, int tokens, int heads, const FlKv8* kv, int mass) {
   if (!sizes_fit(kv) || batch < 1 || tokens < 1 || heads < 1 || heads % kv->heads) return 0;
+  if (batch > MOST_REQUESTS) {
+    const long long whole = fl_kv8_attention_scratch(MOST_REQUESTS, tokens, heads, kv, mass);
+    const long long rest = fl_kv8_attention_scratch(batch % MOST_REQUESTS, tokens, heads, kv, mass);
+    return whole > rest ? whole : rest;
+  }
   const Cut c = cut_of(batch, tokens, heads, kv);
   const long long rows = (long long)batch * heads * tokens, parts = c.clustered ? 1 : c.splits;
   long long bytes = 0;
   if (!c.clustered) bytes += up16(rows * parts * kv->dim * 4);
   if (!c.clustered || mass) bytes += up16(rows * parts * fl::kv8::PART * 4);
-  if (mass) bytes += up16(rows * c.units * 4);
+  if (mass) bytes += up16(rows * c.units * 8);
   return bytes;
 }
 
 extern "C" int fl_kv8_attention(int dtype, const void* q, long long stride_b, long long stride_t, long long stride_h, const long long* start,
                                 const long long* counts, int batch, int tokens, int heads, float scale, const FlKv8* kv, void* out, float* mass,
                                 void* scratch, cudaStream_t stream) {
-  if (!sizes_fit(kv) || kv->layer < 0 || kv->layer >= kv->layers || batch < 0 || batch > 65535 || tokens < 0 || heads < 1 || heads % kv->heads ||
+  if (!sizes_fit(kv) || kv->layer < 0 || kv->layer >= kv->layers || batch < 0 || tokens < 0 || heads < 1 || heads % kv->heads ||
       (long long)heads * tokens > 0x3fffffffll || stride_b % 8 || stride_t % 8 || stride_h % 8)
     return -2;
-  if (mass != nullptr && (long long)heads * tokens > 12 * 1024) return -2;         // rows whose sums a CTA keeps in shared memory
+  if (mass != nullptr && (long long)heads * tokens > FL_KV8_MASS_ROWS) return -2;   // a CTA of the kernel that adds them up keeps each one's sum in shared memory
   if (!aligned({q, out, scratch, kv->k, kv->v})) return -4;
   if (batch == 0 || tokens == 0) return 0;
+  if (batch > MOST_REQUESTS) {
+    if (dtype != FL_DEC_BF16 && dtype != FL_DEC_FP16) return -1;
+    for (long long b = 0; b < batch; b += MOST_REQUESTS) {
+      FlKv8 part = *kv;
+      part.block_table += b * kv->table_stride;
+      const int n = (int)(batch - b < MOST_REQUESTS ? batch - b : MOST_REQUESTS);
+      const int rc = fl_kv8_attention(dtype, (const uint8_t*)q + 2 * b * stride_b, stride_b, stride_t, stride_h, start + b, counts ? counts + b : nullptr, n, tokens, heads,
+                                      scale, &part, (uint8_t*)out + 2 * b * tokens * heads * kv->dim, mass ? mass + b * kv->table_stride : nullptr, scratch, stream);
+      if (rc != 0) return rc;
+    }
+    return 0;
+  }
   const Cut c = cut_of(batch, tokens, heads, kv);
   const long long rows = (long long)batch * heads * tokens, parts = c.clustered ? 1 : c.splits;
   fl::kv8::AttArgs a = {};
@@ -1322,7 +1337,7 @@ extern "C" int fl_kv8_attention(int dtype, const void* q, long long stride_b, lo
   uint8_t* s = reinterpret_cast<uint8_t*>(scratch);
   if (!c.clustered) { a.part_o = reinterpret_cast<float*>(s); s += up16(rows * parts * kv->dim * 4); }
   if (!c.clustered || mass) { a.part_s = reinterpret_cast<float*>(s); s += up16(rows * parts * fl::kv8::PART * 4); }
-  if (mass) a.unit_s = reinterpret_cast<float*>(s);
+  if (mass) a.unit_s = reinterpret_cast<float2*>(s);
   const dim3 grid(kv->heads * c.row_parts, batch, c.splits);
   const bool early = (long long)batch * tokens <= FL_THIN_MAX_ROWS;
   a.early = early;
@@ -1336,7 +1351,7 @@ extern "C" int fl_kv8_attention(int dtype, const void* q, long long stride_b, lo
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(row_ctas + page_ctas, batch, 1);
   cfg.blockDim = dim3(128, 1, 1);
-  cfg.dynamicSmemBytes = mass ? (size_t)heads * tokens * 4 : 0;
+  cfg.dynamicSmemBytes = mass ? (size_t)heads * tokens * sizeof(float2) : 0;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -14,6 +14,8 @@ struct FlKv8 {
   int* status;                                 // FlDecStatus, or null
 };
 
+constexpr int FL_KV8_MASS_ROWS = 6 * 1024;   // new tokens times heads of a call that asks for pages' weights
+
 // dim: a multiple of 16, at most 128.  Tensors start at a multiple of 16 bytes.  Calls return 0, a cudaError, or < 0 for arguments they do
 // not take (-1 type, -2 sizes, -4 addresses); nothing is launched then.
 #ifdef __cplusplus
@@ -31,7 +33,7 @@ int fl_kv8_pack(int dtype, const void* k_pool, const void* v_pool, int src_block
                 int batch, const FlKv8* kv, cudaStream_t stream);
 // out [batch][tokens][heads * dim] = softmax(scale q k^T) v of tokens start[b] .. start[b] + counts[b] - 1 (counts null: `tokens` of them) over the
 // slots up to their own; zeros where there is none.  q: element strides of (request, token, head).  mass (or null): [batch][table_stride], += the
-// weights' sum over this call's tokens and heads, page by page.
+// weights' sum over this call's tokens and heads, page by page; tokens * heads is at most FL_KV8_MASS_ROWS then.
 // scratch: fl_kv8_attention_scratch() bytes, from a multiple of 16 on.
 long long fl_kv8_attention_scratch(int batch, int tokens, int heads, const FlKv8* kv, int mass);
 int fl_kv8_attention(int dtype, const void* q, long long stride_b, long long stride_t, long long stride_h, const long long* start,

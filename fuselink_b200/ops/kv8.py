@@ -101,7 +101,8 @@ def attention(cache: Kv8Cache, layer: int, q: torch.Tensor, block_table: torch.T
     """Attention of new tokens over the cache, their own keys and values (already written) among it: q [batch, tokens, heads, dim], of any strides that
     are multiples of 8 elements; token t of request b sees slots 0 .. start[b] + t.  Returns [batch, tokens, heads * dim]; zeros for tokens behind
     ``counts`` and for those that see nothing.  scale: 1 / sqrt(dim) by default.
-    mass ([batch, pages] fp32) has the weights' sum over this call's tokens and heads added, page by page of ``block_table``."""
+    mass ([batch, pages] fp32) has the weights' sum over this call's tokens and heads added, page by page of ``block_table``; on the GPU such a call
+    takes up to 6144 tokens times heads."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if q.is_cuda:

@@ -294,7 +294,7 @@ def test_c_entries_refuse_sizes(lib):
     def attend(dtype=0, strides=(64, 64, 64), batch=1, tokens=1, heads=4, mass=None):
         return lib.fl_kv8_attention(I(dtype), P(A0), *map(LL, strides), P(8), P(), I(batch), I(tokens), I(heads), F32(1), _kv(), P(A0), P(mass), P(A0), P())
 
-    for kw in (dict(strides=(4, 64, 64)), dict(strides=(64, 60, 64)), dict(strides=(64, 64, 65)), dict(batch=65536), dict(batch=-1), dict(tokens=-1), dict(heads=3), dict(heads=0),
+    for kw in (dict(strides=(4, 64, 64)), dict(strides=(64, 60, 64)), dict(strides=(64, 64, 65)), dict(batch=-1), dict(tokens=-1), dict(heads=3), dict(heads=0),
                dict(tokens=1 << 30), dict(tokens=4000, mass=8)):
         assert attend(**kw) == -2
     assert attend(dtype=7) == -1 and attend(batch=0) == 0 and attend(tokens=0) == 0
@@ -323,5 +323,5 @@ def test_scratch_covers_every_part(lib):
     for batch, tokens, heads, stride in ((1, 1, 8, 4), (2, 1, 32, 8192), (3, 5, 16, 100), (64, 1, 8, 512)):
         kv = _kv(stride=stride, heads=8, dim=128)
         plain, mass = (lib.fl_kv8_attention_scratch(I(batch), I(tokens), I(heads), kv, I(m)) for m in (0, 1))
-        assert plain % 16 == 0 and mass >= plain + 4 * batch * tokens * heads * stride
+        assert plain % 16 == 0 and mass >= plain + 8 * batch * tokens * heads * stride
     assert math.isfinite(plain)

@@ -409,6 +409,24 @@ def test_a_pool_beyond_32_bits():
     assert (_values(cache.k[2, 49999], cache.k_scale[2, 49999]).transpose(0, 1) - rows[0, :16, 16: 24].double()).abs().max() <= 2.0 ** -4 * rows.abs().max()
 
 
+def test_more_requests_than_a_grid_is_high():
+    """70000 requests of one page of eight slots, of which they have used one to eight, with weights; the last ones as much as the first."""
+    from fuselink_b200.ops import kv8
+    B, bs = 70000, 8
+    cache = _cache(1, 100, 1, bs, 16)
+    table = torch.randint(0, 100, (B, 1), generator=_gen(1), device="cuda").int()
+    start = torch.arange(B, device="cuda") % bs
+    q, mass = _randn(B, 1, 2, 16, seed=4, dt=BF), torch.zeros(B, 1, device="cuda")
+    out = kv8.attention(cache, 0, q, table, start, mass=mass).view(B, 2, 16)
+    k, v = (_values(c[0, table[:, 0].long(), 0], s[0, table[:, 0].long(), 0]) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    x = torch.einsum("bhd,bnd->bhn", q[:, 0].double(), k) / 4
+    x = torch.where(torch.arange(bs, device="cuda") <= start[:, None, None], x, torch.full_like(x, -math.inf))
+    want = torch.einsum("bhn,bnd->bhd", x.softmax(-1), v)
+    # as _want_attention: weights of 11 bits, the result's rounding, scores of sums of 16 products
+    assert ((out.double() - want).abs() <= (2.0 ** -11 + 2.0 ** -16) * v.abs().amax((1, 2))[:, None, None] + 2.0 ** -8 * want.abs()).all()
+    assert ((mass - 2).abs() <= 2.0 ** -18).all()
+
+
 # ---- eviction --------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("pages,bs,lens,keep,recent,sinks", [
     (8, 16, [128, 100, 1, 0, 17], 4, 1, 0), (145, 16, [145 * 16 - 3] * 7, 144, 4, 1), (2000, 8, [16000, 9000, 8001], 1000, 3, 2),
