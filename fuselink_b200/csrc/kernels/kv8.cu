@@ -379,14 +379,14 @@ struct AttArgs {
   const void* q; long long sb, st, sh;
   const long long* start; const long long* counts;
   int batch, tokens, heads, group, row_parts;
-  int per_page;                            // steps of a page
+  int per_page;                            // steps of a page, or halves of steps
   int splits, clustered;                   // CTAs per request, KV head and rows; whether they are a cluster
   int early;                               // launched while the kernel before may still run
   float scale;                             // times log2 e
   void* out;
   float* part_o; float* part_s;            // [batch][heads * tokens][parts][dim] and [..][PART]; parts: splits, or 1 if they are a cluster
-  float2* unit_s;                          // [batch][steps of a full table][heads * tokens]: the weights' sum, and the maximum that they refer to; null: not asked for
-  int units;                               // steps of a full table
+  float2* unit_s;                          // [batch][units][heads * tokens]: the weights' sum, and the maximum that they refer to; null: not asked for
+  int units;                               // of a full table: steps, or halves of them
 };
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -470,7 +470,9 @@ __device__ __forceinline__ int seen_by_last(const AttArgs& a, const FlKv8& kv, i
 // parts' outputs are means (divided by their sums), so that joining them overflows nowhere
 __device__ __forceinline__ float share(float m, float l, float mm) { return l == 0.f ? 0.f : exp2f(m - mm) * l; }      // 0: a part without weight; not one whose sum is NaN
 
-template <typename T, int DP, int NT, bool FULL, bool MASS>   // DP: head dimension rounded up to 64 or 128; FULL: it is that
+// DP: head dimension rounded up to 64 or 128.  FULL: it is that, in pages of whole 16s.  HALVES: pages that are not, whose steps are two halves of up to
+// eight tokens, from pages and with scales of their own: with steps of one page, pages of 8 took 1.9 times and pages of 5 three times as long.
+template <typename T, int DP, int NT, bool FULL, bool HALVES, bool MASS>
 __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(const AttArgs a, const FlKv8 kv) {
   using R = Ring<DP>;
   constexpr int KJ = DP / 64, MT = DP / 16, VB = DP / 8, ROWS = 8 * NT, LD = DP + 4;
@@ -486,30 +488,39 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   // The warp's units: every nw-th.  Which pages these are does not depend on the context's length, nor do the queries, so that all three are on
   // their way side by side.
   const int nw = a.splits * WARPS, first = z * WARPS + warp;
-  auto look_up = [&](int u0) {                 // lane i: the page of unit u0 + i nw
-    const int u = u0 + lane * nw;
-    return u < a.units ? page_id(kv, b, a.per_page == 1 ? u : u / a.per_page) : -1;
+  constexpr int H = HALVES ? 2 : 1;            // parts of a unit that have a page of their own, each of SIZE tokens at most
+  constexpr int SIZE = 16 / H;
+  struct Ids { int of[H]; };
+  auto look_up = [&](int u0) {                 // lane i: the pages of unit u0 + i nw
+    Ids ids;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int part = (u0 + lane * nw) * H + h;
+      ids.of[h] = part < a.units ? page_id(kv, b, a.per_page == 1 ? part : part / a.per_page) : -1;
+    }
+    return ids;
   };
   if (a.early) {
     // a look ahead, before the wait for the kernel that writes queries and the new tokens' pages: the first units asked into L2, a line per
     // lane.  Whatever it finds only says what is worth having there; all of it is read again behind the wait.
-    const long long n = __ldcg(a.start + b) + a.tokens, bytes = (long long)16 * D;
-    const int id = look_up(first);
+    const long long n = __ldcg(a.start + b) + a.tokens, bytes = (long long)SIZE * D;
+    const Ids ahead = look_up(first);
 #pragma unroll
-    for (int i = 0; i < R::STAGES - 1; ++i) {
-      const int u = first + i * nw, at = __shfl_sync(0xffffffffu, id, i);
-      const int page = a.per_page == 1 ? u : u / a.per_page, s0 = (u - page * a.per_page) * 16;
-      const long long byte = (lane & 15) * 128;
-      if (at >= 0 && (long long)page * bs + s0 < n && byte < bytes && s0 * D + byte < (long long)bs * D)
-      {
-        const long long cell = ((long long)kv.layer * kv.num_blocks + at) * kv.heads + kh;
-        prefetch_l2(reinterpret_cast<const uint8_t*>(lane < 16 ? kv.k : kv.v) + (cell * bs + s0) * D + byte);
-        if ((lane & 15) == 0) prefetch_l2((lane ? kv.v_scale : kv.k_scale) + cell);
+    for (int i = 0; i < R::STAGES - 1; ++i)
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const int part = (first + i * nw) * H + h, id = __shfl_sync(0xffffffffu, ahead.of[h], i);
+        const int page = a.per_page == 1 ? part : part / a.per_page, s0 = (part - page * a.per_page) * SIZE;
+        const long long byte = (lane & 15) * 128;
+        if (id >= 0 && (long long)page * bs + s0 < n && byte < bytes && s0 * D + byte < (long long)bs * D) {
+          const long long cell = ((long long)kv.layer * kv.num_blocks + id) * kv.heads + kh;
+          prefetch_l2(reinterpret_cast<const uint8_t*>(lane < 16 ? kv.k : kv.v) + (cell * bs + s0) * D + byte);
+          if ((lane & 15) == 0) prefetch_l2((lane ? kv.v_scale : kv.k_scale) + cell);
+        }
       }
-    }
   }
   grid_dep_wait();
-  int ids = look_up(first);
+  Ids ids = look_up(first);
   const long long start = a.start[b];
   const int n_new = tokens_of(a.counts, b, a.tokens);
   uint4 q_raw[NT][KJ][2];
@@ -528,7 +539,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
     }
   }
   const int len = n_new == 0 ? 0 : (int)min(max(start + n_new, 0ll), (long long)kv.table_stride * bs);
-  const int units = (len + bs - 1) / bs * a.per_page;
+  const int units = ((len + bs - 1) / bs * a.per_page + H - 1) / H;
   const int mine = first < units ? (units - first + nw - 1) / nw : 0;
 
   // this lane's 16 bytes of a row, in every PASS-th row
@@ -544,43 +555,51 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
       for (int i = 0; i < 32; i += PASS)
         asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(cell0 + s * R::STAGE + i * R::PITCH), "r"(0u) : "memory");
   }
-  // where a unit begins, and tokens of it that the request has
-  auto place = [&](int u, int& base, int& live) {
-    int page = u, s0 = 0;
-    if (a.per_page > 1) { page = u / a.per_page; s0 = (u - page * a.per_page) * 16; }
-    base = page * bs + s0;
-    live = min(min(bs - s0, len - base), 16);
-    return s0;
+  // where a unit's parts begin, and tokens of them that the request has (none or fewer: it has not got that far)
+  struct Place { int base[H], live[H], s0[H]; };
+  auto place = [&](int u) {
+    Place p;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      int page = u * H + h;
+      p.s0[h] = 0;
+      if (a.per_page > 1) { const int part = page; page /= a.per_page; p.s0[h] = (part - page * a.per_page) * SIZE; }
+      p.base[h] = page * bs + p.s0[h];
+      p.live[h] = min(min(bs - p.s0[h], len - p.base[h]), SIZE);
+    }
+    return p;
   };
   auto fetch = [&](int i, int stage) {         // the warp's i-th unit; every lane calls it, i by i; an empty group behind the last
     if (i < mine) {
       const int u = first + i * nw;
       if (i > 0 && i % 32 == 0) ids = look_up(u);
-      const int id = __shfl_sync(0xffffffffu, ids, i % 32);
-      int base, live;
-      const int s0 = place(u, base, live);
-      if (id < 0 && lane == 0) note(kv.status, FL_DEC_BAD_PAGE);
-      if (id < 0) live = 0;
-      const long long cell = (pool0 + max(id, 0)) * kv.heads + kh, at = (cell * bs + s0) * D;
-      const uint32_t to = cell0 + stage * R::STAGE;
-      if (column) {
-        const uint8_t *k = kp + at, *v = vp + at;
-        if (live == 16) {
+      Place p = place(u);
 #pragma unroll
-          for (int i = 0; i < 16; i += PASS) {
-            copy16(to + i * R::PITCH, k + i * D);
-            copy16(to + R::KEYS + i * R::PITCH, v + i * D);
-          }
-        } else {
+      for (int h = 0; h < H; ++h) {
+        const int id = __shfl_sync(0xffffffffu, ids.of[h], i % 32);
+        if (id < 0 && p.live[h] > 0 && lane == 0) note(kv.status, FL_DEC_BAD_PAGE);
+        if (id < 0) p.live[h] = 0;
+        const long long cell = (pool0 + max(id, 0)) * kv.heads + kh, at = (cell * bs + p.s0[h]) * D;
+        const uint32_t to = cell0 + stage * R::STAGE + h * SIZE * R::PITCH;
+        if (column) {
+          const uint8_t *k = kp + at, *v = vp + at;
+          if (p.live[h] == SIZE) {
 #pragma unroll
-          for (int i = 0; i < 16; i += PASS) {
-            const bool there = i + row0 < live;                  // the addresses of others may be anything
-            copy16(to + i * R::PITCH, there ? k + i * D : reinterpret_cast<const uint8_t*>(kv.k), there);
-            copy16(to + R::KEYS + i * R::PITCH, there ? v + i * D : reinterpret_cast<const uint8_t*>(kv.v), there);
+            for (int j = 0; j < SIZE; j += PASS) {
+              copy16(to + j * R::PITCH, k + j * D);
+              copy16(to + R::KEYS + j * R::PITCH, v + j * D);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < SIZE; j += PASS) {
+              const bool there = j + row0 < p.live[h];           // the addresses of others may be anything
+              copy16(to + j * R::PITCH, there ? k + j * D : reinterpret_cast<const uint8_t*>(kv.k), there);
+              copy16(to + R::KEYS + j * R::PITCH, there ? v + j * D : reinterpret_cast<const uint8_t*>(kv.v), there);
+            }
           }
         }
+        if (lane < 2) copy4(ring + stage * R::STAGE + R::SCALES + 8 * h + 4 * lane, (lane ? kv.v_scale : kv.k_scale) + cell, id >= 0);
       }
-      if (lane < 2) copy4(ring + stage * R::STAGE + R::SCALES + 4 * lane, (lane ? kv.v_scale : kv.k_scale) + cell, id >= 0);
     }
     copies_commit();
   };
@@ -648,11 +667,17 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
     const int u = first + i * nw;
     fetch(i + R::STAGES - 1, stage == 0 ? R::STAGES - 1 : stage - 1);
     stage = stage + 1 == R::STAGES ? 0 : stage + 1;
-    int base, live;
-    place(u, base, live);
-    const uint2 scales = lds_v2(at + R::SCALES);
-    const float ks = __uint_as_float(scales.x), vs = __uint_as_float(scales.y);
-    if (ks == 0.f) live = 0;                     // a page that is not there
+    const Place p = place(u);
+    int base[H], live[H];
+    float ks[H], vs[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const uint2 scales = lds_v2(at + R::SCALES + 8 * h);
+      ks[h] = __uint_as_float(scales.x);
+      vs[h] = __uint_as_float(scales.y);
+      base[h] = p.base[h];
+      live[h] = ks[h] == 0.f ? 0 : p.live[h];    // 0: a page that is not there
+    }
     float s[NT][4], s2[NT][4];                   // two chains of products
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -686,31 +711,41 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
         v[i][0] = w.x; v[i][1] = w.y;
       }
     }
-    const bool cut = live < 16 || base + 16 > fewest;          // some column does not see some of the 16
-    if (cut) {
+    // tokens g and g + 8: the unit's only part, or one each
+    constexpr int H1 = H - 1;
+    const bool seen = base[0] + SIZE <= fewest && base[H1] + SIZE <= fewest;         // by every column
+    if (!seen || live[0] < SIZE || live[H1] < SIZE) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int ends = min(sees[nt][c] - base, live);
-          s[nt][c] = g < ends ? s[nt][c] : -INFINITY;
-          s[nt][2 + c] = g + 8 < ends ? s[nt][2 + c] : -INFINITY;
+          s[nt][c] = g < min(sees[nt][c] - base[0], live[0]) ? s[nt][c] : -INFINITY;
+          s[nt][2 + c] = g + 8 - 8 * H1 < min(sees[nt][c] - base[H1], live[H1]) ? s[nt][2 + c] : -INFINITY;
         }
     }
-    const float page_unit = (float)((int)(__float_as_uint(vs) >> 23) - 127);
-    bool beyond = page_unit > unit && live > 0;
+    float page_unit[H];
+    bool beyond = false;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      page_unit[h] = (float)((int)(__float_as_uint(vs[h]) >> 23) - 127);
+      beyond |= page_unit[h] > unit && live[h] > 0;
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         // -inf stays -inf whatever it meets: a factor of 0 (an underflow, or no page) would make it NaN
-        const float k = fmaxf(factor[nt][c] * ks, 0x1p-126f), top = m[nt][c] + SLACK;
-        s[nt][c] *= k;
-        s[nt][2 + c] *= k;
+        const float k0 = fmaxf(factor[nt][c] * ks[0], 0x1p-126f), k1 = HALVES ? fmaxf(factor[nt][c] * ks[H1], 0x1p-126f) : k0, top = m[nt][c] + SLACK;
+        s[nt][c] *= k0;
+        s[nt][2 + c] *= k1;
         beyond |= s[nt][c] > top || s[nt][2 + c] > top;
       }
     if (__any_sync(0xffffffffu, beyond)) {
-      const float unit_now = live > 0 ? fmaxf(unit, page_unit) : unit, shrink = exp2_fast(unit - unit_now);
+      float unit_now = unit;
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+        if (live[h] > 0) unit_now = fmaxf(unit_now, page_unit[h]);
+      const float shrink = exp2_fast(unit - unit_now);
       unit = unit_now;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -742,21 +777,33 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
         l[nt][c] += add[c];
       }
       if (MASS) {
-        const float s0 = sum_rows(add[0]), s1 = sum_rows(add[1]);
-        if (g == 0) {
-          float2* w = a.unit_s + ((long long)b * a.units + u) * a.heads * a.tokens + kh * all_rows + r0 + 8 * nt + 2 * t;
-          if (8 * nt + 2 * t < n_rows) w[0] = make_float2(s0, m[nt][0]);
-          if (8 * nt + 2 * t + 1 < n_rows) w[1] = make_float2(s1, m[nt][1]);
+        auto keep = [&](int part, float s0, float s1) {
+          s0 = sum_rows(s0);
+          s1 = sum_rows(s1);
+          if (g == 0 && part < a.units) {
+            float2* w = a.unit_s + ((long long)b * a.units + part) * a.heads * a.tokens + kh * all_rows + r0 + 8 * nt + 2 * t;
+            if (8 * nt + 2 * t < n_rows) w[0] = make_float2(s0, m[nt][0]);
+            if (8 * nt + 2 * t + 1 < n_rows) w[1] = make_float2(s1, m[nt][1]);
+          }
+        };
+        if (HALVES) {
+          keep(2 * u, s[nt][0], s[nt][1]);
+          keep(2 * u + 1, s[nt][2], s[nt][3]);
+        } else {
+          keep(u, add[0], add[1]);
         }
       }
     }
-    if (page_unit < unit) {                                      // a page of smaller values than the largest
-      const float w = exp2_fast(page_unit - unit);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int h = 0; h < H; ++h)
+      if (page_unit[h] < unit) {                                   // a page of smaller values than the largest
+        const float w = exp2_fast(page_unit[h] - unit);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[nt][i] *= w;
-    }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!HALVES || i / 2 == h) s[nt][i] *= w;
+      }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       p0[nt] = transposed(half2_of(s[nt][0], s[nt][1]));
@@ -774,20 +821,20 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
           for (int nt = 0; nt < NT; ++nt) each(nt, 2 * w + h, h0.x, h0.y, h1.x, h1.y);
         }
     };
-    if (a.tokens == 1 || base + 16 <= fewest) {
+    if (a.tokens == 1 || seen) {
       values([&](int nt, int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) { mma(o[nt][i], a0, a1, a2, a3, p0[nt], p1[nt]); });
     } else {
       // Among the last tokens a column's weight of 0 must not meet a value of a later token, which may be NaN: one new token at a time, with
       // the values behind it left out (the last one first, so that each leaves out more), and only its own columns take the sums.
       const int t0 = r0 / a.group, t1 = min((r0 + n_rows - 1) / a.group, n_new - 1);
       for (int tok = t1; tok >= t0; --tok) {
-        const int ends = (int)min(start + tok + 1, (long long)len) - base;
-        if (ends <= 0) break;
+        const int sees_now = (int)min(start + tok + 1, (long long)len);
+        if (sees_now <= base[0]) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int w = 0; w < DP / 32; ++w)
-            if (2 * t + (i & 1) + 8 * (i >> 1) >= ends) v[i][w] = 0;
+            if (2 * t + (i & 1) + (HALVES ? 0 : 8 * (i >> 1)) >= sees_now - base[HALVES ? i >> 1 : 0]) v[i][w] = 0;
         values([&](int nt, int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
           float c[4] = {0.f, 0.f, 0.f, 0.f};
           mma(c, a0, a1, a2, a3, p0[nt], p1[nt]);
@@ -1228,18 +1275,21 @@ extern "C" int fl_kv8_pack(int dtype, const void* k_pool, const void* v_pool, in
 
 // How a call is cut up: enough CTAs for the SMs (four of NT = 1, two of NT = 2 each), as a cluster where 8 per request and KV head are enough.
 namespace {
-struct Cut { int nt, row_parts, per_page, units, splits; bool clustered; };
+struct Cut { int nt, row_parts, per_page, units, splits; bool halves, clustered; };
 Cut cut_of(int batch, int tokens, int heads, const FlKv8* kv) {
   Cut c;
   const long long rows = (long long)heads / kv->heads * tokens;
   c.nt = rows > 8 ? 2 : 1;
   c.row_parts = (int)((rows + 8 * c.nt - 1) / (8 * c.nt));
-  c.per_page = (kv->block_size + 15) / 16;
+  c.halves = kv->block_size % 16 != 0;
+  const int size = c.halves ? 8 : 16;
+  c.per_page = (kv->block_size + size - 1) / size;
   c.units = kv->table_stride * c.per_page;
+  const int steps = c.halves ? (c.units + 1) / 2 : c.units;
   const long long ctas = (long long)batch * kv->heads * c.row_parts, want = 148ll * (c.nt == 1 ? 4 : 2);
-  const long long most = (c.units + fl::kv8::FEWEST - 1) / fl::kv8::FEWEST;
+  const long long most = (steps + fl::kv8::FEWEST - 1) / fl::kv8::FEWEST;
   long long splits = want / (ctas < 1 ? 1 : ctas);
-  const long long even = (c.units + fl::kv8::LONGEST - 1) / fl::kv8::LONGEST;
+  const long long even = (steps + fl::kv8::LONGEST - 1) / fl::kv8::LONGEST;
   if (splits < even) splits = even;
   if (splits > most) splits = most;
   if (splits > fl::kv8::MOST_PARTS) splits = fl::kv8::MOST_PARTS;
@@ -1250,7 +1300,7 @@ Cut cut_of(int batch, int tokens, int heads, const FlKv8* kv) {
 }
 long long up16(long long bytes) { return (bytes + 15) / 16 * 16; }
 
-template <typename T, int DP, int NT, bool FULL, bool MASS>
+template <typename T, int DP, int NT, bool FULL, bool HALVES, bool MASS>
 int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, dim3 grid, bool early, cudaStream_t stream) {
   constexpr int smem = fl::kv8::Ring<DP>::BYTES;
   static bool set_on[64];                          // per device: a process may drive several GPUs
@@ -1259,7 +1309,7 @@ int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, dim3 grid, bool
   if (e != cudaSuccess) return (int)e;
   if (dev < 0 || dev >= 64) return -3;
   if (!set_on[dev]) {
-    e = cudaFuncSetAttribute(fl::kv8::attention_kernel<T, DP, NT, FULL, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(fl::kv8::attention_kernel<T, DP, NT, FULL, HALVES, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
     set_on[dev] = true;
   }
@@ -1275,13 +1325,14 @@ int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, dim3 grid, bool
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = early ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, fl::kv8::attention_kernel<T, DP, NT, FULL, MASS>, a, kv);
+  return (int)cudaLaunchKernelEx(&cfg, fl::kv8::attention_kernel<T, DP, NT, FULL, HALVES, MASS>, a, kv);
 }
 template <typename T, int DP>
-int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, int nt, bool mass, dim3 grid, bool early, cudaStream_t stream) {
-#define FL_ATT(N, F) return mass ? launch_attention<T, DP, N, F, true>(a, kv, grid, early, stream) : launch_attention<T, DP, N, F, false>(a, kv, grid, early, stream)
-  if (kv.dim == DP) { if (nt == 1) FL_ATT(1, true); else FL_ATT(2, true); }
-  if (nt == 1) FL_ATT(1, false); else FL_ATT(2, false);
+int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, const Cut& c, bool mass, dim3 grid, bool early, cudaStream_t stream) {
+#define FL_ATT(N, F, S) return mass ? launch_attention<T, DP, N, F, S, true>(a, kv, grid, early, stream) : launch_attention<T, DP, N, F, S, false>(a, kv, grid, early, stream)
+  if (c.halves) { if (c.nt == 1) FL_ATT(1, false, true); else FL_ATT(2, false, true); }
+  if (kv.dim == DP) { if (c.nt == 1) FL_ATT(1, true, false); else FL_ATT(2, true, false); }
+  if (c.nt == 1) FL_ATT(1, false, false); else FL_ATT(2, false, false);
 #undef FL_ATT
 }
 }  // namespace
@@ -1342,8 +1393,8 @@ extern "C" int fl_kv8_attention(int dtype, const void* q, long long stride_b, lo
   const bool early = (long long)batch * tokens <= FL_THIN_MAX_ROWS;
   a.early = early;
   int rc = 0;
-  FL_KV8_TYPES(dtype, rc = kv->dim <= 64 ? launch_attention<T, 64>(a, *kv, c.nt, mass != nullptr, grid, early, stream)
-                                         : launch_attention<T, 128>(a, *kv, c.nt, mass != nullptr, grid, early, stream));
+  FL_KV8_TYPES(dtype, rc = kv->dim <= 64 ? launch_attention<T, 64>(a, *kv, c, mass != nullptr, grid, early, stream)
+                                         : launch_attention<T, 128>(a, *kv, c, mass != nullptr, grid, early, stream));
   if (rc != 0 || (c.clustered && mass == nullptr)) return rc;
   const int row_ctas = c.clustered ? 0 : heads * tokens;
   const int pages = kv->table_stride, most = 8 * 148 / batch;                 // eight CTAs per SM, if there is a page for each warp of theirs
