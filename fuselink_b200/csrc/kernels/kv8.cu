@@ -1100,12 +1100,10 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass,
   mass += (long long)b * pages; table += (long long)b * pages;
   mass_out += (long long)b * pages; table_out += (long long)b * pages;
   float m[EACH];
-  auto load = [&](int piece) {
+  auto place = [&](unsigned piece, int k) { return piece + (unsigned)(k * threads + tid); };
+  auto load = [&](unsigned piece) {
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      const long long i = (long long)piece + k * threads + tid;
-      m[k] = i < pages ? mass[i] : 0.f;
-    }
+    for (int k = 0; k < EACH; ++k) m[k] = place(piece, k) < (unsigned)pages ? mass[place(piece, k)] : 0.f;
   };
   load(0);
   const long long len = max(lengths[b], 0ll);
@@ -1114,22 +1112,33 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass,
     lengths_out[b] = lengths[b] - (long long)extra * bs;
     gone[b] = extra;
   }
-  const int lo = sinks, hi = used - recent;                    // hi - lo >= extra, since keep >= recent + sinks
+  // pages that may go: from `lo` on, `free_pages` of them; at least `extra`, since keep >= recent + sinks
+  const unsigned lo = sinks, free_pages = extra > 0 ? used - recent - sinks : 0;
+  uint32_t key[EACH];
+  unsigned free = 0;                                           // of the thread's
+  auto look = [&](unsigned piece) {
+    if (pages > piece_size) load(piece);
+    free = 0;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      key[k] = evict_key(m[k]);
+      free |= (place(piece, k) - lo < free_pages ? 1u : 0u) << k;
+    }
+  };
+  look(0);
   uint32_t prefix = 0;
   int left = extra;                                            // of those that go, among the weights that begin with the digits found
   if (extra > 0) {
     for (int shift = 24; shift >= 0; shift -= 8) {
       for (int i = tid; i < 256; i += threads) s.hist[i] = 0;
       __syncthreads();
-      for (int piece = 0; piece < pages; piece += piece_size) {
-        if (pages > piece_size) load(piece);
+      for (unsigned piece = 0; piece < (unsigned)pages; piece += piece_size) {
+        if (pages > piece_size) look(piece);
 #pragma unroll
         for (int k = 0; k < EACH; ++k) {
-          const long long i = (long long)piece + k * threads + tid;
-          const uint32_t key = evict_key(m[k]);
-          const bool in = i >= lo && i < hi && (shift == 24 || key >> (shift + 8) == prefix);
+          const bool in = (free >> k & 1) && (shift == 24 || key[k] >> (shift + 8) == prefix);
           // weights that no token ever saw are all alike: those that agree with the first of the warp are added at once
-          const int digit = (int)(key >> shift & 255);
+          const int digit = (int)(key[k] >> shift & 255);
           const unsigned some = __ballot_sync(0xffffffffu, in);
           if (some == 0) continue;
           const int leader = __ffs(some) - 1, first = __shfl_sync(0xffffffffu, digit, leader);
@@ -1138,7 +1147,6 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass,
           if (lane == leader) atomicAdd(&s.hist[digit], __popc(alike));
           else if (in && !like) atomicAdd(&s.hist[digit], 1);
         }
-        if (piece > 0x7fffffff - piece_size) break;
       }
       __syncthreads();
       if (warp == 0) {
@@ -1168,18 +1176,15 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass,
   }
   // kept pages go to the front, those that go to used - extra and on
   int equal_before = 0, gone_before = 0;
-  for (int piece = 0; piece < pages; piece += piece_size) {
-    if (pages > piece_size) load(piece);
+  for (unsigned piece = 0; piece < (unsigned)pages; piece += piece_size) {
+    if (pages > piece_size) look(piece);
     int id[EACH], rank[EACH] = {};
     unsigned below = 0, equal = 0;
 #pragma unroll
     for (int k = 0; k < EACH; ++k) {
-      const long long i = (long long)piece + k * threads + tid;
-      id[k] = i < pages ? table[i] : 0;
-      const bool free = extra > 0 && i >= lo && i < hi;
-      const uint32_t key = evict_key(m[k]);
-      below |= (free && key < prefix ? 1u : 0u) << k;
-      equal |= (free && key == prefix ? 1u : 0u) << k;
+      id[k] = place(piece, k) < (unsigned)pages ? table[place(piece, k)] : 0;
+      below |= ((free >> k & 1) && key[k] < prefix ? 1u : 0u) << k;
+      equal |= ((free >> k & 1) && key[k] == prefix ? 1u : 0u) << k;
     }
     unsigned goes = below;
     if (extra > 0) {
@@ -1195,14 +1200,13 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass,
     }
 #pragma unroll
     for (int k = 0; k < EACH; ++k) {
-      const long long i = (long long)piece + k * threads + tid;
-      if (i >= pages) continue;
+      const unsigned i = place(piece, k);
+      if (i >= (unsigned)pages) continue;
       const bool out = goes >> k & 1;
-      const int to = (int)i >= used ? (int)i : out ? used - extra + rank[k] : (int)i - rank[k];
+      const unsigned to = i >= (unsigned)used ? i : out ? used - extra + rank[k] : i - rank[k];
       table_out[to] = id[k];
       mass_out[to] = out ? 0.f : m[k];
     }
-    if (piece > 0x7fffffff - piece_size) break;
   }
 }
 

@@ -430,7 +430,8 @@ def test_more_requests_than_a_grid_is_high():
 # ---- eviction --------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("pages,bs,lens,keep,recent,sinks", [
     (8, 16, [128, 100, 1, 0, 17], 4, 1, 0), (145, 16, [145 * 16 - 3] * 7, 144, 4, 1), (2000, 8, [16000, 9000, 8001], 1000, 3, 2),
-    (5000, 32, [160000, 77], 3, 2, 1), (9, 5, [45, 44, 41, 5], 9, 1, 0), (9, 5, [45, 44], 1, 1, 0), (12, 16, [10 ** 6, -5], 6, 1, 5),
+    (5000, 32, [160000, 77], 3, 2, 1), (9, 5, [45, 44, 41, 5], 9, 1, 0), (9, 5, [45, 44], 1, 1, 0), (12, 16, [10 ** 6, -5], 6, 1, 5), (1024, 16, [16384, 16369], 1000, 1, 1), (1025, 16, [16400, 9000], 500, 1, 1),
+    (20000, 16, [320000, 250007, 131072], 9000, 2, 1),
 ])
 @pytest.mark.parametrize("masses", ["random", "ties", "odd"])
 def test_evict(pages, bs, lens, keep, recent, sinks, masses):
