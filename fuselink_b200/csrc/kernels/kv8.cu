@@ -78,7 +78,9 @@ __device__ __forceinline__ int page_id(const FlKv8& kv, int b, int page) {
 // Bound by memory: new tokens are read once, written once in the model's type and once in 8 bits.  A warp has one page of one head, of keys or
 // of values: lane (t, c) takes columns 8 c .. 8 c + 7 of the first half of a token's row and the matching ones of the second (the pairs that the
 // rotation mixes), 32 / (dim / 16) tokens at a time.  Four such steps, a page of 16 tokens, stay in registers between finding the largest
-// magnitude and writing codes; larger pages are read again.
+// magnitude and writing codes; larger pages are read again.  16 x 2048 tokens of 32 + 2 x 8 heads of 128: 254 us with a query's columns and angles
+// looked up one by one, now 188 (136 of bytes).  With 128 registers, for the four steps, an SM has 16 warps; 96 spill (253 us), two steps in
+// registers and the others read again take 206, queries in a launch of their own 180 to 193.
 constexpr int STEPS = 4;
 
 struct WriteArgs {
@@ -363,7 +365,9 @@ __global__ void __launch_bounds__(128) pack_kernel(const WriteArgs a, const FlKv
 // follows when a score is 2^8 beyond it (a vote, not a reduction, per step), and the sums of the second product stay in units of the largest
 // value scale seen, which a page's weights are brought to where its own is smaller (scales are powers of two).  With a maximum per step and a
 // multiplication of every sum by the page's scale, and the codes on their way through registers, 16 x 2048 tokens of 8 KV heads of 128 took
-// 25.6 us, now 18.7 (10.3 of bytes).  Codes are on their way through a ring in shared memory, two steps ahead of their use.
+// 25.6 us, now 17.4 (10.3 of bytes; 2 x 131072 tokens 103, 82 of bytes).  Codes are on their way through a ring in shared memory, two steps ahead
+// of their use, which then never wait: of the 17.4 us some 9 go at the memory's rate, the others are launch, the first page ids and rows (4000 to
+// 5000 cycles: a miss each, of pages anywhere in memory), and the joining of warps and CTAs (5000 cycles).
 //
 // A request's context is dealt out evenly over the warps of the CTAs in the grid's third dimension: a cluster of up to 8, which joins their (max, sum,
 // output) through distributed shared memory, or more, whose parts finish_kernel joins.
@@ -1035,8 +1039,8 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
 // ---- eviction ---------------------------------------------------------------------------------------------------------------
 // Bound by the latency of one CTA per request.  How many pages go is known; the weight up to which they go is found digit by digit (four
 // histograms of 256), and the row is dealt out in its order.  Threads keep their weights in registers, so that memory is read once: one each of
-// up to 1024 pages (16 rows of 145: 12.5 us with eight each, 4.4 with one), eight each of more (64 rows of 8192: 28 us with one page per thread and
-// pass, now 17); rows of more than 8192 go by in pieces of that, once for every digit.
+// up to 1024 pages (16 rows of 145: 12.5 us with eight each, 4.3 with one), eight each of more (64 rows of 8192: 28 us with one page per thread and
+// pass, now 14.3); rows of more than 8192 go by in pieces of that, once for every digit.
 constexpr int EVICT_THREADS = 1024, EVICT_WARPS = EVICT_THREADS / 32, EVICT_EACH = 8;
 
 // weights in an order that whole numbers have: NaN last, -0 as 0

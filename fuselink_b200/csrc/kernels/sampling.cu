@@ -8,8 +8,9 @@
 // A cluster of CTAs per row.  Each counts its stretch of the row in shared memory (16-bit counters, 128 KB) and adds up counts and weights of 64 bins (a
 // chunk) at a time; the first one adds up the CTAs' chunks through distributed shared memory.  There a warp finds the
 // limits and the token's bin, by two votes over the sums of 1024 chunks and one over the 64 bins of a chunk each.  The CTA in whose stretch
-// the token lies looks for it among its equals.  Bound by latency: what a row needs beside its bytes is a fixed number of passes over 128 KB of
-// shared memory and some twenty barriers.
+// the token lies looks for it among its equals.  Bound by latency: one row of 128256 takes 14 us (26000 cycles: counting 4000, barriers of the cluster
+// 3500 each, chunks 3500, searches 10000, the look among equals 2500); many rows by the shared memory's atomic additions, of which a warp's 32
+// take some seven cycles: 192 rows 63 us (131 before logits were counted two at a time and weights computed eight at a time).
 #include "sampling.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -451,9 +451,10 @@ def test_evict(pages, bs, lens, keep, recent, sinks, masses):
         m = mass[b].tolist()
         free = sorted(range(sinks, used - recent), key=lambda i: (m[i] != m[i], m[i] if m[i] == m[i] else 0.0, i))
         gone = sorted(free[:extra])
-        order = [i for i in range(used) if i not in set(gone)] + gone + list(range(used, pages))
+        out = set(gone)
+        order = [i for i in range(used) if i not in out] + gone + list(range(used, pages))
         assert got[0][b].tolist() == table[b, order].tolist() and got[1][b] == n - extra * bs and got[3][b] == extra
-        want = torch.where(torch.tensor([i in set(gone) for i in order], device="cuda"), torch.zeros((), device="cuda"), mass[b, order])
+        want = torch.where(torch.tensor([i in out for i in order], device="cuda"), torch.zeros((), device="cuda"), mass[b, order])
         assert torch.equal(got[2][b].nan_to_num(-7.0), want.nan_to_num(-7.0))
 
 
