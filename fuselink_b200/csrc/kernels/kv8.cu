@@ -923,6 +923,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
     *reinterpret_cast<float4*>(&s_o[0][row][d]) = acc;         // read and written by this thread alone
     if (d == 0) { s_cm[row] = mm; s_cl[row] = ll; }
   }
+  __syncwarp();
   cluster_sync_all();
   for (int i = z * WARPS * 32 + threadIdx.x; i < n_rows * pieces; i += a.splits * WARPS * 32) {
     const int row = i / pieces, d = 4 * (i - row * pieces);
@@ -951,6 +952,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
       }
     result(row, d, mm, ll, acc);
   }
+  __syncwarp();
   cluster_sync_all();                            // nobody leaves while its part is being read
 }
 
@@ -1368,7 +1370,7 @@ extern "C" int fl_kv8_attention(int dtype, const void* q, long long stride_b, lo
                                 const long long* counts, int batch, int tokens, int heads, float scale, const FlKv8* kv, void* out, float* mass,
                                 void* scratch, cudaStream_t stream) {
   if (!sizes_fit(kv) || kv->layer < 0 || kv->layer >= kv->layers || batch < 0 || tokens < 0 || heads < 1 || heads % kv->heads ||
-      (long long)heads * tokens > 0x3fffffffll || stride_b % 8 || stride_t % 8 || stride_h % 8)
+      (long long)heads * tokens > 0x3fffffffll || stride_b % 8 || stride_t % 8 || stride_h % 8 || !(scale >= 0.f && scale < INFINITY))
     return -2;
   if (mass != nullptr && (long long)heads * tokens > FL_KV8_MASS_ROWS) return -2;   // a CTA of the kernel that adds them up keeps each one's sum in shared memory
   if (!aligned({q, out, scratch, kv->k, kv->v})) return -4;

@@ -32,7 +32,7 @@ int fl_kv8_write(int dtype, const void* qkv, void* out, const void* bias, const 
 int fl_kv8_pack(int dtype, const void* k_pool, const void* v_pool, int src_blocks, const int* src_table, int src_stride, const long long* lengths,
                 int batch, const FlKv8* kv, cudaStream_t stream);
 // out [batch][tokens][heads * dim] = softmax(scale q k^T) v of tokens start[b] .. start[b] + counts[b] - 1 (counts null: `tokens` of them) over the
-// slots up to their own; zeros where there is none.  q: element strides of (request, token, head).  mass (or null): [batch][table_stride], += the
+// slots up to their own; zeros where there is none.  scale: finite, not negative.  q: element strides of (request, token, head).  mass (or null): [batch][table_stride], += the
 // weights' sum over this call's tokens and heads, page by page; tokens * heads is at most FL_KV8_MASS_ROWS then.
 // scratch: fl_kv8_attention_scratch() bytes, from a multiple of 16 on.
 long long fl_kv8_attention_scratch(int batch, int tokens, int heads, const FlKv8* kv, int mass);

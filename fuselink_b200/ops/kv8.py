@@ -100,11 +100,13 @@ def attention(cache: Kv8Cache, layer: int, q: torch.Tensor, block_table: torch.T
               scale: Optional[float] = None, mass: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, status: int = 0) -> torch.Tensor:
     """Attention of new tokens over the cache, their own keys and values (already written) among it: q [batch, tokens, heads, dim], of any strides that
     are multiples of 8 elements; token t of request b sees slots 0 .. start[b] + t.  Returns [batch, tokens, heads * dim]; zeros for tokens behind
-    ``counts`` and for those that see nothing.  scale: 1 / sqrt(dim) by default.
+    ``counts`` and for those that see nothing.  scale (finite, not negative): 1 / sqrt(dim) by default.
     mass ([batch, pages] fp32) has the weights' sum over this call's tokens and heads added, page by page of ``block_table``; on the GPU such a call
     takes up to 6144 tokens times heads."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
+    elif not 0 <= scale < math.inf:
+        raise ValueError(f"kv8: scale {scale}")
     if q.is_cuda:
         return require_native().kv8_attention(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, layer, q, start, counts, scale, out, mass, status)
     _check_like(cache, q, "queries")

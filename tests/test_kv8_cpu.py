@@ -76,6 +76,8 @@ def test_indices_outside_are_errors():
         kv8.write(cache, 0, rows, table, torch.tensor([0]), rope=torch.zeros(1, 32))
     with pytest.raises(IndexError):
         kv8.attention(cache, 0, rows[:, :, :1], table, torch.tensor([20]))
+    with pytest.raises(ValueError):
+        kv8.attention(cache, 0, rows[:, :, :1], table, torch.tensor([3]), scale=-1.0)
     with pytest.raises(IndexError):
         kv8.pack(cache, torch.zeros(4 * 16 * 32), torch.zeros(4 * 16 * 32), 4, table, table, torch.tensor([40]))
 
@@ -291,11 +293,11 @@ def test_c_entries_refuse_caches(lib, kw):
 
 
 def test_c_entries_refuse_sizes(lib):
-    def attend(dtype=0, strides=(64, 64, 64), batch=1, tokens=1, heads=4, mass=None):
-        return lib.fl_kv8_attention(I(dtype), P(A0), *map(LL, strides), P(8), P(), I(batch), I(tokens), I(heads), F32(1), _kv(), P(A0), P(mass), P(A0), P())
+    def attend(dtype=0, strides=(64, 64, 64), batch=1, tokens=1, heads=4, mass=None, scale=1.0):
+        return lib.fl_kv8_attention(I(dtype), P(A0), *map(LL, strides), P(8), P(), I(batch), I(tokens), I(heads), F32(scale), _kv(), P(A0), P(mass), P(A0), P())
 
     for kw in (dict(strides=(4, 64, 64)), dict(strides=(64, 60, 64)), dict(strides=(64, 64, 65)), dict(batch=-1), dict(tokens=-1), dict(heads=3), dict(heads=0),
-               dict(tokens=1 << 30), dict(tokens=4000, mass=8)):
+               dict(tokens=1 << 30), dict(tokens=4000, mass=8), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan)):
         assert attend(**kw) == -2
     assert attend(dtype=7) == -1 and attend(batch=0) == 0 and attend(tokens=0) == 0
     assert lib.fl_kv8_write(I(7), P(A0), P(A0), P(), P(), LL(0), P(8), P(), P(), I(1), I(1), I(4), _kv(), P()) == -1

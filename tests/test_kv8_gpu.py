@@ -129,6 +129,24 @@ def test_write(dt, heads, kv_heads, dim, bs, tokens, start, counts, how):
         assert torch.equal(got.view(torch.uint8) if got.dtype == F8 else got, exp.view(torch.uint8) if exp.dtype == F8 else exp)
 
 
+def test_rows_of_any_order():
+    """Rows that are no contiguous tensor are written as their copy; scales other than the heads' own, 0 among them."""
+    from fuselink_b200.ops import kv8
+    table = _table(2, 2, 5)
+    x = _randn(3, 2, 8, 64, seed=3, dt=BF).transpose(0, 1)             # [2, 3, 8, 64]
+    a, b = _cache(1, 5, 2, 16, 64), _cache(1, 5, 2, 16, 64)
+    out = kv8.write(a, 0, x, table, _ints([4, 15]))
+    assert torch.equal(out, kv8.write(b, 0, x.contiguous(), table, _ints([4, 15]))) and torch.equal(out, x)
+    for s, t in zip(a.tensors(), b.tensors()):
+        assert torch.equal(s.view(torch.uint8), t.view(torch.uint8))
+    q = _randn(8, 3, 2, 64, seed=4, dt=BF).permute(2, 1, 0, 3)[:, :, ::2]        # [2, 3, 4, 64], strides of multiples of 64
+    for scale in (0.0, 0.01, 1.0):
+        want, _, may = _want_attention(a, 0, q, table, [4, 15], [3, 3], scale)
+        _check(kv8.attention(a, 0, q, table, _ints([4, 15]), scale=scale), want, may, BF)
+    with pytest.raises(ValueError):
+        kv8.attention(a, 0, q, table, _ints([4, 15]), scale=-0.1)
+
+
 def test_a_page_follows_its_scale_token_by_token():
     """Growing magnitudes: every token raises the scale; the earlier codes follow it each time."""
     from fuselink_b200.ops import kv8
@@ -248,6 +266,10 @@ SHAPES = [  # heads, kv_heads, dim, bs, tokens, lengths (slots that the last tok
     (64, 8, 128, 16, 8, [1000, 8, 33]),
     (10, 2, 112, 7, 5, [5, 50, 613]),
     (3, 1, 32, 16, 40, [40, 111, 2500]),
+    (8, 2, 128, 16, 150, [150, 777]),
+    (2, 2, 128, 8, 1, [8, 9, 4000, 7]),
+    (8, 1, 64, 5, 3, [3, 4, 10, 11, 1201]),
+    (16, 2, 96, 20, 2, [2, 20, 21, 44, 999]),
 ]
 
 

@@ -52,11 +52,11 @@ def test_each_limit(limits):
     _check(sample(x, u, *limits), x, u, *limits)
 
 
-@pytest.mark.parametrize("rows,vocab", [(4, 1000), (4, 40000), (4, 128256)])
-def test_rows_that_are_not_ordinary(rows, vocab):
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("vocab", [1000, 40000, 128256])
+def test_rows_that_are_not_ordinary(dt, vocab):
     """Equal logits everywhere, masks by -inf and by the type's lowest value, one token left, none, NaN, +inf; numbers outside [0, 1)."""
     from fuselink_b200.ops.sampling import sample
-    dt = torch.bfloat16
     x = _logits(16, vocab, dt, seed=7)
     x[0] = 0.0
     x[1] = -0.0
@@ -106,7 +106,7 @@ def test_frequencies():
 def test_rows_anywhere_in_memory():
     from fuselink_b200.ops.sampling import sample
     base = _logits(9, 4001, torch.float16, seed=9)
-    for x in (base[:, 1:], base[:, 3: 3998], base[::2, 7:], base.t()[:9, :].t() if False else base[:, ::2]):
+    for x in (base[:, 1:], base[:, 3: 3998], base[::2, 7:], base[:, ::2], base[3:4].expand(5, -1)):
         u = _u(x.shape[0])
         _check(sample(x, u, 1.0, 100, 0.9, 0.0), x, u, 1.0, 100, 0.9, 0.0)
 
