@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 #include "../kernels/grouped_gemm.cuh"
 #include "../kernels/shadow_reduce.cuh"
@@ -424,6 +425,10 @@ static void dec_advance(torch::Tensor next, torch::Tensor tokens, torch::Tensor 
 }
 
 // ------------------------------------------------------------------------------------------------ cache in 8 bits
+// A new tensor without the dispatcher's part, which is half of what one costs the host: these calls take the GPU a few microseconds.
+static torch::Tensor new_like(const torch::Tensor& as, c10::IntArrayRef sizes, torch::ScalarType type) {
+  return torch::Tensor(at::detail::empty_cuda(sizes, type, as.device(), c10::nullopt));
+}
 // k, v: [layers, blocks, heads, block_size, dim] e4m3; scales: [layers, blocks, heads] fp32; table: [batch, pages] int32
 static FlKv8 kv8_of(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& k_scale, const torch::Tensor& v_scale, const torch::Tensor& table,
                     int64_t layer, int64_t batch, int64_t status_addr) {
@@ -454,7 +459,7 @@ static torch::Tensor kv8_write(const torch::Tensor& k, const torch::Tensor& v, c
   const int dt = dec_dtype(qkv);
   c10::cuda::CUDAGuard guard(qkv.device());
   if (!into.has_value()) qkv = qkv.contiguous();
-  const torch::Tensor out = into.has_value() ? *into : torch::empty_like(qkv);
+  const torch::Tensor out = into.has_value() ? *into : new_like(qkv, qkv.sizes(), qkv.scalar_type());
   TORCH_CHECK(qkv.dim() == 4 && qkv.is_contiguous() && qkv.device() == k.device(), "kv8: qkv [batch, tokens, heads + 2 kv_heads, dim], contiguous");
   const int64_t B = qkv.size(0), T = qkv.size(1), all = qkv.size(2), D = qkv.size(3);
   TORCH_CHECK(k.dim() == 5 && D == k.size(4) && all >= 2 * k.size(2) && B <= INT32_MAX && T <= INT32_MAX && all * D <= INT32_MAX, "kv8: qkv of another layout than the cache");
@@ -490,14 +495,14 @@ static torch::Tensor kv8_attention(const torch::Tensor& k, const torch::Tensor& 
   const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3);
   TORCH_CHECK(B <= INT32_MAX && T <= INT32_MAX && H <= INT32_MAX && H % std::max<int64_t>(k.size(2), 1) == 0, "kv8: heads in groups that share a KV head");
   c10::cuda::CUDAGuard guard(k.device());
-  const torch::Tensor out = into.has_value() ? *into : torch::empty({B, T, H * D}, q.options());
+  const torch::Tensor out = into.has_value() ? *into : new_like(q, {B, T, H * D}, q.scalar_type());
   TORCH_CHECK(out.device() == k.device() && out.scalar_type() == q.scalar_type() && out.is_contiguous() && out.numel() == B * T * H * D, "kv8: out [batch, tokens, heads * dim] like q");
   TORCH_CHECK(!mass.has_value() || (mass->device() == k.device() && mass->scalar_type() == torch::kFloat32 && mass->is_contiguous() && mass->sizes() == table.sizes()),
               "kv8: mass [batch, pages] fp32");
   const FlKv8 kv = kv8_of(k, v, k_scale, v_scale, table, layer, B, status_addr);
   const long long bytes = fl_kv8_attention_scratch((int)B, (int)T, (int)H, &kv, mass.has_value());
   torch::Tensor scratch;
-  if (bytes > 0) scratch = torch::empty({bytes}, q.options().dtype(torch::kUInt8));
+  if (bytes > 0) scratch = new_like(q, {(int64_t)bytes}, torch::kUInt8);
   check_rc(fl_kv8_attention(dt, q.data_ptr(), B > 1 ? q.stride(0) : 0, T > 1 ? q.stride(1) : 0, H > 1 ? q.stride(2) : 0, kv8_i64(start, k, B, "kv8: start [batch] int64"),
                             kv8_i64(counts, k, B, "kv8: counts [batch] int64"), (int)B, (int)T, (int)H, (float)scale, &kv, out.data_ptr(),
                             mass.has_value() ? mass->data_ptr<float>() : nullptr, bytes > 0 ? scratch.data_ptr() : nullptr, cur_stream()), "fl_kv8_attention");
@@ -510,7 +515,8 @@ static std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> kv
   TORCH_CHECK(B <= INT32_MAX && M <= INT32_MAX && block_size >= 1 && block_size <= INT32_MAX && keep <= INT32_MAX && recent >= 1 && sinks >= 0 && recent <= keep && sinks <= keep - recent,
               "kv8: keep at least recent + sinks pages, recent at least one");
   c10::cuda::CUDAGuard guard(mass.device());
-  auto mass_out = torch::empty_like(mass), table_out = torch::empty_like(table), lengths_out = torch::empty_like(lengths), gone = torch::empty({B}, table.options());
+  auto mass_out = new_like(mass, mass.sizes(), torch::kFloat32), table_out = new_like(mass, mass.sizes(), torch::kInt32), lengths_out = new_like(mass, lengths.sizes(), torch::kInt64),
+       gone = new_like(mass, {B}, torch::kInt32);
   check_rc(fl_kv8_evict(mass.data_ptr<float>(), table.data_ptr<int>(), kv8_i64(lengths, mass, B, "kv8: lengths [batch] int64"), (int)B, (int)M, (int)block_size, (int)keep,
                         (int)recent, (int)sinks, mass_out.data_ptr<float>(), table_out.data_ptr<int>(), reinterpret_cast<long long*>(lengths_out.data_ptr<int64_t>()),
                         gone.data_ptr<int>(), cur_stream()), "fl_kv8_evict");
@@ -539,7 +545,7 @@ static std::pair<torch::Tensor, torch::Tensor> sample(torch::Tensor logits, torc
   a.top_p = (const float*)per_row(top_p, torch::kFloat32, "sample: top_p [rows] fp32"); a.top_p_all = (float)top_p_all;
   a.min_p = (const float*)per_row(min_p, torch::kFloat32, "sample: min_p [rows] fp32"); a.min_p_all = (float)min_p_all;
   c10::cuda::CUDAGuard guard(logits.device());
-  auto tokens = torch::empty({rows}, logits.options().dtype(torch::kInt64)), logprobs = torch::empty({rows}, logits.options().dtype(torch::kFloat32));
+  auto tokens = new_like(logits, {rows}, torch::kInt64), logprobs = new_like(logits, {rows}, torch::kFloat32);
   a.tokens = reinterpret_cast<long long*>(tokens.data_ptr<int64_t>()); a.logprobs = logprobs.data_ptr<float>();
   if (rows > 0) check_rc(fl_sample(dt, &a, cur_stream()), "fl_sample");
   return {tokens, logprobs};
