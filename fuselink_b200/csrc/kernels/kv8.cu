@@ -1039,10 +1039,11 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
 }
 
 // ---- eviction ---------------------------------------------------------------------------------------------------------------
-// Bound by the latency of one CTA per request.  How many pages go is known; the weight up to which they go is found digit by digit (four
-// histograms of 256), and the row is dealt out in its order.  Threads keep their weights in registers, so that memory is read once: one each of
-// up to 1024 pages (16 rows of 145: 12.5 us with eight each, 4.3 with one), eight each of more (64 rows of 8192: 28 us with one page per thread and
-// pass, now 14.3); rows of more than 8192 go by in pieces of that, once for every digit.
+// Bound by the latency of one CTA per request.  How many pages go is known; the weight up to which they go is found digit by digit (histograms of 256, up
+// to the digit whose whole counter goes), and the row is dealt out in its order.  Threads keep their weights in registers, so that memory is read once: one
+// each of up to 1024 pages (16 rows of 145: 12.5 us with eight each, 3.4 with one), eight each of more (64 rows of 8192: 28 us with one page per thread and
+// pass, 14.3 with a vote per page in every digit and two rankings, now 9.6, of which instructions take half); rows of more than 8192 go by in
+// pieces of that, once for every digit (4 rows of 40000: 52 us).
 constexpr int EVICT_THREADS = 1024, EVICT_WARPS = EVICT_THREADS / 32, EVICT_EACH = 8;
 
 // weights in an order that whole numbers have: NaN last, -0 as 0
@@ -1053,69 +1054,40 @@ __device__ __forceinline__ uint32_t evict_key(float m) {
 }
 
 template <int EACH> struct EvictShared {
-  int hist[256];
-  int before[EACH * EVICT_WARPS];        // by pass and warp: how many, then how many before
-  int all, digit, left;
+  int hist[4][256];                                                            // one per digit
+  uint8_t kind[EACH * EVICT_THREADS];                                          // of the piece's pages
+  unsigned short to[EACH * EVICT_THREADS];                                     // how many go before the page, and whether it does
+  unsigned before[EVICT_WARPS];                                                // a warp's pages below the limit, and from bit 16 on those equal to it
+  int digit, left, whole;
 };
-// How many of the piece's flagged ones come before each of the thread's (bit k of `flags`: the one at k * threads + thread), in `rank`;
-// returns how many there are.
-template <int EACH>
-__device__ __forceinline__ int evict_ranks(EvictShared<EACH>& s, unsigned flags, int (&rank)[EACH]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < EACH; ++k) {
-    const unsigned v = __ballot_sync(0xffffffffu, flags >> k & 1);
-    rank[k] = __popc(v & ((1u << lane) - 1));
-    if (lane == 0) s.before[k * EVICT_WARPS + warp] = __popc(v);
-  }
-  __syncthreads();
-  if (warp == 0) {
-    int n[EACH], sum = 0;
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const int at = lane * EACH + j;
-      n[j] = (at % EVICT_WARPS) * 32 < (int)blockDim.x ? s.before[at] : 0;
-      sum += n[j];
-    }
-    int upto = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    if (lane == 31) s.all = upto;
-    upto -= sum;
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      s.before[lane * EACH + j] = upto;
-      upto += n[j];
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < EACH; ++k) rank[k] += s.before[k * EVICT_WARPS + warp];
-  return s.all;
-}
+constexpr unsigned EVICT_BELOW = 1, EVICT_EQUAL = 2, EVICT_OUT = 0x8000;
 
 template <int EACH>
 __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass, const int* table, const long long* lengths, int pages, int bs, int keep,
                                                               int recent, int sinks, float* mass_out, int* table_out, long long* lengths_out, int* gone) {
-  __shared__ EvictShared<EACH> s;
+  __shared__ __align__(16) EvictShared<EACH> s;
   const int b = blockIdx.x, threads = blockDim.x, piece_size = threads * EACH, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   mass += (long long)b * pages; table += (long long)b * pages;
   mass_out += (long long)b * pages; table_out += (long long)b * pages;
+  const long long given = lengths[b];
   float m[EACH];
+  int id[EACH];
   auto place = [&](unsigned piece, int k) { return piece + (unsigned)(k * threads + tid); };
-  auto load = [&](unsigned piece) {
+  auto load = [&](unsigned piece, bool ids) {
 #pragma unroll
     for (int k = 0; k < EACH; ++k) m[k] = place(piece, k) < (unsigned)pages ? mass[place(piece, k)] : 0.f;
+    if (!ids) return;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) id[k] = place(piece, k) < (unsigned)pages ? table[place(piece, k)] : 0;
   };
-  load(0);
-  const long long len = max(lengths[b], 0ll);
-  const int used = (int)min(len / bs + (len % bs != 0), (long long)pages), extra = max(used - keep, 0);
+  load(0, true);
+  for (int i = tid; i < 4 * 256; i += threads) s.hist[0][i] = 0;
+  const long long len = max(given, 0ll);
+  // (a division in 64 bits would cost each warp as much as a digit)
+  const long long full = len <= 0x7fffffffll ? (long long)((unsigned)len / (unsigned)bs) : len / bs;
+  const int used = (int)min(full + (full * bs != len), (long long)pages), extra = max(used - keep, 0);
   if (tid == 0) {
-    lengths_out[b] = lengths[b] - (long long)extra * bs;
+    lengths_out[b] = given - (long long)extra * bs;
     gone[b] = extra;
   }
   // pages that may go: from `lo` on, `free_pages` of them; at least `extra`, since keep >= recent + sinks
@@ -1123,7 +1095,6 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass,
   uint32_t key[EACH];
   unsigned free = 0;                                           // of the thread's
   auto look = [&](unsigned piece) {
-    if (pages > piece_size) load(piece);
     free = 0;
 #pragma unroll
     for (int k = 0; k < EACH; ++k) {
@@ -1132,86 +1103,113 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_kernel(const float* mass,
     }
   };
   look(0);
+  __syncthreads();
   uint32_t prefix = 0;
-  int left = extra;                                            // of those that go, among the weights that begin with the digits found
-  if (extra > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += threads) s.hist[i] = 0;
-      __syncthreads();
-      for (unsigned piece = 0; piece < (unsigned)pages; piece += piece_size) {
-        if (pages > piece_size) look(piece);
-#pragma unroll
-        for (int k = 0; k < EACH; ++k) {
-          const bool in = (free >> k & 1) && (shift == 24 || key[k] >> (shift + 8) == prefix);
-          // weights that no token ever saw are all alike: those that agree with the first of the warp are added at once
-          const int digit = (int)(key[k] >> shift & 255);
-          const unsigned some = __ballot_sync(0xffffffffu, in);
-          if (some == 0) continue;
-          const int leader = __ffs(some) - 1, first = __shfl_sync(0xffffffffu, digit, leader);
-          const bool like = in && digit == first;
-          const unsigned alike = __ballot_sync(0xffffffffu, like);
-          if (lane == leader) atomicAdd(&s.hist[digit], __popc(alike));
-          else if (in && !like) atomicAdd(&s.hist[digit], 1);
-        }
-      }
-      __syncthreads();
-      if (warp == 0) {
-        int n[8], sum = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { n[j] = s.hist[lane * 8 + j]; sum += n[j]; }
-        int before = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, before, o);
-          if (lane >= o) before += v;
-        }
-        before -= sum;
-        if (before < left && before + sum >= left) {
-          int j = 0;
-#pragma unroll
-          for (int q = 0; q < 7; ++q)
-            if (j == q && before + n[q] < left) { before += n[q]; ++j; }
-          s.digit = lane * 8 + j;
-          s.left = left - before;
-        }
-      }
-      __syncthreads();
-      prefix = prefix << 8 | (uint32_t)s.digit;
-      left = s.left;
-    }
-  }
-  // kept pages go to the front, those that go to used - extra and on
-  int equal_before = 0, gone_before = 0;
-  for (unsigned piece = 0; piece < (unsigned)pages; piece += piece_size) {
-    if (pages > piece_size) look(piece);
-    int id[EACH], rank[EACH] = {};
-    unsigned below = 0, equal = 0;
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      id[k] = place(piece, k) < (unsigned)pages ? table[place(piece, k)] : 0;
-      below |= ((free >> k & 1) && key[k] < prefix ? 1u : 0u) << k;
-      equal |= ((free >> k & 1) && key[k] == prefix ? 1u : 0u) << k;
-    }
-    unsigned goes = below;
-    if (extra > 0) {
-      const int equals = evict_ranks(s, equal, rank);
+  int shift = 32, left = extra;                                // of those that go, among the weights that begin with the digits found
+  bool whole = extra == 0;                                     // all of them do: further digits say nothing
+  while (shift > 0 && !whole) {
+    shift -= 8;
+    int* hist = s.hist[shift / 8];
+    for (unsigned piece = 0; piece < (unsigned)pages; piece += piece_size) {
+      if (pages > piece_size) { load(piece, false); look(piece); }
+      // weights that no token ever saw are all alike: a warp's additions to one counter cost no more than others (adding them up first, 12.3 us)
 #pragma unroll
       for (int k = 0; k < EACH; ++k)
-        if ((equal >> k & 1) && equal_before + rank[k] < left) goes |= 1u << k;
-      equal_before += equals;
-      const int going = evict_ranks(s, goes, rank);
+        if ((free >> k & 1) && (shift == 24 || key[k] >> (shift + 8) == prefix)) atomicAdd(&hist[key[k] >> shift & 255], 1);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      const int4 h0 = reinterpret_cast<const int4*>(hist)[2 * lane], h1 = reinterpret_cast<const int4*>(hist)[2 * lane + 1];
+      const int n[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
+      const int sum = n[0] + n[1] + n[2] + n[3] + n[4] + n[5] + n[6] + n[7];
+      int before = sum;
 #pragma unroll
-      for (int k = 0; k < EACH; ++k) rank[k] += gone_before;
-      gone_before += going;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+      }
+      before -= sum;
+      if (before < left && before + sum >= left) {
+        int j = 0, equals = n[0];
+#pragma unroll
+        for (int q = 0; q < 7; ++q)
+          if (j == q && before + n[q] < left) { before += n[q]; ++j; equals = n[q + 1]; }
+        s.digit = lane * 8 + j;
+        s.left = left - before;
+        s.whole = equals == left - before;
+      }
+    }
+    __syncthreads();
+    prefix = prefix << 8 | (uint32_t)s.digit;
+    left = s.left;
+    whole = s.whole;
+  }
+  // Kept pages go to the front, those that go to used - extra and on.  A thread ranks neighbours, so that a warp has one sum and not one per page of a thread;
+  // what a page is and where it goes change their order through shared memory.
+  unsigned below_before = 0, equal_before = 0;
+  auto going = [&](unsigned below, unsigned equal) { return below + min(equal, (unsigned)left); };          // of those that are equal the first `left` go
+  for (unsigned piece = 0; piece < (unsigned)pages; piece += piece_size) {
+    if (pages > piece_size) { load(piece, true); look(piece); }
+    const unsigned gone_before = going(below_before, equal_before);
+    unsigned to[EACH] = {};
+    if (extra > 0) {
+      unsigned kind[EACH], own = 0;
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const uint32_t digits = key[k] >> shift;
+        kind[k] = !(free >> k & 1) ? 0 : digits < prefix ? EVICT_BELOW : digits == prefix ? EVICT_EQUAL : 0;
+      }
+      if constexpr (EACH > 1) {
+        static_assert(EACH == 8, "a vector of eight bytes and one of eight halves");
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) s.kind[k * threads + tid] = (uint8_t)kind[k];
+        __syncthreads();
+        const uint2 v = reinterpret_cast<const uint2*>(s.kind)[tid];
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) kind[k] = (k < 4 ? v.x : v.y) >> (k % 4 * 8) & 255;
+      }
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        kind[k] = (kind[k] & EVICT_BELOW) | (kind[k] & EVICT_EQUAL) << 15;             // as the sums have them
+        own += kind[k];
+      }
+      unsigned upto = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      if (lane == 31) s.before[warp] = upto;
+      __syncthreads();
+      unsigned all = lane * 32 < threads ? s.before[lane] : 0, others = lane < warp ? all : 0;
+      all = __reduce_add_sync(0xffffffffu, all);
+      others = __reduce_add_sync(0xffffffffu, others);
+      upto += others - own;                                    // of the piece, before the thread's
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const unsigned equals = equal_before + (upto >> 16);
+        const bool out = kind[k] == 1 || (kind[k] != 0 && equals < (unsigned)left);
+        to[k] = going(below_before + (upto & 0xffffu), equals) - gone_before + (out ? EVICT_OUT : 0);
+        upto += kind[k];
+      }
+      below_before += all & 0xffffu;
+      equal_before += all >> 16;
+      if constexpr (EACH > 1) {
+        reinterpret_cast<uint4*>(s.to)[tid] = make_uint4(to[0] | to[1] << 16, to[2] | to[3] << 16, to[4] | to[5] << 16, to[6] | to[7] << 16);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) to[k] = s.to[k * threads + tid];
+      }
     }
 #pragma unroll
     for (int k = 0; k < EACH; ++k) {
       const unsigned i = place(piece, k);
       if (i >= (unsigned)pages) continue;
-      const bool out = goes >> k & 1;
-      const unsigned to = i >= (unsigned)used ? i : out ? used - extra + rank[k] : i - rank[k];
-      table_out[to] = id[k];
-      mass_out[to] = out ? 0.f : m[k];
+      const bool out = to[k] & EVICT_OUT;
+      const unsigned rank = gone_before + (to[k] & (EVICT_OUT - 1));
+      const unsigned at = i >= (unsigned)used ? i : out ? used - extra + rank : i - rank;
+      table_out[at] = id[k];
+      mass_out[at] = out ? 0.f : m[k];
     }
   }
 }
