@@ -116,10 +116,10 @@ struct Columns {                              // of one token: the two vectors t
     unpack<T>(hi, b);
     if (bias != nullptr) {
       float e[8];
-      unpack<T>(ld_v4(bias), e);
+      unpack<T>(*reinterpret_cast<const uint4*>(bias), e);
 #pragma unroll
       for (int j = 0; j < 8; ++j) a[j] += e[j];
-      unpack<T>(ld_v4(bias + half), e);
+      unpack<T>(*reinterpret_cast<const uint4*>(bias + half), e);
 #pragma unroll
       for (int j = 0; j < 8; ++j) b[j] += e[j];
     }
@@ -156,9 +156,9 @@ struct Columns {                              // of one token: the two vectors t
 };
 
 // One page of one head by one warp.  row(i): token i of the `n` that are new, i.e. its vector of this lane's columns; given(i, columns): what becomes
-// of them besides.  again(i): the same after given().
-template <typename T, typename Row, typename Given, typename Again>
-__device__ __forceinline__ void write_page(uint8_t* page, float* scale, bool there, int lead, int n, int dim, Row row, Given given, Again again) {
+// of them; keep(i, columns): where they go besides.  again(i): the vector after given().
+template <typename T, typename Row, typename Given, typename Keep, typename Again>
+__device__ __forceinline__ void write_page(uint8_t* page, float* scale, bool there, int lead, int n, int dim, Row row, Given given, Keep keep, Again again) {
   const int lane = threadIdx.x & 31, chunks = dim / 16, at_once = 32 / chunks, tk = lane / chunks, c = lane - tk * chunks;
   const bool on = tk < at_once;
   const int steps = (n + at_once - 1) / at_once;
@@ -177,6 +177,12 @@ __device__ __forceinline__ void write_page(uint8_t* page, float* scale, bool the
         given(i, c, col[s]);
         amax = max(amax, col[s].amax());
       }
+    }
+    // behind all of them, so that a step's angles and bias are on their way during the one before
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int i = (s0 + s) * at_once + tk;
+      if (on && i < n) keep(i, c, col[s]);
     }
   }
   if (!there) return;
@@ -274,6 +280,8 @@ __global__ void __launch_bounds__(128, 4) write_kernel(const WriteArgs a, const 
               if (rotate) note(kv.status, FL_DEC_BAD_POSITION);
               col.turn(bias_c, nullptr, half);
             }
+          },
+          [&](int i, int c, const Columns<T>& col) {
             T* p = out + (first + (long long)i * all) * D + 8 * c;
             st_v4(p, col.lo);
             st_v4(p + half, col.hi);
@@ -310,6 +318,10 @@ __global__ void __launch_bounds__(128, 4) write_kernel(const WriteArgs a, const 
       for (int s = 0; s < STEPS; ++s)
         if (h0 + s * at_once < heads) {
           if (in) col[s].turn(bias ? bias + (h0 + s * at_once) * D + 8 * c : nullptr, there ? &cs : nullptr, half);
+        }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (h0 + s * at_once < heads) {
           T* p = out + at + (long long)s * at_once * D;
           st_v4(p, col[s].lo);
           st_v4(p + half, col[s].hi);
@@ -348,7 +360,7 @@ __global__ void __launch_bounds__(128) pack_kernel(const WriteArgs a, const FlKv
       return Columns<T>{ld_v4(p), ld_v4(p + half)};
     };
     write_page<T>(reinterpret_cast<uint8_t*>(is_v ? kv.v : kv.k) + cell * bs * D, (is_v ? kv.v_scale : kv.k_scale) + cell, true, 0, n, D, row,
-                  [](int, int, Columns<T>&) {}, row);
+                  [](int, int, Columns<T>&) {}, [](int, int, const Columns<T>&) {}, row);
   }
 }
 
