@@ -488,6 +488,16 @@ def test_evict_on_the_cpu_is_the_same():
     assert all(torch.equal(x.cpu(), y) for x, y in zip(a, b))
 
 
+def test_evict_of_lengths_beyond_32_bits():
+    from fuselink_b200.ops import kv8
+    lens = torch.tensor([2 ** 40 + 3, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 5, 0])
+    for pages, bs in ((12, 16), (3, 2 ** 30), (4, 2 ** 29 + 1)):
+        mass = torch.rand(5, pages, generator=torch.Generator().manual_seed(3))
+        table = torch.arange(5 * pages, dtype=torch.int32).view(5, pages)
+        for a, b in zip(kv8.evict(mass.cuda(), table.cuda(), lens.cuda(), bs, 2), kv8.evict(mass, table, lens, bs, 2)):
+            assert torch.equal(a.cpu(), b)
+
+
 # ---- together --------------------------------------------------------------------------------------------------------------------
 def test_decoding_over_an_evicted_cache():
     """Prompt, weights, eviction, then new tokens behind the kept pages: what is left is attended to as by definition, and freed pages are used again."""
