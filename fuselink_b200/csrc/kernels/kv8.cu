@@ -81,7 +81,7 @@ __device__ __forceinline__ int page_id(const FlKv8& kv, int b, int page) {
 // magnitude and writing codes; larger pages are read again.  16 x 2048 tokens of 32 + 2 x 8 heads of 128: 254 us with a query's columns and angles
 // looked up one by one, now 186 (136 of bytes); 5 x 389 ragged ones of 32 + 2 x 32 heads of 64: 18.6 us (7.0).  With 128 registers, for the four steps, an SM
 // has 16 warps; 96 spill (253 us), two steps in registers and the others read again take 206, queries in a launch of their own 180 to 193.  A warp's
-// next rows copied to shared memory while it works on these: 176 and 23.3 us, since a row's place is worked out twice.
+// next rows copied to shared memory while it works on these, by a grid that stays: 176 us, but 23.3 for the ragged ones.
 constexpr int STEPS = 4;
 
 struct WriteArgs {
