@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const FlSampleArgs a, i
     uint4 u[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (i0 + k * THREADS < vecs) u[k] = ld_nc_v4(xv + (i0 + k * THREADS) * 8);
+      if (i0 + k * THREADS < vecs) u[k] = ld_stream_v4(xv + (i0 + k * THREADS) * 8);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (i0 + k * THREADS >= vecs) break;
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const FlSampleArgs a, i
     uint4 u[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if ((k0 + k) * THREADS + tid < vecs) u[k] = ld_nc_v4(xv + ((k0 + k) * THREADS + tid) * 8);
+      if ((k0 + k) * THREADS + tid < vecs) u[k] = ld_stream_v4(xv + ((k0 + k) * THREADS + tid) * 8);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       uint32_t m = 0;

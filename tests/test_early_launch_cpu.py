@@ -114,3 +114,14 @@ def test_an_epilogue_warp_goes_on_together_behind_a_wait(kernel):
     body = text[start:text.index("\n}\n", start)]
     epilogue = body[body.index("half = (warp - 2) >> 2"):]
     assert "mbar_wait_warp(" in epilogue and "mbar_wait(" not in epilogue
+
+
+@pytest.mark.parametrize("name,kernels", [("sampling.cu", {"sample_kernel"})])
+def test_nor_by_kernels_that_follow_the_decoders(name, kernels):
+    """As for the decoder's passes: what they read may be the output of the kernel before."""
+    functions = _functions(name)
+    early = [k for k, body in functions.items() if "grid_dep_wait()" in body]
+    assert set(early) == kernels
+    for k in early:
+        for n, body in _reached(functions, k).items():
+            assert not re.search(r"ld_nc|\.nc\b|__ldg|__restrict__", body), f"{name}: {n}, reached from {k}"

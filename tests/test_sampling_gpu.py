@@ -147,3 +147,25 @@ def test_calls_that_are_refused():
             sample(*a)
     tokens, logprobs = sample(x[:0], u[:0])
     assert tokens.shape == (0,) and logprobs.shape == (0,)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 50257), (5, 32000), (16, 128256)])
+def test_draws_behind_a_product_see_all_of_it(rows, vocab):
+    """The decoder's last product and the draw, one after the other over and over, the product's output in memory that the last one's held: the draw is
+    on the GPU while the product stores."""
+    from fuselink_b200 import C
+    from fuselink_b200.ops.sampling import sample
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.randn(vocab, 256, generator=g, device="cuda").to(torch.bfloat16)
+    xs = [torch.randn(rows, 256, generator=g, device="cuda").to(torch.bfloat16) / 4 for _ in range(40)]
+    u = _u(rows, seed=4)
+    want = []
+    for x in xs:
+        logits = C.dec_product(x, w, None, 3, True)
+        torch.cuda.synchronize()
+        want.append(sample(logits, u, 0.8, 0, 0.95))
+        torch.cuda.synchronize()
+    got = [sample(C.dec_product(x, w, None, 3, True), u, 0.8, 0, 0.95) for x in xs]
+    torch.cuda.synchronize()
+    for (a, p), (b, q) in zip(got, want):
+        assert torch.equal(a, b) and torch.equal(p, q)
