@@ -93,14 +93,14 @@ struct WriteArgs {
   const void* src_v; const int* src_table; int src_stride, src_blocks;
 };
 
-struct Angles {                               // of a lane's columns
+struct Angles {                               // of a lane's columns; read as what a kernel before may have written
   float co[8], si[8];
   __device__ __forceinline__ void load(const float* rope, int dim, int c) {
     const float4* a = reinterpret_cast<const float4*>(rope + 8 * c);
     const float4* b = reinterpret_cast<const float4*>(rope + dim / 2 + 8 * c);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float4 u = __ldg(a + i), v = __ldg(b + i);
+      const float4 u = a[i], v = b[i];
       co[4 * i] = u.x; co[4 * i + 1] = u.y; co[4 * i + 2] = u.z; co[4 * i + 3] = u.w;
       si[4 * i] = v.x; si[4 * i + 1] = v.y; si[4 * i + 2] = v.z; si[4 * i + 3] = v.w;
     }

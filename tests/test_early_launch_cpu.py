@@ -116,7 +116,7 @@ def test_an_epilogue_warp_goes_on_together_behind_a_wait(kernel):
     assert "mbar_wait_warp(" in epilogue and "mbar_wait(" not in epilogue
 
 
-@pytest.mark.parametrize("name,kernels", [("sampling.cu", {"sample_kernel"})])
+@pytest.mark.parametrize("name,kernels", [("sampling.cu", {"sample_kernel"}), ("kv8.cu", {"write_kernel", "attention_kernel", "finish_kernel"})])
 def test_nor_by_kernels_that_follow_the_decoders(name, kernels):
     """As for the decoder's passes: what they read may be the output of the kernel before."""
     functions = _functions(name)
