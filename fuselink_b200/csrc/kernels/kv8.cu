@@ -242,12 +242,13 @@ __global__ void __launch_bounds__(128, 4) write_kernel(const WriteArgs a, const 
       const int n = a.counts ? (int)min(max(a.counts[b], 0ll), (long long)a.tokens) : a.tokens;
       // tokens [from, to) of the request's are in this page
       int from, to, lead, page;
-      bool inside = st >= 0 && st + n <= cap;
+      const bool inside = st >= 0 && st <= cap - n;             // in this order: st may be any number
       if (inside) {
+        const int used = (int)st % bs;          // of the first page, before them
         page = (int)st / bs + pi;
-        lead = pi == 0 ? (int)st % bs : 0;
-        from = pi == 0 ? 0 : page * bs - (int)st;
-        to = min(n, (page + 1) * bs - (int)st);
+        lead = pi == 0 ? used : 0;
+        from = pi == 0 ? 0 : pi * bs - used;
+        to = min(n, (pi + 1) * bs - used);
       } else {                                  // no pages to write to: the rows are still turned
         page = 0; lead = 0;
         from = (int)min((long long)pi * bs, (long long)n);
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(128, 4) write_kernel(const WriteArgs a, const 
       const int id = inside ? page_id(kv, b, page) : -1;
       if (inside && id < 0 && lane == 0) note(kv.status, FL_DEC_BAD_PAGE);
       const int head = a.heads + (is_v ? kv.heads : 0) + kh;
-      const long long turn = (a.pos ? a.pos[b] : st) + from;
+      const long long turn = min(a.pos ? a.pos[b] : st, a.rope_rows) + from;
       const long long first = ((long long)b * a.tokens + from) * all + head;
       const long long cell = ((long long)kv.layer * kv.num_blocks + max(id, 0)) * kv.heads + kh;
       uint8_t* dst = reinterpret_cast<uint8_t*>(is_v ? kv.v : kv.k) + cell * bs * D;
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(128, 4) write_kernel(const WriteArgs a, const 
     if ((!in || (bias == nullptr && a.rope == nullptr)) && src == out) continue;
     const int at_once = 32 / chunks, tk = lane / chunks, c = lane - tk * chunks, heads = in ? a.heads : all;
     if (tk >= at_once) continue;
-    const long long turn = (a.pos ? a.pos[b] : a.start[b]) + t;
+    const long long turn = min(a.pos ? a.pos[b] : a.start[b], a.rope_rows) + t;
     const bool there = in && a.rope != nullptr && turn >= 0 && turn < a.rope_rows;
     if (in && a.rope != nullptr && !there) note(kv.status, FL_DEC_BAD_POSITION);
     Angles cs;
@@ -478,10 +479,12 @@ __device__ __forceinline__ uint2 lds_v2(uint32_t addr) {
 __device__ __forceinline__ int tokens_of(const long long* counts, int b, int tokens) {
   return counts ? (int)min(max(counts[b], 0ll), (long long)tokens) : tokens;
 }
+// the request's first new slot; one behind the table as the table's end, so that sums with it fit
+__device__ __forceinline__ long long start_of(const AttArgs& a, const FlKv8& kv, int b) { return min(a.start[b], (long long)kv.table_stride * kv.block_size); }
 // slots that the request's new tokens see, the last one's own among them; at most the table's
 __device__ __forceinline__ int seen_by_last(const AttArgs& a, const FlKv8& kv, int b) {
   const int n = tokens_of(a.counts, b, a.tokens);
-  return n == 0 ? 0 : (int)min(max(a.start[b] + n, 0ll), (long long)kv.table_stride * kv.block_size);
+  return n == 0 ? 0 : (int)min(max(start_of(a, kv, b) + n, 0ll), (long long)kv.table_stride * kv.block_size);
 }
 
 // parts' outputs are means (divided by their sums), so that joining them overflows nowhere
@@ -520,7 +523,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   if (a.early) {
     // a look ahead, before the wait for the kernel that writes queries and the new tokens' pages: the first units asked into L2, a line per
     // lane.  Whatever it finds only says what is worth having there; all of it is read again behind the wait.
-    const long long n = __ldcg(a.start + b) + a.tokens, bytes = (long long)SIZE * D;
+    const long long n = min(__ldcg(a.start + b), (long long)kv.table_stride * bs) + a.tokens, bytes = (long long)SIZE * D;
     const Ids ahead = look_up(first);
 #pragma unroll
     for (int i = 0; i < R::STAGES - 1; ++i)
@@ -538,7 +541,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   }
   grid_dep_wait();
   Ids ids = look_up(first);
-  const long long start = a.start[b];
+  const long long start = start_of(a, kv, b);
   const int n_new = tokens_of(a.counts, b, a.tokens);
   uint4 q_raw[NT][KJ][2];
 #pragma unroll
@@ -1005,7 +1008,7 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
     const long long at = ((long long)b * rows + row) * parts;
     const Joined j = joined(a, at, parts, lane);
     const float f = j.sum == 0.f ? 0.f : 1.f / j.sum;
-    const bool none = tok >= tokens_of(a.counts, b, a.tokens) || a.start[b] + tok < 0;
+    const bool none = tok >= tokens_of(a.counts, b, a.tokens) || start_of(a, kv, b) + tok < 0;
     const int d = threadIdx.x;
     const float* part = a.part_o + at * D + min(d, D - 1);
     float acc = 0.f;
@@ -1024,7 +1027,7 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
   const int n_new = tokens_of(a.counts, b, a.tokens);
   auto keep = [&](int r, float m, float sum) {
     const int tok = (r % all_rows) / a.group;
-    s_row[r] = make_float2(m, tok >= n_new || a.start[b] + tok < 0 ? 0.f : sum == 0.f ? NAN : 1.f / sum);
+    s_row[r] = make_float2(m, tok >= n_new || start_of(a, kv, b) + tok < 0 ? 0.f : sum == 0.f ? NAN : 1.f / sum);
   };
   if (parts == 1) {
     for (int r = threadIdx.x; r < rows; r += 128) {
@@ -1240,7 +1243,7 @@ static bool aligned(std::initializer_list<const void*> pointers) {
 }
 static bool sizes_fit(const FlKv8* kv) {
   return kv->dim % 16 == 0 && kv->dim >= 16 && kv->dim <= 128 && kv->heads >= 1 && kv->block_size >= 1 && kv->num_blocks >= 0 && kv->layers >= 1 &&
-         kv->table_stride >= 0 && (long long)kv->table_stride * kv->block_size <= 0x3fffffffll;
+         kv->table_stride >= 0 && (long long)kv->table_stride * kv->block_size <= 0x3fffffffll && (long long)kv->block_size * kv->dim <= 0x7fffffffll;
 }
 static unsigned grid_of(long long warps) {
   const long long ctas = (warps + 3) / 4;
@@ -1262,7 +1265,7 @@ extern "C" int fl_kv8_write(int dtype, const void* qkv, void* out, const void* b
   fl::kv8::WriteArgs a = {};
   a.src = qkv; a.out = out; a.bias = bias; a.rope = rope; a.rope_rows = rope_rows;
   a.start = start; a.pos = pos; a.counts = counts; a.batch = batch; a.tokens = tokens; a.heads = heads;
-  a.reach = (tokens + kv->block_size - 2) / kv->block_size + 1;
+  a.reach = (int)(((long long)tokens + kv->block_size - 2) / kv->block_size + 1);
   const long long page_units = 2ll * batch * a.reach * kv->heads, rows = (long long)batch * tokens;
   const bool q = qkv != out || bias != nullptr || rope != nullptr;
   const int per_warp = fl::kv8::STEPS * (32 / (kv->dim / 16));       // heads

@@ -16,7 +16,7 @@ struct FlKv8 {
 
 constexpr int FL_KV8_MASS_ROWS = 6 * 1024;   // new tokens times heads of a call that asks for pages' weights
 
-// dim: a multiple of 16, at most 128.  Tensors start at a multiple of 16 bytes.  Calls return 0, a cudaError, or < 0 for arguments they do
+// dim: a multiple of 16, at most 128; a page of a head at most 2^31 - 1 codes, a table at most 2^30 - 1 slots.  Tensors start at a multiple of 16 bytes.  Calls return 0, a cudaError, or < 0 for arguments they do
 // not take (-1 type, -2 sizes, -4 addresses); nothing is launched then.
 #ifdef __cplusplus
 extern "C" {

@@ -327,3 +327,13 @@ def test_scratch_covers_every_part(lib):
         plain, mass = (lib.fl_kv8_attention_scratch(I(batch), I(tokens), I(heads), kv, I(m)) for m in (0, 1))
         assert plain % 16 == 0 and mass >= plain + 8 * batch * tokens * heads * stride
     assert math.isfinite(plain)
+
+
+def test_c_entries_refuse_pages_beyond_32_bits(lib):
+    """Places in a page are 32-bit numbers."""
+    for dim, bs, stride in ((16, 1 << 27, 1), (128, 1 << 24, 2), (64, (1 << 31) - 1, 0)):
+        kv = _kv(bs=bs, dim=dim, stride=stride)
+        assert lib.fl_kv8_write(I(0), P(A0), P(A0), P(), P(), LL(0), P(8), P(), P(), I(1), I(1), I(4), kv, P()) == -2
+        assert lib.fl_kv8_attention(I(0), P(A0), LL(64), LL(64), LL(64), P(8), P(), I(1), I(1), I(4), F32(1), kv, P(A0), P(), P(A0), P()) == -2
+        assert lib.fl_kv8_pack(I(0), P(A0), P(A0), I(4), P(8), I(4), P(8), I(1), kv, P()) == -2
+    assert lib.fl_kv8_write(I(0), P(A0), P(A0), P(), P(), LL(0), P(8), P(), P(), I(0), I(1), I(4), _kv(bs=1 << 24, dim=64, stride=2), P()) == 0

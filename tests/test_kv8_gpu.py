@@ -599,3 +599,28 @@ def test_calls_that_are_refused():
     empty = kv8.attention(cache, 0, q[:0], table[:0], start[:0])
     assert empty.shape == (0, 1, 256) and kv8.attention(cache, 0, q[:, :0], table, start).shape == (2, 0, 256)
     assert [t.shape[0] for t in kv8.evict(torch.zeros(0, 4, device="cuda"), table[:0], start[:0], 16, 2)] == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("where", [2 ** 63 - 1, 2 ** 63 - 3, 2 ** 62, 2 ** 31 - 1, -2 ** 63])
+def test_slots_and_positions_at_the_ends_of_64_bits(where):
+    """Slots that are none of the table's are written nowhere and noted, rotations that are not there are left out and noted, however far away; an
+    attention from behind the table sees all of it."""
+    from fuselink_b200.ops import kv8
+    cache, table = _cache(1, 8, 2, 16, 64), _table(2, 3, 8)
+    x, rope = _randn(2, 20, 8, 64, seed=3, dt=BF), torch.full((90, 64), 2.0, device="cuda")
+    before, word = [t.clone() for t in cache.tensors()], torch.zeros(1, dtype=torch.int32).pin_memory()
+    out = kv8.write(cache, 0, x, table, _ints([where, 47]), positions=_ints([0, where]), counts=_ints([20, 0]), status=word.data_ptr())
+    torch.cuda.synchronize()
+    assert int(word) == 2 and torch.equal(out, x)
+    for a, b in zip(before, cache.tensors()):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    word.zero_()
+    out = kv8.write(cache, 0, x, table, _ints([3, 20]), positions=_ints([where, where]), rope=rope, status=word.data_ptr())
+    torch.cuda.synchronize()
+    assert int(word) == 2 and torch.equal(out, x)
+    q = x[:, :5, :4]
+    got = kv8.attention(cache, 0, q, table, _ints([where, 30]), counts=_ints([5, 2]))
+    if where < 0:
+        assert got[0].abs().max() == 0
+    else:
+        assert torch.equal(got, kv8.attention(cache, 0, q, table, _ints([48, 30]), counts=_ints([5, 2])))
