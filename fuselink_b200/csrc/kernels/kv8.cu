@@ -1046,7 +1046,10 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
     float sum = 0.f;
     for (int i = 0; i < a.per_page; ++i) {
       const float2* w = a.unit_s + ((long long)b * a.units + p * a.per_page + i) * rows;
-      for (int r = lane; r < rows; r += 32) sum += w[r].x * exp2_fast(w[r].y - s_row[r].x) * s_row[r].y;
+      for (int r = lane; r < rows; r += 32) {
+        const float2 row = s_row[r];
+        if (row.y != 0.f) sum += w[r].x * exp2_fast(w[r].y - row.x) * row.y;         // what a row that sees nothing left may be NaN
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);

@@ -624,3 +624,31 @@ def test_slots_and_positions_at_the_ends_of_64_bits(where):
         assert got[0].abs().max() == 0
     else:
         assert torch.equal(got, kv8.attention(cache, 0, q, table, _ints([48, 30]), counts=_ints([5, 2])))
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads,kv_heads,tokens,lens", [(8, 2, 4, [200, 130]), (4, 1, 9, [3000, 40]), (64, 8, 2, [100, 5])])
+def test_what_stands_in_padding_reaches_no_pages_weight(heads, kv_heads, tokens, lens, what):
+    """Rows behind a request's count are whatever they are: outputs and weights as with any others, and eviction sees numbers.  So are rows of tokens before slot 0."""
+    from fuselink_b200.ops import kv8
+    each = max(lens) // 16 + 2
+    cache, table = _cache(1, 2 * each, kv_heads, 16, 64), _table(2, each, 2 * each)
+    q = _randn(2, tokens, heads, 64, seed=4, dt=BF)
+    counts, got = [1, tokens - 1], []
+    start = [n - c for n, c in zip(lens, counts)]
+    for fill in (0.5, what):
+        for b, c in enumerate(counts):
+            q[b, c:] = fill
+        mass = torch.zeros(2, each, device="cuda")
+        got.append((kv8.attention(cache, 0, q, table, _ints(start), counts=_ints(counts), mass=mass), mass))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    want, weights, may = _want_attention(cache, 0, q, table, start, counts)
+    _check(got[1][0], want, may, BF)
+    assert ((got[1][1].double() - weights).abs() <= 1e-4 * weights + 1e-12).all()
+    q[:] = _randn(2, tokens, heads, 64, seed=5, dt=BF)
+    q[:, :tokens - 1] = what                                           # all but the last, which sees slot 0
+    mass = torch.zeros(2, each, device="cuda")
+    out = kv8.attention(cache, 0, q, table, _ints([1 - tokens] * 2), mass=mass)
+    want, weights, may = _want_attention(cache, 0, q, table, [1 - tokens] * 2, [tokens] * 2)
+    _check(out, want, may, BF)
+    assert (mass[:, 0] - heads).abs().max() <= 1e-4 and mass[:, 1:].abs().max() == 0
