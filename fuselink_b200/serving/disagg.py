@@ -82,6 +82,7 @@ class ServeParams:
     seed: int = 0
 
     EVICT_SINKS, EVICT_RECENT = 1, 2        # pages that are never given back
+    PREFILL, DECODE = 0, 1                  # stages
 
     def check(self) -> None:
         if self.kv_bits not in (8, 16):
@@ -95,9 +96,10 @@ class ServeParams:
             return None
         return Sampler(torch.zeros(batch, device=device), self.temperature, self.top_k, self.top_p, self.min_p)
 
-    def numbers(self, device) -> torch.Generator:
-        """The source of a stage's uniform numbers, the same one on every shard."""
-        return torch.Generator(device=device).manual_seed(self.seed)
+    def numbers(self, device, stage: int = PREFILL) -> torch.Generator:
+        """The source of a stage's uniform numbers, the same one on every shard, another one in every stage: with one for both, a request's first and second
+        token would be drawn by the same number."""
+        return torch.Generator(device=device).manual_seed((self.seed + stage * 0x9E3779B97F4A7C15) % 2 ** 64)
 
     @property
     def elem_bytes(self) -> int:
@@ -243,7 +245,7 @@ class PrefillStage:
         self.dev = dev
         self.hdr = torch.zeros(HDR_INTS, dtype=torch.int64, device=dev)
         p.check()
-        self.choose, self.numbers = p.sampler(B, dev), p.numbers(dev)
+        self.choose, self.numbers = p.sampler(B, dev), p.numbers(dev, p.PREFILL)
 
     def first_tokens(self, tokens: torch.Tensor, on_layer_done=None) -> torch.Tensor:
         """The prompts through the model, into the stage's own pools."""
@@ -323,7 +325,7 @@ class DecodeStage:
         self.g_step = torch.zeros(1, dtype=torch.long, device=dev)
         p.check()
         self.small = SmallCache(p, model, link) if p.kv_bits == 8 else None
-        self.choose, self.numbers = p.sampler(B, dev), p.numbers(dev)
+        self.choose, self.numbers = p.sampler(B, dev), p.numbers(dev, p.DECODE)
         self.g_u = None if self.choose is None else torch.zeros_like(self.g_hist, dtype=torch.float32)      # what every step draws by
 
     def _step(self, tokens, pos):

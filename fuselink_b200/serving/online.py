@@ -121,7 +121,7 @@ class OnlinePrefill:
         self.batches = 0
         self.stats: List[BatchStats] = []
         p.check()
-        self.numbers = p.numbers(dev)
+        self.numbers = p.numbers(dev, p.PREFILL)
 
     def serve_batch(self, reqs: List[Request]) -> BatchStats:
         p, m = self.p, self.p.model
@@ -208,7 +208,7 @@ class OnlineDecode:
         self.done_on = [0] * len(links)
         p.check()
         self.small = SmallCache(p, model, links[0]) if p.kv_bits == 8 and model is not None else None
-        self.numbers = p.numbers(links[0].k_pool.local.device)
+        self.numbers = p.numbers(links[0].k_pool.local.device, p.DECODE)
 
     def serve_batch(self, max_steps: int) -> dict:
         p = self.p

@@ -337,3 +337,36 @@ def test_c_entries_refuse_pages_beyond_32_bits(lib):
         assert lib.fl_kv8_attention(I(0), P(A0), LL(64), LL(64), LL(64), P(8), P(), I(1), I(1), I(4), F32(1), kv, P(A0), P(), P(A0), P()) == -2
         assert lib.fl_kv8_pack(I(0), P(A0), P(A0), I(4), P(8), I(4), P(8), I(1), kv, P()) == -2
     assert lib.fl_kv8_write(I(0), P(A0), P(A0), P(), P(), LL(0), P(8), P(), P(), I(0), I(1), I(4), _kv(bs=1 << 24, dim=64, stride=2), P()) == 0
+
+
+@pytest.mark.parametrize("online", [False, True])
+@pytest.mark.parametrize("seed", [0, 5, -1, 2 ** 63 - 1])
+def test_every_token_is_drawn_by_numbers_of_its_own(online, seed, monkeypatch):
+    """First tokens and the following ones come from two stages; what one draws by, the other does not."""
+    import cpu_kernel_model
+    from fuselink_b200.parallel.symm import SymmetricHeap
+    from fuselink_b200.serving.disagg import DecodeStage, KVLink, PrefillStage, ServeParams, make_prompts
+    from fuselink_b200.serving.online import OnlineDecode, OnlinePrefill, Request
+    p = ServeParams(model=MODEL_ZOO["tiny"], batch_size=3, input_len=32, num_decoding_step=4, temperature=1.0, seed=seed)
+    seen, call = [], Sampler.__call__
+    monkeypatch.setattr(Sampler, "__call__", lambda self, logits: (seen.append(self.u.clone()), call(self, logits))[1])
+    heaps = SymmetricHeap.emulated(2, 32 << 20)
+    try:
+        with cpu_kernel_model.installed():
+            net = LlamaShard(p.model, device="cpu", seed=1)
+            if online:
+                links = [[KVLink(h, p, net.kvh_local, name=f"kv{i}") for i in range(2)] for h in heaps]
+                pre, dec = OnlinePrefill(p, net, links[0], dst_rank=1), OnlineDecode(p, net, links[1], src_rank=0)
+                for batch in range(2):
+                    pre.serve_batch([Request(0.0, 20, 20, 4) for _ in range(3)])
+                    dec.serve_batch(4)
+            else:
+                links = [KVLink(h, p, net.kvh_local) for h in heaps]
+                pre, dec = PrefillStage(p, net, links[0], dst_rank=1), DecodeStage(p, net, links[1])
+                for batch in range(2):
+                    pre.run(make_prompts(p, "cpu", seed=3))
+                    dec.run()
+    finally:
+        for h in heaps:
+            h.close()
+    assert len(seen) == 2 * (1 + 4) and torch.cat(seen).unique().numel() == 2 * (1 + 4) * 3
