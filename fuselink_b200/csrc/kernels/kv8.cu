@@ -372,15 +372,20 @@ __global__ void __launch_bounds__(128) pack_kernel(const WriteArgs a, const FlKv
 // times weights), the query rows that share the KV head (heads of the group, and new tokens) the 8 NT columns of both, so that no product
 // is spent on padding of a group of 8.  As in decoder.cu the orders that the products do not fix are chosen for 16-byte loads: lane t of a quad takes
 // columns 16 t .. 16 t + 15 of each 64 of a key, lane group g columns DP / 8 g .. of a value.  Codes become halves exactly; queries are
-// brought into their range by a power of two per row, which loses nothing that counts beside the row's largest (2^-40 of it); weights
-// are rounded to 11 bits for the second product, their sum is not.
+// brought into their range by a power of two per row, which loses nothing that counts beside the row's largest (2^-40 of it).
 //
-// What a step of 16 tokens costs beside its 16 products and 64 conversions is kept out of the loop: the maximum that the weights refer to only
-// follows when a score is 2^8 beyond it (a vote, not a reduction, per step), and the sums of the second product stay in units of the largest
-// value scale seen, which a page's weights are brought to where its own is smaller (scales are powers of two).  With a maximum per step and a
+// Weights times their page's scale of values meet the codes as halves, in a unit per row that follows the largest such product: what a page has no
+// weight for takes no bits from the others, however large its values, and what lies below 2^-26 of the largest is lost.  A half has 11 bits.
+// Where a KV head has four rows or fewer, the columns that are left have what is beyond them: 22 bits, and the output's error is that of sums in
+// 32 bits.  Elsewhere the sum that the output is divided by is that of the weights as they were cut, so that what the cuts have in common cancels; as
+// further products the bits beyond would cost 48 ragged requests of eight rows 64.5 us in place of 61.6, and the output is off by 1.650e-3 of its norm in
+// place of 1.646e-3 (bf16; divided by the sum of uncut weights: 1.70e-3).  Weights of pages are of uncut sums.
+//
+// What a step of 16 tokens costs beside its 16 products and 64 conversions is kept out of the loop: the maximum that the weights refer to and the unit
+// of the products only follow when a score is 2^8 or a page's scale 2^7 beyond them (a vote, not a reduction, per step).  With a maximum per step and a
 // multiplication of every sum by the page's scale, and the codes on their way through registers, 16 x 2048 tokens of 8 KV heads of 128 took
-// 25.6 us, now 17.4 (10.3 of bytes; 2 x 131072 tokens 103, 82 of bytes).  Codes are on their way through a ring in shared memory, two steps ahead
-// of their use, which then never wait: of the 17.4 us some 9 go at the memory's rate, the others are launch, the first page ids and rows (4000 to
+// 25.6 us, now 17.5 (10.3 of bytes; 2 x 131072 tokens 101, 82 of bytes).  Codes are on their way through a ring in shared memory, two steps ahead
+// of their use, which then never wait: of the 17.5 us some 9 go at the memory's rate, the others are launch, the first page ids and rows (4000 to
 // 5000 cycles: a miss each, of pages anywhere in memory), and the joining of warps and CTAs (5000 cycles).
 //
 // A request's context is dealt out evenly over the warps of the CTAs in the grid's third dimension: a cluster of up to 8, which joins their (max, sum,
@@ -389,9 +394,11 @@ constexpr int WARPS = 4;
 constexpr int FEWEST = 2 * WARPS;          // steps that make a CTA worth having
 constexpr int LONGEST = 64 * WARPS;        // steps beyond which a context is cut even where there are CTAs enough: ragged batches end together
 constexpr int MOST_PARTS = 64;             // two for a lane of the kernel that joins them
-constexpr int PART = 2;                    // floats of a part besides its output: maximum, sum
+constexpr int PART = 4;                    // floats of a part besides its output: maximum, sum of the weights as they meet the values, sum as they are
 constexpr float LOWEST = -3e38f;           // a maximum of nothing: masked scores are -inf, which is below it
-constexpr float SLACK = 8.f;               // log2 of the largest weight; halves hold 2^15
+constexpr float SLACK = 8.f;               // log2 of the largest weight, whose reference only follows when a score is beyond it
+constexpr float ROOM = 7.f;                // log2 of the largest page's scale in the column's unit: halves hold 2^(SLACK + ROOM)
+constexpr float START = 3.f;               // log2 of the largest weight times its page's scale, in a unit that has just been chosen
 
 struct AttArgs {
   const void* q; long long sb, st, sh;
@@ -420,6 +427,12 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {              // an 
 __device__ __forceinline__ uint32_t half2_of(float a, float b) {
   __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ float eleven_bits(float x, uint32_t keep = 0xffffe000u) { return __uint_as_float(__float_as_uint(x) & keep); }     // cut to what a half holds
+__device__ __forceinline__ uint32_t half2_cut(float a, float b) {
+  uint32_t r;
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {                     // the hardware's: 2^-22 off, relatively; 0 below 2^-126
   float r;
@@ -492,19 +505,22 @@ __device__ __forceinline__ float share(float m, float l, float mm) { return l ==
 
 // DP: head dimension rounded up to 64 or 128.  FULL: it is that, in pages of whole 16s.  HALVES: pages that are not, whose steps are two halves of up to
 // eight tokens, from pages and with scales of their own: with steps of one page, pages of 8 took 1.9 times and pages of 5 three times as long.
-template <typename T, int DP, int NT, bool FULL, bool HALVES, bool MASS>
+template <typename T, int DP, int NT, bool BOTH, bool FULL, bool HALVES, bool MASS>
 __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(const AttArgs a, const FlKv8 kv) {
   using R = Ring<DP>;
   constexpr int KJ = DP / 64, MT = DP / 16, VB = DP / 8, ROWS = 8 * NT, LD = DP + 4;
   static_assert(WARPS * ROWS * LD * 4 <= R::BYTES, "the warps' parts take the rings' place");
   extern __shared__ __align__(16) uint8_t s_ring[];
   auto s_o = reinterpret_cast<float(*)[ROWS][LD]>(s_ring);
-  __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_cm[ROWS], s_cl[ROWS];
+  __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_x[WARPS][ROWS], s_cm[ROWS], s_cl[ROWS], s_cx[ROWS];
   grid_dep_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int kh = blockIdx.x / a.row_parts, rp = blockIdx.x - kh * a.row_parts, b = blockIdx.y, z = blockIdx.z;
   const int D = FULL ? DP : kv.dim, bs = kv.block_size, all_rows = a.group * a.tokens, r0 = rp * ROWS;
   const int n_rows = min(ROWS, all_rows - r0);
+  static_assert(!BOTH || NT == 1, "half of the only eight columns");
+  constexpr int COL = BOTH ? 3 : 7;            // a column's row, of eight
+  constexpr bool EXACT = MASS && !BOTH;        // the weights' sums are kept apart from the sums of the weights as they meet the values
   // The warp's units: every nw-th.  Which pages these are does not depend on the context's length, nor do the queries, so that all three are on
   // their way side by side.
   const int nw = a.splits * WARPS, first = z * WARPS + warp;
@@ -546,7 +562,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   uint4 q_raw[NT][KJ][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int r = r0 + 8 * nt + g, tok = a.tokens == 1 ? 0 : r / a.group, h = r - tok * a.group;
+    const int r = r0 + 8 * nt + (g & COL), tok = a.tokens == 1 ? 0 : r / a.group, h = r - tok * a.group;
     const T* q = reinterpret_cast<const T*>(a.q) + b * a.sb + tok * a.st + (long long)(kh * a.group + h) * a.sh;
 #pragma unroll
     for (int j = 0; j < KJ; ++j) {
@@ -635,6 +651,14 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   for (int nt = 0; nt < NT; ++nt) {
     float f[KJ][16];
     float m = 0.f;
+    if (MASS) {
+      // rows that are no token's count as zeros: whatever stands in them would move the references of the columns beside them, by a rounding
+      const int row = r0 + 8 * nt + (g & COL), tok = a.tokens == 1 ? 0 : row / a.group;
+      if (tok >= n_new || start + tok < 0) {
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) q_raw[nt][j][0] = q_raw[nt][j][1] = make_uint4(0, 0, 0, 0);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < KJ; ++j) {
       float v0[8], v1[8];
@@ -660,14 +684,17 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       factor[nt][c] = __shfl_sync(0xffffffffu, back, (2 * t + c) * 4) * a.scale;
-      const int rc = r0 + 8 * nt + 2 * t + c, tc = a.tokens == 1 ? 0 : rc / a.group;
+      const int rc = r0 + 8 * nt + (2 * t + c & COL), tc = a.tokens == 1 ? 0 : rc / a.group;
       sees[nt][c] = rc < all_rows && tc < n_new ? max((int)min(start + tc + 1, (long long)len), 0) : 0;
       if (sees[nt][c] > 0) fewest = min(fewest, sees[nt][c]);
     }
   }
   fewest = __reduce_min_sync(0xffffffffu, fewest);
 
-  float o[NT][MT][4], m[NT][2], l[NT][2], unit = -200.f;       // unit: log2 of what the sums o are in
+  // A column's sums: weights 2^(score - m) in l (lx: before they were cut), the same times values in o, in units of 2^down.  m and down are whole numbers,
+  // so that neither reference leaves a rounding behind when it moves.
+  float o[NT][MT][4], m[NT][2], l[NT][2], lx[NT][2], down[NT][2];
+  const uint32_t rest = t < 2 ? 0u : 0xffffe000u;              // BOTH: the bits of a weight that are not this column's
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -675,7 +702,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) { m[nt][c] = LOWEST; l[nt][c] = 0.f; }
+    for (int c = 0; c < 2; ++c) { m[nt][c] = LOWEST; l[nt][c] = lx[nt][c] = 0.f; down[nt][c] = LOWEST; }
   }
 
   int stage = 0;
@@ -743,40 +770,36 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
           s[nt][2 + c] = g + 8 - 8 * H1 < min(sees[nt][c] - base[H1], live[H1]) ? s[nt][2 + c] : -INFINITY;
         }
     }
-    float page_unit[H];
+    float page_unit[H];                          // log2 of the values' scale
+#pragma unroll
+    for (int h = 0; h < H; ++h) page_unit[h] = (float)((int)(__float_as_uint(vs[h]) >> 23) - 127);
+    float wt[NT][4];                             // weights, first their logarithms
     bool beyond = false;
+    // -inf stays -inf whatever it meets: a factor of 0 (an underflow, or no page) would make it NaN
+    auto by = [&](int nt, int i) { return fmaxf(factor[nt][i & 1] * ks[i >> 1 ? H1 : 0], 0x1p-126f); };
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      page_unit[h] = (float)((int)(__float_as_uint(vs[h]) >> 23) - 127);
-      beyond |= page_unit[h] > unit && live[h] > 0;
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) wt[nt][i] = fmaf(s[nt][i], by(nt, i), -m[nt][i & 1]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) beyond |= fmaxf(wt[nt][c], wt[nt][2 + c]) > SLACK || fmaxf(page_unit[0], page_unit[H1]) - down[nt][c] > ROOM;
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        // -inf stays -inf whatever it meets: a factor of 0 (an underflow, or no page) would make it NaN
-        const float k0 = fmaxf(factor[nt][c] * ks[0], 0x1p-126f), k1 = HALVES ? fmaxf(factor[nt][c] * ks[H1], 0x1p-126f) : k0, top = m[nt][c] + SLACK;
-        s[nt][c] *= k0;
-        s[nt][2 + c] *= k1;
-        beyond |= s[nt][c] > top || s[nt][2 + c] > top;
-      }
     if (__any_sync(0xffffffffu, beyond)) {
-      float unit_now = unit;
-#pragma unroll
-      for (int h = 0; h < H; ++h)
-        if (live[h] > 0) unit_now = fmaxf(unit_now, page_unit[h]);
-      const float shrink = exp2_fast(unit - unit_now);
-      unit = unit_now;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float f[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const float before = m[nt][c];
-          m[nt][c] = fmaxf(before, max_rows(fmaxf(s[nt][c], s[nt][2 + c])));
-          const float e = exp2_fast(before - m[nt][c]);
+          const float from = m[nt][c], was = down[nt][c];
+          const float s0 = s[nt][c] * by(nt, c), s1 = s[nt][2 + c] * by(nt, 2 + c);
+          m[nt][c] = fmaxf(from, ceilf(max_rows(fmaxf(s0, s1))));
+          wt[nt][c] = s0 - m[nt][c];
+          wt[nt][2 + c] = s1 - m[nt][c];
+          const float fall = from - m[nt][c], e = exp2_fast(fall);
           l[nt][c] *= e;
-          f[c] = e * shrink;
+          if (EXACT) lx[nt][c] *= e;
+          down[nt][c] = fmaxf(was + fall, ceilf(max_rows(fmaxf(wt[nt][c] + page_unit[0], wt[nt][2 + c] + page_unit[H1]))) - START);
+          f[c] = exp2_fast(was - down[nt][c] + fall);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
@@ -788,14 +811,28 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
     uint32_t p0[NT], p1[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float add[2];
+      float add[2], w[4];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        s[nt][c] = exp2_fast(s[nt][c] - m[nt][c]);
-        s[nt][2 + c] = exp2_fast(s[nt][2 + c] - m[nt][c]);
-        add[c] = s[nt][c] + s[nt][2 + c];
-        l[nt][c] += add[c];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          wt[nt][2 * h + c] = exp2_fast(wt[nt][2 * h + c]);
+          w[2 * h + c] = BOTH ? wt[nt][2 * h + c] : eleven_bits(wt[nt][2 * h + c]);
+        }
+        add[c] = wt[nt][c] + wt[nt][2 + c];
+        l[nt][c] += w[c] + w[2 + c];
+        if (EXACT) lx[nt][c] += add[c];
+        // a page whose values are so much larger than what counts has no weight beyond the smallest numbers
+        const float u0 = exp2_fast(fminf(page_unit[0] - down[nt][c], 126.f)), u1 = HALVES ? exp2_fast(fminf(page_unit[H1] - down[nt][c], 126.f)) : u0;
+        w[c] *= u0;
+        w[2 + c] *= u1;
       }
+      if (BOTH) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] -= eleven_bits(w[i], rest);
+      }
+      p0[nt] = transposed(half2_cut(w[0], w[1]));
+      p1[nt] = transposed(half2_cut(w[2], w[3]));
       if (MASS) {
         auto keep = [&](int part, float s0, float s1) {
           s0 = sum_rows(s0);
@@ -807,27 +844,12 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
           }
         };
         if (HALVES) {
-          keep(2 * u, s[nt][0], s[nt][1]);
-          keep(2 * u + 1, s[nt][2], s[nt][3]);
+          keep(2 * u, wt[nt][0], wt[nt][1]);
+          keep(2 * u + 1, wt[nt][2], wt[nt][3]);
         } else {
           keep(u, add[0], add[1]);
         }
       }
-    }
-#pragma unroll
-    for (int h = 0; h < H; ++h)
-      if (page_unit[h] < unit) {                                   // a page of smaller values than the largest
-        const float w = exp2_fast(page_unit[h] - unit);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!HALVES || i / 2 == h) s[nt][i] *= w;
-      }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      p0[nt] = transposed(half2_of(s[nt][0], s[nt][1]));
-      p1[nt] = transposed(half2_of(s[nt][2], s[nt][3]));
     }
     auto values = [&](auto each) {
 #pragma unroll
@@ -860,7 +882,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
           mma(c, a0, a1, a2, a3, p0[nt], p1[nt]);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if ((r0 + 8 * nt + 2 * t + (j & 1)) / a.group == tok) o[nt][i][j] += c[j];
+            if ((r0 + 8 * nt + (2 * t + (j & 1) & COL)) / a.group == tok) o[nt][i][j] += c[j];
         });
       }
     }
@@ -869,15 +891,18 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   __syncthreads();                               // the rings' memory is free
 
   // the warps' parts become one
-  const float scale_o = exp2f(unit);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int row = 8 * nt + 2 * t + c;
-      const float sum = sum_rows(l[nt][c]), f = sum == 0.f ? 0.f : 1.f / sum;
+      const float sum = sum_rows(l[nt][c]), f = sum == 0.f ? 0.f : 1.f / sum, unit = exp2f(down[nt][c]);
       if (g == 0) { s_m[warp][row] = m[nt][c]; s_l[warp][row] = sum; }
-      auto mean = [&](float v) { return v * f * scale_o; };
+      if (EXACT) {
+        const float x = sum_rows(lx[nt][c]);
+        if (g == 0) s_x[warp][row] = x;
+      }
+      auto mean = [&](float v) { return v * f * unit; };
 #pragma unroll
       for (int i = 0; i < MT; i += 2)
         *reinterpret_cast<float4*>(&s_o[warp][row][VB * g + 2 * i]) = make_float4(mean(o[nt][i][c]), mean(o[nt][i][2 + c]), mean(o[nt][i + 1][c]), mean(o[nt][i + 1][2 + c]));
@@ -886,25 +911,35 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
   // Four columns of a row per thread.  `joined4` adds up the warps' means by what they count for in the CTA's.
   const long long row_at = (long long)b * a.heads * a.tokens + kh * all_rows + r0;
   const int pieces = D / 4;
-  auto joined4 = [&](int row, int d, float& mm, float& ll) {
+  auto joined4 = [&](int row, int d, float& mm, float& ll, float& xx) {
     float w[WARPS];
     mm = LOWEST;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) mm = fmaxf(mm, s_m[i][row]);
-    ll = 0.f;
+    ll = xx = 0.f;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) { w[i] = share(s_m[i][row], s_l[i][row], mm); ll += w[i]; }
+    if (EXACT) {
+#pragma unroll
+      for (int i = 0; i < WARPS; ++i) xx += share(s_m[i][row], s_x[i][row], mm);
+    } else {
+      xx = ll;
+    }
     const float f = ll == 0.f ? 0.f : 1.f / ll;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) {
-      const float4 v = *reinterpret_cast<const float4*>(&s_o[i][row][d]);
+      float4 v = *reinterpret_cast<const float4*>(&s_o[i][row][d]);
+      if (BOTH) {
+        const float4 more = *reinterpret_cast<const float4*>(&s_o[i][row + 4][d]);
+        v.x += more.x; v.y += more.y; v.z += more.z; v.w += more.w;
+      }
       const float k = w[i] * f;
       acc.x += k * v.x; acc.y += k * v.y; acc.z += k * v.z; acc.w += k * v.w;
     }
     return acc;
   };
-  auto result = [&](int row, int d, float mm, float ll, float4 acc) {
+  auto result = [&](int row, int d, float mm, float ll, float xx, float4 acc) {
     const int r = r0 + row, tok = a.tokens == 1 ? 0 : r / a.group, h = kh * a.group + r - tok * a.group;
     const bool none = tok >= n_new || start + tok < 0 || len == 0;
     if (none) acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -913,44 +948,44 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
         make_uint2(Typed<T>::pack(acc.x, acc.y), Typed<T>::pack(acc.z, acc.w));
     if (MASS && d == 0) {
       float* p = a.part_s + (row_at + row) * (a.clustered ? 1 : a.splits) * PART;
-      p[0] = mm;
-      p[1] = ll;
+      *reinterpret_cast<float4*>(p) = make_float4(mm, ll, xx, 0.f);
     }
   };
   if (!a.clustered || a.splits == 1) {
     for (int i = threadIdx.x; i < n_rows * pieces; i += WARPS * 32) {
       const int row = i / pieces, d = 4 * (i - row * pieces);
-      float mm, ll;
-      const float4 acc = joined4(row, d, mm, ll);
+      float mm, ll, xx;
+      const float4 acc = joined4(row, d, mm, ll, xx);
       if (a.splits == 1) {
-        result(row, d, mm, ll, acc);
+        result(row, d, mm, ll, xx, acc);
       } else {
         const long long part = (row_at + row) * a.splits + z;
         *reinterpret_cast<float4*>(a.part_o + part * D + d) = acc;
-        if (d == 0) { a.part_s[part * PART] = mm; a.part_s[part * PART + 1] = ll; }
+        if (d == 0) *reinterpret_cast<float4*>(a.part_s + part * PART) = make_float4(mm, ll, xx, 0.f);
       }
     }
     return;
   }
   for (int i = threadIdx.x; i < n_rows * pieces; i += WARPS * 32) {
     const int row = i / pieces, d = 4 * (i - row * pieces);
-    float mm, ll;
-    const float4 acc = joined4(row, d, mm, ll);
+    float mm, ll, xx;
+    const float4 acc = joined4(row, d, mm, ll, xx);
     *reinterpret_cast<float4*>(&s_o[0][row][d]) = acc;         // read and written by this thread alone
-    if (d == 0) { s_cm[row] = mm; s_cl[row] = ll; }
+    if (d == 0) { s_cm[row] = mm; s_cl[row] = ll; s_cx[row] = xx; }
   }
   __syncwarp();
   cluster_sync_all();
   for (int i = z * WARPS * 32 + threadIdx.x; i < n_rows * pieces; i += a.splits * WARPS * 32) {
     const int row = i / pieces, d = 4 * (i - row * pieces);
     const uint32_t am = smem_u32(&s_cm[row]), al = smem_u32(&s_cl[row]), ao = smem_u32(&s_o[0][row][d]);
-    float pm[8], pl[8], mm = LOWEST, ll = 0.f;
+    float pm[8], pl[8], px[8], mm = LOWEST, ll = 0.f;
     float4 po[8], acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int x = 0; x < 8; ++x)
       if (x < a.splits) {
         pm[x] = ld_cluster_f32(map_to_cta(am, x));
         pl[x] = ld_cluster_f32(map_to_cta(al, x));
+        if (EXACT) px[x] = ld_cluster_f32(map_to_cta(smem_u32(&s_cx[row]), x));
         po[x] = ld_cluster_f32x4(map_to_cta(ao, x));
       }
 #pragma unroll
@@ -959,6 +994,12 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
 #pragma unroll
     for (int x = 0; x < 8; ++x)
       if (x < a.splits) { pl[x] = share(pm[x], pl[x], mm); ll += pl[x]; }
+    float xx = EXACT ? 0.f : ll;
+    if (EXACT) {
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (x < a.splits) xx += share(pm[x], px[x], mm);
+    }
     const float f = ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll
     for (int x = 0; x < 8; ++x)
@@ -966,22 +1007,23 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2) attention_kernel(
         const float k = pl[x] * f;
         acc.x += k * po[x].x; acc.y += k * po[x].y; acc.z += k * po[x].z; acc.w += k * po[x].w;
       }
-    result(row, d, mm, ll, acc);
+    result(row, d, mm, ll, xx, acc);
   }
   __syncwarp();
   cluster_sync_all();                            // nobody leaves while its part is being read
 }
 
 struct Joined { float m, sum, w0, w1; };       // of a row's parts: their maximum and sum; what parts `lane` and `lane` + 32 count for in it
+template <int SUM>                              // which of the parts' sums
 __device__ __forceinline__ Joined joined(const AttArgs& a, long long at, int parts, int lane) {
   Joined j;
   float m[2] = {LOWEST, LOWEST}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     if (lane + 32 * i < parts) {
-      const float2 p = *reinterpret_cast<const float2*>(a.part_s + (at + lane + 32 * i) * PART);
+      const float4 p = *reinterpret_cast<const float4*>(a.part_s + (at + lane + 32 * i) * PART);
       m[i] = p.x;
-      l[i] = p.y;
+      l[i] = SUM == 1 ? p.y : p.z;
     }
   j.m = fmaxf(m[0], m[1]);
 #pragma unroll
@@ -1006,7 +1048,7 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
   if ((int)blockIdx.x < row_ctas) {
     const int row = blockIdx.x, kh = row / all_rows, r = row - kh * all_rows, tok = r / a.group, h = kh * a.group + r - tok * a.group;
     const long long at = ((long long)b * rows + row) * parts;
-    const Joined j = joined(a, at, parts, lane);
+    const Joined j = joined<1>(a, at, parts, lane);
     const float f = j.sum == 0.f ? 0.f : 1.f / j.sum;
     const bool none = tok >= tokens_of(a.counts, b, a.tokens) || start_of(a, kv, b) + tok < 0;
     const int d = threadIdx.x;
@@ -1032,11 +1074,11 @@ __global__ void __launch_bounds__(128) finish_kernel(const AttArgs a, const FlKv
   if (parts == 1) {
     for (int r = threadIdx.x; r < rows; r += 128) {
       const float* p = a.part_s + ((long long)b * rows + r) * PART;
-      keep(r, p[0], p[1]);
+      keep(r, p[0], p[2]);
     }
   } else {
     for (int r = threadIdx.x >> 5; r < rows; r += 4) {
-      const Joined j = joined(a, ((long long)b * rows + r) * parts, parts, lane);
+      const Joined j = joined<2>(a, ((long long)b * rows + r) * parts, parts, lane);
       if (lane == 0) keep(r, j.m, j.sum);
     }
   }
@@ -1302,11 +1344,12 @@ extern "C" int fl_kv8_pack(int dtype, const void* k_pool, const void* v_pool, in
 
 // How a call is cut up: enough CTAs for the SMs (four of NT = 1, two of NT = 2 each), as a cluster where 8 per request and KV head are enough.
 namespace {
-struct Cut { int nt, row_parts, per_page, units, splits; bool halves, clustered; };
+struct Cut { int nt, row_parts, per_page, units, splits; bool both, halves, clustered; };
 Cut cut_of(int batch, int tokens, int heads, const FlKv8* kv) {
   Cut c;
   const long long rows = (long long)heads / kv->heads * tokens;
   c.nt = rows > 8 ? 2 : 1;
+  c.both = rows <= 4;
   c.row_parts = (int)((rows + 8 * c.nt - 1) / (8 * c.nt));
   c.halves = kv->block_size % 16 != 0;
   const int size = c.halves ? 8 : 16;
@@ -1327,7 +1370,7 @@ Cut cut_of(int batch, int tokens, int heads, const FlKv8* kv) {
 }
 long long up16(long long bytes) { return (bytes + 15) / 16 * 16; }
 
-template <typename T, int DP, int NT, bool FULL, bool HALVES, bool MASS>
+template <typename T, int DP, int NT, bool BOTH, bool FULL, bool HALVES, bool MASS>
 int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, dim3 grid, bool early, cudaStream_t stream) {
   constexpr int smem = fl::kv8::Ring<DP>::BYTES;
   static bool set_on[64];                          // per device: a process may drive several GPUs
@@ -1336,7 +1379,7 @@ int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, dim3 grid, bool
   if (e != cudaSuccess) return (int)e;
   if (dev < 0 || dev >= 64) return -3;
   if (!set_on[dev]) {
-    e = cudaFuncSetAttribute(fl::kv8::attention_kernel<T, DP, NT, FULL, HALVES, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(fl::kv8::attention_kernel<T, DP, NT, BOTH, FULL, HALVES, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
     set_on[dev] = true;
   }
@@ -1352,14 +1395,16 @@ int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, dim3 grid, bool
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = early ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, fl::kv8::attention_kernel<T, DP, NT, FULL, HALVES, MASS>, a, kv);
+  return (int)cudaLaunchKernelEx(&cfg, fl::kv8::attention_kernel<T, DP, NT, BOTH, FULL, HALVES, MASS>, a, kv);
 }
 template <typename T, int DP>
 int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, const Cut& c, bool mass, dim3 grid, bool early, cudaStream_t stream) {
-#define FL_ATT(N, F, S) return mass ? launch_attention<T, DP, N, F, S, true>(a, kv, grid, early, stream) : launch_attention<T, DP, N, F, S, false>(a, kv, grid, early, stream)
-  if (c.halves) { if (c.nt == 1) FL_ATT(1, false, true); else FL_ATT(2, false, true); }
-  if (kv.dim == DP) { if (c.nt == 1) FL_ATT(1, true, false); else FL_ATT(2, true, false); }
-  if (c.nt == 1) FL_ATT(1, false, false); else FL_ATT(2, false, false);
+#define FL_ATT(N, B, F, S) return mass ? launch_attention<T, DP, N, B, F, S, true>(a, kv, grid, early, stream) : launch_attention<T, DP, N, B, F, S, false>(a, kv, grid, early, stream)
+#define FL_ATT_ROWS(F, S) do { if (c.both) FL_ATT(1, true, F, S); if (c.nt == 1) FL_ATT(1, false, F, S); FL_ATT(2, false, F, S); } while (0)
+  if (c.halves) FL_ATT_ROWS(false, true);
+  if (kv.dim == DP) FL_ATT_ROWS(true, false);
+  FL_ATT_ROWS(false, false);
+#undef FL_ATT_ROWS
 #undef FL_ATT
 }
 }  // namespace

@@ -652,3 +652,46 @@ def test_what_stands_in_padding_reaches_no_pages_weight(heads, kv_heads, tokens,
     want, weights, may = _want_attention(cache, 0, q, table, [1 - tokens] * 2, [tokens] * 2)
     _check(out, want, may, BF)
     assert (mass[:, 0] - heads).abs().max() <= 1e-4 and mass[:, 1:].abs().max() == 0
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,bs,tokens", [(4, 2, 64, 16, 1), (8, 2, 128, 16, 1), (16, 2, 128, 16, 1), (12, 1, 80, 16, 1), (2, 2, 64, 8, 3), (8, 1, 128, 5, 2), (8, 2, 128, 32, 4)])
+@pytest.mark.parametrize("apart", [12, 20, 30, -30, 60])
+@pytest.mark.parametrize("nats", [0.0, 7.0, 14.0, 40.0])
+def test_values_of_different_magnitude(heads, kv_heads, dim, bs, tokens, apart, nats):
+    """Every third page has values 2^apart times the others', and scores `nats` below theirs: what such a page has no weight for takes nothing from the others."""
+    from fuselink_b200.ops import kv8
+    lens = [37 * bs, 5 * bs + 2, 3 * bs]
+    batch, each, dt = len(lens), 37, HF
+    cache, table = _cache(1, batch * each, kv_heads, bs, dim, spread=0.3), _table(batch, each, batch * each)
+    q = _randn(batch, tokens, heads, dim, seed=4).abs().to(dt)
+    # in the far pages every key has -nats for a score: -nats / (scale sum q) in all columns, as near as a code comes to it
+    far = torch.zeros(batch * each, dtype=torch.bool, device="cuda")
+    far[table[:, torch.arange(each, device="cuda") % 3 == 1].flatten().long()] = True
+    key = torch.tensor(-nats / (dim ** 0.5 * 0.8), device="cuda").to(F8)
+    cache.k[0, far], cache.k_scale[0, far] = key, 1.0
+    cache.v_scale[0, far] *= 2.0 ** apart
+    start = [n - tokens for n in lens]
+    mass = torch.zeros(batch, each, device="cuda")
+    out = kv8.attention(cache, 0, q, table, _ints(start), mass=mass)
+    assert torch.equal(out, kv8.attention(cache, 0, q, table, _ints(start)))
+    for b in range(batch):
+        pages = table[b].long()
+        k, v = (_values(c[0][pages], s[0][pages]).transpose(0, 1).reshape(kv_heads, -1, dim).repeat_interleave(heads // kv_heads, 0) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+        scale = cache.v_scale[0][pages].double().transpose(0, 1).repeat_interleave(bs, 1).repeat_interleave(heads // kv_heads, 0)      # [heads, slots]
+        for t in range(tokens):
+            seen = start[b] + t + 1
+            qq = q[b, t].double()
+            p = (torch.einsum("hd,hnd->hn", qq, k[:, :seen]) * dim ** -0.5).softmax(-1)
+            want = torch.einsum("hn,hnd->hd", p, v[:, :seen])
+            # Weights are cut to 11 bits, off by 0 to 2^-10 each: what that has in common cancels against their sum, and 2^-11 to either side of it is left
+            # of the differences between values and output, whose weighed magnitudes are at most twice the values'.  As halves they come in steps of 2^-24
+            # where the largest product of a weight and its page's scale is 2^2 at least: 2^-26 of that for each code of at most 448.  Scores and sums over the
+            # tokens in fp32 as in _want_attention.
+            size = (torch.einsum("hd,hnd->hn", qq.abs(), k[:, :seen].abs()) * dim ** -0.5).amax(-1)
+            relative = 2.0 ** -10 + 2 * (dim + 6) * 2.0 ** -23 * size + (seen + 8) * 2.0 ** -23
+            may = relative[:, None] * torch.einsum("hn,hnd->hd", p, v[:, :seen].abs()) + (seen * 2.0 ** -26 * 448 * (p * scale[:, :seen]).amax(-1))[:, None]
+            got = out[b, t].view(heads, dim).double()
+            there = want.abs() < 65000.0                               # beyond fp16 there is infinity
+            off = (got - want).abs() - may - 2.0 ** -11 * want.abs() * 1.01 - 2.0 ** -25
+            assert (off[there] <= 0).all(), (b, t, off[there].max().item())
+    assert (mass.sum(1) - heads * tokens).abs().max() <= 1e-4 * heads * tokens
