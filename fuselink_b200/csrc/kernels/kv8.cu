@@ -1409,23 +1409,31 @@ int launch_attention(const fl::kv8::AttArgs& a, const FlKv8& kv, const Cut& c, b
 }
 }  // namespace
 
-// More requests than a grid's second dimension takes go in several launches, which use the same scratch one after the other.
+// Requests beyond a grid's second dimension, and those whose scratch would be more than this, go in launches one after the other, which share the
+// scratch: weights cost 8 bytes per row and unit of the table, 4 MB per request of 64 heads and 8192 pages of 16.
 constexpr int MOST_REQUESTS = 65535;
+constexpr long long MOST_SCRATCH = 256ll << 20;
 
-extern "C" long long fl_kv8_attention_scratch(int batch, int tokens, int heads, const FlKv8* kv, int mass) {
-  if (!sizes_fit(kv) || batch < 1 || tokens < 1 || heads < 1 || heads % kv->heads) return 0;
-  if (batch > MOST_REQUESTS) {
-    const long long whole = fl_kv8_attention_scratch(MOST_REQUESTS, tokens, heads, kv, mass);
-    const long long rest = fl_kv8_attention_scratch(batch % MOST_REQUESTS, tokens, heads, kv, mass);
-    return whole > rest ? whole : rest;
-  }
-  const Cut c = cut_of(batch, tokens, heads, kv);
+static long long scratch_of(const Cut& c, int batch, int tokens, int heads, const FlKv8* kv, bool mass) {
   const long long rows = (long long)batch * heads * tokens, parts = c.clustered ? 1 : c.splits;
   long long bytes = 0;
   if (!c.clustered) bytes += up16(rows * parts * kv->dim * 4);
   if (!c.clustered || mass) bytes += up16(rows * parts * fl::kv8::PART * 4);
   if (mass) bytes += up16(rows * c.units * 8);
   return bytes;
+}
+static int at_once(int batch, int tokens, int heads, const FlKv8* kv, bool mass) {
+  int n = batch < MOST_REQUESTS ? batch : MOST_REQUESTS;
+  while (n > 1 && scratch_of(cut_of(n, tokens, heads, kv), n, tokens, heads, kv, mass) > MOST_SCRATCH) n = (n + 1) / 2;
+  return n;
+}
+
+extern "C" long long fl_kv8_attention_scratch(int batch, int tokens, int heads, const FlKv8* kv, int mass) {
+  if (!sizes_fit(kv) || batch < 1 || tokens < 1 || heads < 1 || heads % kv->heads) return 0;
+  const int n = at_once(batch, tokens, heads, kv, mass != 0);
+  const long long whole = scratch_of(cut_of(n, tokens, heads, kv), n, tokens, heads, kv, mass != 0);
+  const long long rest = batch % n == 0 ? 0 : fl_kv8_attention_scratch(batch % n, tokens, heads, kv, mass);
+  return whole > rest ? whole : rest;
 }
 
 extern "C" int fl_kv8_attention(int dtype, const void* q, long long stride_b, long long stride_t, long long stride_h, const long long* start,
@@ -1437,12 +1445,13 @@ extern "C" int fl_kv8_attention(int dtype, const void* q, long long stride_b, lo
   if (mass != nullptr && (long long)heads * tokens > FL_KV8_MASS_ROWS) return -2;   // a CTA of the kernel that adds them up keeps each one's sum in shared memory
   if (!aligned({q, out, scratch, kv->k, kv->v})) return -4;
   if (batch == 0 || tokens == 0) return 0;
-  if (batch > MOST_REQUESTS) {
+  const int once = at_once(batch, tokens, heads, kv, mass != nullptr);
+  if (batch > once) {
     if (dtype != FL_DEC_BF16 && dtype != FL_DEC_FP16) return -1;
-    for (long long b = 0; b < batch; b += MOST_REQUESTS) {
+    for (long long b = 0; b < batch; b += once) {
       FlKv8 part = *kv;
       part.block_table += b * kv->table_stride;
-      const int n = (int)(batch - b < MOST_REQUESTS ? batch - b : MOST_REQUESTS);
+      const int n = (int)(batch - b < once ? batch - b : once);
       const int rc = fl_kv8_attention(dtype, (const uint8_t*)q + 2 * b * stride_b, stride_b, stride_t, stride_h, start + b, counts ? counts + b : nullptr, n, tokens, heads,
                                       scale, &part, (uint8_t*)out + 2 * b * tokens * heads * kv->dim, mass ? mass + b * kv->table_stride : nullptr, scratch, stream);
       if (rc != 0) return rc;

@@ -34,7 +34,8 @@ int fl_kv8_pack(int dtype, const void* k_pool, const void* v_pool, int src_block
 // out [batch][tokens][heads * dim] = softmax(scale q k^T) v of tokens start[b] .. start[b] + counts[b] - 1 (counts null: `tokens` of them) over the
 // slots up to their own; zeros where there is none.  scale: finite, not negative.  q: element strides of (request, token, head).  mass (or null): [batch][table_stride], += the
 // weights' sum over this call's tokens and heads, page by page; tokens * heads is at most FL_KV8_MASS_ROWS then.
-// scratch: fl_kv8_attention_scratch() bytes, from a multiple of 16 on.
+// scratch: fl_kv8_attention_scratch() bytes, from a multiple of 16 on: what one request needs (with weights 8 bytes per token, head and 16 slots of the table, or
+// part of a page), or 256 MiB at most.
 long long fl_kv8_attention_scratch(int batch, int tokens, int heads, const FlKv8* kv, int mass);
 int fl_kv8_attention(int dtype, const void* q, long long stride_b, long long stride_t, long long stride_h, const long long* start,
                      const long long* counts, int batch, int tokens, int heads, float scale, const FlKv8* kv, void* out, float* mass, void* scratch,

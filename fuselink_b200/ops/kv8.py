@@ -102,7 +102,7 @@ def attention(cache: Kv8Cache, layer: int, q: torch.Tensor, block_table: torch.T
     are multiples of 8 elements; token t of request b sees slots 0 .. start[b] + t.  Returns [batch, tokens, heads * dim]; zeros for tokens behind
     ``counts`` and for those that see nothing.  scale (finite, not negative): 1 / sqrt(dim) by default.
     mass ([batch, pages] fp32) has the weights' sum over this call's tokens and heads added, page by page of ``block_table``; on the GPU such a call
-    takes up to 6144 tokens times heads."""
+    takes up to 6144 tokens times heads, and memory while it runs: 8 bytes per request, token, head and 16 slots of the table (at most 256 MiB, or one request's)."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     elif not 0 <= scale < math.inf:

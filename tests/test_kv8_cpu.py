@@ -370,3 +370,12 @@ def test_every_token_is_drawn_by_numbers_of_its_own(online, seed, monkeypatch):
         for h in heaps:
             h.close()
     assert len(seen) == 2 * (1 + 4) and torch.cat(seen).unique().numel() == 2 * (1 + 4) * 3
+
+
+def test_scratch_is_bounded(lib):
+    """A large batch with a wide table goes in pieces that share their scratch: what one request needs, or 256 MiB."""
+    for batch, tokens, heads, stride in ((64, 8, 64, 8192), (65535, 1, 64, 8192), (70000, 4, 8, 1000), (65535, 1, 64, 65535), (3, 96, 64, 8192)):
+        kv = _kv(stride=stride, heads=8, dim=128)
+        for mass in (0, 1):
+            one, all_ = (lib.fl_kv8_attention_scratch(I(b), I(tokens), I(heads), kv, I(mass)) for b in (1, batch))
+            assert 0 <= all_ <= max(1 << 28, one)

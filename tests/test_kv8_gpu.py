@@ -695,3 +695,21 @@ def test_values_of_different_magnitude(heads, kv_heads, dim, bs, tokens, apart, 
             off = (got - want).abs() - may - 2.0 ** -11 * want.abs() * 1.01 - 2.0 ** -25
             assert (off[there] <= 0).all(), (b, t, off[there].max().item())
     assert (mass.sum(1) - heads * tokens).abs().max() <= 1e-4 * heads * tokens
+
+
+def test_a_batch_that_goes_in_pieces():
+    """Weights of 70 requests of 64 heads with tables of 8192 pages: more than one piece's scratch; the last request as much as the first."""
+    from fuselink_b200.ops import kv8
+    B, H, KH, D, each = 70, 64, 8, 16, 8192
+    cache = _cache(1, 400, KH, 16, D)
+    table = torch.randint(0, 400, (B, each), generator=_gen(1), device="cuda").int()
+    lens = [1 + (37 * b) % 90 for b in range(B)]
+    q, mass = _randn(B, 1, H, D, seed=4, dt=HF), torch.zeros(B, each, device="cuda")
+    word = torch.zeros(1, dtype=torch.int32).pin_memory()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = kv8.attention(cache, 0, q, table, _ints(lens) - 1, mass=mass, status=word.data_ptr())
+    assert torch.cuda.max_memory_allocated() - before <= (1 << 28) + 2 * out.nbytes
+    want, weights, may = _want_attention(cache, 0, q, table[:, :6], [n - 1 for n in lens], [1] * B)
+    _check(out, want, may, HF)
+    assert ((mass[:, :6].double() - weights).abs() <= 1e-4 * weights + 1e-12).all() and mass[:, 6:].abs().max() == 0 and int(word) == 0
