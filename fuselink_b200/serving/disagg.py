@@ -84,11 +84,22 @@ class ServeParams:
     EVICT_SINKS, EVICT_RECENT = 1, 2        # pages that are never given back
     PREFILL, DECODE = 0, 1                  # stages
 
-    def check(self) -> None:
+    def check(self, device=None) -> None:
+        """``device``: where the stage runs, if that is known; the kernels take less than the plain forms on the CPU."""
         if self.kv_bits not in (8, 16):
             raise ValueError(f"kv_bits {self.kv_bits}: 8 or 16")
         if self.keep_blocks and (self.kv_bits != 8 or self.keep_blocks < self.EVICT_SINKS + self.EVICT_RECENT):
             raise ValueError(f"keep_blocks {self.keep_blocks}: at least {self.EVICT_SINKS + self.EVICT_RECENT}, of a cache in 8 bits")
+        if device is None or torch.device(device).type != "cuda":
+            return
+        small, drawn = self.kv_bits == 8, self.temperature > 0
+        if (small or drawn) and self.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"{'kv_bits 8' if small else f'temperature {self.temperature}'} with {self.dtype}: bf16 or fp16 on the GPU")
+        if small and (self.model.head_dim % 16 or self.model.head_dim > 128):
+            raise ValueError(f"kv_bits 8 with heads of {self.model.head_dim}: a multiple of 16, at most 128, on the GPU")
+        most = require_native().SAMPLE_MAX_VOCAB
+        if drawn and self.model.vocab > most:
+            raise ValueError(f"temperature {self.temperature} with a vocabulary of {self.model.vocab}: at most {most} on the GPU")
 
     def sampler(self, batch: int, device) -> Optional[Sampler]:
         """What chooses the tokens of a batch; None: the greedy choice."""
@@ -244,7 +255,7 @@ class PrefillStage:
         self.side = torch.cuda.Stream(device=dev) if dev.type == "cuda" else None
         self.dev = dev
         self.hdr = torch.zeros(HDR_INTS, dtype=torch.int64, device=dev)
-        p.check()
+        p.check(dev)
         self.choose, self.numbers = p.sampler(B, dev), p.numbers(dev, p.PREFILL)
 
     def first_tokens(self, tokens: torch.Tensor, on_layer_done=None) -> torch.Tensor:
@@ -323,7 +334,7 @@ class DecodeStage:
         # lengths a caller may change; longer runs than the history has rows for are read out in between.
         self.g_hist = torch.zeros(max(1, p.num_decoding_step), B, dtype=torch.long, device=dev)
         self.g_step = torch.zeros(1, dtype=torch.long, device=dev)
-        p.check()
+        p.check(dev)
         self.small = SmallCache(p, model, link) if p.kv_bits == 8 else None
         self.choose, self.numbers = p.sampler(B, dev), p.numbers(dev, p.DECODE)
         self.g_u = None if self.choose is None else torch.zeros_like(self.g_hist, dtype=torch.float32)      # what every step draws by

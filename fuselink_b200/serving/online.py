@@ -120,7 +120,7 @@ class OnlinePrefill:
         self.credit_pad = links[0].heap.alloc_tensor([16], torch.uint8)     # landing zone of the decoder's credit write
         self.batches = 0
         self.stats: List[BatchStats] = []
-        p.check()
+        p.check(dev)
         self.numbers = p.numbers(dev, p.PREFILL)
 
     def serve_batch(self, reqs: List[Request]) -> BatchStats:
@@ -206,7 +206,7 @@ class OnlineDecode:
         self.credit_pad = links[0].heap.alloc_tensor([16], torch.uint8)
         self.batches = 0
         self.done_on = [0] * len(links)
-        p.check()
+        p.check(links[0].k_pool.local.device)
         self.small = SmallCache(p, model, links[0]) if p.kv_bits == 8 and model is not None else None
         self.numbers = p.numbers(links[0].k_pool.local.device, p.DECODE)
 

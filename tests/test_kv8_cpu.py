@@ -379,3 +379,20 @@ def test_scratch_is_bounded(lib):
         for mass in (0, 1):
             one, all_ = (lib.fl_kv8_attention_scratch(I(b), I(tokens), I(heads), kv, I(mass)) for b in (1, batch))
             assert 0 <= all_ <= max(1 << 28, one)
+
+
+def test_options_that_the_gpu_does_not_take():
+    """Known before a batch is on its way: types, heads and vocabularies that only the plain forms take."""
+    import dataclasses
+    from fuselink_b200.serving.disagg import ServeParams
+    tiny = MODEL_ZOO["tiny"]
+    odd, wide = dataclasses.replace(tiny, head_dim=72), dataclasses.replace(tiny, vocab=600000)
+    bad = [(tiny, dict(kv_bits=8, dtype=torch.float32)), (tiny, dict(temperature=0.5, dtype=torch.float32)), (odd, dict(kv_bits=8)), (wide, dict(temperature=1.0))]
+    for model, kw in bad:
+        p = ServeParams(model, **kw)
+        p.check()
+        p.check("cpu")
+        with pytest.raises(ValueError):
+            p.check("cuda")
+    for model, kw in ((tiny, dict(dtype=torch.float32)), (odd, dict(temperature=1.0)), (wide, dict(kv_bits=8)), (tiny, dict(kv_bits=8, temperature=1.0, dtype=torch.float16))):
+        ServeParams(model, **kw).check(torch.device("cuda", 0))

@@ -321,3 +321,21 @@ def test_a_position_outside_a_small_cache_is_an_error():
         torch.cuda.synchronize()
         with pytest.raises(IndexError, match=what):
             net.check_status()
+
+
+def test_stages_refuse_a_small_cache_and_sampling_in_fp32():
+    from fuselink_b200.models.llama import MODEL_ZOO, LlamaShard
+    from fuselink_b200.parallel.symm import SymmetricHeap
+    from fuselink_b200.serving.disagg import DecodeStage, KVLink, PrefillStage, ServeParams
+    from fuselink_b200.serving.online import OnlineDecode, OnlinePrefill
+    heap, = SymmetricHeap.emulated(1, 64 << 20)
+    try:
+        net = LlamaShard(MODEL_ZOO["tiny"], device="cuda", dtype=torch.float32)
+        for i, options in enumerate((dict(kv_bits=8), dict(temperature=0.7))):
+            p = ServeParams(model=MODEL_ZOO["tiny"], batch_size=3, input_len=32, num_decoding_step=4, dtype=torch.float32, **options)
+            link = KVLink(heap, p, net.kvh_local, name=f"kv{i}")
+            for make in (lambda: PrefillStage(p, net, link, 0), lambda: DecodeStage(p, net, link), lambda: OnlinePrefill(p, net, [link], 0), lambda: OnlineDecode(p, net, [link], 0)):
+                with pytest.raises(ValueError, match="bf16 or fp16"):
+                    make()
+    finally:
+        heap.close()
