@@ -418,7 +418,7 @@ class LlamaShard(torch.nn.Module):
         counts = None if counts is None else self._indices(counts)
         x = torch.empty(B * T, cfg.hidden, dtype=self.embed.dtype, device=dev)
         each = positions if T == 1 else (positions.unsqueeze(1) + torch.arange(T, device=dev)).flatten()
-        if T > 1 and self.pos_embed is not None and counts is not None:      # padding has no position
+        if self.pos_embed is not None and counts is not None:      # padding has no position
             each = torch.where((torch.arange(T, device=dev) < counts.unsqueeze(1)).flatten(), each, torch.zeros_like(each))
         C.dec_embed(tokens, each, self.embed, self.pos_embed, x, 1, cfg.pos_offset, status)
         out = torch.empty(B, T, hl * D, dtype=x.dtype, device=dev)

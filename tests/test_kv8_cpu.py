@@ -396,3 +396,21 @@ def test_options_that_the_gpu_does_not_take():
             p.check("cuda")
     for model, kw in ((tiny, dict(dtype=torch.float32)), (odd, dict(temperature=1.0)), (wide, dict(kv_bits=8)), (tiny, dict(kv_bits=8, temperature=1.0, dtype=torch.float16))):
         ServeParams(model, **kw).check(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("model", FAMILIES)
+@pytest.mark.parametrize("r", [FUSED, PLAIN])
+@pytest.mark.parametrize("shape", [(3,), (3, 1), (3, 2)])
+def test_a_padded_row_has_no_position(model, r, shape, route):  # noqa: F811
+    """A batch with a request that has no new token: whatever its position says, single tokens and pieces alike, the others go on as without it."""
+    net = _net(model)
+    route(r)
+    toks, table = _tokens(net, 3, 32), _table(3, 4)
+    new, got = _tokens(net, 3, 2)[:, :1 if len(shape) == 1 else shape[1]].reshape(shape), []
+    for where in (32, 10 ** 7):
+        cache = _cache(net.cfg, 12)
+        net.prefill(toks, cache, None, table)
+        positions = torch.tensor([32, where, 32])
+        out = net.extend(new, positions, cache, table, slots=torch.tensor([32, 32, 32]), counts=torch.tensor([len(new[0].reshape(-1)), 0, 1]))
+        got.append((out.view(3, -1)[[0, 2], 0], *(scales[:, table[[0, 2], :3].long()] for scales in (cache.k_scale, cache.v_scale))))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
