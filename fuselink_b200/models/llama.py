@@ -558,6 +558,8 @@ class LlamaShard(torch.nn.Module):
         most = block_table.shape[1] * cfg.block_size if max_positions is None else max_positions
         if B == 0 or T == 0:
             return torch.zeros(shape, dtype=torch.long, device=tokens.device)
+        if counts is not None:                                                   # padding is none of the vocabulary
+            tokens = torch.where(torch.arange(T, device=tokens.device) < counts.to(tokens.device).unsqueeze(1), tokens, torch.zeros_like(tokens))
         if self._fused(None):
             return self._extend_fused(tokens, positions, cache, block_table, slots, counts, mass, most, choose).view(shape)
         table, hl, status = self._pages(block_table), self.h_local, self._status_or_0()

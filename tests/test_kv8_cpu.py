@@ -414,3 +414,19 @@ def test_a_padded_row_has_no_position(model, r, shape, route):  # noqa: F811
         out = net.extend(new, positions, cache, table, slots=torch.tensor([32, 32, 32]), counts=torch.tensor([len(new[0].reshape(-1)), 0, 1]))
         got.append((out.view(3, -1)[[0, 2], 0], *(scales[:, table[[0, 2], :3].long()] for scales in (cache.k_scale, cache.v_scale))))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("r", [FUSED, PLAIN])
+@pytest.mark.parametrize("shape", [(3,), (3, 4)])
+def test_what_stands_behind_counts_is_no_token(r, shape, route):  # noqa: F811
+    """Padding need not be an entry of the vocabulary."""
+    net = _net("tiny")
+    route(r)
+    toks, table, counts = _tokens(net, 3, 32), _table(3, 4), torch.tensor([1, 0, 1])
+    new, got = _tokens(net, 3, 4)[:, :1 if len(shape) == 1 else 4].reshape(shape), []
+    for fill in (0, -10 ** 9, net.cfg.vocab):
+        cache = _cache(net.cfg, 12)
+        net.prefill(toks, cache, None, table)
+        new = torch.where(torch.arange(new.numel() // 3) < counts[:, None], new.reshape(3, -1), fill).reshape(shape)
+        got.append(net.extend(new, torch.full((3,), 32), cache, table, counts=counts).view(3, -1)[[0, 2], 0])
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
