@@ -42,7 +42,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Limit = 1.0, top_
            min_p: Limit = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """logits [rows, vocab]; u [rows], fp32 or fp64 in [0, 1); the limits numbers, or tensors with one for each row (top_k 0, top_p 1 and min_p 0 leave
     nothing out).  Returns the tokens [rows] int64 and the logarithm of each one's probability among those that were left, fp32.
-    On the GPU bf16 and fp16; on the CPU any floating type."""
+    On the GPU bf16 and fp16, and logarithms without a gradient; on the CPU any floating type."""
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"sample: logits [rows, vocab] expected, not {tuple(logits.shape)}")
     rows, dev = logits.shape[0], logits.device

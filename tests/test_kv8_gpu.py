@@ -713,3 +713,15 @@ def test_a_batch_that_goes_in_pieces():
     want, weights, may = _want_attention(cache, 0, q, table[:, :6], [n - 1 for n in lens], [1] * B)
     _check(out, want, may, HF)
     assert ((mass[:, :6].double() - weights).abs() <= 1e-4 * weights + 1e-12).all() and mass[:, 6:].abs().max() == 0 and int(word) == 0
+
+
+def test_gradients_are_refused():
+    from fuselink_b200.ops import kv8
+    cache, table, start = _cache(1, 8, 2, 16, 64), _table(2, 4, 8), _ints([5, 6])
+    q, qkv = _randn(2, 1, 4, 64, dt=BF).requires_grad_(), _randn(2, 1, 8, 64, dt=BF).requires_grad_()
+    bias = _randn(8 * 64, dt=BF).requires_grad_()
+    for call in (lambda: kv8.attention(cache, 0, q, table, start), lambda: kv8.write(cache, 0, qkv, table, start), lambda: kv8.write(cache, 0, qkv.detach(), table, start, bias=bias)):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
