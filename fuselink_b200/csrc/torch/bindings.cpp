@@ -453,10 +453,15 @@ static const long long* kv8_i64(const c10::optional<torch::Tensor>& t, const tor
   TORCH_CHECK(!t.has_value() || t->device() == as.device(), what);
   return dec_i64(t, numel, what);
 }
+static void kv8_no_gradient(std::initializer_list<const torch::Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const auto* t : tensors) TORCH_CHECK(t == nullptr || !t->requires_grad(), "kv8: no gradient is computed on the GPU; call this under torch.no_grad()");
+}
 static torch::Tensor kv8_write(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& k_scale, const torch::Tensor& v_scale, const torch::Tensor& table, int64_t layer,
                                torch::Tensor qkv, c10::optional<torch::Tensor> into, const c10::optional<torch::Tensor>& bias, const c10::optional<torch::Tensor>& rope,
                                const torch::Tensor& start, const c10::optional<torch::Tensor>& pos, const c10::optional<torch::Tensor>& counts, int64_t status_addr) {
   const int dt = dec_dtype(qkv);
+  kv8_no_gradient({&qkv, bias.has_value() ? &*bias : nullptr, rope.has_value() ? &*rope : nullptr});
   c10::cuda::CUDAGuard guard(qkv.device());
   if (!into.has_value()) qkv = qkv.contiguous();
   const torch::Tensor out = into.has_value() ? *into : new_like(qkv, qkv.sizes(), qkv.scalar_type());
@@ -491,6 +496,7 @@ static torch::Tensor kv8_attention(const torch::Tensor& k, const torch::Tensor& 
                                    const torch::Tensor& q, const torch::Tensor& start, const c10::optional<torch::Tensor>& counts, double scale,
                                    c10::optional<torch::Tensor> into, const c10::optional<torch::Tensor>& mass, int64_t status_addr) {
   const int dt = dec_dtype(q);
+  kv8_no_gradient({&q});
   TORCH_CHECK(q.dim() == 4 && q.device() == k.device() && k.dim() == 5 && q.size(3) == k.size(4) && q.stride(3) == 1, "kv8: q [batch, tokens, heads, dim] with contiguous heads");
   const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3);
   TORCH_CHECK(B <= INT32_MAX && T <= INT32_MAX && H <= INT32_MAX && H % std::max<int64_t>(k.size(2), 1) == 0, "kv8: heads in groups that share a KV head");

@@ -58,11 +58,6 @@ def _check_like(cache: Kv8Cache, t: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"kv8: {what} on {cache.k.device} expected, not on {t.device}")
 
 
-def _check_no_gradient(*tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("kv8: no gradient is computed on the GPU; call this under torch.no_grad()")
-
-
 def write(cache: Kv8Cache, layer: int, qkv: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor, *, counts: Optional[torch.Tensor] = None,
           positions: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
           out: Optional[torch.Tensor] = None, status: int = 0) -> torch.Tensor:
@@ -70,13 +65,11 @@ def write(cache: Kv8Cache, layer: int, qkv: torch.Tensor, block_table: torch.Ten
     keys and values to their pages.
 
     qkv: [batch, tokens, heads + 2 kv_heads, dim]; token t of request b is the cache's slot ``start[b] + t`` ([batch] int64) of the pages
-    ``block_table[b]`` ([batch, pages] int32).  What the last page written held behind that is no longer valid, and no page
-    is written for two requests of a call.  counts ([batch] int64): tokens
-    that a request has, of a padded batch; rows behind them stay as they are.  rope ([positions, dim] fp32): cosines, then sines;
-    positions ([batch] int64): what the first token is rotated by, where that is not its slot.  bias: [(heads + 2 kv_heads) * dim].  Returns the rows as the
+    ``block_table[b]`` ([batch, pages] int32).  What the last page written held behind that is no longer valid, and no page is written for two
+    requests of a call.  counts ([batch] int64): tokens that a request has, of a padded batch; rows behind them stay as they are.  rope ([positions,
+    dim] fp32): cosines, then sines; positions ([batch] int64): what the first token is rotated by, where that is not its slot.  bias: [(heads + 2 kv_heads) * dim].  Returns the rows as the
     attention takes them: ``out``, which may be qkv, or a new tensor."""
     if qkv.is_cuda:
-        _check_no_gradient(qkv, bias, rope)
         return require_native().kv8_write(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, layer, qkv, out, bias, rope, start, positions, counts, status)
     _check_like(cache, qkv, "rows")
     return _plain_write(cache, layer, qkv, torch.empty_like(qkv) if out is None else out, block_table, start, counts, positions, rope, bias)
@@ -116,7 +109,6 @@ def attention(cache: Kv8Cache, layer: int, q: torch.Tensor, block_table: torch.T
     elif not 0 <= scale < math.inf:
         raise ValueError(f"kv8: scale {scale}")
     if q.is_cuda:
-        _check_no_gradient(q)
         return require_native().kv8_attention(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, layer, q, start, counts, scale, out, mass, status)
     _check_like(cache, q, "queries")
     B, T, H, D = q.shape
