@@ -79,7 +79,7 @@ __device__ __forceinline__ int page_id(const FlKv8& kv, int b, int page) {
 // of values: lane (t, c) takes columns 8 c .. 8 c + 7 of the first half of a token's row and the matching ones of the second (the pairs that the
 // rotation mixes), 32 / (dim / 16) tokens at a time.  Four such steps, a page of 16 tokens, stay in registers between finding the largest
 // magnitude and writing codes; larger pages are read again.  16 x 2048 tokens of 32 + 2 x 8 heads of 128: 254 us with a query's columns and angles
-// looked up one by one, now 186 (136 of bytes); 5 x 389 ragged ones of 32 + 2 x 32 heads of 64: 18.6 us (7.0).  With 128 registers, for the four steps, an SM
+// looked up one by one, now 186 (136 of bytes); 5 x 389 ragged ones of 32 + 2 x 32 heads of 64: 18.5 us (7.0).  With 128 registers, for the four steps, an SM
 // has 16 warps; 96 spill (253 us), two steps in registers and the others read again take 206, queries in a launch of their own 180 to 193.  A warp's
 // next rows copied to shared memory while it works on these, by a grid that stays: 176 us, but 23.3 for the ragged ones.
 constexpr int STEPS = 4;
@@ -456,13 +456,13 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
-// A warp's ring in shared memory.  Rows are 16 bytes further apart than they are long, so that the 16-byte (values of heads up to 64: 8-byte) reads of
-// a product's rows meet different banks.
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
+// A warp's ring in shared memory.  Rows are 16 bytes further apart than they are long, so that the 16-byte (values of heads up to 64: 8-byte) reads of
+// a product's rows meet different banks.
 template <int DP> struct Ring {
   static constexpr int STAGES = DP == 128 ? 3 : 6;
   static constexpr int PITCH = DP + 16, KEYS = 16 * PITCH, SCALES = 2 * KEYS;

@@ -547,7 +547,8 @@ class LlamaShard(torch.nn.Module):
         ``block_table[b]``; counts ([B]): how many of a padded row's T are tokens.  Returns tokens of the same shape; what stands behind counts
         says nothing.
         mass ([B, pages] fp32): this shard's heads' attention weights are added to it, all layers, page by page (ops/kv8.py, ``evict``).
-        max_positions: positions there may be (the table's slots, if not given); one beyond is an IndexError from the next call on."""
+        max_positions: how many positions have rotations (the table's slots, if not given; more than that are kept); one without is an IndexError from
+        the next call on."""
         self._check_cache(cache)
         cfg, shape = self.cfg, tokens.shape
         tokens = tokens.unsqueeze(1) if tokens.dim() == 1 else tokens
