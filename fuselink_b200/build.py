@@ -41,7 +41,7 @@ NVCC_FLAGS = [
 ]
 CXX_FLAGS = ["-O2", "-g", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-pthread"]
 
-KERNELS = ["grouped_gemm", "comm_kernels", "embbag", "kv_pack", "moe_dispatch", "moe_dispatch_noalloc", "fp8_gemm", "shadow_reduce", "decoder", "thin_gemm", "kv8", "sampling", "interact", "mlp_bwd", "moe_route"]
+KERNELS = ["grouped_gemm", "comm_kernels", "embbag", "kv_pack", "moe_dispatch", "moe_dispatch_noalloc", "fp8_gemm", "shadow_reduce", "decoder", "thin_gemm", "kv8", "sampling", "interact", "mlp_bwd", "moe_route", "embedding", "routing", "losses", "adamw"]
 NET_SRCS = ["plugin", "tcp_transport", "tcp_endpoints", "params", "conn_manager", "ib_transport", "nvl_channel", "logging", "rdma_transport", "soft_provider", "verbs_provider", "nic_rate"]
 
 
@@ -135,7 +135,7 @@ def build_all(verbose: bool = False, jobs: int | None = None) -> dict:
     # ---- torch extension ------------------------------------------------------------------------
     inc, defs, tlink = _torch_flags()
     ext_objs = []
-    for rel in ["torch/bindings.cpp", "monitor/monitor_py.cpp"]:
+    for rel in ["torch/bindings.cpp", "torch/train_ops.cpp", "monitor/monitor_py.cpp"]:
         src = CSRC / rel
         out = OBJ / (Path(rel).stem + ".o")
         ext_objs.append(add(out, [src], [CXX, *CXX_FLAGS, *defs, *inc, "-c", src, "-o", out]))

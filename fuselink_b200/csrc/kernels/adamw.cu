@@ -1,0 +1,233 @@
+// AdamW over many tensors.
+//
+//   m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2      w = w (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Moments are kept in fp32, or as e4m3 codes of m and of sqrt(v) with a scale for each 256 values of a tensor: the smallest power of two,
+// 2^-100 at least, that keeps their largest finite magnitude within 448.  The root halves the range that a code has to span, and a root above 0 keeps
+// the smallest code at least: were it lost while m is not, the next steps would divide by eps.  Values that are not finite are kept
+// as NaN.  The step itself uses m and v as they are before they become codes.  These roundings are each IEEE's, without fused
+// multiply-adds between them, so that the codes are the same wherever they are computed.
+//
+// Bound by memory: 10 bytes per bf16 weight with codes, 22 with fp32 moments, 28 with an fp32 copy of the weight as well.  A CTA takes 8192
+// values of one tensor; the tensors' addresses are kernel arguments, 400 tensors a launch, so that a captured step needs no copy of a table.
+// The number of steps is on the device: every CTA of a tensor adds 2^40 to it when it has read it, and the last one puts the next number.
+#include "adamw.cuh"
+#include <cuda_fp8.h>
+#include <math.h>
+#include <string.h>
+#include "../common/fl_ptx.cuh"
+
+namespace fl {
+namespace adamw {
+
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int BLOCK = FL_ADAMW_BLOCK, CHUNK = 8192;
+constexpr int MOST = 400, FEW = 32;              // tensors of a launch: 32 KB of arguments, or 2.5
+constexpr unsigned ALL = 0xffffffffu;
+constexpr long long ARRIVED = 1ll << 40;
+
+template <int CAP>
+struct Launch {
+  FlAdamwTensor t[CAP];
+  int first[CAP];                                // chunks before the tensor's
+  int count;
+  float b1, c1, b2, c2, eps;
+  double lr, decay, log_b1, log_b2;
+  const float* lr_on_device;
+};
+
+// the smallest power of two, 2^-100 at least, that brings `bits` (of a finite number, not negative) within 448 = 1.75 * 2^8
+__device__ __forceinline__ uint32_t scale_bits(uint32_t bits) {
+  const int e = (int)(bits >> 23) + ((bits & 0x7fffffu) > 0x600000u) - 8;
+  return (uint32_t)max(e, 27) << 23;
+}
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+__device__ __forceinline__ float no_inf(float x) { return (__float_as_uint(x) & 0x7fffffffu) == 0x7f800000u ? NAN : x; }
+__device__ __forceinline__ uint32_t codes_of(const float* x, float inverse) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(no_inf(x[1]) * inverse), "f"(no_inf(x[0]) * inverse));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(no_inf(x[3]) * inverse), "f"(no_inf(x[2]) * inverse));
+  return (uint32_t)hi << 16 | lo;
+}
+__device__ __forceinline__ void values_of(float* x, uint32_t codes, float scale) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t two;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"((uint16_t)(codes >> 16 * h)));
+    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&two));
+    x[2 * h] = f.x * scale;
+    x[2 * h + 1] = f.y * scale;
+  }
+}
+
+// four values from `at` on; those behind the end are 0
+template <typename T>
+__device__ __forceinline__ Pack<T, 4> load4(const void* p, long long at, long long n, bool wide) {
+  Pack<T, 4> x;
+  if (wide && at + 4 <= n) return *reinterpret_cast<const Pack<T, 4>*>((const T*)p + at);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x.v[i] = at + i < n ? ((const T*)p)[at + i] : T{};
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ void store4(void* p, long long at, long long n, bool wide, const Pack<T, 4>& x) {
+  if (wide && at + 4 <= n) {
+    *reinterpret_cast<Pack<T, 4>*>((T*)p + at) = x;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i < n) ((T*)p)[at + i] = x.v[i];
+}
+
+template <typename T, bool CODES, bool MASTER, int CAP>
+__global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ Launch<CAP> a) {
+  __shared__ float shared[3];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (a.first[mid] <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
+  }
+  const FlAdamwTensor& t = a.t[lo];
+  const int chunk = (int)blockIdx.x - a.first[lo], chunks = t.n > CHUNK ? (int)((t.n + CHUNK - 1) / CHUNK) : 1;
+  if (threadIdx.x == 0) {
+    const long long step = *reinterpret_cast<volatile long long*>(t.step) & (ARRIVED - 1);
+    const double lr = a.lr_on_device != nullptr ? (double)*a.lr_on_device : a.lr;
+    shared[0] = (float)(lr / -expm1((double)(step + 1) * a.log_b1));
+    shared[1] = (float)(1.0 / sqrt(-expm1((double)(step + 1) * a.log_b2)));
+    shared[2] = (float)(1.0 - lr * a.decay);
+    const unsigned long long before = atomicAdd(reinterpret_cast<unsigned long long*>(t.step), (unsigned long long)ARRIVED);
+    if ((int)(before >> 40) == chunks - 1) atomicExch(reinterpret_cast<unsigned long long*>(t.step), (unsigned long long)(step + 1));
+  }
+  __syncthreads();
+  const float first = shared[0], second = shared[1], keep = shared[2];
+  uintptr_t bits = (uintptr_t)t.param | (uintptr_t)t.grad;
+  bool wide = (bits & (4 * sizeof(T) - 1)) == 0;
+  bits = (uintptr_t)t.m | (uintptr_t)t.v;
+  wide = wide && (bits & (CODES ? 3 : 15)) == 0 && (!MASTER || ((uintptr_t)t.master & 15) == 0);
+  const long long end = min(t.n, (long long)(chunk + 1) * CHUNK);
+  for (long long b = (long long)chunk * CHUNK + warp * BLOCK; b < end; b += WARPS * BLOCK) {
+    float m[2][4], root[2][4];
+    uint32_t m_most = 0, r_most = 0;
+    const float ms = CODES ? t.m_scale[b / BLOCK] : 1.f, rs = CODES ? t.v_scale[b / BLOCK] : 1.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long at = b + h * (BLOCK / 2) + lane * 4;
+      const Pack<T, 4> g4 = load4<T>(t.grad, at, t.n, wide);
+      float v[4], w[4];
+      if (CODES) {
+        const Pack<uint8_t, 4> mc = load4<uint8_t>(t.m, at, t.n, wide), vc = load4<uint8_t>(t.v, at, t.n, wide);
+        values_of(m[h], *reinterpret_cast<const uint32_t*>(&mc), ms);
+        values_of(v, *reinterpret_cast<const uint32_t*>(&vc), rs);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __fmul_rn(v[i], v[i]);
+      } else {
+        const Pack<float, 4> m4 = load4<float>(t.m, at, t.n, wide), v4 = load4<float>(t.v, at, t.n, wide);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { m[h][i] = m4.v[i]; v[i] = v4.v[i]; }
+      }
+      if (MASTER) {
+        const Pack<float, 4> w4 = load4<float>(t.master, at, t.n, wide);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = w4.v[i];
+      } else {
+        const Pack<T, 4> w4 = load4<T>(t.param, at, t.n, wide);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = to_f32(w4.v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float g = to_f32(g4.v[i]);
+        m[h][i] = __fadd_rn(__fmul_rn(m[h][i], a.b1), __fmul_rn(g, a.c1));
+        v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(g, g), a.c2));
+        root[h][i] = __fsqrt_rn(v[i]);
+        w[i] = fmaf(w[i], keep, -first * __fdividef(m[h][i], fmaf(root[h][i], second, a.eps)));
+        if (CODES) {
+          m_most = max(m_most, finite_bits(m[h][i]));
+          r_most = max(r_most, finite_bits(root[h][i]));
+        }
+      }
+      Pack<T, 4> w_out;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w_out.v[i] = from_f32<T>(w[i]);
+      store4<T>(t.param, at, t.n, wide, w_out);
+      if (MASTER) store4<float>(t.master, at, t.n, wide, Pack<float, 4>{{w[0], w[1], w[2], w[3]}});
+      if (!CODES) {
+        store4<float>(t.m, at, t.n, wide, Pack<float, 4>{{m[h][0], m[h][1], m[h][2], m[h][3]}});
+        store4<float>(t.v, at, t.n, wide, Pack<float, 4>{{v[0], v[1], v[2], v[3]}});
+      }
+    }
+    if (CODES) {
+      const uint32_t mb = scale_bits(__reduce_max_sync(ALL, m_most)), rb = scale_bits(__reduce_max_sync(ALL, r_most));
+      const float m_inv = __uint_as_float((254u << 23) - mb), r_inv = __uint_as_float((254u << 23) - rb);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long long at = b + h * (BLOCK / 2) + lane * 4;
+        const uint32_t mc = codes_of(m[h], m_inv);
+        uint32_t rc = codes_of(root[h], r_inv);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (root[h][i] > 0.f && (rc >> 8 * i & 0xffu) == 0) rc |= 1u << 8 * i;
+        store4<uint8_t>(t.m, at, t.n, wide, *reinterpret_cast<const Pack<uint8_t, 4>*>(&mc));
+        store4<uint8_t>(t.v, at, t.n, wide, *reinterpret_cast<const Pack<uint8_t, 4>*>(&rc));
+      }
+      if (lane == 0) {
+        t.m_scale[b / BLOCK] = __uint_as_float(mb);
+        t.v_scale[b / BLOCK] = __uint_as_float(rb);
+      }
+    }
+  }
+}
+
+template <typename T, bool CODES, bool MASTER, int CAP>
+static int launch(const FlAdamwTensor* t, int count, const FlAdamwArgs* a, cudaStream_t stream) {
+  static thread_local Launch<CAP> l;
+  long long chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    l.t[i] = t[i];
+    l.first[i] = (int)chunks;
+    chunks += t[i].n > CHUNK ? (t[i].n + CHUNK - 1) / CHUNK : 1;
+    if (chunks > INT32_MAX) return -1;
+  }
+  l.count = count;
+  l.b1 = (float)a->beta1; l.c1 = (float)(1.0 - a->beta1);
+  l.b2 = (float)a->beta2; l.c2 = (float)(1.0 - a->beta2);
+  l.eps = (float)a->eps; l.lr = a->lr; l.decay = a->weight_decay;
+  l.log_b1 = log(a->beta1); l.log_b2 = log(a->beta2);
+  l.lr_on_device = a->lr_on_device;
+  adamw_kernel<T, CODES, MASTER, CAP><<<(unsigned)chunks, THREADS, 0, stream>>>(l);
+  return (int)cudaGetLastError();
+}
+
+template <typename T, bool CODES, bool MASTER>
+static int run(const FlAdamwTensor* t, long long count, const FlAdamwArgs* a, cudaStream_t stream) {
+  for (long long i = 0; i < count;) {
+    const int n = (int)(count - i < MOST ? count - i : MOST);
+    const int rc = n <= FEW ? launch<T, CODES, MASTER, FEW>(t + i, n, a, stream) : launch<T, CODES, MASTER, MOST>(t + i, n, a, stream);
+    if (rc != 0) return rc;
+    i += n;
+  }
+  return 0;
+}
+
+}  // namespace adamw
+}  // namespace fl
+
+extern "C" int fl_adamw(int dtype, const FlAdamwTensor* t, long long count, const FlAdamwArgs* a, cudaStream_t stream) {
+  using namespace fl::adamw;
+  if (count < 0 || !(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0)) return -1;
+  for (long long i = 0; i < count; ++i)
+    if (t[i].n < 0 || t[i].n > (long long)CHUNK * (1 << 22) || t[i].step == nullptr) return -1;
+  return fl_by_dtype(dtype, [&](auto type) {
+    using T = decltype(type);
+    if (a->master) {
+      if constexpr (sizeof(T) == 2) return a->codes ? run<T, true, true>(t, count, a, stream) : run<T, false, true>(t, count, a, stream);
+      else return -1;
+    }
+    return a->codes ? run<T, true, false>(t, count, a, stream) : run<T, false, false>(t, count, a, stream);
+  });
+}

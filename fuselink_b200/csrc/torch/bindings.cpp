@@ -23,6 +23,7 @@
 #include "../mem/vmm.h"
 #include "../monitor/monitor.h"
 void fl_monitor_bind(pybind11::module& m);
+void fl_train_bind(pybind11::module& m);
 
 namespace py = pybind11;
 
@@ -885,4 +886,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("vmm_usage", [](int64_t dev) { return (int64_t)fl_vmm_usage((int)dev); });
 
   fl_monitor_bind(m);
+  fl_train_bind(m);
 }

@@ -15,6 +15,7 @@ import torch.nn as nn
 
 from .._ext import require_native
 from ..ops import gemm, ref
+from ..ops.checks import ordinary as _ordinary
 from ..ops.moe import MoEConfig, MoEFunction, MoEWorkspace, balanced_placement, expert_home
 from ..parallel.symm import SymmetricHeap
 
@@ -50,15 +51,6 @@ def load_balancing_loss(probs: torch.Tensor, idx: torch.Tensor, num_experts: int
     me = probs.mean(0)
     ce = torch.nn.functional.one_hot(idx[:, 0].long(), num_experts).float().mean(0)
     return (me * ce).sum() * num_experts
-
-
-def _ordinary(t: torch.Tensor) -> bool:
-    """Whether a kernel may read this tensor in place of the framework's operations: no subclass, and neither a function transform
-    (vmap, grad, jvp), forward-mode differentiation, a dispatch mode nor tracing that has to see the operations."""
-    # a batched gradient reaches the backward on a thread without the transform, and shows itself by having no memory
-    return (type(t) in (torch.Tensor, nn.Parameter) and torch._C._has_storage(t) and not torch._C._are_functorch_transforms_active()
-            and torch.autograd.forward_ad._current_level < 0 and torch._C._len_torch_dispatch_stack() == 0
-            and not torch.jit.is_tracing() and not torch.compiler.is_compiling())
 
 
 class _Route(torch.autograd.Function):
