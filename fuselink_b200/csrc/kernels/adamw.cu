@@ -68,8 +68,9 @@ template <typename T>
 __device__ __forceinline__ Pack<T, 4> load4(const void* p, long long at, long long n, bool wide) {
   Pack<T, 4> x;
   if (wide && at + 4 <= n) return *reinterpret_cast<const Pack<T, 4>*>((const T*)p + at);
+  T* y = reinterpret_cast<T*>(&x.raw);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x.v[i] = at + i < n ? ((const T*)p)[at + i] : T{};
+  for (int i = 0; i < 4; ++i) y[i] = at + i < n ? ((const T*)p)[at + i] : T{};
   return x;
 }
 template <typename T>
@@ -80,7 +81,14 @@ __device__ __forceinline__ void store4(void* p, long long at, long long n, bool 
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (at + i < n) ((T*)p)[at + i] = x.v[i];
+    if (at + i < n) ((T*)p)[at + i] = reinterpret_cast<const T*>(&x.raw)[i];
+}
+
+template <typename T>
+__device__ __forceinline__ Pack<T, 4> pack(const float* f) {
+  Pack<T, 4> x;
+  x.set(f);
+  return x;
 }
 
 template <typename T, bool CODES, bool MASTER, int CAP>
@@ -118,32 +126,27 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
     for (int h = 0; h < 2; ++h) {
       const long long at = b + h * (BLOCK / 2) + lane * 4;
       const Pack<T, 4> g4 = load4<T>(t.grad, at, t.n, wide);
-      float v[4], w[4];
+      float g[4], v[4], w[4];
+      g4.get(g);
       if (CODES) {
         const Pack<uint8_t, 4> mc = load4<uint8_t>(t.m, at, t.n, wide), vc = load4<uint8_t>(t.v, at, t.n, wide);
-        values_of(m[h], *reinterpret_cast<const uint32_t*>(&mc), ms);
-        values_of(v, *reinterpret_cast<const uint32_t*>(&vc), rs);
+        values_of(m[h], mc.raw, ms);
+        values_of(v, vc.raw, rs);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = __fmul_rn(v[i], v[i]);
       } else {
-        const Pack<float, 4> m4 = load4<float>(t.m, at, t.n, wide), v4 = load4<float>(t.v, at, t.n, wide);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { m[h][i] = m4.v[i]; v[i] = v4.v[i]; }
+        load4<float>(t.m, at, t.n, wide).get(m[h]);
+        load4<float>(t.v, at, t.n, wide).get(v);
       }
       if (MASTER) {
-        const Pack<float, 4> w4 = load4<float>(t.master, at, t.n, wide);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = w4.v[i];
+        load4<float>(t.master, at, t.n, wide).get(w);
       } else {
-        const Pack<T, 4> w4 = load4<T>(t.param, at, t.n, wide);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = to_f32(w4.v[i]);
+        load4<T>(t.param, at, t.n, wide).get(w);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float g = to_f32(g4.v[i]);
-        m[h][i] = __fadd_rn(__fmul_rn(m[h][i], a.b1), __fmul_rn(g, a.c1));
-        v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(g, g), a.c2));
+        m[h][i] = __fadd_rn(__fmul_rn(m[h][i], a.b1), __fmul_rn(g[i], a.c1));
+        v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(g[i], g[i]), a.c2));
         root[h][i] = __fsqrt_rn(v[i]);
         w[i] = fmaf(w[i], keep, -first * __fdividef(m[h][i], fmaf(root[h][i], second, a.eps)));
         if (CODES) {
@@ -151,14 +154,11 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
           r_most = max(r_most, finite_bits(root[h][i]));
         }
       }
-      Pack<T, 4> w_out;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w_out.v[i] = from_f32<T>(w[i]);
-      store4<T>(t.param, at, t.n, wide, w_out);
-      if (MASTER) store4<float>(t.master, at, t.n, wide, Pack<float, 4>{{w[0], w[1], w[2], w[3]}});
+      store4<T>(t.param, at, t.n, wide, pack<T>(w));
+      if (MASTER) store4<float>(t.master, at, t.n, wide, pack<float>(w));
       if (!CODES) {
-        store4<float>(t.m, at, t.n, wide, Pack<float, 4>{{m[h][0], m[h][1], m[h][2], m[h][3]}});
-        store4<float>(t.v, at, t.n, wide, Pack<float, 4>{{v[0], v[1], v[2], v[3]}});
+        store4<float>(t.m, at, t.n, wide, pack<float>(m[h]));
+        store4<float>(t.v, at, t.n, wide, pack<float>(v));
       }
     }
     if (CODES) {
@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (root[h][i] > 0.f && (rc >> 8 * i & 0xffu) == 0) rc |= 1u << 8 * i;
-        store4<uint8_t>(t.m, at, t.n, wide, *reinterpret_cast<const Pack<uint8_t, 4>*>(&mc));
-        store4<uint8_t>(t.v, at, t.n, wide, *reinterpret_cast<const Pack<uint8_t, 4>*>(&rc));
+        store4<uint8_t>(t.m, at, t.n, wide, Pack<uint8_t, 4>{mc});
+        store4<uint8_t>(t.v, at, t.n, wide, Pack<uint8_t, 4>{rc});
       }
       if (lane == 0) {
         t.m_scale[b / BLOCK] = __uint_as_float(mb);

@@ -8,8 +8,9 @@
 //
 // Gradient: embed_sort_kernel lists the tokens' places sorted by id, places of one id in order.  A CTA has a range of ids, counts its own ones
 // (each warp a stretch of the batch, in counters of its own) and those below the range, which says where its stretch of the list begins
-// without a word from the other CTAs.  embed_sum_kernel then adds rows up: ids of up to 32 places by a warp each, up to 1024 by a CTA, and
-// more of them (padding, say) by CTAs that take 1024 places each; the one that is done last adds up the parts in their order.
+// without a word from the other CTAs.  embed_sum_kernel then takes 32 places of the list a CTA, however many ids they are of: rows of ids whose places
+// are all among them are written at once, of the others (frequent words, padding) the CTA that is done last adds up the parts in their order, 32 at a
+// time.  Other CTAs of the same launch have the copy engine write the rows of ids that do not occur, from zeros in shared memory.
 #include "embedding.cuh"
 #include "../common/fl_ptx.cuh"
 
@@ -18,11 +19,10 @@ namespace embedding {
 
 constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32;
 constexpr int RANGE = 512;                       // ids of a sorting CTA
-constexpr int SUM_WARPS = 8, SUM_THREADS = SUM_WARPS * 32;
-constexpr int GROUP = 64;                        // ids of a summing CTA
-constexpr int FEW = 32;                          // places of an id that a warp adds up alone
-constexpr int MANY = 1024;                       // places that a CTA adds up alone
-constexpr int AHEAD = 8;                         // rows on their way per warp
+constexpr int BATCH = 8;                         // tokens on their way per sorting thread
+constexpr int PART = 32;                         // places of a summing CTA, and parts that are added up at a time
+constexpr int ZERO_IDS = 4;                      // ids that a warp looks at for rows of zeros
+constexpr int ZEROS = 8192;                      // bytes of zeros that a copy takes at most
 
 template <typename I>
 __device__ __forceinline__ long long token_at(const I* tokens, long long t, long long vocab) {
@@ -49,8 +49,11 @@ __global__ void __launch_bounds__(128) embed_kernel(const FlEmbedArgs a, int tpr
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (at + j * tpr >= packs) break;
+    float f[N];
+    x[j].get(f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[j].v[i] = from_f32<T>(ok ? to_f32(x[j].v[i]) * a.scale : 0.f);
+    for (int i = 0; i < N; ++i) f[i] = ok ? f[i] * a.scale : 0.f;
+    x[j].set(f);
     out[at + j * tpr] = x[j];
   }
 }
@@ -58,21 +61,28 @@ __global__ void __launch_bounds__(128) embed_kernel(const FlEmbedArgs a, int tpr
 // ------------------------------------------------------------------------------------------------------------------ sort
 struct Scratch {
   int* first;       // [vocab + 1]: where an id's places begin in the list
-  int* places;      // [n]
-  int* done;        // [parts][slices]: parts of an id of many places that are there
-  float* parts;     // [parts][2][hidden]
+  int2* list;       // [n]: place and id
+  int* done;        // [2][parts][2][tiles]: parts (then groups of them) of an id that are there
+  float* sums;      // [parts][2][columns]: of the id that a part begins with, and of the one that begins in it and goes on
 };
 __host__ __device__ inline long long up256(long long x) { return (x + 255) / 256 * 256; }
-__host__ __device__ inline long long parts_of(long long n) { return n > MANY ? (n + MANY - 1) / MANY : 0; }
-__host__ __device__ inline Scratch scratch_of(void* p, long long n, long long vocab, long long hidden) {
+__host__ __device__ inline long long parts_of(long long n) { return (n + PART - 1) / PART; }
+__host__ __device__ inline Scratch scratch_of(void* p, long long n, long long vocab, long long tiles) {
   char* c = (char*)p;
   Scratch s;
   s.first = (int*)c; c += up256((vocab + 1) * 4);
-  s.places = (int*)c; c += up256(n * 4);
-  s.done = (int*)c; c += up256(parts_of(n) * ((hidden + 31) / 32) * 4);
-  s.parts = (float*)c;
+  s.list = (int2*)c; c += up256(n * 8);
+  s.done = (int*)c; c += up256(parts_of(n) * 4 * tiles * 4);
+  s.sums = (float*)c;
   return s;
 }
+// threads of a summing CTA, 16 bytes of a row each, and how many of their widths a row has
+static int threads_of(long long hidden, int size) {
+  int t = 32;
+  while (t < 256 && t * 16 < hidden * size) t *= 2;
+  return t;
+}
+static long long tiles_of(long long hidden, int size) { return (hidden * size + threads_of(hidden, size) * 16 - 1) / (threads_of(hidden, size) * 16); }
 
 // exclusive sum over the block; total in *all
 __device__ __forceinline__ int block_scan(int x, int* warp_sums, int* all) {
@@ -96,53 +106,76 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums, int* all) {
 }
 
 template <typename I>
-__global__ void __launch_bounds__(SORT_THREADS) embed_sort_kernel(const FlEmbedArgs a, int slices) {
+__global__ void __launch_bounds__(SORT_THREADS) embed_sort_kernel(const FlEmbedArgs a, int tiles) {
   extern __shared__ int counters[];              // [SORT_WARPS][RANGE]
   __shared__ int warp_sums[SORT_WARPS];
-  const Scratch s = scratch_of(a.scratch, a.n, a.vocab, a.hidden);
+  grid_dep_launch();
+  const Scratch s = scratch_of(a.scratch, a.n, a.vocab, tiles);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long lo = (long long)blockIdx.x * RANGE, hi = lo + RANGE < a.vocab ? lo + RANGE : a.vocab;
   const I* tokens = (const I*)a.tokens;
-  for (int i = threadIdx.x; i < SORT_WARPS * RANGE; i += SORT_THREADS) counters[i] = 0;
-  for (long long i = (long long)blockIdx.x * SORT_THREADS + threadIdx.x; i < parts_of(a.n) * slices; i += (long long)gridDim.x * SORT_THREADS) s.done[i] = 0;
-  __syncthreads();
-  const long long each = ((a.n + SORT_WARPS - 1) / SORT_WARPS + 31) / 32 * 32, begin = warp * each, end = begin + each < a.n ? begin + each : a.n;
+  const int each = (int)((a.n + SORT_WARPS - 1) / SORT_WARPS + 31) / 32 * 32;
+  const long long begin = (long long)warp * each, end = begin + each < a.n ? begin + each : a.n;
   int* mine = counters + warp * RANGE;
+  // a token's id less the first of the range; what is no id at all becomes one behind it
+  auto fetch = [&](int* x, long long t0) {
+    long long id[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j)
+      if (t0 + j * 32 + lane < end) id[j] = token_at(tokens, t0 + j * 32 + lane, a.vocab);
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) x[j] = t0 + j * 32 + lane < end && id[j] >= 0 && id[j] < a.vocab ? (int)(id[j] - lo) : RANGE;
+  };
+  int x[BATCH];
+  fetch(x, begin);                               // a warp of up to 256 tokens keeps them
+  for (int i = lane; i < RANGE / 4; i += 32) reinterpret_cast<int4*>(mine)[i] = make_int4(0, 0, 0, 0);
+  for (long long i = (long long)blockIdx.x * SORT_THREADS + threadIdx.x; i < parts_of(a.n) * 4 * tiles; i += (long long)gridDim.x * SORT_THREADS) s.done[i] = 0;
+  __syncwarp();
+  const int ids = (int)(hi - lo);
   int below = 0;
-  for (long long t = begin + lane; t < end; t += 32) {
-    const long long id = token_at(tokens, t, a.vocab);
-    below += id >= 0 && id < lo;
-    if (id >= lo && id < hi) atomicAdd(&mine[id - lo], 1);
+  for (long long t0 = begin; t0 < end; t0 += 32 * BATCH) {
+    if (t0 > begin) fetch(x, t0);
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      below += x[j] < 0;
+      if (x[j] >= 0 && x[j] < ids) atomicAdd(&mine[x[j]], 1);
+    }
   }
   __syncthreads();
   int base;
   block_scan(below, warp_sums, &base);
   int total = 0;
   if (threadIdx.x < RANGE)
-    for (int w = 0; w < SORT_WARPS; ++w) {       // counters become offsets of the warps within an id
-      const int c = counters[w * RANGE + threadIdx.x];
-      counters[w * RANGE + threadIdx.x] = total;
-      total += c;
-    }
+#pragma unroll 8
+    for (int w = 0; w < SORT_WARPS; ++w) total += counters[w * RANGE + threadIdx.x];
   int all;
-  const int first = base + block_scan(total, warp_sums, &all);
+  int first = base + block_scan(total, warp_sums, &all);
   if (threadIdx.x < RANGE) {
-    for (int w = 0; w < SORT_WARPS; ++w) counters[w * RANGE + threadIdx.x] += first;
-    if (lo + threadIdx.x < hi) s.first[lo + threadIdx.x] = first;
+    if (threadIdx.x < ids) s.first[lo + threadIdx.x] = first;
+#pragma unroll 8
+    for (int w = 0; w < SORT_WARPS; ++w) {       // counters become where a warp's places of an id begin
+      const int c = counters[w * RANGE + threadIdx.x];
+      counters[w * RANGE + threadIdx.x] = first;
+      first += c;
+    }
   }
   if (threadIdx.x == 0 && hi == a.vocab) s.first[a.vocab] = base + all;
   __syncthreads();
-  for (long long t0 = begin; t0 < end; t0 += 32) {
-    const long long t = t0 + lane, id = t < end ? token_at(tokens, t, a.vocab) : -1;
-    const bool in = id >= lo && id < hi;
-    if (__ballot_sync(0xffffffffu, in)) {
-      const unsigned same = __match_any_sync(0xffffffffu, in ? (int)(id - lo) : -1);
+  const bool kept = end - begin <= 32 * BATCH;
+  for (long long t0 = begin; t0 < end; t0 += 32 * BATCH) {
+    if (!kept) fetch(x, t0);
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const bool in = x[j] >= 0 && x[j] < ids;
+      if (!__any_sync(0xffffffffu, in)) continue;
+      const unsigned same = __match_any_sync(0xffffffffu, in ? x[j] : -1);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      int at = 0;
+      if (in) at = mine[x[j]] + rank;
+      __syncwarp();
       if (in) {
-        const int rank = __popc(same & ((1u << lane) - 1));
-        const int at = mine[id - lo] + rank;
-        s.places[at] = (int)t;
-        __syncwarp(same);
-        if (rank == 0) mine[id - lo] = at + __popc(same);
+        s.list[at] = make_int2((int)(t0 + j * 32 + lane), (int)lo + x[j]);
+        if (rank == 0) mine[x[j]] = at + __popc(same);
       }
       __syncwarp();
     }
@@ -150,110 +183,176 @@ __global__ void __launch_bounds__(SORT_THREADS) embed_sort_kernel(const FlEmbedA
 }
 
 // ------------------------------------------------------------------------------------------------------------------ sums
+// A thread has W values of a row, 16 bytes in all, as W / N packs of N values, `apart` values from one another; AHEAD rows are on their way.
 template <typename T, int N>
-__device__ __forceinline__ void add_rows(float* sum, const T* dout, long long hidden, const int* places, int n, long long col, bool live) {
-  for (int i = 0; i < n; i += AHEAD) {
-    Pack<T, N> x[AHEAD];
+struct Way {
+  static constexpr int W = 16 / (int)sizeof(T), C = W / N, AHEAD = C == 1 ? 8 : C == 2 ? 4 : 2;
+  static __device__ __forceinline__ void load(Pack<T, N>* x, const T* row, long long col, int apart, long long hidden) {
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      if (i + j < n && live) x[j] = *reinterpret_cast<const Pack<T, N>*>(dout + (long long)places[i + j] * hidden + col);
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      if (i + j < n && live)
-#pragma unroll
-        for (int k = 0; k < N; ++k) sum[k] += to_f32(x[j].v[k]);
+    for (int c = 0; c < C; ++c)
+      if (col + c * apart < hidden) x[c] = *reinterpret_cast<const Pack<T, N>*>(row + col + c * apart);
   }
-}
-template <typename T, int N>
-__device__ __forceinline__ void put_row(T* to, const float* sum, float scale) {
-  Pack<T, N> y;
+  static __device__ __forceinline__ void add(float* sum, const Pack<T, N>* x, long long col, int apart, long long hidden) {
 #pragma unroll
-  for (int k = 0; k < N; ++k) y.v[k] = from_f32<T>(sum[k] * scale);
-  *reinterpret_cast<Pack<T, N>*>(to) = y;
-}
-// the warps' sums, added up in the warps' order by the first warp
-template <int N>
-__device__ __forceinline__ void join_warps(float* sum, float (*shared)[32 * N]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __syncthreads();
+    for (int c = 0; c < C; ++c)
+      if (col + c * apart < hidden) {
+        float f[N];
+        x[c].get(f);
 #pragma unroll
-  for (int k = 0; k < N; ++k) shared[warp][k * 32 + lane] = sum[k];
-  __syncthreads();
-  if (warp == 0)
+        for (int k = 0; k < N; ++k) sum[c * N + k] += f[k];
+      }
+  }
+  static __device__ __forceinline__ void store(T* row, const float* sum, float scale, long long col, int apart, long long hidden) {
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      for (int w = 1; w < SUM_WARPS; ++w) sum[k] += shared[w][k * 32 + lane];
+    for (int c = 0; c < C; ++c)
+      if (col + c * apart < hidden) {
+        Pack<T, N> y;
+        float f[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) f[k] = sum[c * N + k] * scale;
+        y.set(f);
+        *reinterpret_cast<Pack<T, N>*>(row + col + c * apart) = y;
+      }
+  }
+};
+
+// n zeros, by the copy engine as far as whole 16 bytes go
+template <typename T>
+__device__ __forceinline__ void put_zeros(T* to, long long n, const uint4* zeros) {
+  while (n > 0 && ((uintptr_t)to & 15)) { *to++ = T{}; --n; }
+  char* at = reinterpret_cast<char*>(to);
+  long long bytes = n * (long long)sizeof(T);
+  while (bytes >= 16) {
+    const uint32_t k = (uint32_t)(bytes < ZEROS ? bytes & ~15ll : ZEROS);
+    bulk_store(at, zeros, k);
+    at += k;
+    bytes -= k;
+  }
+  for (to = reinterpret_cast<T*>(at); bytes > 0; bytes -= sizeof(T)) *to++ = T{};
 }
 
-// blockIdx.x: the ids' group, and behind the groups the parts of 1024 places; blockIdx.y: the slice of 32 * N columns
+// The rows of ids without a place among ZERO_IDS for each warp: runs of them at a time.
+template <typename T>
+__device__ __forceinline__ void zero_rows(const FlEmbedArgs& a, const Scratch& s, unsigned block) {
+  __shared__ __align__(128) uint4 zeros[ZEROS / 16];
+  for (int i = threadIdx.x; i < ZEROS / 16; i += blockDim.x) zeros[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const long long v0 = ((long long)block * (blockDim.x / 32) + threadIdx.x / 32) * ZERO_IDS;
+  const int f = v0 + lane <= a.vocab && lane <= ZERO_IDS ? s.first[v0 + lane] : -1, next = __shfl_down_sync(0xffffffffu, f, 1);
+  unsigned none = __ballot_sync(0xffffffffu, lane < ZERO_IDS && v0 + lane < a.vocab && f == next);
+  if (lane != 0) return;
+  while (none) {
+    const int from = __ffs(none) - 1, n = __ffs(~(none >> from)) - 1;
+    put_zeros((T*)a.dtable + (v0 + from) * a.hidden, n * a.hidden, zeros);
+    none &= ~(((1u << n) - 1) << from);
+  }
+  tma_store_commit();
+  tma_store_wait_read<0>();
+}
+
+// Whether the CTA is the last of `all` that come here with this counter; then it sees what they have written.
+__device__ __forceinline__ bool last_of(int* counter, int all, int* shared) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) *shared = atomicAdd(counter, 1) == all - 1;
+  __syncthreads();
+  const bool last = *shared;
+  if (last) __threadfence();
+  return last;
+}
+
+// blockIdx.x: the zeros' CTAs, which then write for as long as the others sum; then a CTA per part and tile of blockDim.x * W columns.
 template <typename T, int N>
-__global__ void __launch_bounds__(SUM_THREADS) embed_sum_kernel(const FlEmbedArgs a, int groups) {
-  __shared__ float shared[SUM_WARPS][32 * N];
-  __shared__ int first[GROUP + 1];
+__global__ void __launch_bounds__(256, 3) embed_sum_kernel(const FlEmbedArgs a, int zero_blocks, int tiles) {
+  using way = Way<T, N>;
+  __shared__ int2 list[PART + 2];                // the place before the part's, its own, the one behind them
   __shared__ int last_one;
-  const Scratch s = scratch_of(a.scratch, a.n, a.vocab, a.hidden);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long col = ((long long)blockIdx.y * 32 + lane) * N;
-  const bool live = col < a.hidden;
-  const T* dout = (const T*)a.dout;
-  T* dtable = (T*)a.dtable;
-  if (blockIdx.x < groups) {
-    const long long v0 = (long long)blockIdx.x * GROUP;
-    const int ids = (int)(a.vocab - v0 < GROUP ? a.vocab - v0 : GROUP);
-    if (threadIdx.x <= ids) first[threadIdx.x] = s.first[v0 + threadIdx.x];
-    __syncthreads();
-    for (int r = warp; r < ids; r += SUM_WARPS) {
-      const int n = first[r + 1] - first[r];
-      if (n > FEW) continue;
-      float sum[N] = {};
-      add_rows<T, N>(sum, dout, a.hidden, s.places + first[r], n, col, live);
-      if (live) put_row<T, N>(dtable + (v0 + r) * a.hidden + col, sum, a.scale);
-    }
-    for (int r = 0; r < ids; ++r) {
-      const int n = first[r + 1] - first[r];
-      if (n <= FEW || n > MANY) continue;
-      const int each = (n + SUM_WARPS - 1) / SUM_WARPS, b = warp * each;
-      float sum[N] = {};
-      add_rows<T, N>(sum, dout, a.hidden, s.places + first[r] + b, max(0, min(each, n - b)), col, live);
-      join_warps<N>(sum, shared);
-      if (warp == 0 && live) put_row<T, N>(dtable + (v0 + r) * a.hidden + col, sum, a.scale);
-    }
+  const Scratch s = scratch_of(a.scratch, a.n, a.vocab, tiles);
+  grid_dep_wait();
+  if (blockIdx.x < (unsigned)zero_blocks) {
+    zero_rows<T>(a, s, blockIdx.x);
     return;
   }
-  // places [b, e) of the list: those of ids with more than MANY, of which there are at most two here, the first's and the last's
-  const int part = blockIdx.x - groups, total = s.first[a.vocab], b = part * MANY, e = min(b + MANY, total);
-  if (b >= e) return;
-  for (int which = 0; which < 2; ++which) {
-    const int place = s.places[which == 0 ? b : e - 1];
-    const long long id = a.token_bytes == 8 ? token_at((const long long*)a.tokens, place, a.vocab) : token_at((const int*)a.tokens, place, a.vocab);
-    const int from = s.first[id], to = s.first[id + 1];
-    if (to - from <= MANY) continue;
-    if (which == 1 && from <= b) continue;                             // the same id as at the part's beginning
-    const int p0 = max(from, b), n = min(to, e) - p0, each = (n + SUM_WARPS - 1) / SUM_WARPS, off = warp * each;
-    float sum[N] = {};
-    add_rows<T, N>(sum, dout, a.hidden, s.places + p0 + off, max(0, min(each, n - off)), col, live);
-    join_warps<N>(sum, shared);
-    if (warp == 0 && live)
+  const int part = (blockIdx.x - zero_blocks) / tiles, tile = (blockIdx.x - zero_blocks) % tiles;
+  const long long col = (long long)tile * blockDim.x * way::W + threadIdx.x * N, columns = (long long)tiles * blockDim.x * way::W;
+  const int apart = blockDim.x * N, total = s.first[a.vocab], b = part * PART, n = min(PART, total - b);
+  if (n <= 0) return;                            // tokens outside the vocabulary have no place
+  for (int i = threadIdx.x; i < n + 2; i += blockDim.x) list[i] = b + i > 0 && b + i <= total ? s.list[b + i - 1] : make_int2(-1, -1);
+  __syncthreads();
+  const T* dout = (const T*)a.dout;
+  T* dtable = (T*)a.dtable;
+  float sum[way::W] = {};
+  int begun = -1, goes_on = -1;                  // ids of which there is a part here: begun before, or at its beginning and going on; begun in it
+  for (int i = 0; i < n; i += way::AHEAD) {
+    Pack<T, N> x[way::AHEAD][way::C];
 #pragma unroll
-      for (int k = 0; k < N; ++k) __stcg(&s.parts[((long long)part * 2 + which) * a.hidden + col + k], sum[k]);
-    const int p_first = from / MANY, parts = (to - 1) / MANY - p_first + 1;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) last_one = atomicAdd(&s.done[(long long)p_first * gridDim.y + blockIdx.y], 1) == parts - 1;
-    __syncthreads();
-    if (!last_one) continue;
-    __threadfence();
-    const int per = (parts + SUM_WARPS - 1) / SUM_WARPS;
+    for (int j = 0; j < way::AHEAD; ++j)
+      if (i + j < n) way::load(x[j], dout + (long long)list[i + j + 1].x * a.hidden, col, apart, a.hidden);
 #pragma unroll
-    for (int k = 0; k < N; ++k) sum[k] = 0.f;
-    for (int i = warp * per; i < min((warp + 1) * per, parts); ++i) {
-      const int slot = i == 0 && from > p_first * MANY;                // only in its first part may others stand before it
-      if (live)
+    for (int j = 0; j < way::AHEAD; ++j) {
+      if (i + j >= n) break;
+      way::add(sum, x[j], col, apart, a.hidden);
+      const int id = list[i + j + 1].y;
+      if (i + j + 1 < n && list[i + j + 2].y == id) continue;
+      const bool from_here = list[0].y != id, to_here = i + j + 1 < n || list[n + 1].y != id;
+      if (from_here && to_here) {
+        way::store(dtable + id * a.hidden, sum, a.scale, col, apart, a.hidden);
+      } else if (!from_here || list[1].y == id) {
+        begun = id;
+        float* to = s.sums + (long long)part * 2 * columns + tile * blockDim.x * way::W + threadIdx.x;
 #pragma unroll
-        for (int k = 0; k < N; ++k) sum[k] += __ldcg(&s.parts[((long long)(p_first + i) * 2 + slot) * a.hidden + col + k]);
+        for (int k = 0; k < way::W; ++k) __stcg(to + k * blockDim.x, sum[k]);
+      } else {
+        goes_on = id;
+        float* to = s.sums + ((long long)part * 2 + 1) * columns + tile * blockDim.x * way::W + threadIdx.x;
+#pragma unroll
+        for (int k = 0; k < way::W; ++k) __stcg(to + k * blockDim.x, sum[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < way::W; ++k) sum[k] = 0.f;
     }
-    join_warps<N>(sum, shared);
-    if (warp == 0 && live) put_row<T, N>(dtable + id * a.hidden + col, sum, a.scale);
+  }
+  const long long all_parts = parts_of(a.n);
+  for (int which = 0; which < 2; ++which) {
+    const int id = which == 0 ? begun : goes_on;
+    if (id < 0) continue;
+    const int from = s.first[id], p0 = from / PART, p1 = (s.first[id + 1] - 1) / PART, slot0 = from > p0 * PART;
+    auto at = [&](int p) { return s.sums + ((long long)p * 2 + (p == p0 ? slot0 : 0)) * columns + tile * blockDim.x * way::W + threadIdx.x; };
+    auto counter = [&](int level, int p) { return s.done + ((level * all_parts + p) * 2 + (p == p0 ? slot0 : 0)) * tiles + tile; };
+    auto gather = [&](int first, int last, int step) {          // parts first, first + step (rounded down to step) ... last
+#pragma unroll
+      for (int k = 0; k < way::W; ++k) sum[k] = 0.f;
+      for (int p = first; p <= last;) {
+        float y[4][way::W];
+        int q = p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (q <= last)
+#pragma unroll
+            for (int k = 0; k < way::W; ++k) y[j][k] = __ldcg(at(q) + k * blockDim.x);
+          q = (q / step + 1) * step;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (p <= last)
+#pragma unroll
+            for (int k = 0; k < way::W; ++k) sum[k] += y[j][k];
+          p = (p / step + 1) * step;
+        }
+      }
+    };
+    const int g0 = max(part / PART * PART, p0), g1 = min(part / PART * PART + PART - 1, p1);
+    if (!last_of(counter(0, g0), g1 - g0 + 1, &last_one)) continue;
+    gather(g0, g1, 1);
+    if (p0 / PART != p1 / PART) {
+#pragma unroll
+      for (int k = 0; k < way::W; ++k) __stcg(at(g0) + k * blockDim.x, sum[k]);
+      if (!last_of(counter(1, p0), p1 / PART - p0 / PART + 1, &last_one)) continue;
+      gather(p0, p1, PART);
+    }
+    way::store(dtable + id * a.hidden, sum, a.scale, col, apart, a.hidden);
   }
 }
 
@@ -286,8 +385,9 @@ static int embed_check(const FlEmbedArgs* a) {
 
 extern "C" long long fl_embed_scratch(long long n, long long vocab, long long hidden) {
   if (n < 0 || n >= INT32_MAX || vocab < 1 || vocab >= INT32_MAX || hidden < 1 || hidden >= INT32_MAX) return -1;
-  const Scratch s = scratch_of(nullptr, n, vocab, hidden);
-  return (long long)((char*)s.parts - (char*)nullptr) + parts_of(n) * 2 * hidden * 4;
+  const long long most = (hidden * 4 + 511) / 512;                       // tiles of 32 threads, fp32
+  const Scratch s = scratch_of(nullptr, n, vocab, most);
+  return (long long)((char*)s.sums - (char*)nullptr) + parts_of(n) * 2 * (hidden + 2048) * 4;
 }
 
 extern "C" int fl_embed(int dtype, const FlEmbedArgs* a, cudaStream_t stream) {
@@ -316,16 +416,22 @@ extern "C" int fl_embed_grad(int dtype, const FlEmbedArgs* a, cudaStream_t strea
     using T = decltype(type);
     return by_pack<T>(pack_of<T>(a->hidden, a->hidden, a->dout, a->dtable), [&](auto width) {
       constexpr int N = decltype(width)::value;
-      const long long slices = (a->hidden + 32 * N - 1) / (32 * N), groups = (a->vocab + GROUP - 1) / GROUP;
-      if (slices > 65535) return -1;
+      const int threads = threads_of(a->hidden, sizeof(T));
+      const long long tiles = tiles_of(a->hidden, sizeof(T)), ranges = (a->vocab + RANGE - 1) / RANGE, ids = threads / 32 * ZERO_IDS,
+                      zero_blocks = (a->vocab + ids - 1) / ids, blocks = zero_blocks + parts_of(a->n) * tiles;
+      if (blocks > INT32_MAX) return -1;
       constexpr int bytes = SORT_WARPS * RANGE * 4;
-      const unsigned ranges = (unsigned)((a->vocab + RANGE - 1) / RANGE);
       auto sort = a->token_bytes == 8 ? embed_sort_kernel<long long> : embed_sort_kernel<int>;
       cudaError_t e = cudaFuncSetAttribute(sort, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
       if (e != cudaSuccess) return (int)e;
-      sort<<<ranges, SORT_THREADS, bytes, stream>>>(*a, (int)slices);
-      embed_sum_kernel<T, N><<<dim3((unsigned)(groups + parts_of(a->n)), (unsigned)slices), SUM_THREADS, 0, stream>>>(*a, (int)groups);
-      return (int)cudaGetLastError();
+      sort<<<(unsigned)ranges, SORT_THREADS, bytes, stream>>>(*a, (int)tiles);
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      at[0].val.programmaticStreamSerializationAllowed = 1;
+      cudaLaunchConfig_t c = {};
+      c.gridDim = dim3((unsigned)blocks); c.blockDim = dim3(threads); c.stream = stream; c.attrs = at; c.numAttrs = 1;
+      e = cudaLaunchKernelEx(&c, embed_sum_kernel<T, N>, *a, (int)zero_blocks, (int)tiles);
+      return (int)(e != cudaSuccess ? e : cudaGetLastError());
     });
   });
 }
