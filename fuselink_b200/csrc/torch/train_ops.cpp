@@ -135,7 +135,7 @@ tensor_list route_forward(const Tensor& logits, const RouteHow& h, const OptTens
   const int64_t T = logits.size(0), E = logits.size(1);
   Tensor w = new_like(logits, {T, h.topk}, torch::kFloat32), chosen = new_like(logits, {T, h.topk}, torch::kInt32), load = new_like(logits, {E}, torch::kInt32), term;
   if (balance) term = new_like(logits, {}, torch::kFloat32);
-  const Tensor scratch = new_bytes(logits, fl_route_scratch(T, a.experts, balance));
+  const Tensor scratch = new_bytes(logits, fl_route_scratch(a.experts));
   a.weights = w.data_ptr<float>(); a.chosen = chosen.data_ptr<int>(); a.load = load.data_ptr<int>(); a.balance = balance ? term.data_ptr<float>() : nullptr;
   a.scratch = scratch.data_ptr();
   check(fl_route(dtype_of(logits, "route"), &a, stream_of()), "fl_route");
