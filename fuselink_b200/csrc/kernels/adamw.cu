@@ -9,7 +9,7 @@
 // multiply-adds between them, so that the codes are the same wherever they are computed.
 //
 // Bound by memory: 10 bytes per bf16 weight with codes, 22 with fp32 moments, 28 with an fp32 copy of the weight as well.  A CTA takes 8192
-// values of one tensor; the tensors' addresses are kernel arguments, 400 tensors a launch, so that a captured step needs no copy of a table.
+// or 32768 values of one tensor; the tensors' addresses are kernel arguments, 400 tensors a launch, so that a captured step needs no copy of a table.
 // The number of steps is on the device: every CTA of a tensor adds 2^40 to it when it has read it, and the last one puts the next number.
 #include "adamw.cuh"
 #include <cuda_fp8.h>
@@ -21,7 +21,7 @@ namespace fl {
 namespace adamw {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int BLOCK = FL_ADAMW_BLOCK, CHUNK = 8192;
+constexpr int BLOCK = FL_ADAMW_BLOCK, LEAST_CHUNK = 8192, MOST_CHUNK = 32768;
 constexpr int MOST = 400, FEW = 32;              // tensors of a launch: 32 KB of arguments, or 2.5
 constexpr unsigned ALL = 0xffffffffu;
 constexpr long long ARRIVED = 1ll << 40;
@@ -30,8 +30,8 @@ template <int CAP>
 struct Launch {
   FlAdamwTensor t[CAP];
   int first[CAP];                                // chunks before the tensor's
-  int count;
-  float b1, c1, b2, c2, eps;
+  int count, chunk;                              // chunk: values of a CTA
+  float b1, c1, b2, c2, eps, one;
   double lr, decay, log_b1, log_b2;
   const float* lr_on_device;
 };
@@ -91,8 +91,180 @@ __device__ __forceinline__ Pack<T, 4> pack(const float* f) {
   return x;
 }
 
+__device__ __forceinline__ float rcp(float x) {   // 1 unit in the last place; 0 beyond 2^126
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two at a time, each rounded as one alone would be
+struct F2 {
+  unsigned long long bits;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ void get(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(bits)); }
+};
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits)); return r; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits)); return r; }
+// A sum as a one + b, where `one` is an argument of the kernel: add.rn.f32x2 of a product, and fma.rn.f32x2 with a 1 that the compiler knows, became
+// one rounding with it (46 of 16384 codes were another).
+__device__ __forceinline__ F2 sum2(F2 a, F2 b, F2 one) { return fma2(a, one, b); }
+
+// A lane's eight values of 256: consecutive ones, or, where some array has them in fp32, four and four that lie 128 apart, so that an access of the warp is
+// without gaps.
+template <typename T, bool APART>
+struct Eight {
+  static constexpr int M = APART ? 4 : sizeof(T) == 4 ? 4 : 8, LEAP = APART ? BLOCK / 2 : 4;
+  Pack<T, M> p[8 / M];
+  static __device__ __forceinline__ long long place(long long b) { return b + (threadIdx.x & 31) * (APART ? 4 : 8); }
+  __device__ __forceinline__ void load(const T* from, long long b) {
+#pragma unroll
+    for (int j = 0; j < 8 / M; ++j) p[j] = *reinterpret_cast<const Pack<T, M>*>(from + place(b) + j * LEAP);
+  }
+  __device__ __forceinline__ void store(T* to, long long b) const {
+#pragma unroll
+    for (int j = 0; j < 8 / M; ++j) *reinterpret_cast<Pack<T, M>*>(to + place(b) + j * LEAP) = p[j];
+  }
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int j = 0; j < 8 / M; ++j) p[j].get(f + j * M);
+  }
+  __device__ __forceinline__ void set(const float* f) {
+#pragma unroll
+    for (int j = 0; j < 8 / M; ++j) p[j].set(f + j * M);
+  }
+};
+template <bool APART>
+__device__ __forceinline__ uint2 load_codes(const void* from, long long b) {
+  const uint8_t* at = (const uint8_t*)from + Eight<uint8_t, APART>::place(b);
+  if (APART) return make_uint2(*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + BLOCK / 2));
+  return *reinterpret_cast<const uint2*>(at);
+}
+template <bool APART>
+__device__ __forceinline__ void store_codes(void* to, long long b, uint2 c) {
+  uint8_t* at = (uint8_t*)to + Eight<uint8_t, APART>::place(b);
+  if (APART) {
+    *reinterpret_cast<uint32_t*>(at) = c.x;
+    *reinterpret_cast<uint32_t*>(at + BLOCK / 2) = c.y;
+  } else {
+    *reinterpret_cast<uint2*>(at) = c;
+  }
+}
+__device__ __forceinline__ F2 values_of2(uint16_t codes) {
+  uint32_t two;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"(codes));
+  const float2 f = __half22float2(*reinterpret_cast<__half2*>(&two));
+  return F2(f.x, f.y);
+}
+__device__ __forceinline__ uint32_t codes_of2(float x, float y) {
+  uint16_t c;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(y), "f"(x));
+  return c;
+}
+__device__ __forceinline__ float at_least(float x, float least) {      // NaN stays
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(least));
+  return y;
+}
+
+// 256 values with codes, whole and from multiples of 16 bytes on (codes: of 8).  What a lane has loaded of them:
+template <typename T, bool MASTER>
+struct Loaded {
+  using W = typename std::conditional<MASTER, float, T>::type;
+  static constexpr bool APART = sizeof(W) == 4;
+  Eight<T, APART> g;
+  Eight<W, APART> w;
+  uint2 m, v;
+  float ms, rs;
+  __device__ __forceinline__ void load(const FlAdamwTensor& t, long long b) {
+    g.load((const T*)t.grad, b);
+    w.load(MASTER ? (const W*)t.master : (const W*)t.param, b);
+    m = load_codes<APART>(t.m, b);
+    v = load_codes<APART>(t.v, b);
+    ms = t.m_scale[b / BLOCK];
+    rs = t.v_scale[b / BLOCK];
+  }
+};
+// Instructions go two values at a time where the hardware has that; the largest magnitudes are taken over numbers (a NaN is left out by itself), and
+// infinities looked for only in them.
+template <typename T, bool MASTER, typename L>
+__device__ __forceinline__ void step_codes(const Loaded<T, MASTER>& in, const FlAdamwTensor& t, const L& a, long long b, float first, float second, float keep) {
+  constexpr bool APART = Loaded<T, MASTER>::APART;
+  float g[8], w[8], m[8], root[8];
+  const uint2 mc = in.m, vc = in.v;
+  in.g.get(g);
+  in.w.get(w);
+  const float ms = in.ms, rs = in.rs;
+  const F2 one(a.one, a.one);
+  const F2 ms2(ms, ms), rs2(rs, rs), b1(a.b1, a.b1), c1(a.c1, a.c1), b2(a.b2, a.b2), c2(a.c2, a.c2), keep2(keep, keep), eps2(a.eps, a.eps), second2(second, second), first2(-first, -first);
+  float m_most = 0.f, r_most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t mw = j < 2 ? mc.x : mc.y, vw = j < 2 ? vc.x : vc.y;
+    const F2 g2(g[2 * j], g[2 * j + 1]);
+    const F2 r_old = values_of2((uint16_t)(vw >> 16 * (j & 1))) * rs2;
+    const F2 m_new = sum2(values_of2((uint16_t)(mw >> 16 * (j & 1))) * ms2 * b1, g2 * c1, one), v_new = sum2(r_old * r_old * b2, g2 * g2 * c2, one);
+    float v0, v1;
+    v_new.get(v0, v1);
+    m_new.get(m[2 * j], m[2 * j + 1]);
+    root[2 * j] = __fsqrt_rn(v0);
+    root[2 * j + 1] = __fsqrt_rn(v1);
+    m_most = fmaxf(m_most, fmaxf(fabsf(m[2 * j]), fabsf(m[2 * j + 1])));
+    r_most = fmaxf(r_most, fmaxf(root[2 * j], root[2 * j + 1]));
+    float d0, d1;
+    fma2(F2(root[2 * j], root[2 * j + 1]), second2, eps2).get(d0, d1);
+    const F2 w2 = fma2(m_new * first2, F2(rcp(d0), rcp(d1)), F2(w[2 * j], w[2 * j + 1]) * keep2);
+    w2.get(w[2 * j], w[2 * j + 1]);
+  }
+  Eight<T, APART> out;
+  out.set(w);
+  out.store((T*)t.param, b);
+  if (MASTER) {
+    Eight<float, APART> copy;
+    copy.set(w);
+    copy.store(t.master, b);
+  }
+  uint32_t mb = __reduce_max_sync(ALL, __float_as_uint(m_most)), rb = __reduce_max_sync(ALL, __float_as_uint(r_most));
+  if (mb >= 0x7f800000u || rb >= 0x7f800000u) {  // infinities: no number decides a scale, and NaN is kept
+    uint32_t most = 0, r = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      most = max(most, finite_bits(m[j]));
+      r = max(r, finite_bits(root[j]));
+      m[j] = no_inf(m[j]);
+      root[j] = no_inf(root[j]);
+    }
+    mb = __reduce_max_sync(ALL, most);
+    rb = __reduce_max_sync(ALL, r);
+  }
+  mb = scale_bits(mb);
+  rb = scale_bits(rb);
+  const float m_inv = __uint_as_float((254u << 23) - mb), r_inv = __uint_as_float((254u << 23) - rb);
+  uint2 mo, ro;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t x[2], y[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int k = 4 * h + 2 * j;
+      x[j] = codes_of2(m[k] * m_inv, m[k + 1] * m_inv);
+      float r0 = root[k] * r_inv, r1 = root[k + 1] * r_inv;
+      if (root[k] != 0.f) r0 = at_least(r0, 0x1p-9f);      // the smallest code
+      if (root[k + 1] != 0.f) r1 = at_least(r1, 0x1p-9f);
+      y[j] = codes_of2(r0, r1);
+    }
+    (h == 0 ? mo.x : mo.y) = x[1] << 16 | x[0];
+    (h == 0 ? ro.x : ro.y) = y[1] << 16 | y[0];
+  }
+  store_codes<APART>(t.m, b, mo);
+  store_codes<APART>(t.v, b, ro);
+  if ((threadIdx.x & 31) == 0) {
+    t.m_scale[b / BLOCK] = __uint_as_float(mb);
+    t.v_scale[b / BLOCK] = __uint_as_float(rb);
+  }
+}
+
 template <typename T, bool CODES, bool MASTER, int CAP>
-__global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ Launch<CAP> a) {
+__global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant__ Launch<CAP> a) {
   __shared__ float shared[3];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int lo = 0, hi = a.count - 1;
@@ -101,7 +273,7 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
     if (a.first[mid] <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
   }
   const FlAdamwTensor& t = a.t[lo];
-  const int chunk = (int)blockIdx.x - a.first[lo], chunks = t.n > CHUNK ? (int)((t.n + CHUNK - 1) / CHUNK) : 1;
+  const int chunk = (int)blockIdx.x - a.first[lo], chunks = t.n > a.chunk ? (int)((t.n + a.chunk - 1) / a.chunk) : 1;
   if (threadIdx.x == 0) {
     const long long step = *reinterpret_cast<volatile long long*>(t.step) & (ARRIVED - 1);
     const double lr = a.lr_on_device != nullptr ? (double)*a.lr_on_device : a.lr;
@@ -117,8 +289,25 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
   bool wide = (bits & (4 * sizeof(T) - 1)) == 0;
   bits = (uintptr_t)t.m | (uintptr_t)t.v;
   wide = wide && (bits & (CODES ? 3 : 15)) == 0 && (!MASTER || ((uintptr_t)t.master & 15) == 0);
-  const long long end = min(t.n, (long long)(chunk + 1) * CHUNK);
-  for (long long b = (long long)chunk * CHUNK + warp * BLOCK; b < end; b += WARPS * BLOCK) {
+  const long long begin = (long long)chunk * a.chunk, end = min(t.n, begin + a.chunk);
+  long long b = begin + warp * BLOCK;
+  if constexpr (CODES) {
+    const bool eights = (((uintptr_t)t.param | (uintptr_t)t.grad | (uintptr_t)t.master) & 15) == 0 && (((uintptr_t)t.m | (uintptr_t)t.v) & 7) == 0;
+    if (eights && b + BLOCK <= end) {            // the next block's loads are on their way while one is computed
+      Loaded<T, MASTER> now, next;
+      now.load(t, b);
+      for (;;) {
+        const long long to = b + WARPS * BLOCK;
+        const bool more = to + BLOCK <= end;
+        if (more) next.load(t, to);
+        step_codes<T, MASTER>(now, t, a, b, first, second, keep);
+        b = to;
+        if (!more) break;
+        now = next;
+      }
+    }
+  }
+  for (; b < end; b += WARPS * BLOCK) {
     float m[2][4], root[2][4];
     uint32_t m_most = 0, r_most = 0;
     const float ms = CODES ? t.m_scale[b / BLOCK] : 1.f, rs = CODES ? t.v_scale[b / BLOCK] : 1.f;
@@ -148,7 +337,7 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
         m[h][i] = __fadd_rn(__fmul_rn(m[h][i], a.b1), __fmul_rn(g[i], a.c1));
         v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(g[i], g[i]), a.c2));
         root[h][i] = __fsqrt_rn(v[i]);
-        w[i] = fmaf(w[i], keep, -first * __fdividef(m[h][i], fmaf(root[h][i], second, a.eps)));
+        w[i] = fmaf(-first * m[h][i], rcp(fmaf(root[h][i], second, a.eps)), w[i] * keep);
         if (CODES) {
           m_most = max(m_most, finite_bits(m[h][i]));
           r_most = max(r_most, finite_bits(root[h][i]));
@@ -186,17 +375,21 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
 template <typename T, bool CODES, bool MASTER, int CAP>
 static int launch(const FlAdamwTensor* t, int count, const FlAdamwArgs* a, cudaStream_t stream) {
   static thread_local Launch<CAP> l;
-  long long chunks = 0;
+  long long all = 0, chunks = 0;
+  for (int i = 0; i < count; ++i) all += t[i].n;
+  // Each chunk begins with its tensor and its step, 2 us before the first value: with codes, which instructions bound, larger ones where there are many (285 M
+  // bf16 weights: 604 us against 663); in fp32 the memory has enough to do with others' values (958 us against 1017).
+  l.chunk = CODES && all / MOST_CHUNK > 148 * 16 ? MOST_CHUNK : LEAST_CHUNK;
   for (int i = 0; i < count; ++i) {
     l.t[i] = t[i];
     l.first[i] = (int)chunks;
-    chunks += t[i].n > CHUNK ? (t[i].n + CHUNK - 1) / CHUNK : 1;
+    chunks += t[i].n > l.chunk ? (t[i].n + l.chunk - 1) / l.chunk : 1;
     if (chunks > INT32_MAX) return -1;
   }
   l.count = count;
   l.b1 = (float)a->beta1; l.c1 = (float)(1.0 - a->beta1);
   l.b2 = (float)a->beta2; l.c2 = (float)(1.0 - a->beta2);
-  l.eps = (float)a->eps; l.lr = a->lr; l.decay = a->weight_decay;
+  l.one = 1.f; l.eps = (float)a->eps; l.lr = a->lr; l.decay = a->weight_decay;
   l.log_b1 = log(a->beta1); l.log_b2 = log(a->beta2);
   l.lr_on_device = a->lr_on_device;
   adamw_kernel<T, CODES, MASTER, CAP><<<(unsigned)chunks, THREADS, 0, stream>>>(l);
@@ -221,7 +414,7 @@ extern "C" int fl_adamw(int dtype, const FlAdamwTensor* t, long long count, cons
   using namespace fl::adamw;
   if (count < 0 || !(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0)) return -1;
   for (long long i = 0; i < count; ++i)
-    if (t[i].n < 0 || t[i].n > (long long)CHUNK * (1 << 22) || t[i].step == nullptr) return -1;
+    if (t[i].n < 0 || t[i].n > (long long)LEAST_CHUNK * (1 << 22) || t[i].step == nullptr) return -1;
   return fl_by_dtype(dtype, [&](auto type) {
     using T = decltype(type);
     if (a->master) {
