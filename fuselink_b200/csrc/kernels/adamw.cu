@@ -96,19 +96,6 @@ __device__ __forceinline__ float rcp(float x) {   // 1 unit in the last place; 0
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Two at a time, each rounded as one alone would be
-struct F2 {
-  unsigned long long bits;
-  __device__ __forceinline__ F2() {}
-  __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(x), "f"(y)); }
-  __device__ __forceinline__ void get(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(bits)); }
-};
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits)); return r; }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits)); return r; }
-// A sum as a one + b, where `one` is an argument of the kernel: add.rn.f32x2 of a product, and fma.rn.f32x2 with a 1 that the compiler knows, became
-// one rounding with it (46 of 16384 codes were another).
-__device__ __forceinline__ F2 sum2(F2 a, F2 b, F2 one) { return fma2(a, one, b); }
-
 // A lane's eight values of 256: consecutive ones, or, where some array has them in fp32, four and four that lie 128 apart, so that an access of the warp is
 // without gaps.
 template <typename T, bool APART>

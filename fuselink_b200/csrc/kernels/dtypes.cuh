@@ -70,6 +70,21 @@ struct Pack {
   }
 };
 
+// Two at a time, each rounded as one alone would be
+struct F2 {
+  unsigned long long bits;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ void get(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(bits)); }
+};
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits)); return r; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits)); return r; }
+// A sum as a one + b, where `one` is an argument of the kernel: add.rn.f32x2 of a product, and fma.rn.f32x2 with a 1 that the compiler knows, became
+// one rounding with it (46 of 16384 codes were another).
+__device__ __forceinline__ F2 sum2(F2 a, F2 b, F2 one) { return fma2(a, one, b); }
+
+__device__ __forceinline__ F2 plain_sum2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits)); return r; }      // where one rounding in place of two does no harm
+
 }  // namespace fl
 
 // Calls f(T{}) with the element type of `dtype`
