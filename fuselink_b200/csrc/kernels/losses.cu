@@ -17,7 +17,7 @@ namespace fl {
 namespace losses {
 
 constexpr int SMS = 148;
-constexpr int MOST_CTAS = SMS * 4;                 // 256 threads each, or half as many of 512
+constexpr int MOST_CTAS = SMS * 32;
 constexpr unsigned ALL = 0xffffffffu;
 constexpr int AHEAD = 4;                           // vectors on their way per thread
 
@@ -34,11 +34,10 @@ __device__ __forceinline__ int head_of(const T* row, long long vocab) {      // 
   return n < vocab ? n : (int)vocab;
 }
 
-// 16 bytes of logits as pairs, and the largest of them
+// 16 bytes of logits as fp32, and the largest of them
 template <typename T> struct Logits;
 template <> struct Logits<float> {
   static constexpr uint32_t NONE = 0xff800000u;    // -inf
-  static __device__ __forceinline__ F2 pair(const uint4& x, int i) { return i == 0 ? F2(__uint_as_float(x.x), __uint_as_float(x.y)) : F2(__uint_as_float(x.z), __uint_as_float(x.w)); }
   static __device__ __forceinline__ uint4 larger(const uint4& a, const uint4& b) {
     return make_uint4(__float_as_uint(fmaxf(__uint_as_float(a.x), __uint_as_float(b.x))), __float_as_uint(fmaxf(__uint_as_float(a.y), __uint_as_float(b.y))),
                       __float_as_uint(fmaxf(__uint_as_float(a.z), __uint_as_float(b.z))), __float_as_uint(fmaxf(__uint_as_float(a.w), __uint_as_float(b.w))));
@@ -47,12 +46,8 @@ template <> struct Logits<float> {
     return fmaxf(fmaxf(__uint_as_float(x.x), __uint_as_float(x.y)), fmaxf(__uint_as_float(x.z), __uint_as_float(x.w)));
   }
 };
-template <typename T> struct Logits16 {
-  static __device__ __forceinline__ uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
-};
-template <> struct Logits<__nv_bfloat16> : Logits16<__nv_bfloat16> {
+template <> struct Logits<__nv_bfloat16> {
   static constexpr uint32_t NONE = 0xff80ff80u;
-  static __device__ __forceinline__ F2 pair(const uint4& x, int i) { return F2(__uint_as_float(word(x, i) << 16), __uint_as_float(word(x, i) & 0xffff0000u)); }
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -63,13 +58,8 @@ template <> struct Logits<__nv_bfloat16> : Logits16<__nv_bfloat16> {
     return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
   }
 };
-template <> struct Logits<__half> : Logits16<__half> {
+template <> struct Logits<__half> {
   static constexpr uint32_t NONE = 0xfc00fc00u;
-  static __device__ __forceinline__ F2 pair(const uint4& x, int i) {
-    const uint32_t w = word(x, i);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-    return F2(f.x, f.y);
-  }
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
     const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -90,23 +80,26 @@ __device__ __forceinline__ void merge(Running& a, const Running& b, float unit) 
   a.sum = a.sum * ex2((a.top - top) * unit) + b.sum * ex2((b.top - top) * unit);
   a.top = top;
 }
-// 2^(unit (x - top)) of both
-__device__ __forceinline__ F2 powers(F2 x, F2 minus_top, F2 unit) {
+// Exponents are unit x - base, one instruction for two, with base = unit top rounded: all terms of a row are 2^r too large then, r the rounding's error, and the
+// row's sum with them.  Logits of such size that r would matter are taken one by one, as unit (x - top).
+constexpr float LARGE = 1e6f;
+__device__ __forceinline__ bool large(float top) { return !(fabsf(top) < LARGE); }
+__device__ __forceinline__ F2 powers(float x, float y, F2 unit, F2 minus) {
   float a, b;
-  (plain_sum2(x, minus_top) * unit).get(a, b);
+  fma2(F2(x, y), unit, minus).get(a, b);
   return F2(ex2(a), ex2(b));
 }
 
-// The row's running sum, the same in all threads.  It starts from the least finite number: a row's -inf then make no difference of infinities.
+// The row's running sum, the same in all threads.  It starts from a finite number: a row's -inf then make no difference of infinities.
 template <typename T, int THREADS>
 __device__ __forceinline__ Running sum_row(const T* row, long long vocab, float unit, Running* shared) {
   constexpr int P = PER<T>;
   const int head = head_of(row, vocab);
   const int packs = (int)((vocab - head) / P);
   const uint4* v = reinterpret_cast<const uint4*>(row + head);
-  const F2 unit2(unit, unit);
-  float top = -3.402823466e38f;
+  float top = -LARGE;
   F2 sum(0.f, 0.f);
+  const F2 unit2(unit, unit);
   for (int i = threadIdx.x; i < packs; i += THREADS * AHEAD) {
     uint4 x[AHEAD];
 #pragma unroll
@@ -121,46 +114,63 @@ __device__ __forceinline__ Running sum_row(const T* row, long long vocab, float 
       sum = sum * F2(fall, fall);
       top = to;
     }
-    const F2 minus(-top, -top);
+    const float base = -(top * unit);
+    const F2 minus(base, base);
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
+    for (int j = 0; j < AHEAD; ++j) {
+      float f[P];
+      Pack<T, P>{x[j]}.get(f);
 #pragma unroll
-      for (int k = 0; k < P / 2; ++k) sum = plain_sum2(sum, powers(Logits<T>::pair(x[j], k), minus, unit2));
+      for (int k = 0; k < P; k += 2) sum = plain_sum2(sum, powers(f[k], f[k + 1], unit2, minus));
+    }
   }
+  // the thread's sum as one of 2^(unit (x - top)), whatever its base's rounding
   float one, other;
   sum.get(one, other);
-  Running r{top, one + other};
+  Running r{top, (one + other) * ex2(-fmaf(top, unit, -(top * unit)))};
   for (long long i = threadIdx.x; i < vocab - (long long)packs * P; i += THREADS) {
     const float x = to_f32(row[i < head ? i : (long long)packs * P + i]), to = fmaxf(x, r.top);
     r.sum = r.sum * ex2((r.top - to) * unit) + ex2((x - to) * unit);
     r.top = to;
   }
+  auto join = [&]() {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) merge(r, Running{__shfl_xor_sync(ALL, r.top, o), __shfl_xor_sync(ALL, r.sum, o)}, unit);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = r;
-  __syncthreads();
-  r = shared[0];
+    for (int o = 16; o > 0; o >>= 1) merge(r, Running{__shfl_xor_sync(ALL, r.top, o), __shfl_xor_sync(ALL, r.sum, o)}, unit);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = r;
+    __syncthreads();
+    r = shared[0];
 #pragma unroll
-  for (int w = 1; w < THREADS / 32; ++w) merge(r, shared[w], unit);
+    for (int w = 1; w < THREADS / 32; ++w) merge(r, shared[w], unit);
+  };
+  join();
+  if (large(r.top)) {                              // or nothing above -LARGE: once more, one by one
+    r = Running{-3.402823466e38f, 0.f};
+    for (long long i = threadIdx.x; i < vocab; i += THREADS) {
+      const float x = to_f32(row[i]), to = fmaxf(x, r.top);
+      r.sum = r.sum * ex2((r.top - to) * unit) + ex2((x - to) * unit);
+      r.top = to;
+    }
+    join();
+  }
   return r;
 }
 
-// out_j = factor (1[j = tok] - p_j).  The row is read from L2 for the most part, and what is written not kept there.
+// out_j = factor (1[j = tok] - p_j).  The row is in L2 for the most part; what is written is not kept there.  inverse: 1 / sum_j 2^(unit (x_j - top))
 template <typename T, int THREADS>
 __device__ __forceinline__ void write_row(T* out, const T* row, long long vocab, float unit, float top, float inverse, float factor, long long tok) {
   constexpr int P = PER<T>;
   const int head = head_of(row, vocab);
-  const int packs = (int)((vocab - head) / P);
+  const int packs = large(top) && factor != 0.f ? 0 : (int)((vocab - head) / P);
   const uint4* v = reinterpret_cast<const uint4*>(row + head);
   uint4* to = reinterpret_cast<uint4*>(out + head);
-  const float share = -factor * inverse;
   if (factor == 0.f) {                             // nothing is read
     for (int i = threadIdx.x; i < packs; i += THREADS) st_cs_v4(to + i, make_uint4(0, 0, 0, 0));
     for (long long i = threadIdx.x; i < vocab - (long long)packs * P; i += THREADS) out[i < head ? i : (long long)packs * P + i] = from_f32<T>(0.f);
     return;
   }
-  const F2 unit2(unit, unit), minus(-top, -top), share2(share, share);
+  const float base = -(top * unit), share = -factor * inverse, fine = share * ex2(-fmaf(top, unit, base));      // the latter without the base's rounding
+  const F2 unit2(unit, unit), minus(base, base), fine2(fine, fine);
   for (int i = threadIdx.x; i < packs; i += THREADS * AHEAD) {
     uint4 x[AHEAD];
 #pragma unroll
@@ -170,16 +180,17 @@ __device__ __forceinline__ void write_row(T* out, const T* row, long long vocab,
     for (int j = 0; j < AHEAD; ++j) {
       if (i + j * THREADS >= packs) break;
       float f[P];
+      Pack<T, P>{x[j]}.get(f);
 #pragma unroll
-      for (int k = 0; k < P / 2; ++k) (powers(Logits<T>::pair(x[j], k), minus, unit2) * share2).get(f[2 * k], f[2 * k + 1]);
+      for (int k = 0; k < P; k += 2) (powers(f[k], f[k + 1], unit2, minus) * fine2).get(f[k], f[k + 1]);
       Pack<T, P> y;
       y.set(f);
-      st_cs_v4(to + i + j * THREADS, y.raw);
+      st_cs_v4(to + i + j * THREADS, *reinterpret_cast<const uint4*>(&y.raw));
     }
   }
   for (long long i = threadIdx.x; i < vocab - (long long)packs * P; i += THREADS) {
-    const long long at = i < head ? i : (long long)packs * P + i;
-    out[at] = from_f32<T>(ex2((to_f32(row[at]) - top) * unit) * share);
+    const long long j = i < head ? i : (long long)packs * P + i;
+    out[j] = from_f32<T>(ex2((to_f32(row[j]) - top) * unit) * share);
   }
   // the token's own value, by the thread that has written it already
   if (tok >= 0 && tok < vocab) {
@@ -188,6 +199,15 @@ __device__ __forceinline__ void write_row(T* out, const T* row, long long vocab,
     if ((int)threadIdx.x == owner) out[tok] = from_f32<T>(fmaf(ex2((to_f32(row[tok]) - top) * unit), share, factor));
   }
 }
+
+struct Sums {
+  double loss, divergence, clipped;
+};
+struct Scratch {
+  double* total;                                   // the weights' sum
+  Sums* sums;                                      // [CTAs]
+};
+__host__ __device__ inline Scratch scratch_of(void* p) { return {(double*)p, (Sums*)((char*)p + 256)}; }
 
 template <int THREADS>
 __device__ __forceinline__ double block_sum(double x, double* shared) {       // in a fixed order
@@ -201,26 +221,48 @@ __device__ __forceinline__ double block_sum(double x, double* shared) {       //
   return x;
 }
 
-struct Sums {
-  double loss, divergence, clipped;
+__global__ void __launch_bounds__(1024) weights_kernel(const FlLossArgs a) {
+  __shared__ double sums[32];
+  grid_dep_launch();
+  const long long rows = a.outer * a.inner;
+  double w = 0.0;
+#pragma unroll 8
+  for (long long r = threadIdx.x; r < rows; r += 1024) w += a.weights[r];
+  w = block_sum<1024>(w, sums);
+  if (threadIdx.x == 0) *scratch_of(a.scratch).total = w;
+}
+
+// What one row adds to the loss, and the derivative of that by its log-probability; without the weight.  In 64 bits as far as numbers are taken from one another.
+struct Term {
+  double loss, divergence, slope;
+  bool clipped;
 };
+__device__ __forceinline__ Term term_of(const FlLossArgs& a, double lp, float old, float advantage, float reference) {
+  Term t{0.0, 0.0, 0.0, false};
+  const float q = expf((float)(lp - (double)old)), A = advantage;
+  const float held = fminf(fmaxf(q, (float)(1.0 - a.clip_low)), (float)(1.0 + a.clip_high)) * A, open = q * A;
+  t.loss = open <= held ? -open : -held;
+  t.slope = open <= held ? -open : 0.f;
+  if (q != q) t.loss = t.slope = q;
+  t.clipped = open > held;
+  if (a.reference != nullptr) {
+    const double gap = (double)reference - lp, more = expm1(gap);
+    t.divergence = more < 1e300 ? more - gap : more;
+    t.loss += a.kl * t.divergence;
+    t.slope -= a.kl * more;
+  }
+  return t;
+}
 
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const FlLossArgs a) {
   __shared__ Running shared[THREADS / 32];
-  __shared__ double sums[THREADS / 32];
-  __shared__ float said[2];
+  __shared__ float said;
   const float unit = (float)(1.4426950408889634 / a.temperature);
   const long long rows = a.outer * a.inner;
+  const bool policy = a.loss != nullptr;
   double total = (double)rows;
-  if (a.loss != nullptr) {
-    if (a.total != nullptr) total = *a.total;
-    else if (a.weights != nullptr) {
-      double w = 0.0;
-      for (long long r = threadIdx.x; r < rows; r += THREADS) w += a.weights[r];
-      total = block_sum<THREADS>(w, sums);
-    }
-  }
+  bool asked = false;
   Sums mine{0.0, 0.0, 0.0};
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = (const T*)a.logits + r / a.inner * a.outer_stride + r % a.inner * a.inner_stride;
@@ -235,58 +277,58 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const FlL
       if (a.dlogits != nullptr) write_row<T, THREADS>(out, row, a.vocab, unit, 0.f, 0.f, 0.f, -1);
       continue;
     }
-    const Running s = sum_row<T, THREADS>(row, a.vocab, unit, shared);
+    // asked for before the row, used behind it
     const long long tok = a.tokens[r];
+    float old = 0.f, advantage = 0.f, reference = 0.f;
+    if (threadIdx.x == 0 && policy) {
+      old = a.old[r];
+      advantage = a.advantages[r];
+      if (a.reference != nullptr) reference = a.reference[r];
+    }
+    const Running s = sum_row<T, THREADS>(row, a.vocab, unit, shared);
     if (threadIdx.x == 0) {
       const bool ok = tok >= 0 && tok < a.vocab;
       const double x = ok ? (double)to_f32(row[tok]) - (double)s.top : (double)NAN;
       const double lp = x / a.temperature - log((double)s.sum);
       a.logprobs[r] = (float)lp;
       if (a.top != nullptr) { a.top[r] = s.top; a.inverse[r] = 1.f / s.sum; }
-      if (a.loss != nullptr) {
-        const double adv = a.advantages[r], q = exp(lp - (double)a.old[r]);
-        const double held = fmin(fmax(q, 1.0 - a.clip_low), 1.0 + a.clip_high) * adv, open = q * adv;
-        double term = open <= held ? -open : -held, d = open <= held ? -open : 0.0;
-        if (q != q) term = d = q;
-        if (open > held) mine.clipped += w;
-        if (a.reference != nullptr) {
-          const double gap = (double)a.reference[r] - lp, more = expm1(gap);
-          const double far = more < 1e300 ? more - gap : more;
-          mine.divergence += w * far;
-          term += a.kl * far;
-          d -= a.kl * more;
+      if (policy) {
+        const Term t = term_of(a, lp, old, advantage, reference);
+        if (!asked) {
+          asked = true;
+          grid_dep_wait();                         // the weights' sum
+          if (a.total != nullptr) total = *a.total;
+          else if (a.weights != nullptr) total = *scratch_of(a.scratch).total;
+          total = total == 0.0 ? 0.0 : 1.0 / total;
         }
-        mine.loss += w * term;
-        said[0] = total == 0.0 ? 0.f : (float)(d * w / total);
-        if (a.coefficient != nullptr) a.coefficient[r] = said[0];
+        mine.loss += w * t.loss;
+        mine.divergence += w * t.divergence;
+        if (t.clipped) mine.clipped += w;
+        said = total == 0.0 ? 0.f : (float)(t.slope * (w * total));
+        if (a.coefficient != nullptr) a.coefficient[r] = said;
       }
     }
     if (a.dlogits != nullptr) {
       __syncthreads();
-      write_row<T, THREADS>(out, row, a.vocab, unit, s.top, 1.f / s.sum, (float)((double)said[0] / a.temperature), tok);
+      write_row<T, THREADS>(out, row, a.vocab, unit, s.top, 1.f / s.sum, (float)((double)said / a.temperature), tok);
     }
   }
-  if (a.loss != nullptr && threadIdx.x == 0) {
-    Sums* out = (Sums*)a.scratch;
-    const double inv = total == 0.0 ? 0.0 : 1.0 / total;
-    out[blockIdx.x] = Sums{mine.loss * inv, mine.divergence * inv, mine.clipped * inv};
-  }
+  if (policy && threadIdx.x == 0) scratch_of(a.scratch).sums[blockIdx.x] = asked ? Sums{mine.loss * total, mine.divergence * total, mine.clipped * total} : mine;
 }
 
-__global__ void __launch_bounds__(32) loss_sum_kernel(const FlLossArgs a, int ctas) {
+__global__ void __launch_bounds__(256) loss_sum_kernel(const FlLossArgs a, int ctas) {
+  __shared__ double sums[8];
+  const Sums* parts = scratch_of(a.scratch).sums;
   Sums s{0.0, 0.0, 0.0};
-  for (int b = threadIdx.x; b < ctas; b += 32) {
-    const Sums x = ((const Sums*)a.scratch)[b];
-    s.loss += x.loss;
-    s.divergence += x.divergence;
-    s.clipped += x.clipped;
+#pragma unroll 4
+  for (int b = threadIdx.x; b < ctas; b += 256) {
+    s.loss += parts[b].loss;
+    s.divergence += parts[b].divergence;
+    s.clipped += parts[b].clipped;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    s.loss += __shfl_xor_sync(ALL, s.loss, o);
-    s.divergence += __shfl_xor_sync(ALL, s.divergence, o);
-    s.clipped += __shfl_xor_sync(ALL, s.clipped, o);
-  }
+  s.loss = block_sum<256>(s.loss, sums);
+  s.divergence = block_sum<256>(s.divergence, sums);
+  s.clipped = block_sum<256>(s.clipped, sums);
   if (threadIdx.x == 0) {
     *a.loss = (float)s.loss;
     *a.divergence = (float)s.divergence;
@@ -320,21 +362,26 @@ static bool bad(const FlLossArgs* a) {
 static bool apart(const FlLossArgs* a, int size) {
   return (((uintptr_t)a->dlogits - (uintptr_t)a->logits) | (uintptr_t)((a->dlogits_outer - a->outer_stride) * size) | (uintptr_t)((a->dlogits_inner - a->inner_stride) * size)) & 15;
 }
-// Calls f(threads, CTAs).  256 threads a row, four rows an SM, where all rows that are in work stay in L2 until they are read again; 512, two rows an SM,
-// where they would not, and where rows are so few that an SM has no more.
+// Calls f(threads, CTAs).  Short rows are a warp's or 128 threads' (32768 rows of 1000 bf16: 115 us with the gradient, 259 with 256 threads a row); others 256 threads',
+// four an SM, whatever their length (1024 x 128256, two of 512: 15% slower); 512 where rows are so few that an SM has no more than two.
 template <typename F>
 static int by_rows(const FlLossArgs* a, int size, F&& f) {
-  const long long rows = a->outer * a->inner;
-  const bool wide = a->vocab * size > 96 * 1024 || rows <= 2 * SMS;
-  const long long most = wide ? MOST_CTAS / 2 : MOST_CTAS;
+  const long long rows = a->outer * a->inner, bytes = a->vocab * size;
+  const int threads = bytes <= 8 * 1024 && rows > SMS * 8 ? 32 : bytes <= 24 * 1024 && rows > SMS * 4 ? 128 : rows > SMS * 2 ? 256 : 512;
+  const long long most = SMS * (1024 / threads);
   const int ctas = (int)(rows < most ? rows : most);
-  return wide ? f(std::integral_constant<int, 512>{}, ctas) : f(std::integral_constant<int, 256>{}, ctas);
+  switch (threads) {
+    case 32: return f(std::integral_constant<int, 32>{}, ctas);
+    case 128: return f(std::integral_constant<int, 128>{}, ctas);
+    case 256: return f(std::integral_constant<int, 256>{}, ctas);
+    default: return f(std::integral_constant<int, 512>{}, ctas);
+  }
 }
 
 }  // namespace losses
 }  // namespace fl
 
-extern "C" long long fl_policy_scratch(void) { return fl::losses::MOST_CTAS * (long long)sizeof(fl::losses::Sums); }
+extern "C" long long fl_policy_scratch(void) { return 256 + fl::losses::MOST_CTAS * (long long)sizeof(fl::losses::Sums); }
 
 extern "C" int fl_token_logprobs(int dtype, const FlLossArgs* a, cudaStream_t stream) {
   using namespace fl::losses;
@@ -357,8 +404,20 @@ extern "C" int fl_policy_loss(int dtype, const FlLossArgs* a, cudaStream_t strea
     using T = decltype(type);
     return by_rows(a, sizeof(T), [&](auto threads, int ctas) {
       constexpr int N = decltype(threads)::value;
-      if (ctas > 0) loss_kernel<T, N><<<ctas, N, 0, stream>>>(*a);
-      loss_sum_kernel<<<1, 32, 0, stream>>>(*a, ctas);
+      if (ctas > 0) {
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t c = {};
+        c.gridDim = dim3(ctas); c.blockDim = dim3(N); c.stream = stream; c.attrs = at;
+        if (a->weights != nullptr && a->total == nullptr) {
+          weights_kernel<<<1, 1024, 0, stream>>>(*a);
+          c.numAttrs = 1;                          // the rows begin beside that; what came before is behind both
+        }
+        const cudaError_t e = cudaLaunchKernelEx(&c, loss_kernel<T, N>, *a);
+        if (e != cudaSuccess) return (int)e;
+      }
+      loss_sum_kernel<<<1, 256, 0, stream>>>(*a, ctas);
       return (int)cudaGetLastError();
     });
   });
