@@ -33,6 +33,12 @@ def main():
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--log-every", type=int, default=5)
     ap.add_argument("--lr", type=float, default=0.01)
+    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adamw", "adamw8"], help="adamw: moments in fp32; adamw8: in 8 bits; both keep fp32 copies of the "
+                                                                                           "weights and update the experts too (sgd updates them in their gradients' GEMM)")
+    ap.add_argument("--objective", default="tokens", choices=["tokens", "policy"], help="policy: the clipped policy loss on the model's own log-probabilities, with a "
+                                                                                        "random advantage for each sequence")
+    ap.add_argument("--gate", default="", choices=["", "softmax", "sigmoid"], help="routers that choose by these scores and a balance bias (ops/routing.py)")
+    ap.add_argument("--embed-scale", type=float, default=0.0, help="factor of the embedding's rows (0: as they are)")
     ap.add_argument("--device", default="cuda", choices=["cuda", "cpu"])
     ap.add_argument("--shadow", type=int, default=0, help="replicate the N most favoured experts of every layer on every rank (CUDA, several ranks)")
     ap.add_argument("--reshadow-every", type=int, default=0, help="with --shadow: every K steps choose the shadowed experts of each layer "
@@ -43,6 +49,8 @@ def main():
     ap.add_argument("--checkpoint", default="", help="save the last state here (per rank: experts differ)")
     ap.add_argument("--resume", default="", help="load <path>.rank<r> written by --checkpoint (same world size) before training")
     a = ap.parse_args()
+    if a.reshadow_every and a.optimizer != "sgd":
+        ap.error("--reshadow-every moves experts between copy slots, and AdamW's moments and fp32 copies stay with the slots: --optimizer sgd")
     from fuselink_b200.models.moe_transformer import MOE_ZOO, MoETransformer
     rank, local, world = (int(os.environ.get(k, d)) for k, d in (("RANK", 0), ("LOCAL_RANK", 0), ("WORLD_SIZE", 1)))
     cpu = a.device == "cpu"
@@ -51,6 +59,11 @@ def main():
         cfg = dataclasses.replace(cfg, layers=a.layers)
     if a.shadow:
         cfg = dataclasses.replace(cfg, shadow_experts=a.shadow)
+    if a.gate:
+        from fuselink_b200.models.moe import Gate
+        cfg = dataclasses.replace(cfg, gate=Gate(score=a.gate, balance_bias=True))
+    if a.embed_scale:
+        cfg = dataclasses.replace(cfg, embed_scale=a.embed_scale)
     heap = None
     if cpu:
         dev = torch.device("cpu")
@@ -70,11 +83,16 @@ def main():
         if a.shadow and world > 1:                                                     # + expert weights and gradient staging of the copies
             per_layer += (E // world + 2 * a.shadow) * 3 * H * cfg.ffn * 2 + (1 << 20)
         heap = SymmetricHeap.create(cfg.layers * per_layer + (64 << 20), device=-1 if cpu else local)
-    net = MoETransformer(cfg, a.batch * a.seq, heap, rank, world, device=dev, seed=0, fused_sgd_lr=a.lr if fused else 0.0)
+    net = MoETransformer(cfg, a.batch * a.seq, heap, rank, world, device=dev, seed=0,
+                         fused_sgd_lr=a.lr if fused and a.optimizer == "sgd" else 0.0)
     if a.resume:
         net.load_state_dict(torch.load(f"{a.resume}.rank{rank}", map_location=dev))
-    params = net.dense_parameters() if fused else net.parameters()     # on the fused path the expert update is part of the wgrad GEMM
-    opt = torch.optim.SGD(params, lr=a.lr)
+    if a.optimizer == "sgd":
+        params = net.dense_parameters() if fused else net.parameters()     # on the fused path the expert update is part of the wgrad GEMM
+        opt = torch.optim.SGD(params, lr=a.lr)
+    else:
+        from fuselink_b200.ops.adamw import AdamW
+        opt = AdamW(net.parameters(), lr=a.lr, state_bits=8 if a.optimizer == "adamw8" else 32, master=True)
     gen = torch.Generator(device=dev).manual_seed(100 + rank)
     t_mark, tok = time.perf_counter(), 0
     ev = None if cpu else (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
@@ -83,7 +101,11 @@ def main():
     for step in range(1, a.steps + 1):
         tokens = torch.randint(0, cfg.vocab, (a.batch, a.seq), device=dev, generator=gen)
         labels = torch.roll(tokens, -1, 1)
-        loss = net.train_step(tokens, labels, opt)
+        if a.objective == "policy":
+            advantages = torch.randn(a.batch, 1, device=dev, generator=gen)
+            loss = net.policy_step(tokens, net.token_logprobs(tokens), advantages, opt).loss
+        else:
+            loss = net.train_step(tokens, labels, opt)
         tok += a.batch * a.seq
         if a.reshadow_every and step % a.reshadow_every == 0:
             for b in net.blocks:                 # between steps: nothing of the layer is in flight

@@ -8,16 +8,29 @@ from __future__ import annotations
 
 import dataclasses
 import os
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
 import torch.nn as nn
 
 from .._ext import require_native
-from ..ops import gemm, ref
+from ..ops import gemm, ref, routing
 from ..ops.checks import ordinary as _ordinary
 from ..ops.moe import MoEConfig, MoEFunction, MoEWorkspace, balanced_placement, expert_home
 from ..parallel.symm import SymmetricHeap
+
+
+@dataclass(frozen=True)
+class Gate:
+    """How a layer's router chooses, beyond the softmax of its logits (ops/routing.py)."""
+    score: str = "sigmoid"                # or "softmax"
+    groups: int = 1                       # groups of consecutive experts, ...
+    topk_groups: Optional[int] = None     # ... of which so many are chosen from (None: all)
+    group_best: int = 2                   # a group goes by the sum of its 1 or 2 best
+    renormalize: bool = True              # a token's weights sum to `scale`
+    scale: float = 1.0
+    balance_bias: bool = False            # a bias of the choice that MoELayer.update_balance moves towards even loads
 
 
 def zipf_log_bias(num_experts: int, s: float = 1.2) -> torch.Tensor:
@@ -94,13 +107,17 @@ class MoELayer(nn.Module):
     with ``drop_tokens`` (choices over an expert's capacity contribute nothing; on the fused path their rows still
     travel, with weight zero, because the transport is sized for the worst case), ``noisy_gate`` ("jitter": inputs of
     the router are scaled by U(1-eps, 1+eps) in training; "rsample": Gumbel noise on the logits), and the
-    load-balancing auxiliary loss of the last forward in ``self.l_aux``."""
+    load-balancing auxiliary loss of the last forward in ``self.l_aux``.  With a ``gate`` the choice is that of ops/routing.py: any number of experts up to 1024,
+    sigmoid or softmax scores, groups, and a bias that ``update_balance`` keeps even loads with; ``l_aux`` is its balance term while training, ``last_load`` the
+    tokens that chose each expert, and the router's bias counts where ``zipf_s`` asks for it."""
 
     def __init__(self, cfg: MoEConfig, heap: Optional[SymmetricHeap] = None, rank: int = 0, world: int = 1,
                  device="cuda", zipf_s: Optional[float] = 1.2, seed: int = 0, fused_sgd_lr: float = 0.0,
                  name: str = "moe", capacity_factor: float = 0.0, drop_tokens: bool = False, min_capacity: int = 4,
-                 noisy_gate: Optional[str] = None, jitter_eps: float = 1e-2, shadow_experts=0, placement=None):
+                 noisy_gate: Optional[str] = None, jitter_eps: float = 1e-2, shadow_experts=0, placement=None, gate: Optional[Gate] = None):
         super().__init__()
+        if gate is not None and noisy_gate == "rsample":
+            raise ValueError("MoELayer: a gate draws no Gumbel noise; noisy_gate 'jitter' or None")
         bias = zipf_log_bias(cfg.num_experts, zipf_s) if zipf_s else torch.zeros(cfg.num_experts)
         # which rank owns which expert: in order by default; "balanced" evens out the rows per rank the router's bias
         # predicts (the same on every rank, since the bias is); or an explicit tuple of homes
@@ -126,6 +143,9 @@ class MoELayer(nn.Module):
         H, F, E = cfg.hidden, cfg.ffn, cfg.num_experts
         self.router = nn.Parameter((torch.randn(E, H, generator=g) * 0.02).to(torch.bfloat16).to(device))
         self.register_buffer("router_bias", bias.to(device))
+        self.gate, self.skewed = gate, bool(zipf_s)
+        if gate is not None and gate.balance_bias:
+            self.register_buffer("balance_bias", torch.zeros(E, device=device))
         # this rank's experts, then its copies of the shadowed experts (ops.moe.slot_table); every expert's init depends on
         # (seed, global expert id), not on the layout, so a copy starts out equal to the owner's expert
         w13, w2 = [], []
@@ -181,6 +201,13 @@ class MoELayer(nn.Module):
         if self.training and self.noisy_gate == "jitter":
             xr = x * torch.empty_like(x).uniform_(1.0 - self.jitter_eps, 1.0 + self.jitter_eps)
         y = xr @ self.router.t()
+        if self.gate is not None:
+            g = self.gate
+            r = routing.route(y, self.cfg.topk, score=g.score, bias=self.balance_bias if g.balance_bias else None, offset=self.router_bias if self.skewed else None,
+                              groups=g.groups, topk_groups=g.topk_groups, group_best=g.group_best, renormalize=g.renormalize, scale=g.scale, balance=self.training)
+            self.last_topk_idx, self.last_load = r.experts, r.load
+            self.l_aux = r.balance if self.training else torch.zeros((), device=y.device)
+            return self._drop(r.weights, r.experts), r.experts
         if self._fused_route(y):
             w, idx, self.last_topk_idx, self.l_aux = _Route.apply(y, self.router_bias, self.cfg.topk)
             return self._drop(w, idx), idx
@@ -214,6 +241,18 @@ class MoELayer(nn.Module):
             self.dropped_fraction = 1.0 - keep.float().mean()
             w = w * keep.to(w.dtype)
         return w
+
+    @torch.no_grad()
+    def update_balance(self, rate: float, group=None) -> None:
+        """Between steps, with a gate that has a balance bias: it moves by ``rate``, up for experts that the last batch chose less than on average, down for those
+        that it chose more.  Collective over the ranks of the layer, whose loads are added up."""
+        if self.gate is None or not self.gate.balance_bias:
+            raise RuntimeError("MoELayer: no balance bias to update")
+        load = self.last_load.float()
+        if self.world > 1:
+            import torch.distributed as dist
+            dist.all_reduce(load, group=group)
+        self.balance_bias += rate * (load.mean() - load).sign()
 
     def home(self, e: int):
         """(owner rank, local index) of expert e."""

@@ -7,7 +7,8 @@ embeddings, attention, norms, routers, output head -- is replicated and its grad
 in one bucket.  Every rank feeds its own micro-batch.
 
 The attention and the dense GEMMs are library calls (``scaled_dot_product_attention``, ``matmul``); the hand-written
-kernels are the ones inside the MoE layer.
+kernels are the ones inside the MoE layer and, where the configuration or the call asks for them, around it: the embedding with a factor
+(``embed_scale``), a router with groups and a balance bias (``gate``), the policy loss (``policy_step``) and AdamW (ops/adamw.py) as the optimizer.
 """
 from __future__ import annotations
 
@@ -18,10 +19,11 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops import embedding, losses
 from ..ops.moe import MoEConfig
 from ..parallel.symm import SymmetricHeap
-from .llama import _rms, _rope
-from .moe import MoELayer
+from .llama import _rms, _rope, _Status
+from .moe import Gate, MoELayer
 
 
 @dataclass
@@ -42,6 +44,9 @@ class MoEModelConfig:
     drop_tokens: bool = False
     placement: Optional[str] = None       # "balanced": experts' homes evened out by the router's bias (MoELayer)
     shadow_experts: int = 0               # copies of the n experts the router favours most on every rank (CUDA path)
+    gate: Optional[Gate] = None           # how the routers choose; None: softmax, at most 64 experts in one kernel
+    balance_rate: float = 1e-3            # by which a step moves the gate's balance bias, if it has one
+    embed_scale: float = 0.0              # factor of the embedding's rows (ops/embedding.py); 0: the rows as they are
 
 
 MOE_ZOO = {
@@ -97,9 +102,10 @@ class MoETransformer(nn.Module):
         for l in range(cfg.layers):
             moe = MoELayer(mcfg, heap, rank, world, device=device, zipf_s=None, seed=seed * 100 + l, fused_sgd_lr=fused_sgd_lr,
                            name=f"moe{l}", capacity_factor=cfg.capacity_factor, drop_tokens=cfg.drop_tokens,
-                           shadow_experts=cfg.shadow_experts if world > 1 else 0, placement=cfg.placement)
+                           shadow_experts=cfg.shadow_experts if world > 1 else 0, placement=cfg.placement, gate=cfg.gate)
             blocks.append(_Block(cfg, moe, device, gen, dtype))
         self.blocks = nn.ModuleList(blocks)
+        self._status = _Status() if cfg.embed_scale and torch.device(device).type == "cuda" else None
 
     # ---- parameters by parallelism ------------------------------------------------------------------------
     def expert_parameters(self) -> List[nn.Parameter]:
@@ -110,20 +116,54 @@ class MoETransformer(nn.Module):
         return [p for p in self.parameters() if id(p) not in experts]
 
     # ---- forward / loss -------------------------------------------------------------------------------------
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+    def check_status(self) -> None:
+        """Raise IndexError if the embedding met a token outside the vocabulary since the last call.  Does not wait: behind a synchronisation it covers everything
+        before it.  Every forward pass begins with it."""
+        if self._status is not None and int(self._status.word):
+            self._status.word.zero_()
+            raise IndexError(f"embedding: {_Status.WHAT[1]}")
+
+    def _logits(self, tokens: torch.Tensor) -> torch.Tensor:
+        """In the model's type."""
         B, S = tokens.shape
         pos = torch.arange(S, device=tokens.device).unsqueeze(0).expand(B, S)
-        x = self.embed[tokens]
+        if self.cfg.embed_scale:
+            self.check_status()
+            x = embedding.lookup(self.embed, tokens, self.cfg.embed_scale, status=self._status.word.data_ptr() if self._status is not None else 0)
+        else:
+            x = self.embed[tokens]
         for b in self.blocks:
             x = b(x, pos)
-        return (_rms(x, self.final_norm, self.cfg.eps) @ self.lm_head.t()).float()
+        return _rms(x, self.final_norm, self.cfg.eps) @ self.lm_head.t()
+
+    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+        return self._logits(tokens).float()
+
+    def _aux(self) -> torch.Tensor:
+        return self.cfg.aux_loss_coef * (sum(b.moe.l_aux for b in self.blocks) / len(self.blocks))
 
     def loss(self, tokens: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
         """Next-token cross entropy plus the load-balancing term of every MoE layer."""
         logits = self(tokens)
         ce = F.cross_entropy(logits.view(-1, logits.shape[-1]), labels.reshape(-1))
-        aux = sum(b.moe.l_aux for b in self.blocks) / len(self.blocks)
-        return ce + self.cfg.aux_loss_coef * aux
+        return ce + self._aux()
+
+    @torch.no_grad()
+    def token_logprobs(self, tokens: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
+        """[batch, seq]: at every position the logarithm of the next token's probability, 0 at the last: what policy_loss takes as ``old`` and ``reference``."""
+        lp = losses.token_logprobs(self._logits(tokens), torch.roll(tokens, -1, 1), temperature=temperature)
+        lp[:, -1] = 0
+        return lp
+
+    def policy_loss(self, tokens: torch.Tensor, old: torch.Tensor, advantages: torch.Tensor, *, weights: Optional[torch.Tensor] = None,
+                    reference: Optional[torch.Tensor] = None, kl: float = 0.0, clip=(0.2, 0.2), temperature: float = 1.0, total=None):
+        """(policy loss plus the load-balancing term, losses.PolicyLoss) over next tokens.  Entries of old, advantages, weights (a mask of answers, say) and
+        reference belong to the token after their position; the last position's do not count."""
+        w = torch.ones(tokens.shape, device=tokens.device) if weights is None else weights.to(torch.float32).broadcast_to(tokens.shape).clone()
+        w[:, -1] = 0
+        r = losses.policy_loss(self._logits(tokens), torch.roll(tokens, -1, 1), old, advantages, weights=w, reference=reference, kl=kl, clip=clip,
+                               temperature=temperature, total=total)
+        return r.loss + self._aux(), r
 
     def allreduce_dense_grads(self) -> None:
         """Data-parallel average of the replicated parameters' gradients, one bucket (expert gradients stay local)."""
@@ -138,10 +178,22 @@ class MoETransformer(nn.Module):
         for g, r in zip(grads, _unflatten_dense_tensors(flat, grads)):
             g.copy_(r)
 
-    def train_step(self, tokens: torch.Tensor, labels: torch.Tensor, opt: torch.optim.Optimizer) -> torch.Tensor:
-        loss = self.loss(tokens, labels)
+    def _update(self, loss: torch.Tensor, opt: torch.optim.Optimizer) -> None:
         loss.backward()
         self.allreduce_dense_grads()
         opt.step()
         opt.zero_grad(set_to_none=True)
+        if self.cfg.gate is not None and self.cfg.gate.balance_bias:
+            for b in self.blocks:
+                b.moe.update_balance(self.cfg.balance_rate)
+
+    def train_step(self, tokens: torch.Tensor, labels: torch.Tensor, opt: torch.optim.Optimizer) -> torch.Tensor:
+        loss = self.loss(tokens, labels)
+        self._update(loss, opt)
         return loss.detach()
+
+    def policy_step(self, tokens: torch.Tensor, old: torch.Tensor, advantages: torch.Tensor, opt: torch.optim.Optimizer, **how) -> losses.PolicyLoss:
+        """One step on answers that an earlier policy gave, see policy_loss."""
+        loss, r = self.policy_loss(tokens, old, advantages, **how)
+        self._update(loss, opt)
+        return r._replace(loss=loss.detach())

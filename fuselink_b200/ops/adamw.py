@@ -115,8 +115,8 @@ def _plain_step(p, grad, m, v, steps, lr, betas, eps, weight_decay, scales, mast
 
 
 class AdamW(torch.optim.Optimizer):
-    """The optimizer around :func:`step`: ``state_bits`` 32 or 8, ``master`` keeps fp32 copies of bf16 and fp16 parameters.  Parameters without a gradient are left
-    out of a step, their counts too.  ``lr`` of a group may be one fp32 value on the device, which a schedule writes between replays of a captured step; the first
+    """The optimizer around :func:`step`: ``state_bits`` 32 or 8, ``master`` keeps fp32 copies of bf16 and fp16 parameters, from which the next step starts:
+    parameters that are written otherwise (loaded, broadcast) call for ``refresh_masters``.  Parameters without a gradient are left out of a step, their counts too.  ``lr`` of a group may be one fp32 value on the device, which a schedule writes between replays of a captured step; the first
     step, which makes the state, is not captured.  Sparse gradients are refused."""
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, *,
@@ -167,6 +167,13 @@ class AdamW(torch.optim.Optimizer):
                 step(ps, gs, ms, vs, steps, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                      scales=(m_scales, v_scales) if group["state_bits"] == 8 else None, master=masters if has_master else None)
         return loss
+
+    @torch.no_grad()
+    def refresh_masters(self) -> None:
+        """Takes the fp32 copies anew from the parameters."""
+        for p, state in self.state.items():
+            if "master" in state:
+                state["master"].copy_(p)
 
     def load_state_dict(self, state_dict):
         """As the base class does, which turns floating state to the parameter's type: here it keeps its own."""

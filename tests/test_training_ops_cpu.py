@@ -121,13 +121,13 @@ def test_logprobs_and_policy_loss():
     a, b = call(x + h * d), call(x - h * d)
     # no ratio crosses its border on the way: then only the third derivative (of order 1 along d, per token) and fp32 results part the two
     assert float(a.clipped) == float(b.clipped) == float(r.clipped)
-    assert abs(float((g * d).sum()) - (float(a.loss) - float(b.loss)) / (2 * h)) < 50 * h * h + 2.0 ** -23 * 2 / h
+    assert abs(float((g * d).sum()) - (float(a.loss.detach()) - float(b.loss.detach())) / (2 * h)) < 50 * h * h + 2.0 ** -23 * 2 / h
     # rows of weight 0 are not looked at
     y = x.detach().clone()
     y[0], w[0] = math.nan, 0
     assert losses.policy_loss(y, t, old, A, weights=w).loss.isfinite()
     half = losses.policy_loss(x, t, old, A, total=48.0)
-    assert abs(float(half.loss) * 2 - float(losses.policy_loss(x, t, old, A).loss)) < 1e-6
+    assert abs(float(half.loss.detach()) * 2 - float(losses.policy_loss(x, t, old, A).loss.detach())) < 1e-6
     assert losses.token_logprobs(x, torch.full_like(t, 11)).isnan().all()
 
 
@@ -217,3 +217,87 @@ def test_c_entries_refuse_what_the_kernels_do_not_take():
     assert need == sorted(need) and need[0] >= 4004
     c.fl_adamw.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p]
     assert c.fl_adamw(0, None, -1, zeros, None) == -1 and c.fl_adamw(7, None, 0, zeros, None) == -1 and c.fl_adamw(0, None, 0, zeros, None) == 0
+
+
+def test_masters_start_anew_from_parameters_that_were_written():
+    p = torch.nn.Parameter(torch.ones(4, dtype=torch.bfloat16))
+    opt = adamw.AdamW([p], lr=1e-3, master=True, weight_decay=0.0)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with torch.no_grad():
+        p.fill_(5.0)
+    opt.refresh_masters()
+    opt.step()
+    assert (opt.state[p]["master"] - 5).abs().max() <= 2e-3 and (p == 5).all()
+
+
+def _net(**how):
+    import dataclasses
+
+    from fuselink_b200.models.moe import Gate
+    from fuselink_b200.models.moe_transformer import MOE_ZOO, MoETransformer
+    cfg = dataclasses.replace(MOE_ZOO["tiny_moe"], **{**dict(embed_scale=2.0, gate=Gate(groups=2, topk_groups=1, scale=1.5, balance_bias=True)), **how})
+    return MoETransformer(cfg, 2 * 12, None, 0, 1, device="cpu", seed=2)
+
+
+def test_gated_layers_route_as_the_operator_does():
+    from fuselink_b200.models.moe import Gate, MoELayer
+    from fuselink_b200.ops.moe import MoEConfig
+    layer = MoELayer(MoEConfig(hidden=32, ffn=128, num_experts=8, topk=2, tokens=50), None, 0, 1, device="cpu", gate=Gate(score="softmax", balance_bias=True))
+    x = torch.randn(50, 32, generator=_gen()).to(torch.bfloat16)
+    w, idx = layer.route(x)
+    r = routing.route(x @ layer.router.t(), 2, bias=layer.balance_bias, offset=layer.router_bias, balance=True)
+    assert torch.equal(w, r.weights) and torch.equal(idx, r.experts) and torch.equal(layer.l_aux, r.balance) and torch.equal(layer.last_load, r.load)
+    before = layer.balance_bias.clone()
+    layer.update_balance(0.5)
+    assert torch.equal(layer.balance_bias - before, 0.5 * torch.sign(50 * 2 / 8 - r.load.float()))
+    assert "balance_bias" in layer.state_dict()
+    layer.eval()
+    layer.route(x)
+    assert layer.l_aux == 0
+    plain = MoELayer(MoEConfig(hidden=32, ffn=128, num_experts=8, topk=2, tokens=50), None, 0, 1, device="cpu")
+    assert "balance_bias" not in plain.state_dict()
+    with pytest.raises(RuntimeError):
+        plain.update_balance(0.1)
+    with pytest.raises(ValueError):
+        MoELayer(MoEConfig(hidden=32, ffn=128, num_experts=8, topk=2, tokens=50), None, 0, 1, device="cpu", gate=Gate(), noisy_gate="rsample")
+
+
+def test_a_transformer_around_its_experts():
+    net = _net()
+    tokens = torch.randint(0, 512, (2, 12), generator=_gen(4))
+    lp = net.token_logprobs(tokens)
+    want = torch.log_softmax(net(tokens).detach(), -1)[:, :-1].gather(-1, tokens[:, 1:, None])[..., 0]
+    # the same logits in fp32 on either side; logarithms of magnitude 6 rounded to it
+    assert lp.shape == (2, 12) and (lp[:, -1] == 0).all() and (lp[:, :-1] - want).abs().max() <= 8 * 2.0 ** -22
+    old, A = lp + 0.1, torch.randn(2, 1, generator=_gen(5))
+    loss, r = net.policy_loss(tokens, old, A, reference=lp, kl=0.1)
+    loss.backward()
+    # ratios of e^-0.1 lie inside the borders: the mean of -q A, and the divergence of a reference that is the policy itself
+    assert abs(float(r.loss.detach()) + math.exp(-0.1) * float(A.mean())) < 1e-4 and float(r.clipped) == 0 and abs(float(r.divergence)) < 1e-9
+    assert all(p.grad is not None and p.grad.isfinite().all() for p in net.parameters())
+    seen = {}
+    net.blocks[0].register_forward_pre_hook(lambda m, x: x[0].register_hook(lambda g: seen.update(g=g.detach().clone())))
+    net.embed.grad = None
+    net.policy_loss(tokens, old, A, reference=lp, kl=0.1)[0].backward()
+    rows = torch.zeros(net.embed.shape, dtype=torch.float64).index_add_(0, tokens.reshape(-1), seen["g"].reshape(-1, 128).double()) * 2.0
+    # bf16 gradients added up row by row by the library, each sum of at most 24 rounded to bf16
+    assert ((net.embed.grad.double() - rows).abs() <= 24 * 2.0 ** -8 * rows.abs().amax(1, keepdim=True) + 1e-30).all()
+    from fuselink_b200.ops.adamw import AdamW
+    opt = AdamW(net.parameters(), lr=1e-3, state_bits=8)
+    bias = net.blocks[0].moe.balance_bias.clone()
+    r = net.policy_step(tokens, old, A, opt, weights=torch.arange(12) > 3)
+    assert r.loss.isfinite() and not r.loss.requires_grad and (r.logprobs[:, :4] == 0).all() and (r.logprobs[:, -1] == 0).all()
+    assert not torch.equal(bias, net.blocks[0].moe.balance_bias) and all(p.grad is None for p in net.parameters())
+    assert net.train_step(tokens, torch.roll(tokens, -1, 1), opt).isfinite()
+
+
+def test_the_training_command_with_every_choice():
+    import subprocess
+    import sys
+    script = os.path.join(ROOT, "experiments", "run_moe_training.py")
+    small = ["--model", "tiny_moe", "--device", "cpu", "--steps", "2", "--batch", "2", "--seq", "32", "--log-every", "1", "--lr", "0.001"]
+    r = subprocess.run([sys.executable, script, *small, "--optimizer", "adamw8", "--objective", "policy", "--gate", "sigmoid", "--embed-scale", "11.3"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.count('"loss"') == 2, r.stderr[-2000:]
+    r = subprocess.run([sys.executable, script, *small, "--optimizer", "adamw", "--reshadow-every", "1"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 2 and "copy slots" in r.stderr
