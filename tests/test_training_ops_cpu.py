@@ -277,7 +277,11 @@ def test_a_transformer_around_its_experts():
     assert abs(float(r.loss.detach()) + math.exp(-0.1) * float(A.mean())) < 1e-4 and float(r.clipped) == 0 and abs(float(r.divergence)) < 1e-9
     assert all(p.grad is not None and p.grad.isfinite().all() for p in net.parameters())
     seen = {}
-    net.blocks[0].register_forward_pre_hook(lambda m, x: x[0].register_hook(lambda g: seen.update(g=g.detach().clone())))
+
+    def look(module, inputs):
+        inputs[0].register_hook(lambda g: seen.update(g=g.detach().clone()))
+
+    net.blocks[0].register_forward_pre_hook(look)
     net.embed.grad = None
     net.policy_loss(tokens, old, A, reference=lp, kl=0.1)[0].backward()
     rows = torch.zeros(net.embed.shape, dtype=torch.float64).index_add_(0, tokens.reshape(-1), seen["g"].reshape(-1, 128).double()) * 2.0
