@@ -616,7 +616,9 @@ static bool bad(const FlRouteArgs* a) {
 }  // namespace routing
 }  // namespace fl
 
-extern "C" long long fl_route_scratch(int experts) { return (long long)experts * 12 + 8; }
+extern "C" long long fl_route_scratch(long long tokens, int experts) {
+  return tokens <= (experts <= 256 ? fl::routing::MOST_WARPS<8> : fl::routing::MOST_WARPS<16>) ? 0 : (long long)experts * 12 + 8;
+}
 
 extern "C" int fl_route(int dtype, const FlRouteArgs* a, cudaStream_t stream) {
   using namespace fl::routing;
@@ -633,7 +635,7 @@ extern "C" int fl_route(int dtype, const FlRouteArgs* a, cudaStream_t stream) {
       const bool in_lanes = size % N == 0 && (lanes & (lanes - 1)) == 0;
       const int bytes = (warps * 32 * (N + 1) + 2 * a->experts) * 4 + (a->topk_groups < a->groups && !in_lanes ? warps * a->experts * 8 : 0);
       if (ctas > 1) {
-        const cudaError_t e = cudaMemsetAsync(a->scratch, 0, (size_t)fl_route_scratch(a->experts), stream);
+        const cudaError_t e = cudaMemsetAsync(a->scratch, 0, (size_t)fl_route_scratch(a->tokens, a->experts), stream);
         if (e != cudaSuccess) return (int)e;
       }
       auto kernel = a->experts == 32 * N ? route_kernel<N, true, T> : route_kernel<N, false, T>;

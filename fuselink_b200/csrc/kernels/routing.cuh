@@ -28,7 +28,7 @@ typedef struct {
   int* chosen;                   // [tokens][topk], best first, of equals the lowest first
   int* load;                     // [experts]: tokens that chose each
   float* balance;                // E / (T k) sum_e load_e mean_t p_te / sum p_t, 0 without tokens; or null
-  void* scratch;                 // fl_route_scratch() bytes
+  void* scratch;                 // fl_route_scratch() bytes, or null where that is 0
   // gradient
   const float* dweights;         // [tokens][topk] or null
   const float* dbalance;         // one value or null
@@ -38,7 +38,7 @@ typedef struct {
 // dtype: FlDtype of the logits.  -1: sizes that the kernels do not take
 int fl_route(int dtype, const FlRouteArgs* a, cudaStream_t stream);
 int fl_route_grad(int dtype, const FlRouteArgs* a, cudaStream_t stream);
-long long fl_route_scratch(int experts);
+long long fl_route_scratch(long long tokens, int experts);
 
 #ifdef __cplusplus
 }

@@ -6,6 +6,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <string>
 #include <vector>
@@ -135,9 +136,11 @@ tensor_list route_forward(const Tensor& logits, const RouteHow& h, const OptTens
   const int64_t T = logits.size(0), E = logits.size(1);
   Tensor w = new_like(logits, {T, h.topk}, torch::kFloat32), chosen = new_like(logits, {T, h.topk}, torch::kInt32), load = new_like(logits, {E}, torch::kInt32), term;
   if (balance) term = new_like(logits, {}, torch::kFloat32);
-  const Tensor scratch = new_bytes(logits, fl_route_scratch(a.experts));
+  const long long bytes = fl_route_scratch(T, a.experts);
+  Tensor scratch;
+  if (bytes > 0) scratch = new_bytes(logits, bytes);
   a.weights = w.data_ptr<float>(); a.chosen = chosen.data_ptr<int>(); a.load = load.data_ptr<int>(); a.balance = balance ? term.data_ptr<float>() : nullptr;
-  a.scratch = scratch.data_ptr();
+  a.scratch = bytes > 0 ? scratch.data_ptr() : nullptr;
   check(fl_route(dtype_of(logits, "route"), &a, stream_of()), "fl_route");
   return {w, chosen, load, term};
 }
@@ -175,22 +178,37 @@ struct Route : torch::autograd::Function<Route> {
     return said;
   }
 };
-std::tuple<Tensor, Tensor, Tensor, OptTensor> route(Tensor logits, int64_t topk, int64_t score, int64_t groups, int64_t topk_groups, int64_t group_best, bool renormalize, double scale,
-                                                    OptTensor bias, OptTensor offset, bool balance) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "route: logits [tokens, experts] on the GPU");
-  const int64_t E = logits.size(1);
-  TORCH_CHECK(E >= 1 && E <= FL_ROUTE_MAX_EXPERTS && topk <= FL_ROUTE_MAX_TOPK && groups <= FL_ROUTE_MAX_GROUPS, 
-              "route: at most 1024 experts, 32 choices and 32 groups on the GPU");
+// What is wrong with an argument's value is a ValueError, as from the plain form in Python; these checks are here because the calls are short.
+void value(bool ok, const char* what) {
+  if (!ok) throw pybind11::value_error(what);
+}
+std::tuple<Tensor, Tensor, Tensor, OptTensor> route(Tensor logits, int64_t topk, const std::string& score, int64_t groups, c10::optional<int64_t> topk_groups, int64_t group_best,
+                                                    bool renormalize, double scale, OptTensor bias, OptTensor offset, bool balance) {
+  TORCH_CHECK(logits.is_cuda(), "route: logits on the GPU");
+  value(logits.dim() == 2 && logits.size(1) >= 1, "route: logits [tokens, experts] expected");
+  const int64_t E = logits.size(1), how = score == "softmax" ? FL_ROUTE_SOFTMAX : score == "sigmoid" ? FL_ROUTE_SIGMOID : -1;
+  value(how >= 0, "route: a score of softmax or sigmoid expected");
+  value(groups >= 1 && E % groups == 0, "route: the experts do not make so many equal groups");
+  const int64_t kept = topk_groups.value_or(groups);
+  value(kept >= 1 && kept <= groups, "route: topk_groups, one at least and no more than there are groups");
+  value(topk >= 1 && topk <= E / groups * kept, "route: topk, one at least and no more than the groups chosen from have experts");
+  if (groups == 1) group_best = 1;
+  value((group_best == 1 || group_best == 2) && group_best <= E / groups, "route: a group goes by its 1 or 2 best");
+  value(scale != 0.0 && std::isfinite(scale), "route: a factor that is finite and not 0");
+  TORCH_CHECK(E <= FL_ROUTE_MAX_EXPERTS && topk <= FL_ROUTE_MAX_TOPK && groups <= FL_ROUTE_MAX_GROUPS, "route: at most 1024 experts, 32 choices and 32 groups on the GPU");
   static_assert(FL_ROUTE_MAX_EXPERTS == 1024 && FL_ROUTE_MAX_TOPK == 32 && FL_ROUTE_MAX_GROUPS == 32, "what the message says");
   dtype_of(logits, "route");
-  floats(bias, logits, E, "route: bias [experts] fp32, contiguous, on the logits' device");
-  floats(offset, logits, E, "route: offset [experts] fp32, contiguous, on the logits' device");
-  for (const auto* t : {&bias, &offset})
-    TORCH_CHECK(!t->has_value() || !records(**t), "route: bias and offset get no gradient; detach them");
+  for (auto* t : {&bias, &offset}) {
+    if (!t->has_value()) continue;
+    value((*t)->dim() == 1 && (*t)->size(0) == E && (*t)->scalar_type() == torch::kFloat32, "route: bias and offset [experts] fp32");
+    TORCH_CHECK((*t)->device() == logits.device(), "route: bias and offset on the logits' device");
+    TORCH_CHECK(!records(**t), "route: bias and offset get no gradient; detach them");
+    if (!(*t)->is_contiguous()) *t = (*t)->contiguous();
+  }
   if ((E > 1 && logits.stride(1) != 1) || (logits.size(0) > 1 && logits.stride(0) < E)) logits = logits.contiguous();
   tensor_list out;
-  if (records(logits)) out = Route::apply(logits, topk, score, groups, topk_groups, group_best, renormalize, scale, bias, offset, balance);
-  else out = route_forward(logits, RouteHow{topk, score, groups, topk_groups, group_best, renormalize, scale}, bias, offset, balance);
+  if (records(logits)) out = Route::apply(logits, topk, how, groups, kept, group_best, renormalize, scale, bias, offset, balance);
+  else out = route_forward(logits, RouteHow{topk, how, groups, kept, group_best, renormalize, scale}, bias, offset, balance);
   return {out[0], out[1], out[2], balance ? OptTensor(out[3]) : OptTensor()};
 }
 
@@ -266,11 +284,15 @@ Tensor rows_gradient(const Tensor& logits, const Tensor& tokens, double temperat
   return out;
 }
 
-void logits_and_tokens(const Tensor& logits, const Tensor& tokens, const char* what) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() >= 1 && logits.size(-1) > 0, what, ": logits [..., vocab] on the GPU");
-  TORCH_CHECK(tokens.device() == logits.device() && tokens.scalar_type() == torch::kInt64 && tokens.is_contiguous() && tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1),
-              what, ": tokens int64, one for each row of the logits, on their device");
-  dtype_of(logits, what);
+Tensor logits_and_tokens(const Tensor& logits, Tensor tokens, double temperature) {
+  TORCH_CHECK(logits.is_cuda(), "losses: logits on the GPU");
+  value(logits.dim() >= 1 && logits.size(-1) > 0, "losses: logits [..., vocab] expected");
+  value(tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1), "losses: tokens, one for each row of the logits");
+  value(tokens.scalar_type() == torch::kInt64 || tokens.scalar_type() == torch::kInt32, "losses: tokens of int64 or int32 expected");
+  TORCH_CHECK(tokens.device() == logits.device(), "losses: tokens on ", logits.device(), " expected, not on ", tokens.device());
+  value(temperature > 0.0 && std::isfinite(temperature), "losses: a temperature above 0");
+  dtype_of(logits, "losses");
+  return tokens.scalar_type() == torch::kInt64 && tokens.is_contiguous() ? tokens : tokens.to(torch::kInt64).contiguous();
 }
 // log-probabilities and, where the gradient will be asked for, the rows' largest logits and inverse sums
 tensor_list logprobs_forward(const Tensor& logits, const Tensor& tokens, double temperature, bool gradient) {
@@ -305,8 +327,8 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
             Tensor(), Tensor()};
   }
 };
-Tensor token_logprobs(const Tensor& logits, const Tensor& tokens, double temperature) {
-  logits_and_tokens(logits, tokens, "token_logprobs");
+Tensor token_logprobs(const Tensor& logits, Tensor tokens, double temperature) {
+  tokens = logits_and_tokens(logits, tokens, temperature);
   return records(logits) ? LogProbs::apply(logits, tokens, temperature) : logprobs_forward(logits, tokens, temperature, false)[0];
 }
 
@@ -366,11 +388,33 @@ struct Policy : torch::autograd::Function<Policy> {
     return said;
   }
 };
-std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& tokens, const Tensor& old, const Tensor& advantages, OptTensor reference, OptTensor weights,
-                                                       OptTensor total, double kl, double low, double high, double temperature) {
-  logits_and_tokens(logits, tokens, "policy_loss");
-  for (const auto& t : {OptTensor(old), OptTensor(advantages), reference, weights, total})
-    TORCH_CHECK(!t.has_value() || !records(*t), "policy_loss: only the logits get a gradient; detach the others");
+// `total`: None, a number, or one value on the device
+std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, Tensor tokens, Tensor old, Tensor advantages, OptTensor reference, OptTensor weights,
+                                                       pybind11::object total_of, double kl, double low, double high, double temperature) {
+  tokens = logits_and_tokens(logits, tokens, temperature);
+  value(low >= 0.0 && std::isfinite(low) && high >= 0.0 && std::isfinite(high) && kl >= 0.0 && std::isfinite(kl), "policy_loss: borders and a factor of the KL term that are not negative");
+  auto like_tokens = [&](Tensor& t, const char* what) {
+    TORCH_CHECK(t.device() == tokens.device(), "policy_loss: ", what, " on ", tokens.device(), " expected, not on ", t.device());
+    TORCH_CHECK(!records(t), "policy_loss: only the logits get a gradient; detach ", what);
+    if (t.scalar_type() != torch::kFloat32) t = t.to(torch::kFloat32);
+    if (t.sizes() != tokens.sizes()) t = t.broadcast_to(tokens.sizes());
+    if (!t.is_contiguous()) t = t.contiguous();
+  };
+  like_tokens(old, "old");
+  like_tokens(advantages, "advantages");
+  if (reference.has_value()) like_tokens(*reference, "reference");
+  if (weights.has_value()) like_tokens(*weights, "weights");
+  OptTensor total;
+  if (!total_of.is_none()) {
+    if (THPVariable_Check(total_of.ptr())) {
+      total = THPVariable_Unpack(total_of.ptr());
+      value(total->numel() == 1 && total->device() == logits.device(), "policy_loss: total, a number or one value on the logits' device");
+      TORCH_CHECK(!records(*total), "policy_loss: only the logits get a gradient; detach total");
+      if (total->scalar_type() != torch::kFloat32) total = total->to(torch::kFloat32);
+    } else {
+      total = torch::full({}, total_of.cast<double>(), logits.options().dtype(torch::kFloat32).requires_grad(false));
+    }
+  }
   tensor_list out;
   if (records(logits)) out = Policy::apply(logits, tokens, old, advantages, reference, weights, total, kl, low, high, temperature);
   else out = policy_forward(logits, tokens, old, advantages, reference, weights, total, PolicyHow{kl, low, high, temperature}, false);
@@ -378,9 +422,21 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, con
 }
 
 // ------------------------------------------------------------------------------------------------ AdamW
-void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& m, const std::vector<Tensor>& v, const std::vector<Tensor>& steps,
-                const std::vector<Tensor>& m_scales, const std::vector<Tensor>& v_scales, const std::vector<Tensor>& masters, double lr, OptTensor lr_on_device, double beta1,
-                double beta2, double eps, double weight_decay, bool codes) {
+// The tensors of a list or tuple, borrowed from it: of some hundred a conversion to a vector is half of what the call costs the host.
+struct Tensors {
+  pybind11::object held;
+  Tensors(const pybind11::object& from) : held(pybind11::reinterpret_steal<pybind11::object>(PySequence_Fast(from.ptr(), "adamw: lists of tensors expected"))) {
+    if (!held) throw pybind11::error_already_set();
+    for (size_t i = 0; i < size(); ++i) TORCH_CHECK(THPVariable_Check(PySequence_Fast_GET_ITEM(held.ptr(), (Py_ssize_t)i)), "adamw: lists of tensors expected");
+  }
+  size_t size() const { return (size_t)PySequence_Fast_GET_SIZE(held.ptr()); }
+  bool empty() const { return size() == 0; }
+  const Tensor& operator[](size_t i) const { return THPVariable_Unpack(PySequence_Fast_GET_ITEM(held.ptr(), (Py_ssize_t)i)); }
+};
+void adamw_step(const pybind11::object& params_, const pybind11::object& grads_, const pybind11::object& m_, const pybind11::object& v_, const pybind11::object& steps_,
+                const pybind11::object& m_scales_, const pybind11::object& v_scales_, const pybind11::object& masters_, double lr, OptTensor lr_on_device, double beta1, double beta2, double eps,
+                double weight_decay, bool codes) {
+  const Tensors params(params_), grads(grads_), m(m_), v(v_), steps(steps_), m_scales(m_scales_), v_scales(v_scales_), masters(masters_);
   const size_t n = params.size();
   TORCH_CHECK(grads.size() == n && m.size() == n && v.size() == n && steps.size() == n && (!codes || (m_scales.size() == n && v_scales.size() == n)) &&
                   (masters.empty() || masters.size() == n), "adamw: one of each for every parameter");
@@ -422,6 +478,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
     }
     Tensor g = grads[i];
     if (g.strides() != p.strides() && t.n > 1) {
+      const at::NoGradGuard none;
       g = at::empty_like(p).copy_(g);
       kept.push_back(g);
     }
@@ -437,7 +494,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
   for (int dt = 0; dt < 3; ++dt)
     if (!of[dt].empty()) check(fl_adamw(dt, of[dt].data(), (long long)of[dt].size(), &a, stream_of()), "fl_adamw");
   for (const auto* list : {&params, &m, &v, &steps, &m_scales, &v_scales, &masters})
-    for (const auto& t : *list) t.unsafeGetTensorImpl()->bump_version();
+    for (size_t i = 0; i < list->size(); ++i) (*list)[i].unsafeGetTensorImpl()->bump_version();
 }
 
 }  // namespace

@@ -29,7 +29,6 @@ def _settings(lr, betas, eps, weight_decay):
         raise ValueError(f"adamw: betas {tuple(betas)}, eps {eps}, weight_decay {weight_decay}")
 
 
-@torch.no_grad()
 def step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m: Sequence[torch.Tensor], v: Sequence[torch.Tensor], steps: Sequence[torch.Tensor], *,
          lr: Union[float, torch.Tensor], betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
          scales: Optional[Tuple[Sequence[torch.Tensor], Sequence[torch.Tensor]]] = None, master: Optional[Sequence[torch.Tensor]] = None) -> None:
@@ -44,13 +43,17 @@ def step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m: Seque
         require_native().adamw_step(params, grads, m, v, steps, m_scales, v_scales, master or (), 0.0 if on_device else lr, lr if on_device else None,
                                     betas[0], betas[1], eps, weight_decay, scales is not None)
         return
-    every = [grads, m, v, steps] + ([m_scales, v_scales] if scales is not None else []) + ([master] if master else [])
-    if any(len(x) != len(params) for x in every):
+    _plain(params, grads, m, v, steps, lr, betas, eps, weight_decay, scales, master)
+
+
+@torch.no_grad()
+def _plain(params, grads, m, v, steps, lr, betas, eps, weight_decay, scales, master):
+    if any(len(x) != len(params) for x in [grads, m, v, steps, *(scales or ()), *([master] if master else ())]):
         raise RuntimeError("adamw: one of each for every parameter")
     for i, p in enumerate(params):
         if grads[i].layout != torch.strided or grads[i].shape != p.shape or grads[i].dtype != p.dtype:
             raise RuntimeError("adamw: a dense gradient of its parameter's type, shape and device")
-        _plain_step(p, grads[i], m[i], v[i], steps[i], lr, betas, eps, weight_decay, (m_scales[i], v_scales[i]) if scales is not None else None,
+        _plain_step(p, grads[i], m[i], v[i], steps[i], lr, betas, eps, weight_decay, (scales[0][i], scales[1][i]) if scales is not None else None,
                     master[i] if master else None)
 
 

@@ -42,9 +42,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     """logits [..., vocab]; tokens [...]: the logarithm of each token's probability in its row, fp32.  On the GPU bf16, fp16 and fp32 logits whose rows are
     contiguous and lie at one or two distances (a slice of positions, say; others are copied); on the CPU any floating type.  What preference losses and
     sequence likelihoods are sums of."""
-    _check("token_logprobs", logits, tokens, temperature)
     if logits.is_cuda and ordinary(logits):
-        return require_native().token_logprobs(logits, tokens.long().contiguous(), temperature)
+        return require_native().token_logprobs(logits, tokens, temperature)
+    _check("token_logprobs", logits, tokens, temperature)
     ok = (tokens >= 0) & (tokens < logits.shape[-1])
     return torch.where(ok, _plain_logprobs(logits, tokens, temperature), math.nan).float()
 
@@ -72,8 +72,10 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, a
     weights (a mask, say) and reference are broadcast to the tokens.  ``total``: what the weighted sums are divided by in place of the weights' own sum, a number
     or one fp32 value on the device, where a batch is spread over several calls or ranks; a sum of 0 gives a loss of 0.  A ratio exactly at its border still
     has a gradient.  Only the logits get one, and it cannot be differentiated again on the GPU."""
-    _check("policy_loss", logits, tokens, temperature)
     low, high = clip
+    if logits.is_cuda and ordinary(logits):
+        return PolicyLoss(*require_native().policy_loss(logits, tokens, old, advantages, reference, weights, total, kl, low, high, temperature))
+    _check("policy_loss", logits, tokens, temperature)
     if not (0 <= low < math.inf and 0 <= high < math.inf and 0 <= kl < math.inf):
         raise ValueError(f"policy_loss: clip {clip}, kl {kl}")
     old, advantages, weights, reference = (_like_tokens(n, t, tokens) for n, t in (("old", old), ("advantages", advantages), ("weights", weights), ("reference", reference)))
@@ -85,8 +87,6 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, a
         total = total.reshape(()).float()
     elif total is not None:
         total = torch.full((), float(total), device=logits.device)
-    if logits.is_cuda and ordinary(logits):
-        return PolicyLoss(*require_native().policy_loss(logits, tokens.long().contiguous(), old, advantages, reference, weights, total, kl, low, high, temperature))
     return _plain_policy(logits, tokens, old, advantages, weights, reference, kl, low, high, temperature, total)
 
 

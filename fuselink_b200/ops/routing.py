@@ -34,6 +34,8 @@ def route(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias: Opti
     alone.  ``renormalize``: a token's weights sum to ``scale``; else they are its scores times ``scale``.  A token whose chosen scores are all 0
     (logits of -inf) has weights of 0 and no gradient from them.  On the GPU bf16, fp16 and fp32, at most 1024 experts, 32 choices and 32 groups; on the
     CPU any floating type."""
+    if logits.is_cuda and ordinary(logits):
+        return Routing(*require_native().route(logits, topk, score, groups, topk_groups, group_best, renormalize, scale, bias, offset, balance))
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"route: logits [tokens, experts] expected, not {tuple(logits.shape)}")
     T, E = logits.shape
@@ -61,9 +63,6 @@ def route(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias: Opti
             raise RuntimeError(f"route: {name} on {logits.device} expected, not on {t.device}")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("route: bias and offset get no gradient; detach them")
-    if logits.is_cuda and ordinary(logits):
-        c = lambda t: None if t is None else t.contiguous()  # noqa: E731
-        return Routing(*require_native().route(logits, topk, SCORES.index(score), groups, topk_groups, group_best, renormalize, scale, c(bias), c(offset), balance))
     return _plain_route(logits, topk, score, bias, offset, groups, topk_groups, group_best, renormalize, scale, balance)
 
 
