@@ -3,7 +3,8 @@
 Layers (bottom up):
 
 * ``csrc/``      sm_100a kernels (tcgen05 grouped GEMM, fused dispatch/combine, embedding-bag + all-to-all,
-                 KV pack + transfer, attention over 8-bit pages, sampling, chunked peer copies), the cuMem region layer, the idleness monitor and
+                 KV pack + transfer, attention over 8-bit pages, sampling, embedding, routing,
+                 policy loss, AdamW, chunked peer copies), the cuMem region layer, the idleness monitor and
                  the ncclNet plugin (``lib/libnccl-net-fuselink.so``).
 * ``parallel/``  symmetric heap over cuMem regions, path selector, process-group helpers.
 * ``ops/``       Python entry points of the kernels plus plain-PyTorch fp32 references.

@@ -5,8 +5,8 @@
 //   dL / dlp_r = w_r / sum w (-q A where q A is the smaller, else 0;  + k (1 - exp(d)))
 //
 // A row's sum runs once over its logits in fp32, with the running maximum; what follows per row is one thread's, in 64 bits.  The policy loss
-// knows dL / dlp as soon as it has the row's sum, so the kernel goes over the row once more right then, out of L2, and writes the
-// gradient of a derivative of 1: the logits come from memory once.  Should the derivative turn out to be another number, the gradient is computed
+// knows dL / dlp as soon as it has the row's sum, so the kernel goes over the row once more right then, out of the caches as far as they go, and writes the
+// gradient of a derivative of 1.  Should the derivative turn out to be another number, the gradient is computed
 // anew from the logits (fl_logprobs_grad), so that it is rounded once.
 #include "losses.cuh"
 #include <math.h>
@@ -106,7 +106,7 @@ __device__ __forceinline__ Running sum_row(const T* row, long long vocab, float 
     for (int j = 0; j < AHEAD; ++j) {
       constexpr uint32_t none = Logits<T>::NONE;
       x[j] = make_uint4(none, none, none, none);
-      if (i + j * THREADS < packs) x[j] = ld_stream_v4(v + i + j * THREADS);
+      if (i + j * THREADS < packs) x[j] = ld_v4(v + i + j * THREADS);
     }
     const float to = Logits<T>::largest(Logits<T>::larger(Logits<T>::larger(x[0], x[1]), Logits<T>::larger(x[2], x[3])));
     if (to > top) {
@@ -156,7 +156,8 @@ __device__ __forceinline__ Running sum_row(const T* row, long long vocab, float 
   return r;
 }
 
-// out_j = factor (1[j = tok] - p_j).  The row is in L2 for the most part; what is written is not kept there.  inverse: 1 / sum_j 2^(unit (x_j - top))
+// out_j = factor (1[j = tok] - p_j), from the row's end to its beginning: what was read last is in L1 and L2 still (of rows of 128256 bf16, 600 in work, L2 had
+// lost 85% when they were read from the beginning again).  What is written is not kept.  inverse: 1 / sum_j 2^(unit (x_j - top))
 template <typename T, int THREADS>
 __device__ __forceinline__ void write_row(T* out, const T* row, long long vocab, float unit, float top, float inverse, float factor, long long tok) {
   constexpr int P = PER<T>;
@@ -171,11 +172,11 @@ __device__ __forceinline__ void write_row(T* out, const T* row, long long vocab,
   }
   const float base = -(top * unit), share = -factor * inverse, fine = share * ex2(-fmaf(top, unit, base));      // the latter without the base's rounding
   const F2 unit2(unit, unit), minus(base, base), fine2(fine, fine);
-  for (int i = threadIdx.x; i < packs; i += THREADS * AHEAD) {
+  for (int i = (packs - 1) / (THREADS * AHEAD) * (THREADS * AHEAD) + (int)threadIdx.x; i >= 0; i -= THREADS * AHEAD) {
     uint4 x[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)
-      if (i + j * THREADS < packs) x[j] = ld_stream_v4(v + i + j * THREADS);
+      if (i + j * THREADS < packs) x[j] = ld_v4(v + i + j * THREADS);
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       if (i + j * THREADS >= packs) break;
@@ -414,7 +415,10 @@ extern "C" int fl_policy_loss(int dtype, const FlLossArgs* a, cudaStream_t strea
           weights_kernel<<<1, 1024, 0, stream>>>(*a);
           c.numAttrs = 1;                          // the rows begin beside that; what came before is behind both
         }
-        const cudaError_t e = cudaLaunchKernelEx(&c, loss_kernel<T, N>, *a);
+        cudaError_t e = cudaSuccess;
+        // the ends of rows are read again out of L1 (8192 x 32000: 241 us without this, 231 with it; warps of their own have no use for it and want their CTAs' share)
+        if (N == 256) e = cudaFuncSetAttribute(loss_kernel<T, N>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxL1);
+        if (e == cudaSuccess) e = cudaLaunchKernelEx(&c, loss_kernel<T, N>, *a);
         if (e != cudaSuccess) return (int)e;
       }
       loss_sum_kernel<<<1, 256, 0, stream>>>(*a, ctas);

@@ -2,7 +2,8 @@
 //
 //   kernels   grouped GEMM (bf16 and block-scaled fp8), chunked peer copies / all-to-all / flag waits,
 //             MoE dispatch + combine, embedding-bag + all-to-all, KV page pack + send,
-//             sum + update of replicated experts' weight gradients                         (launch on a cudaStream_t)
+//             sum + update of replicated experts' weight gradients, embedding, routing,
+//             log-probabilities and policy loss, AdamW                                     (launch on a cudaStream_t)
 //   regions   cuMem regions that can be exported, imported, aliased and re-homed; slab pool  (vmm.h)
 //   monitor   lock-free idleness table and path selection                                    (monitor.h)
 //
