@@ -20,7 +20,7 @@ namespace fl {
 namespace routing {
 
 constexpr unsigned ALL = 0xffffffffu;
-constexpr int GRAD_WARPS = 8;
+constexpr int GRAD_WARPS = 8, GRAD_CTAS = 148 * 6;
 constexpr int WARPS = 8;                         // of a CTA; a launch of one CTA has up to MOST_WARPS
 template <int N> constexpr int MOST_WARPS = N <= 8 ? 16 : 8;
 constexpr int CTAS = 148 * 4;
@@ -510,88 +510,87 @@ __global__ void __launch_bounds__(GRAD_WARPS * 32) route_grad_kernel(const FlRou
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = lane * N, E = a.experts;
   const bool sigmoid = a.score == FL_ROUTE_SIGMOID, wide = whole<N, T>(a.logits, a.stride, E), wide_out = whole<N, T>(a.dlogits, E, E);
   const float each = a.dbalance != nullptr ? (float)((double)*a.dbalance * E / ((double)a.tokens * a.tokens * a.topk)) : 0.f;
-  const long long t = (long long)blockIdx.x * GRAD_WARPS + warp;
-  if (t >= a.tokens) return;
-  const T* row = (const T*)a.logits + t * a.stride;
-  T* out = (T*)a.dlogits + t * E;
-  float w = 0.f, dw = 0.f, x = 0.f, own_load = 0.f;
-  int expert = 0;
-  const bool is = lane < a.topk && a.dweights != nullptr;
-  if (is) {
-    w = a.weights[t * a.topk + lane];
-    dw = a.dweights[t * a.topk + lane];
-    expert = a.chosen[t * a.topk + lane];
-  }
-  float p[N], l[N];
-  const bool whole_row = a.dbalance != nullptr || (!a.renormalize && !sigmoid);
-  if (whole_row) {
-    load_logits<N, T>(l, row, e0, E, wide);
-    if (a.offset != nullptr)
+  float b[N];                                    // what the balance term asks of each expert, before a token's mean of it
+#pragma unroll
+  for (int i = 0; i < N; ++i) b[i] = a.dbalance != nullptr && e0 + i < E ? each * (float)a.load[e0 + i] : 0.f;
+  for (long long t = (long long)blockIdx.x * GRAD_WARPS + warp; t < a.tokens; t += (long long)gridDim.x * GRAD_WARPS) {
+    const T* row = (const T*)a.logits + t * a.stride;
+    T* out = (T*)a.dlogits + t * E;
+    float w = 0.f, dw = 0.f, x = 0.f, own_load = 0.f;
+    int expert = 0;
+    const bool is = lane < a.topk && a.dweights != nullptr;
+    if (is) {
+      w = a.weights[t * a.topk + lane];
+      dw = a.dweights[t * a.topk + lane];
+      expert = a.chosen[t * a.topk + lane];
+    }
+    float p[N], l[N];
+    const bool whole_row = a.dbalance != nullptr || (!a.renormalize && !sigmoid);
+    if (whole_row) {
+      load_logits<N, T>(l, row, e0, E, wide);
+      if (a.offset != nullptr)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (e0 + i < E) l[i] += a.offset[e0 + i];
+    }
+    if (is) {
+      x = to_f32(row[expert]) + (a.offset != nullptr ? a.offset[expert] : 0.f);
+      if (a.dbalance != nullptr) own_load = (float)a.load[expert];
+    }
+    const float dot = warp_sum(dw * w);
+    float qb = 0.f, inv = 0.f, top = 0.f;
+    const float all = a.dweights != nullptr && !a.renormalize && !sigmoid ? dot : 0.f;
+    if (whole_row) {
+      float sum = 0.f;
+      if (!sigmoid) {
+        top = l[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) top = fmaxf(top, l[i]);
+        top = fmaxf(warp_max(top), -3.402823466e38f);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        p[i] = e0 + i >= E ? 0.f : sigmoid ? rcp(1.f + ex2(l[i] * -1.4426950408889634f)) : ex2((l[i] - top) * 1.4426950408889634f);
+        sum += p[i];
+      }
+      sum = warp_sum(sum);
+      inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int i = 0; i < N; ++i) qb += p[i] * b[i];
+      qb = warp_sum(qb) * inv;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float q = p[i] * inv, y = q * (b[i] - qb - all);
+        l[i] = sigmoid ? y * (1.f - p[i]) : y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) l[i] = 0.f;
+    }
+    if (wide_out) {
+      constexpr int M = N * (int)sizeof(T) <= 16 ? N : 16 / (int)sizeof(T);
+      if (e0 < E)
+#pragma unroll
+        for (int j = 0; j < N / M; ++j) {
+          Pack<T, M> y;
+          y.set(l + j * M);
+          reinterpret_cast<Pack<T, M>*>(out + e0)[j] = y;
+        }
+    } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (e0 + i < E) l[i] += a.offset[e0 + i];
-  }
-  if (is) {
-    x = to_f32(row[expert]) + (a.offset != nullptr ? a.offset[expert] : 0.f);
-    if (a.dbalance != nullptr) own_load = (float)a.load[expert];
-  }
-  const float dot = warp_sum(dw * w);
-  float qb = 0.f, inv = 0.f, top = 0.f;
-  const float all = a.dweights != nullptr && !a.renormalize && !sigmoid ? dot : 0.f;
-  if (whole_row) {
-    float sum = 0.f;
-    if (!sigmoid) {
-      top = l[0];
-#pragma unroll
-      for (int i = 1; i < N; ++i) top = fmaxf(top, l[i]);
-      top = fmaxf(warp_max(top), -3.402823466e38f);
+        if (e0 + i < E) out[e0 + i] = from_f32<T>(l[i]);
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      p[i] = e0 + i >= E ? 0.f : sigmoid ? rcp(1.f + ex2(l[i] * -1.4426950408889634f)) : ex2((l[i] - top) * 1.4426950408889634f);
-      sum += p[i];
+    if (a.dweights == nullptr) continue;
+    __syncwarp();
+    if (is) {
+      // the chosen ones with the library's exponential: theirs are the large values
+      float y = a.renormalize ? (w == 0.f ? 0.f : (a.scale * dw - dot) * (w / a.scale)) : dw * w;
+      const float e = sigmoid ? expf(-fabsf(x)) : 0.f, r = 1.f / (1.f + e);
+      const float other = sigmoid ? (x >= 0.f ? e * r : r) : 1.f, own = sigmoid ? (x >= 0.f ? r : e * r) : expf(x - top);     // 1 - p and p of a sigmoid
+      if (whole_row) y += (x == -INFINITY ? 0.f : own) * inv * (each * own_load - qb - all);
+      out[expert] = from_f32<T>(y * (x != x ? x : other));
     }
-    sum = warp_sum(sum);
-    inv = sum == 0.f ? 0.f : 1.f / sum;
-    float d[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      d[i] = a.dbalance != nullptr && e0 + i < E ? each * (float)a.load[e0 + i] : 0.f;
-      qb += p[i] * inv * d[i];
-    }
-    qb = warp_sum(qb);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float q = p[i] * inv, y = q * (d[i] - qb - all);
-      l[i] = sigmoid ? y * (1.f - p[i]) : y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) l[i] = 0.f;
-  }
-  if (wide_out) {
-    constexpr int M = N * (int)sizeof(T) <= 16 ? N : 16 / (int)sizeof(T);
-    if (e0 < E)
-#pragma unroll
-      for (int j = 0; j < N / M; ++j) {
-        Pack<T, M> y;
-        y.set(l + j * M);
-        reinterpret_cast<Pack<T, M>*>(out + e0)[j] = y;
-      }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (e0 + i < E) out[e0 + i] = from_f32<T>(l[i]);
-  }
-  if (a.dweights == nullptr) return;
-  __syncwarp();
-  if (is) {
-    // the chosen ones with the library's exponential: theirs are the large values
-    float y = a.renormalize ? (w == 0.f ? 0.f : (a.scale * dw - dot) * (w / a.scale)) : dw * w;
-    const float e = sigmoid ? expf(-fabsf(x)) : 0.f, r = 1.f / (1.f + e);
-    const float other = sigmoid ? (x >= 0.f ? e * r : r) : 1.f, own = sigmoid ? (x >= 0.f ? r : e * r) : expf(x - top);     // 1 - p and p of a sigmoid
-    if (whole_row) y += (x == -INFINITY ? 0.f : own) * inv * (each * own_load - qb - all);
-    out[expert] = from_f32<T>(y * (x != x ? x : other));
   }
 }
 
@@ -657,7 +656,8 @@ extern "C" int fl_route_grad(int dtype, const FlRouteArgs* a, cudaStream_t strea
     using T = decltype(type);
     return by_experts(a->experts, [&](auto width) {
       constexpr int N = decltype(width)::value;
-      route_grad_kernel<N, T><<<(unsigned)((a->tokens + GRAD_WARPS - 1) / GRAD_WARPS), GRAD_WARPS * 32, 0, stream>>>(*a);
+      const long long need = (a->tokens + GRAD_WARPS - 1) / GRAD_WARPS;
+      route_grad_kernel<N, T><<<(unsigned)(need < GRAD_CTAS ? need : GRAD_CTAS), GRAD_WARPS * 32, 0, stream>>>(*a);
       return (int)cudaGetLastError();
     });
   });
