@@ -321,11 +321,13 @@ __global__ void __launch_bounds__(MOST_WARPS<N> * 32, N <= 8 ? 2 : 1) route_kern
   const bool in_lanes = size % N == 0 && (lanes & (lanes - 1)) == 0;
   for (int e = threadIdx.x; e < E; e += blockDim.x) load[e] = 0;
   float mean[N], bias[N], most = 0.f;
+  bool numbers = true;                           // no NaN among the biases
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     mean[i] = 0.f;
     bias[i] = i >= here ? -INFINITY : biased ? a.bias[e0 + i] : 0.f;
-    if (i < here) most = fmaxf(most, fabsf(bias[i]));
+    if (i < here && fabsf(bias[i]) < INFINITY) most = fmaxf(most, fabsf(bias[i]));      // an infinite one is far from all others
+    numbers = numbers && bias[i] == bias[i];
   }
   most = 1.f + warp_max(most);                   // no score and no sum with its bias is larger
   __syncthreads();
@@ -338,10 +340,10 @@ __global__ void __launch_bounds__(MOST_WARPS<N> * 32, N <= 8 ? 2 : 1) route_kern
 #pragma unroll
       for (int i = 0; i < N; ++i)
         if (i < here) l[i] += a.offset[e0 + i];
-    bool sure = true;
+    bool sure = numbers;
     if (scored) {
       const float sum = scores32<N>(c, l, sigmoid);
-      sure = sum == sum;                         // no NaN
+      sure = sure && sum == sum;                 // no NaN
       if (a.balance != nullptr) {
         const float inv = sum == 0.f ? 0.f : rcp(sum);
 #pragma unroll

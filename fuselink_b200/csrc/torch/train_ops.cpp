@@ -290,7 +290,7 @@ Tensor logits_and_tokens(const Tensor& logits, Tensor tokens, double temperature
   value(tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1), "losses: tokens, one for each row of the logits");
   value(tokens.scalar_type() == torch::kInt64 || tokens.scalar_type() == torch::kInt32, "losses: tokens of int64 or int32 expected");
   TORCH_CHECK(tokens.device() == logits.device(), "losses: tokens on ", logits.device(), " expected, not on ", tokens.device());
-  value(temperature > 0.0 && std::isfinite(temperature), "losses: a temperature above 0");
+  value(temperature >= 1e-30 && std::isfinite(temperature), "losses: a temperature of 1e-30 at least");
   dtype_of(logits, "losses");
   return tokens.scalar_type() == torch::kInt64 && tokens.is_contiguous() ? tokens : tokens.to(torch::kInt64).contiguous();
 }

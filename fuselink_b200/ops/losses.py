@@ -34,7 +34,7 @@ def _check(what: str, logits: torch.Tensor, tokens: torch.Tensor, temperature: f
         raise ValueError(f"{what}: tokens of int64 or int32 expected, not {tokens.dtype}")
     if tokens.device != logits.device:
         raise RuntimeError(f"{what}: tokens on {logits.device} expected, not on {tokens.device}")
-    if not (0 < temperature < math.inf):
+    if not (1e-30 <= temperature < math.inf):
         raise ValueError(f"{what}: a temperature of {temperature}")
 
 

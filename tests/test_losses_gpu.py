@@ -252,7 +252,7 @@ def test_what_is_refused():
     x, t = _logits((4, 9), torch.float32), _tokens((4,), 9)
     f = torch.zeros(4, device="cuda")
     for bad, args, how in ((ValueError, (x, t[:3]), {}), (ValueError, (x, t.float()), {}), (RuntimeError, (x, t.cpu()), {}), (ValueError, (x, t), dict(temperature=0.0)),
-                           (ValueError, (x, t), dict(temperature=math.nan)), (ValueError, (x[:, :0], t), {}), (RuntimeError, (x.double(), t), {})):
+                           (ValueError, (x, t), dict(temperature=math.nan)), (ValueError, (x, t), dict(temperature=1e-40)), (ValueError, (x[:, :0], t), {}), (RuntimeError, (x.double(), t), {})):
         with pytest.raises(bad):
             token_logprobs(*args, **how)
     for bad, how in ((RuntimeError, dict(old=f.cpu())), (RuntimeError, dict(advantages=torch.zeros(3, device="cuda"))), (RuntimeError, dict(weights=f.clone().requires_grad_(True))),

@@ -107,6 +107,23 @@ def test_rows_that_are_not_ordinary(groups, score, dt):
         assert (got.weights[2] == 0).all() and (grad[2] == 0).all()
 
 
+@pytest.mark.parametrize("groups", [1, 4])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_biases_that_are_not_ordinary(score, groups):
+    """Experts that a bias of -inf or the lowest number leaves out, one that +inf always takes, and a NaN, which comes before all numbers."""
+    x = _logits(60, 64, torch.bfloat16)
+    bias = 0.1 * torch.randn(64, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda")
+    bias[::3] = -math.inf
+    bias[1] = torch.finfo(torch.float32).min
+    _check(x, 6, score=score, groups=groups, topk_groups=max(1, groups // 2), bias=bias)
+    bias[17] = math.inf
+    got, _ = _check(x, 6, score=score, groups=groups, topk_groups=max(1, groups // 2), bias=bias)
+    assert (got.experts[:, 0] == 17).all()
+    bias[40] = math.nan
+    got, _ = _check(x, 6, score=score, groups=groups, topk_groups=max(1, groups // 2), bias=bias)
+    assert (got.experts[:, 0] == 40).all()
+
+
 def test_strides_offsets_and_captured_calls():
     from fuselink_b200.ops.routing import route
     wide = _logits(50, 100, torch.bfloat16)

@@ -134,7 +134,7 @@ def test_logprobs_and_policy_loss():
 def test_what_the_losses_refuse():
     x, t, f = torch.zeros(4, 9), torch.zeros(4, dtype=torch.int64), torch.zeros(4)
     for error, args, how in ((ValueError, (x, t[:3]), {}), (ValueError, (x, t.float()), {}), (ValueError, (x[:, :0], t), {}), (ValueError, (x, t), dict(temperature=0.0)),
-                             (ValueError, (x, t), dict(temperature=math.inf))):
+                             (ValueError, (x, t), dict(temperature=math.inf)), (ValueError, (x, t), dict(temperature=1e-40))):
         with pytest.raises(error):
             losses.token_logprobs(*args, **how)
     for error, how in ((RuntimeError, dict(advantages=torch.zeros(3))), (RuntimeError, dict(old=f.clone().requires_grad_(True))), (ValueError, dict(clip=(0.2, math.nan))),
