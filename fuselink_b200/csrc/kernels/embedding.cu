@@ -11,6 +11,8 @@
 // without a word from the other CTAs.  embed_sum_kernel then takes 32 places of the list a CTA, however many ids they are of: rows of ids whose places
 // are all among them are written at once, of the others (frequent words, padding) the CTA that is done last adds up the parts in their order, 32 at a
 // time.  Other CTAs of the same launch have the copy engine write the rows of ids that do not occur, from zeros in shared memory.
+// 8192 tokens, 32000 x 4096 bf16: lookup 15 us, sort 8, sums 58 to 64 (0.8 of the measured copy rate; an id's places all by one row of threads: 171, since one of
+// 98 places keeps its threads busy for 23).
 #include "embedding.cuh"
 #include "../common/fl_ptx.cuh"
 
@@ -21,7 +23,7 @@ constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32;
 constexpr int RANGE = 512;                       // ids of a sorting CTA
 constexpr int BATCH = 8;                         // tokens on their way per sorting thread
 constexpr int PART = 32;                         // places of a summing CTA, and parts that are added up at a time
-constexpr int ZERO_IDS = 4;                      // ids that a warp looks at for rows of zeros
+constexpr int ZERO_IDS = 4;                      // ids that a warp looks at for rows of zeros (a table of 32000 x 4096 without tokens: 16 ids 66 us, 8 55, 4 50, 2 52)
 constexpr int ZEROS = 8192;                      // bytes of zeros that a copy takes at most
 
 template <typename I>

@@ -8,6 +8,9 @@
 // knows dL / dlp as soon as it has the row's sum, so the kernel goes over the row once more right then, out of the caches as far as they go, and writes the
 // gradient of a derivative of 1.  Should the derivative turn out to be another number, the gradient is computed
 // anew from the logits (fl_logprobs_grad), so that it is rounded once.
+//
+// 8192 x 32000 bf16 with the gradient: 208 us, 0.70 of the measured copy rate; 4095 x 128256: 443 us.  Bound by exponentials (two a logit, 16 a cycle and SM: 56% of what the
+// pipe could) and by what a row's two passes wait for one another.  Without the gradient 0.65 and 0.8.
 #include "losses.cuh"
 #include <math.h>
 #include <type_traits>
