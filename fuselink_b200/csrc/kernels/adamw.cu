@@ -9,7 +9,7 @@
 // multiply-adds between them, so that the codes are the same wherever they are computed.
 //
 // Bound by memory in fp32: 22 bytes per bf16 weight, 28 with an fp32 copy of the weight as well (698 M weights: 2981 us, the measured copy rate).  With codes 10
-// bytes, and by instructions, 48 a weight (657 M weights: 1403 us, 0.72 of the copy rate).  A CTA takes 8192
+// bytes, and by instructions, 48 a weight (657 M weights: 1399 us, 0.72 of the copy rate; fp32 weights, or with copies, 0.9).  A CTA takes 8192
 // or 32768 values of one tensor; the tensors' addresses are kernel arguments, 400 tensors a launch, so that a captured step needs no copy of a table.
 // The number of steps is on the device: every CTA of a tensor adds 2^40 to it when it has read it, and the last one puts the next number.
 #include "adamw.cuh"
@@ -148,12 +148,6 @@ __device__ __forceinline__ uint32_t codes_of2(float x, float y) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(y), "f"(x));
   return c;
 }
-__device__ __forceinline__ float at_least(float x, float least) {      // NaN stays
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(least));
-  return y;
-}
-
 // 256 values with codes, whole and from multiples of 16 bytes on (codes: of 8).  What a lane has loaded of them:
 template <typename T, bool MASTER>
 struct Loaded {
@@ -172,6 +166,14 @@ struct Loaded {
     rs = t.v_scale[b / BLOCK];
   }
 };
+template <typename T, bool MASTER>
+__device__ __forceinline__ void prefetch(const FlAdamwTensor& t, long long b) {
+  bulk_prefetch_l2((const T*)t.grad + b, BLOCK * sizeof(T));
+  if (MASTER) bulk_prefetch_l2(t.master + b, BLOCK * 4);
+  else bulk_prefetch_l2((const T*)t.param + b, BLOCK * sizeof(T));
+  bulk_prefetch_l2((const uint8_t*)t.m + b, BLOCK);
+  bulk_prefetch_l2((const uint8_t*)t.v + b, BLOCK);
+}
 // Instructions go two values at a time where the hardware has that; the largest magnitudes are taken over numbers (a NaN is left out by itself), and
 // infinities looked for only in them.
 template <typename T, bool MASTER, typename L>
@@ -227,24 +229,30 @@ __device__ __forceinline__ void step_codes(const Loaded<T, MASTER>& in, const Fl
   mb = scale_bits(mb);
   rb = scale_bits(rb);
   const float m_inv = __uint_as_float((254u << 23) - mb), r_inv = __uint_as_float((254u << 23) - rb);
-  uint2 mo, ro;
+  const F2 m_inv2(m_inv, m_inv), r_inv2(r_inv, r_inv);
+  uint32_t mo[2], ro[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t x[2], y[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int k = 4 * h + 2 * j;
-      x[j] = codes_of2(m[k] * m_inv, m[k + 1] * m_inv);
-      float r0 = root[k] * r_inv, r1 = root[k + 1] * r_inv;
-      if (root[k] != 0.f) r0 = at_least(r0, 0x1p-9f);      // the smallest code
-      if (root[k + 1] != 0.f) r1 = at_least(r1, 0x1p-9f);
-      y[j] = codes_of2(r0, r1);
+      float p, q;
+      (F2(m[k], m[k + 1]) * m_inv2).get(p, q);
+      x[j] = codes_of2(p, q);
+      (F2(root[k], root[k + 1]) * r_inv2).get(p, q);
+      y[j] = codes_of2(p, q);
     }
-    (h == 0 ? mo.x : mo.y) = x[1] << 16 | x[0];
-    (h == 0 ? ro.x : ro.y) = y[1] << 16 | y[0];
+    mo[h] = x[1] << 16 | x[0];
+    ro[h] = y[1] << 16 | y[0];
+    if ((ro[h] - 0x01010101u) & ~ro[h] & 0x80808080u) {    // a code of 0 among the four: the smallest in its place, where the root is none
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (root[4 * h + i] > 0.f && (ro[h] >> 8 * i & 0xffu) == 0u) ro[h] |= 1u << 8 * i;
+    }
   }
-  store_codes<APART>(t.m, b, mo);
-  store_codes<APART>(t.v, b, ro);
+  store_codes<APART>(t.m, b, make_uint2(mo[0], mo[1]));
+  store_codes<APART>(t.v, b, make_uint2(ro[0], ro[1]));
   if ((threadIdx.x & 31) == 0) {
     t.m_scale[b / BLOCK] = __uint_as_float(mb);
     t.v_scale[b / BLOCK] = __uint_as_float(rb);
@@ -281,13 +289,17 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
   long long b = begin + warp * BLOCK;
   if constexpr (CODES) {
     const bool eights = (((uintptr_t)t.param | (uintptr_t)t.grad | (uintptr_t)t.master) & 15) == 0 && (((uintptr_t)t.m | (uintptr_t)t.v) & 7) == 0;
-    if (eights && b + BLOCK <= end) {            // the next block's loads are on their way while one is computed
+    // The next block's loads are on their way while one is computed.  Where weights are fp32 (or have a copy that is) the block behind it is asked into L2 as well: 285 M
+    // weights 906 -> 770 us, with copies 979 -> 796; of 16-bit ones alone 588 -> 599, so there it is not.
+    const bool far = Loaded<T, MASTER>::APART && (((uintptr_t)t.m | (uintptr_t)t.v) & 15) == 0 && lane == 0;
+    if (eights && b + BLOCK <= end) {
       Loaded<T, MASTER> now, next;
       now.load(t, b);
       for (;;) {
         const long long to = b + WARPS * BLOCK;
         const bool more = to + BLOCK <= end;
         if (more) next.load(t, to);
+        if (far && to + WARPS * BLOCK + BLOCK <= end) prefetch<T, MASTER>(t, to + WARPS * BLOCK);
         step_codes<T, MASTER>(now, t, a, b, first, second, keep);
         b = to;
         if (!more) break;
