@@ -277,7 +277,8 @@ __device__ __forceinline__ bool weights32(Chosen& c, const FlRouteArgs& a, const
     }
   }
   if (a.renormalize) total = warp_sum(e);
-  c.weight = __fdividef(e, total) * a.scale;
+  e /= total;                                    // IEEE's: the only choice of all weighs `scale` and has no gradient
+  c.weight = e * a.scale;
   return __all_sync(ALL, !is || x == -INFINITY || (e >= 1e-30f && e <= 1.f)) && total > 1e-30f && total < 1e30f;
 }
 
@@ -541,7 +542,7 @@ __global__ void __launch_bounds__(GRAD_WARPS * 32) route_grad_kernel(const FlRou
       x = to_f32(row[expert]) + (a.offset != nullptr ? a.offset[expert] : 0.f);
       if (a.dbalance != nullptr) own_load = (float)a.load[expert];
     }
-    const float dot = warp_sum(dw * w);
+    const float dot = warp_sum(__fmul_rn(dw, w));      // rounded as scale dw is below: of one choice the two are the same
     float qb = 0.f, inv = 0.f, top = 0.f;
     const float all = a.dweights != nullptr && !a.renormalize && !sigmoid ? dot : 0.f;
     if (whole_row) {
@@ -589,7 +590,7 @@ __global__ void __launch_bounds__(GRAD_WARPS * 32) route_grad_kernel(const FlRou
     __syncwarp();
     if (is) {
       // the chosen ones with the library's exponential: theirs are the large values
-      float y = a.renormalize ? (w == 0.f ? 0.f : (a.scale * dw - dot) * (w / a.scale)) : dw * w;
+      float y = a.renormalize ? (w == 0.f ? 0.f : (__fmul_rn(a.scale, dw) - dot) * (w / a.scale)) : dw * w;
       const float e = sigmoid ? expf(-fabsf(x)) : 0.f, r = 1.f / (1.f + e);
       const float other = sigmoid ? (x >= 0.f ? e * r : r) : 1.f, own = sigmoid ? (x >= 0.f ? r : e * r) : expf(x - top);     // 1 - p and p of a sigmoid
       if (whole_row) y += (x == -INFINITY ? 0.f : own) * inv * (each * own_load - qb - all);

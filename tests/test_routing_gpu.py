@@ -107,6 +107,18 @@ def test_rows_that_are_not_ordinary(groups, score, dt):
         assert (got.weights[2] == 0).all() and (grad[2] == 0).all()
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("scale", [1.0, 2.5, 0.3])
+def test_the_only_choice_weighs_all_and_has_no_gradient(scale, score, dt):
+    from fuselink_b200.ops.routing import route
+    x = _logits(300, 96, dt).requires_grad_(True)
+    r = route(x, 1, score=score, scale=scale, groups=4, topk_groups=2)
+    assert (r.weights == torch.tensor(scale)).all()
+    g, = torch.autograd.grad(r.weights, x, torch.randn(300, 1, device="cuda"))
+    assert (g == 0).all()
+
+
 @pytest.mark.parametrize("groups", [1, 4])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_biases_that_are_not_ordinary(score, groups):
