@@ -213,9 +213,14 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> route(Tensor logits, int64_t topk,
 }
 
 // ------------------------------------------------------------------------------------------------ losses
-// The logits as rows at (i, j), or a contiguous copy of them where they do not lie so.
+// The logits as rows at (i, j), or a contiguous copy of them where they do not lie so.  Without a value there is no row, whatever the sizes and strides are.
 Tensor as_rows(const Tensor& logits, FlLossArgs& a) {
   const int64_t V = logits.size(-1);
+  if (logits.numel() == 0) {
+    a.logits = nullptr; a.vocab = V;
+    a.outer = a.inner = 0; a.outer_stride = a.inner_stride = V;
+    return logits;
+  }
   const int d = (int)logits.dim() - 1;
   int64_t size[2] = {1, 1}, stride[2] = {V, V};             // [0]: the inner rows
   int n = 0;
@@ -227,9 +232,10 @@ Tensor as_rows(const Tensor& logits, FlLossArgs& a) {
     else fits = false;
   }
   for (int i = 0; i < n; ++i) fits = fits && stride[i] >= (i == 0 ? V : stride[0] * (size[0] - 1) + V);
-  if (!fits && logits.numel() > 0) return as_rows(logits.contiguous(), a);
+  if (!fits) return as_rows(logits.contiguous(), a);
   a.logits = logits.const_data_ptr(); a.vocab = V;
   a.outer = size[1]; a.inner = size[0]; a.outer_stride = stride[1]; a.inner_stride = stride[0];
+  TORCH_CHECK(a.outer * a.inner == logits.numel() / V, "losses: the logits' rows are not as many as they should be");
   return logits;
 }
 // A gradient whose rows begin as far behind multiples of 16 bytes as those of the logits: contiguous where that does it, else with up to 15 bytes
