@@ -5,11 +5,15 @@
 // Moments are kept in fp32, or as e4m3 codes of m and of sqrt(v) with a scale for each 256 values of a tensor: the smallest power of two,
 // 2^-100 at least, that keeps their largest finite magnitude within 448.  The root halves the range that a code has to span, and a root above 0 keeps
 // the smallest code at least: were it lost while m is not, the next steps would divide by eps.  Values that are not finite are kept
-// as NaN.  The step itself uses m and v as they are before they become codes.  These roundings are each IEEE's, without fused
+// as NaN.  The step itself uses m and v as they are before they become codes.  The roundings of m, v and the root are each IEEE's, without fused
 // multiply-adds between them, so that the codes are the same wherever they are computed.
 //
+// A value becomes one of the two codes around it, the upper one with a chance equal to its place between them.  Codes lie 6 to 12% of a value apart, while a step
+// changes a root by 0.05% with b2 = 0.999: to the nearest code, all but the largest changes would be rounded away at every step, for good.  The chance goes by a hash of the
+// value's place and of the step's number: adding its bits below those of the code carries into the code where it has to.
+//
 // Bound by memory in fp32: 22 bytes per bf16 weight, 28 with an fp32 copy of the weight as well (698 M weights: 2981 us, the measured copy rate).  With codes 10
-// bytes, and by instructions, 48 a weight (657 M weights: 1399 us, 0.72 of the copy rate; fp32 weights, or with copies, 0.9).  A CTA takes 8192
+// bytes, and by instructions (657 M weights: 1490 us, 0.67 of the copy rate; to the nearest code, which does not train, it was 1370).  A CTA takes 8192
 // or 32768 values of one tensor; the tensors' addresses are kernel arguments, 400 tensors a launch, so that a captured step needs no copy of a table.
 // The number of steps is on the device: every CTA of a tensor adds 2^40 to it when it has read it, and the last one puts the next number.
 #include "adamw.cuh"
@@ -47,11 +51,44 @@ __device__ __forceinline__ uint32_t finite_bits(float x) {
   return b < 0x7f800000u ? b : 0u;
 }
 __device__ __forceinline__ float no_inf(float x) { return (__float_as_uint(x) & 0x7fffffffu) == 0x7f800000u ? NAN : x; }
-__device__ __forceinline__ uint32_t codes_of(const float* x, float inverse) {
-  uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(no_inf(x[1]) * inverse), "f"(no_inf(x[0]) * inverse));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(no_inf(x[3]) * inverse), "f"(no_inf(x[2]) * inverse));
-  return (uint32_t)hi << 16 | lo;
+__device__ __forceinline__ uint32_t codes_of2(float x, float y) {
+  uint16_t c;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(y), "f"(x));
+  return c;
+}
+// 32 bits for each of four values, the first of which is at 4 q: draw(q, salt of the step), and what follows
+constexpr uint32_t BY = 0x9e3779b9u, AND = 0x6a09e667u;      // 2^32 times the fractional parts of the golden section and of the root of 2
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x *= BY;
+  x = (x ^ x >> 15) * AND;
+  return x ^ x >> 16;
+}
+__device__ __forceinline__ uint32_t draw(long long place, uint32_t salt) { return mix(salt ^ (uint32_t)(place >> 2)); }
+__device__ __forceinline__ uint32_t next_draw(uint32_t u) { return u * BY + AND; }
+__device__ __forceinline__ uint32_t for_m(uint32_t u) { return u & 0xfffffu; }
+__device__ __forceinline__ uint32_t for_root(uint32_t u) { return u >> 12; }
+// x rounded to e4m3 by 20 bits.  Right from 2^-6 on, where a code has 3 bits behind the first
+__device__ __forceinline__ float rounded_by(float x, uint32_t bits) { return __uint_as_float((__float_as_uint(x) + bits) & 0xfff00000u); }
+// The same for all numbers: codes below 2^-6 are as far apart as those of the next power of two
+__device__ __forceinline__ float any_rounded_by(float x, uint32_t bits) {
+  const float size = fabsf(x), small = size < 0.015625f ? 0.015625f : 0.f;
+  return x != x ? x : copysignf(__fsub_rn(rounded_by(__fadd_rn(size, small), bits), small), x);
+}
+// Codes of four values and roots, as far as scaled by powers of two already
+__device__ __forceinline__ void any_codes(uint32_t& mc, uint32_t& rc, const float* m, const float* root, uint32_t u) {
+  uint32_t x[2], y[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t v = next_draw(u);
+    x[j] = codes_of2(any_rounded_by(m[2 * j], for_m(u)), any_rounded_by(m[2 * j + 1], for_m(v)));
+    y[j] = codes_of2(any_rounded_by(root[2 * j], for_root(u)), any_rounded_by(root[2 * j + 1], for_root(v)));
+    u = next_draw(v);
+  }
+  mc = x[1] << 16 | x[0];
+  rc = y[1] << 16 | y[0];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (root[i] > 0.f && (rc >> 8 * i & 0xffu) == 0u) rc |= 1u << 8 * i;         // the smallest in the place of 0, where the root is none
 }
 __device__ __forceinline__ void values_of(float* x, uint32_t codes, float scale) {
 #pragma unroll
@@ -143,11 +180,6 @@ __device__ __forceinline__ F2 values_of2(uint16_t codes) {
   const float2 f = __half22float2(*reinterpret_cast<__half2*>(&two));
   return F2(f.x, f.y);
 }
-__device__ __forceinline__ uint32_t codes_of2(float x, float y) {
-  uint16_t c;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(y), "f"(x));
-  return c;
-}
 // 256 values with codes, whole and from multiples of 16 bytes on (codes: of 8).  What a lane has loaded of them:
 template <typename T, bool MASTER>
 struct Loaded {
@@ -177,7 +209,7 @@ __device__ __forceinline__ void prefetch(const FlAdamwTensor& t, long long b) {
 // Instructions go two values at a time where the hardware has that; the largest magnitudes are taken over numbers (a NaN is left out by itself), and
 // infinities looked for only in them.
 template <typename T, bool MASTER, typename L>
-__device__ __forceinline__ void step_codes(const Loaded<T, MASTER>& in, const FlAdamwTensor& t, const L& a, long long b, float first, float second, float keep) {
+__device__ __forceinline__ void step_codes(const Loaded<T, MASTER>& in, const FlAdamwTensor& t, const L& a, long long b, float first, float second, float keep, uint32_t salt) {
   constexpr bool APART = Loaded<T, MASTER>::APART;
   float g[8], w[8], m[8], root[8];
   const uint2 mc = in.m, vc = in.v;
@@ -233,23 +265,27 @@ __device__ __forceinline__ void step_codes(const Loaded<T, MASTER>& in, const Fl
   uint32_t mo[2], ro[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t x[2], y[2];
+    const uint32_t drawn = draw(Eight<uint8_t, APART>::place(b) + h * (APART ? BLOCK / 2 : 4), salt);
+    float p[4], q[4];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int k = 4 * h + 2 * j;
-      float p, q;
-      (F2(m[k], m[k + 1]) * m_inv2).get(p, q);
-      x[j] = codes_of2(p, q);
-      (F2(root[k], root[k + 1]) * r_inv2).get(p, q);
-      y[j] = codes_of2(p, q);
+      (F2(m[k], m[k + 1]) * m_inv2).get(p[2 * j], p[2 * j + 1]);
+      (F2(root[k], root[k + 1]) * r_inv2).get(q[2 * j], q[2 * j + 1]);
+    }
+    uint32_t x[2], y[2], u = drawn;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t v = next_draw(u);
+      x[j] = codes_of2(rounded_by(p[2 * j], for_m(u)), rounded_by(p[2 * j + 1], for_m(v)));
+      y[j] = codes_of2(rounded_by(q[2 * j], for_root(u)), rounded_by(q[2 * j + 1], for_root(v)));
+      u = next_draw(v);
     }
     mo[h] = x[1] << 16 | x[0];
     ro[h] = y[1] << 16 | y[0];
-    if ((ro[h] - 0x01010101u) & ~ro[h] & 0x80808080u) {    // a code of 0 among the four: the smallest in its place, where the root is none
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (root[4 * h + i] > 0.f && (ro[h] >> 8 * i & 0xffu) == 0u) ro[h] |= 1u << 8 * i;
-    }
+    // A code of up to 2^-6 (8) among the eight: a value that may lie below 2^-6, or a NaN, of which the bits may have made 0.  Then by the form for all numbers; one that was
+    // 2^-6 at least is the same in both.
+    if ((((mo[h] | 0x80808080u) - 0x09090909u) & ((ro[h] | 0x80808080u) - 0x09090909u) & 0x80808080u) != 0x80808080u) any_codes(mo[h], ro[h], p, q, drawn);
   }
   store_codes<APART>(t.m, b, make_uint2(mo[0], mo[1]));
   store_codes<APART>(t.v, b, make_uint2(ro[0], ro[1]));
@@ -262,6 +298,7 @@ __device__ __forceinline__ void step_codes(const Loaded<T, MASTER>& in, const Fl
 template <typename T, bool CODES, bool MASTER, int CAP>
 __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant__ Launch<CAP> a) {
   __shared__ float shared[3];
+  __shared__ uint32_t shared_salt;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
@@ -276,11 +313,13 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
     shared[0] = (float)(lr / -expm1((double)(step + 1) * a.log_b1));
     shared[1] = (float)(1.0 / sqrt(-expm1((double)(step + 1) * a.log_b2)));
     shared[2] = (float)(1.0 - lr * a.decay);
+    if (CODES) shared_salt = mix((uint32_t)(step + 1));
     const unsigned long long before = atomicAdd(reinterpret_cast<unsigned long long*>(t.step), (unsigned long long)ARRIVED);
     if ((int)(before >> 40) == chunks - 1) atomicExch(reinterpret_cast<unsigned long long*>(t.step), (unsigned long long)(step + 1));
   }
   __syncthreads();
   const float first = shared[0], second = shared[1], keep = shared[2];
+  const uint32_t salt = CODES ? shared_salt : 0u;
   uintptr_t bits = (uintptr_t)t.param | (uintptr_t)t.grad;
   bool wide = (bits & (4 * sizeof(T) - 1)) == 0;
   bits = (uintptr_t)t.m | (uintptr_t)t.v;
@@ -300,7 +339,7 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
         const bool more = to + BLOCK <= end;
         if (more) next.load(t, to);
         if (far && to + WARPS * BLOCK + BLOCK <= end) prefetch<T, MASTER>(t, to + WARPS * BLOCK);
-        step_codes<T, MASTER>(now, t, a, b, first, second, keep);
+        step_codes<T, MASTER>(now, t, a, b, first, second, keep, salt);
         b = to;
         if (!more) break;
         now = next;
@@ -356,11 +395,13 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const long long at = b + h * (BLOCK / 2) + lane * 4;
-        const uint32_t mc = codes_of(m[h], m_inv);
-        uint32_t rc = codes_of(root[h], r_inv);
+        uint32_t mc, rc;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (root[h][i] > 0.f && (rc >> 8 * i & 0xffu) == 0) rc |= 1u << 8 * i;
+        for (int i = 0; i < 4; ++i) {
+          m[h][i] = no_inf(m[h][i]) * m_inv;
+          root[h][i] = no_inf(root[h][i]) * r_inv;
+        }
+        any_codes(mc, rc, m[h], root[h], draw(at, salt));
         store4<uint8_t>(t.m, at, t.n, wide, Pack<uint8_t, 4>{mc});
         store4<uint8_t>(t.v, at, t.n, wide, Pack<uint8_t, 4>{rc});
       }

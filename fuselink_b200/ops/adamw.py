@@ -3,7 +3,10 @@
     m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2      w = w (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
 Codes are e4m3 of m and of sqrt(v) with a scale for each 256 values of a tensor, as they lie in memory: the smallest power of two, 2^-100 at least, that keeps their
-largest finite magnitude within 448.  A root above 0 keeps the smallest code at least; values that are not finite are kept as NaN.  The step itself uses the moments before
+largest finite magnitude within 448.  A step rounds to one of the two codes around a value, to the upper one with a chance equal to the value's place between them: a
+code's step is 6 to 12% of its value, a step of the optimizer changes a moment by less (its root by 0.05% with b2 = 0.999), and the nearest code would for the most part be
+the old one for good.  What decides is a hash of the place in the tensor and of the count of steps (:func:`draws`), so that a step can be done again, and tensors that
+several ranks hold stay equal.  A root above 0 keeps the smallest code at least; values that are not finite are kept as NaN.  The step itself uses the moments before
 they become codes.  The roundings of m, v and the root are IEEE's, one by one, so that the codes are the same on the CPU and on the GPU.
 
 The number of steps is a tensor's own and lives on its device, and the learning rate may: a captured step counts on when it is replayed.
@@ -62,13 +65,44 @@ def _in_memory(t: torch.Tensor) -> torch.Tensor:
     return t.detach().as_strided((t.numel(),), (1,))
 
 
-def encode(x: torch.Tensor, root: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(codes like x, scales [ceil(n / 256)]) of fp32 values; ``root``: none above 0 becomes the code of 0."""
+_WORD, _BY, _AND = 0xffffffff, 0x9e3779b9, 0x6a09e667      # 2^32 times the fractional parts of the golden section and of the root of 2
+
+
+def _mix(x: torch.Tensor) -> torch.Tensor:
+    x = x * _BY & _WORD
+    x = (x ^ x >> 15) * _AND & _WORD
+    return x ^ x >> 16
+
+
+def draws(n: int, step: int, device=None) -> torch.Tensor:
+    """The 32 bits, as int64, by which the ``n`` values of a tensor are rounded in its step number ``step``, the first being 1: a hash of each four values' place and
+    of the step, and numbers that follow it.  Roots go by the upper 20 of them, means by the lower 20."""
+    x = _mix(_mix(torch.tensor(step & _WORD, device=device)) ^ torch.arange((n + 3) // 4, device=device) & _WORD)
+    four = [x]
+    for _ in range(3):
+        four.append(four[-1] * _BY + _AND & _WORD)
+    return torch.stack(four, 1).reshape(-1)[:n]
+
+
+def _rounded_by(x: torch.Tensor, bits: torch.Tensor) -> torch.Tensor:
+    """x, of at most 448, rounded to e4m3: up where its 20 bits below those of a code and ``bits`` make a whole step.  Codes below 2^-6 are as far apart as those above."""
+    small = torch.where(x.abs() < 2.0 ** -6, 2.0 ** -6, 0.0)
+    y = ((x.abs() + small).view(torch.int32) + bits.int() & -(1 << 20)).view(torch.float32) - small
+    return torch.where(x.isnan(), x, torch.copysign(y, x))
+
+
+def encode(x: torch.Tensor, root: bool = False, draws: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes like x, scales [ceil(n / 256)]) of fp32 values; ``root``: none above 0 becomes the code of 0.  To the nearest code, or with ``draws``, 32 bits for each
+    value as it lies in memory, to the one below or above."""
     flat = _in_memory(x)
     blocks = torch.nn.functional.pad(flat, (0, -flat.numel() % BLOCK)).view(-1, BLOCK)
     finite = torch.where(blocks.isfinite(), blocks, torch.zeros_like(blocks))
     scale = scale_of(finite.abs().amax(1)) if blocks.numel() else flat.new_empty(0)
-    codes = torch.where(blocks.isinf(), torch.full_like(blocks, math.nan), blocks / scale[:, None]).to(FP8).view(torch.uint8)
+    scaled = torch.where(blocks.isinf(), torch.full_like(blocks, math.nan), blocks / scale[:, None])
+    if draws is not None:
+        bits = torch.nn.functional.pad(draws, (0, -flat.numel() % BLOCK)).view(-1, BLOCK)
+        scaled = _rounded_by(scaled, bits >> 12 if root else bits & 0xfffff)
+    codes = scaled.to(FP8).view(torch.uint8)
     if root:
         codes = torch.where((blocks > 0) & (codes == 0), torch.ones_like(codes), codes)
     out = torch.empty_like(x, dtype=FP8)
@@ -111,8 +145,9 @@ def _plain_step(p, grad, m, v, steps, lr, betas, eps, weight_decay, scales, mast
         v.copy_(new_v)
         return
     like = torch.empty_like(m, dtype=torch.float32)         # laid out as the parameter, whatever the gradient's strides
+    bits = draws(p.numel(), t, p.device)
     for codes, scale, x, is_root in ((m, scales[0], new_m, False), (v, scales[1], root, True)):
-        c, s = encode(like.copy_(x), is_root)
+        c, s = encode(like.copy_(x), is_root, bits)
         codes.view(torch.uint8).copy_(c.view(torch.uint8))
         scale.copy_(s)
 
