@@ -78,29 +78,33 @@ template <> struct Logits<__half> {
 struct Running {
   float top, sum;                                  // the largest logit so far, and the sum of 2^(unit (x - top))
 };
+// log2(e) / temperature, not 0: -inf times it stays -inf
+__device__ __forceinline__ float unit_of(double temperature) { return fmaxf((float)(1.4426950408889634 / temperature), 1.4e-45f); }
+__device__ __forceinline__ float below(float x, float top, float unit) { return (0.5f * x - 0.5f * top) * (2.f * unit); }      // unit (x - top), of any two numbers
 __device__ __forceinline__ void merge(Running& a, const Running& b, float unit) {
   const float top = fmaxf(a.top, b.top);
-  a.sum = a.sum * ex2((a.top - top) * unit) + b.sum * ex2((b.top - top) * unit);
+  a.sum = a.sum * ex2(below(a.top, top, unit)) + b.sum * ex2(below(b.top, top, unit));
   a.top = top;
 }
 // Exponents are unit x - base, one instruction for two, with base = unit top rounded: all terms of a row are 2^r too large then, r the rounding's error, and the
-// row's sum with them.  Logits of such size that r would matter are taken one by one, as unit (x - top).
-constexpr float LARGE = 1e6f;
-__device__ __forceinline__ bool large(float top) { return !(fabsf(top) < LARGE); }
+// row's sum with them.  Where base is so large that r would matter (far logits, or a low temperature) exponents are taken one by one, as unit (x - top).
+constexpr float LARGE = 1048576.f;                 // r is 1/32 at most
+__device__ __forceinline__ bool large(float base) { return !(fabsf(base) < LARGE); }
 __device__ __forceinline__ F2 powers(float x, float y, F2 unit, F2 minus) {
   float a, b;
   fma2(F2(x, y), unit, minus).get(a, b);
   return F2(ex2(a), ex2(b));
 }
 
-// The row's running sum, the same in all threads.  It starts from a finite number: a row's -inf then make no difference of infinities.
+// The row's running sum, the same in all threads.  It starts from a finite number, whose base is beyond LARGE but small enough for its r: a row's -inf then make no
+// difference of infinities, and a thread without a value has a sum of 0.
 template <typename T, int THREADS>
 __device__ __forceinline__ Running sum_row(const T* row, long long vocab, float unit, Running* shared) {
   constexpr int P = PER<T>;
   const int head = head_of(row, vocab);
   const int packs = (int)((vocab - head) / P);
   const uint4* v = reinterpret_cast<const uint4*>(row + head);
-  float top = -LARGE;
+  float top = fmaxf(-2.f * LARGE / unit, -3.402823466e38f);
   F2 sum(0.f, 0.f);
   const F2 unit2(unit, unit);
   for (int i = threadIdx.x; i < packs; i += THREADS * AHEAD) {
@@ -133,7 +137,7 @@ __device__ __forceinline__ Running sum_row(const T* row, long long vocab, float 
   Running r{top, (one + other) * ex2(-fmaf(top, unit, -(top * unit)))};
   for (long long i = threadIdx.x; i < vocab - (long long)packs * P; i += THREADS) {
     const float x = to_f32(row[i < head ? i : (long long)packs * P + i]), to = fmaxf(x, r.top);
-    r.sum = r.sum * ex2((r.top - to) * unit) + ex2((x - to) * unit);
+    r.sum = r.sum * ex2(below(r.top, to, unit)) + ex2(below(x, to, unit));
     r.top = to;
   }
   auto join = [&]() {
@@ -147,11 +151,11 @@ __device__ __forceinline__ Running sum_row(const T* row, long long vocab, float 
     for (int w = 1; w < THREADS / 32; ++w) merge(r, shared[w], unit);
   };
   join();
-  if (large(r.top)) {                              // or nothing above -LARGE: once more, one by one
+  if (large(r.top * unit)) {                       // or nothing above what it started from: once more, one by one
     r = Running{-3.402823466e38f, 0.f};
     for (long long i = threadIdx.x; i < vocab; i += THREADS) {
       const float x = to_f32(row[i]), to = fmaxf(x, r.top);
-      r.sum = r.sum * ex2((r.top - to) * unit) + ex2((x - to) * unit);
+      r.sum = r.sum * ex2(below(r.top, to, unit)) + ex2(below(x, to, unit));
       r.top = to;
     }
     join();
@@ -165,7 +169,7 @@ template <typename T, int THREADS>
 __device__ __forceinline__ void write_row(T* out, const T* row, long long vocab, float unit, float top, float inverse, float factor, long long tok) {
   constexpr int P = PER<T>;
   const int head = head_of(row, vocab);
-  const int packs = large(top) && factor != 0.f ? 0 : (int)((vocab - head) / P);
+  const int packs = large(top * unit) && factor != 0.f ? 0 : (int)((vocab - head) / P);
   const uint4* v = reinterpret_cast<const uint4*>(row + head);
   uint4* to = reinterpret_cast<uint4*>(out + head);
   if (factor == 0.f) {                             // nothing is read
@@ -194,13 +198,13 @@ __device__ __forceinline__ void write_row(T* out, const T* row, long long vocab,
   }
   for (long long i = threadIdx.x; i < vocab - (long long)packs * P; i += THREADS) {
     const long long j = i < head ? i : (long long)packs * P + i;
-    out[j] = from_f32<T>(ex2((to_f32(row[j]) - top) * unit) * share);
+    out[j] = from_f32<T>(ex2(below(to_f32(row[j]), top, unit)) * share);
   }
   // the token's own value, by the thread that has written it already
   if (tok >= 0 && tok < vocab) {
     const long long in = tok - head;
     const int owner = in < 0 ? (int)tok : in < (long long)packs * P ? (int)(in / P % THREADS) : (int)((tok - (long long)packs * P) % THREADS);
-    if ((int)threadIdx.x == owner) out[tok] = from_f32<T>(fmaf(ex2((to_f32(row[tok]) - top) * unit), share, factor));
+    if ((int)threadIdx.x == owner) out[tok] = from_f32<T>(fmaf(ex2(below(to_f32(row[tok]), top, unit)), share, factor));
   }
 }
 
@@ -262,7 +266,7 @@ template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const FlLossArgs a) {
   __shared__ Running shared[THREADS / 32];
   __shared__ float said;
-  const float unit = (float)(1.4426950408889634 / a.temperature);
+  const float unit = unit_of(a.temperature);
   const long long rows = a.outer * a.inner;
   const bool policy = a.loss != nullptr;
   double total = (double)rows;
@@ -344,7 +348,7 @@ template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_grad_kernel(const FlLossArgs a) {
   const float up = a.upstream != nullptr ? *a.upstream : 1.f;
   if (a.unless_one && up == 1.f) return;
-  const float unit = (float)(1.4426950408889634 / a.temperature);
+  const float unit = unit_of(a.temperature);
   const long long rows = a.outer * a.inner;
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = (const T*)a.logits + r / a.inner * a.outer_stride + r % a.inner * a.inner_stride;
