@@ -81,30 +81,55 @@ struct Running {
 // log2(e) / temperature, not 0: -inf times it stays -inf
 __device__ __forceinline__ float unit_of(double temperature) { return fmaxf((float)(1.4426950408889634 / temperature), 1.4e-45f); }
 __device__ __forceinline__ float below(float x, float top, float unit) { return (0.5f * x - 0.5f * top) * (2.f * unit); }      // unit (x - top), of any two numbers
-__device__ __forceinline__ void merge(Running& a, const Running& b, float unit) {
+__device__ __forceinline__ Running merge(const Running& a, const Running& b, float unit) {
   const float top = fmaxf(a.top, b.top);
-  a.sum = a.sum * ex2(below(a.top, top, unit)) + b.sum * ex2(below(b.top, top, unit));
-  a.top = top;
+  return {top, a.sum * ex2(below(a.top, top, unit)) + b.sum * ex2(below(b.top, top, unit))};
 }
-// Exponents are unit x - base, one instruction for two, with base = unit top rounded: all terms of a row are 2^r too large then, r the rounding's error, and the
-// row's sum with them.  Where base is so large that r would matter (far logits, or a low temperature) exponents are taken one by one, as unit (x - top).
-constexpr float LARGE = 1048576.f;                 // r is 1/32 at most
-__device__ __forceinline__ bool large(float base) { return !(fabsf(base) < LARGE); }
+// Exponents are unit x - base, one instruction for two, with base = unit top rounded.  While a row is summed, threads joined and maxima rise, sums are ones of 2^(unit x - base),
+// which fall by the difference of two bases; the rounding's error comes in once, behind all that.  Where base is so large that it would matter (logits beyond `far`: 7e5 times
+// the temperature) exponents are taken one by one, as unit (x - top).
+constexpr float LARGE = 1048576.f;                 // of a base; the error is 1/32 at most
+__device__ __forceinline__ float far_of(double temperature) { return fminf((float)temperature * (0.69314718f * LARGE), 3.402823466e38f); }
+__device__ __forceinline__ bool is_far(float top, float far) { return !(fabsf(top) < far); }
+__device__ __forceinline__ Running merge_based(const Running& a, const Running& b, float unit) {
+  const float top = fmaxf(a.top, b.top), base = __fmul_rn(top, unit);
+  return {top, a.sum * ex2(__fmul_rn(a.top, unit) - base) + b.sum * ex2(__fmul_rn(b.top, unit) - base)};
+}
 __device__ __forceinline__ F2 powers(float x, float y, F2 unit, F2 minus) {
   float a, b;
   fma2(F2(x, y), unit, minus).get(a, b);
   return F2(ex2(a), ex2(b));
 }
 
-// The row's running sum, the same in all threads.  It starts from a finite number, whose base is beyond LARGE but small enough for its r: a row's -inf then make no
-// difference of infinities, and a thread without a value has a sum of 0.
+// The sum of a row of far logits.  Seldom: its loops stay loops.
 template <typename T, int THREADS>
-__device__ __forceinline__ Running sum_row(const T* row, long long vocab, float unit, Running* shared) {
+__device__ __forceinline__ Running sum_far_row(const T* row, long long vocab, float unit, Running* shared) {
+  Running r{-3.402823466e38f, 0.f};
+  for (long long i = threadIdx.x; i < vocab; i += THREADS) {
+    const float x = to_f32(row[i]), to = fmaxf(x, r.top);
+    r.sum = r.sum * ex2(below(r.top, to, unit)) + ex2(below(x, to, unit));
+    r.top = to;
+  }
+#pragma unroll 1
+  for (int o = 16; o > 0; o >>= 1) r = merge(r, Running{__shfl_xor_sync(ALL, r.top, o), __shfl_xor_sync(ALL, r.sum, o)}, unit);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = r;
+  __syncthreads();
+  r = shared[0];
+#pragma unroll 1
+  for (int w = 1; w < THREADS / 32; ++w) r = merge(r, shared[w], unit);
+  return r;
+}
+
+// The row's running sum, the same in all threads.  It starts from a finite number: a row's -inf then make no difference of infinities, and a thread without a value
+// has a sum of 0.
+template <typename T, int THREADS>
+__device__ __forceinline__ Running sum_row(const T* row, long long vocab, float unit, float far, Running* shared) {
   constexpr int P = PER<T>;
   const int head = head_of(row, vocab);
   const int packs = (int)((vocab - head) / P);
   const uint4* v = reinterpret_cast<const uint4*>(row + head);
-  float top = fmaxf(-2.f * LARGE / unit, -3.402823466e38f);
+  float top = -far;
   F2 sum(0.f, 0.f);
   const F2 unit2(unit, unit);
   for (int i = threadIdx.x; i < packs; i += THREADS * AHEAD) {
@@ -116,12 +141,12 @@ __device__ __forceinline__ Running sum_row(const T* row, long long vocab, float 
       if (i + j * THREADS < packs) x[j] = ld_v4(v + i + j * THREADS);
     }
     const float to = Logits<T>::largest(Logits<T>::larger(Logits<T>::larger(x[0], x[1]), Logits<T>::larger(x[2], x[3])));
-    if (to > top) {
-      const float fall = ex2((top - to) * unit);
+    if (to > top) {                                // the terms' new base is a rounded one too: they fall by the bases' difference, not by the logits'
+      const float fall = ex2(__fmul_rn(top, unit) - __fmul_rn(to, unit));
       sum = sum * F2(fall, fall);
       top = to;
     }
-    const float base = -(top * unit);
+    const float base = -__fmul_rn(top, unit);
     const F2 minus(base, base);
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
@@ -131,45 +156,34 @@ __device__ __forceinline__ Running sum_row(const T* row, long long vocab, float 
       for (int k = 0; k < P; k += 2) sum = plain_sum2(sum, powers(f[k], f[k + 1], unit2, minus));
     }
   }
-  // the thread's sum as one of 2^(unit (x - top)), whatever its base's rounding
   float one, other;
   sum.get(one, other);
-  Running r{top, (one + other) * ex2(-fmaf(top, unit, -(top * unit)))};
+  Running r{top, one + other};
   for (long long i = threadIdx.x; i < vocab - (long long)packs * P; i += THREADS) {
-    const float x = to_f32(row[i < head ? i : (long long)packs * P + i]), to = fmaxf(x, r.top);
-    r.sum = r.sum * ex2(below(r.top, to, unit)) + ex2(below(x, to, unit));
+    const float x = to_f32(row[i < head ? i : (long long)packs * P + i]), to = fmaxf(x, r.top), higher = __fmul_rn(to, unit);
+    r.sum = r.sum * ex2(__fmul_rn(r.top, unit) - higher) + ex2(fmaf(x, unit, -higher));
     r.top = to;
   }
-  auto join = [&]() {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) merge(r, Running{__shfl_xor_sync(ALL, r.top, o), __shfl_xor_sync(ALL, r.sum, o)}, unit);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = r;
-    __syncthreads();
-    r = shared[0];
+  for (int o = 16; o > 0; o >>= 1) r = merge_based(r, Running{__shfl_xor_sync(ALL, r.top, o), __shfl_xor_sync(ALL, r.sum, o)}, unit);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = r;
+  __syncthreads();
+  r = shared[0];
 #pragma unroll
-    for (int w = 1; w < THREADS / 32; ++w) merge(r, shared[w], unit);
-  };
-  join();
-  if (large(r.top * unit)) {                       // or nothing above what it started from: once more, one by one
-    r = Running{-3.402823466e38f, 0.f};
-    for (long long i = threadIdx.x; i < vocab; i += THREADS) {
-      const float x = to_f32(row[i]), to = fmaxf(x, r.top);
-      r.sum = r.sum * ex2(below(r.top, to, unit)) + ex2(below(x, to, unit));
-      r.top = to;
-    }
-    join();
-  }
+  for (int w = 1; w < THREADS / 32; ++w) r = merge_based(r, shared[w], unit);
+  if (is_far(r.top, far)) return sum_far_row<T, THREADS>(row, vocab, unit, shared);      // or nothing above -far
+  r.sum *= ex2(-fmaf(r.top, unit, -__fmul_rn(r.top, unit)));       // without the base's rounding
   return r;
 }
 
 // out_j = factor (1[j = tok] - p_j), from the row's end to its beginning: what was read last is in L1 and L2 still (of rows of 128256 bf16, 600 in work, L2 had
 // lost 85% when they were read from the beginning again).  What is written is not kept.  inverse: 1 / sum_j 2^(unit (x_j - top))
 template <typename T, int THREADS>
-__device__ __forceinline__ void write_row(T* out, const T* row, long long vocab, float unit, float top, float inverse, float factor, long long tok) {
+__device__ __forceinline__ void write_row(T* out, const T* row, long long vocab, float unit, float far, float top, float inverse, float factor, long long tok) {
   constexpr int P = PER<T>;
   const int head = head_of(row, vocab);
-  const int packs = large(top * unit) && factor != 0.f ? 0 : (int)((vocab - head) / P);
+  const int packs = is_far(top, far) && factor != 0.f ? 0 : (int)((vocab - head) / P);
   const uint4* v = reinterpret_cast<const uint4*>(row + head);
   uint4* to = reinterpret_cast<uint4*>(out + head);
   if (factor == 0.f) {                             // nothing is read
@@ -266,7 +280,7 @@ template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const FlLossArgs a) {
   __shared__ Running shared[THREADS / 32];
   __shared__ float said;
-  const float unit = unit_of(a.temperature);
+  const float unit = unit_of(a.temperature), far = far_of(a.temperature);
   const long long rows = a.outer * a.inner;
   const bool policy = a.loss != nullptr;
   double total = (double)rows;
@@ -282,7 +296,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const FlL
         if (a.top != nullptr) { a.top[r] = 0.f; a.inverse[r] = 0.f; }
         if (a.coefficient != nullptr) a.coefficient[r] = 0.f;
       }
-      if (a.dlogits != nullptr) write_row<T, THREADS>(out, row, a.vocab, unit, 0.f, 0.f, 0.f, -1);
+      if (a.dlogits != nullptr) write_row<T, THREADS>(out, row, a.vocab, unit, far, 0.f, 0.f, 0.f, -1);
       continue;
     }
     // asked for before the row, used behind it
@@ -293,7 +307,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const FlL
       advantage = a.advantages[r];
       if (a.reference != nullptr) reference = a.reference[r];
     }
-    const Running s = sum_row<T, THREADS>(row, a.vocab, unit, shared);
+    const Running s = sum_row<T, THREADS>(row, a.vocab, unit, far, shared);
     if (threadIdx.x == 0) {
       const bool ok = tok >= 0 && tok < a.vocab;
       const double x = ok ? (double)to_f32(row[tok]) - (double)s.top : (double)NAN;
@@ -318,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const FlL
     }
     if (a.dlogits != nullptr) {
       __syncthreads();
-      write_row<T, THREADS>(out, row, a.vocab, unit, s.top, 1.f / s.sum, (float)((double)said / a.temperature), tok);
+      write_row<T, THREADS>(out, row, a.vocab, unit, far, s.top, 1.f / s.sum, (float)((double)said / a.temperature), tok);
     }
   }
   if (policy && threadIdx.x == 0) scratch_of(a.scratch).sums[blockIdx.x] = asked ? Sums{mine.loss * total, mine.divergence * total, mine.clipped * total} : mine;
@@ -348,7 +362,7 @@ template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_grad_kernel(const FlLossArgs a) {
   const float up = a.upstream != nullptr ? *a.upstream : 1.f;
   if (a.unless_one && up == 1.f) return;
-  const float unit = unit_of(a.temperature);
+  const float unit = unit_of(a.temperature), far = far_of(a.temperature);
   const long long rows = a.outer * a.inner;
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = (const T*)a.logits + r / a.inner * a.outer_stride + r % a.inner * a.inner_stride;
@@ -358,7 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_grad_kernel(
     double g = (double)a.dlogprobs[r] * (double)up / a.temperature;
     if (inverse == 0.f) g = 0.0;                   // a row of weight 0
     else if (g != 0.0 && (tok < 0 || tok >= a.vocab)) g = NAN;
-    write_row<T, THREADS>(out, row, a.vocab, unit, a.top[r], inverse, (float)g, tok);
+    write_row<T, THREADS>(out, row, a.vocab, unit, far, a.top[r], inverse, (float)g, tok);
   }
 }
 
