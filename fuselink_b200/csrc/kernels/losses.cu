@@ -335,7 +335,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const FlL
       write_row<T, THREADS>(out, row, a.vocab, unit, far, s.top, 1.f / s.sum, (float)((double)said / a.temperature), tok);
     }
   }
-  if (policy && threadIdx.x == 0) scratch_of(a.scratch).sums[blockIdx.x] = asked ? Sums{mine.loss * total, mine.divergence * total, mine.clipped * total} : mine;
+  if (policy && threadIdx.x == 0) {
+    if (!asked) grid_dep_wait();                   // rows of weight 0 alone: whoever is done behind this launch knows the one in front to be done too
+    scratch_of(a.scratch).sums[blockIdx.x] = asked ? Sums{mine.loss * total, mine.divergence * total, mine.clipped * total} : mine;
+  }
 }
 
 __global__ void __launch_bounds__(256) loss_sum_kernel(const FlLossArgs a, int ctas) {
