@@ -136,3 +136,23 @@ def test_logits_far_from_zero(n, vocab, temperature, shift):
     x = 2 * torch.randn(n, vocab, generator=_gen(11), device="cuda")
     x = x.sort(dim=1)[0] if n == 388 else x                             # maxima that rise all the time
     _check_rows(x + shift, temperature, torch.randint(0, vocab, (n,), generator=_gen(12), device="cuda"))
+
+
+def test_at_a_border_exactly_the_ratio_still_counts():
+    """Two equal logits: lp is -ln 2, and rounded to 32 bits it is 1.9e-9 from that, so the ratio rounds to 1, the border of a clip of 0 on either side.  Nothing is clipped, and the
+    gradient is that of the open term; one unit away, on the side where the advantage is held, it is 0."""
+    from fuselink_b200.ops.losses import policy_loss
+    t, A = torch.tensor([0, 1, 0, 1], device="cuda"), torch.tensor([1.0, -1.0, 2.0, -0.5], device="cuda")
+    leaf = torch.zeros(4, 2, device="cuda").requires_grad_(True)
+    old = torch.full((4,), -math.log(2), device="cuda")
+    for dt in (torch.float32, torch.bfloat16):
+        x = leaf.to(dt)
+        r = policy_loss(x, t, old, A, clip=(0.0, 0.0))
+        assert r.clipped == 0 and r.loss == -A.mean()
+        g, = torch.autograd.grad(r.loss, leaf)
+        onehot = torch.nn.functional.one_hot(t, 2).float()
+        assert torch.equal(g, -A[:, None] / 4 * (onehot - 0.5))
+        away = policy_loss(x, t, old - torch.where(A > 0, 1e-4, -1e-4), A, clip=(0.0, 0.0))
+        assert away.clipped == 1 and (torch.autograd.grad(away.loss, leaf)[0] == 0).all()
+    one = policy_loss(torch.full((3, 1), 5.0, device="cuda"), t[:3] * 0, old[:3] * 0, A[:3], clip=(0.0, 0.0))
+    assert one.clipped == 0 and one.loss == -A[:3].mean() and (one.logprobs == 0).all()
