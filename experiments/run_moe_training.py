@@ -24,6 +24,27 @@ import torch
 import torch.distributed as dist
 
 
+def last_state(net, opt) -> dict:
+    """What --checkpoint keeps: the model's state alone with SGD, which has none of its own; with AdamW its moments, counts of steps and fp32 copies too."""
+    return net.state_dict() if isinstance(opt, torch.optim.SGD) else {"model": net.state_dict(), "optimizer": opt.state_dict()}
+
+
+def go_on_from(state: dict, net, opt) -> None:
+    """Loads what last_state gave.  AdamW begins anew behind a model's state alone, SGD takes the model's part of either; moments of another width are refused.  The
+    learning rate stays the one that ``opt`` was made with."""
+    whole = set(state) == {"model", "optimizer"}
+    net.load_state_dict(state["model"] if whole else state)
+    if not whole or isinstance(opt, torch.optim.SGD):
+        return
+    saved = [g["state_bits"] for g in state["optimizer"]["param_groups"]]
+    if saved != [g["state_bits"] for g in opt.param_groups]:
+        raise SystemExit(f"--resume: the checkpoint's moments have {saved[0]} bits, --optimizer's {opt.param_groups[0]['state_bits']}")
+    rates = [g["lr"] for g in opt.param_groups]
+    opt.load_state_dict(state["optimizer"])
+    for g, lr in zip(opt.param_groups, rates):
+        g["lr"] = lr
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--model", default="tiny_moe")
@@ -46,8 +67,9 @@ def main():
     ap.add_argument("--reshadow-tolerance", type=float, default=0.15, help="copy slots stay empty once the busiest rank is within (1 + this) of the mean load")
     ap.add_argument("--host-heap", action="store_true", help="with --device cpu: build the symmetric heap in host memory and take the fused path "
                                                              "(only under a model of the device entry points, as the tests run it)")
-    ap.add_argument("--checkpoint", default="", help="save the last state here (per rank: experts differ)")
-    ap.add_argument("--resume", default="", help="load <path>.rank<r> written by --checkpoint (same world size) before training")
+    ap.add_argument("--checkpoint", default="", help="save the last state here (per rank: experts differ), AdamW's with it")
+    ap.add_argument("--resume", default="", help="load <path>.rank<r> written by --checkpoint (same world size, same width of AdamW's moments) before training; "
+                                                     "the learning rate is --lr's")
     a = ap.parse_args()
     if a.reshadow_every and a.optimizer != "sgd":
         ap.error("--reshadow-every moves experts between copy slots, and AdamW's moments and fp32 copies stay with the slots: --optimizer sgd")
@@ -85,14 +107,14 @@ def main():
         heap = SymmetricHeap.create(cfg.layers * per_layer + (64 << 20), device=-1 if cpu else local)
     net = MoETransformer(cfg, a.batch * a.seq, heap, rank, world, device=dev, seed=0,
                          fused_sgd_lr=a.lr if fused and a.optimizer == "sgd" else 0.0)
-    if a.resume:
-        net.load_state_dict(torch.load(f"{a.resume}.rank{rank}", map_location=dev))
     if a.optimizer == "sgd":
         params = net.dense_parameters() if fused else net.parameters()     # on the fused path the expert update is part of the wgrad GEMM
         opt = torch.optim.SGD(params, lr=a.lr)
     else:
         from fuselink_b200.ops.adamw import AdamW
         opt = AdamW(net.parameters(), lr=a.lr, state_bits=8 if a.optimizer == "adamw8" else 32, master=True)
+    if a.resume:
+        go_on_from(torch.load(f"{a.resume}.rank{rank}", map_location=dev), net, opt)
     gen = torch.Generator(device=dev).manual_seed(100 + rank)
     t_mark, tok = time.perf_counter(), 0
     ev = None if cpu else (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
@@ -131,7 +153,7 @@ def main():
                                   "n_gpus": world, "model": a.model, "layers": cfg.layers}), flush=True)
             tok = 0
     if a.checkpoint:
-        torch.save(net.state_dict(), f"{a.checkpoint}.rank{rank}")
+        torch.save(last_state(net, opt), f"{a.checkpoint}.rank{rank}")
     wd = threading.Timer(60.0, lambda: os._exit(0))
     wd.daemon = True
     wd.start()

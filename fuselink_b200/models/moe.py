@@ -310,7 +310,8 @@ class MoELayer(nn.Module):
         """Choose the shadows from the routing of a batch (``topk_idx`` of this rank, by default the last one routed; the
         loads are summed over the ranks) and install them; with ``tolerance`` copy slots are left empty (-1) once the busiest rank is within (1 + tolerance) of the
         mean load.  Returns the experts now shadowed.  An optimizer that keeps
-        per-parameter state (momentum, Adam moments) keeps the state of a slot, not of the expert that moves into it."""
+        per-parameter state (momentum, Adam moments) keeps the state of a slot, not of the expert that moves into it.  One that keeps fp32 copies of the
+        weights would undo the move in its next step: ``AdamW.refresh_masters`` behind this call, behind set_shadows and rebalance."""
         from ..ops.moe import choose_shadows
         n = len(self.cfg.shadow)
         if topk_idx is None:
