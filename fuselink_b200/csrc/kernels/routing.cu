@@ -252,27 +252,43 @@ __device__ __forceinline__ void sort_down(uint32_t* k) {
       }
 }
 
-// Weights of the lanes' choices, in fp32 from their own logits; false where fp32 does not do: what is not finite, and scores that all but vanish.
+// What a + b, rounded to s, has lost; 0 where s is no number
+__device__ __forceinline__ float lost_of(float a, float b, float s) {
+  const float c = s - a;
+  return fabsf(s) < INFINITY ? (a - (s - c)) + (b - c) : 0.f;
+}
+
+// Weights of the lanes' choices, in fp32 from their own logits; false where fp32 does not do: what is not finite, and scores that all but vanish.  The exponential of
+// a logit with its offset is one of the sum times one of what rounding took from it, which logits of 1000 would have 6e-5 of.
 template <int N, typename T>
 __device__ __forceinline__ bool weights32(Chosen& c, const FlRouteArgs& a, const T* row, const float* l) {
   const int lane = threadIdx.x & 31;
   const bool is = lane < a.topk;
-  const float x = is ? to_f32(row[c.expert]) + (a.offset != nullptr ? a.offset[c.expert] : 0.f) : -INFINITY;
+  float x = is ? to_f32(row[c.expert]) : -INFINITY, lost = 1.f;
+  if (a.offset != nullptr && is) {
+    const float o = a.offset[c.expert], s = x + o;
+    lost = expf(a.score == FL_ROUTE_SIGMOID ? -lost_of(x, o, s) : lost_of(x, o, s));
+    x = s;
+  }
   float e = 0.f, total = 1.f;
   if (a.score == FL_ROUTE_SIGMOID) {
-    if (is) e = __fdividef(1.f, 1.f + expf(-x));
+    if (is) e = __fdividef(1.f, 1.f + expf(-x) * lost);
   } else {
     float top = x;                               // of all: a choice by other values may leave out the largest, beside which its scores may be nothing
     if (!a.renormalize || a.bias != nullptr || a.topk_groups < a.groups)
 #pragma unroll
       for (int i = 0; i < N; ++i) top = fmaxf(top, l[i]);
     top = warp_max(top);
-    if (x > -INFINITY) e = expf(x - top);
+    if (x > -INFINITY) e = expf(x - top) * lost;
     if (!a.renormalize) {
       total = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (l[i] > -INFINITY) total += expf(l[i] - top);
+        if (l[i] > -INFINITY) {
+          float y = expf(l[i] - top);
+          if (a.offset != nullptr) y *= expf(lost_of(to_f32(row[lane * N + i]), a.offset[lane * N + i], l[i]));
+          total += y;
+        }
       total = warp_sum(total);
     }
   }
@@ -355,6 +371,14 @@ __global__ void __launch_bounds__(MOST_WARPS<N> * 32, N <= 8 ? 2 : 1) route_kern
 #pragma unroll
       for (int i = 0; i < N; ++i) c[i] += bias[i];
     }
+    // A softmax's scores are off by 2^-24 of the largest logit where an offset is added in fp32, their sum by as much, and two of them differ by both
+    float spread = 0.f;
+    if (a.offset != nullptr && !sigmoid) {
+      uint32_t bits = 0u;
+#pragma unroll
+      for (int i = 0; i < N; ++i) bits = max(bits, fabsf(l[i]) < INFINITY ? __float_as_uint(l[i]) & 0x7fffffffu : 0u);
+      spread = __uint_as_float(__reduce_max_sync(ALL, bits)) * 2.3841858e-7f;      // 2^-22
+    }
     bool whole_lane = true;                      // whether the lane's experts are in a group that stays; else `kept` says it of each group
     unsigned kept = ALL;
     if (some_groups) {
@@ -396,7 +420,7 @@ __global__ void __launch_bounds__(MOST_WARPS<N> * 32, N <= 8 ? 2 : 1) route_kern
       const bool keep = is && rank < a.topk_groups;
       // the worst that stays against the best that goes
       const float least = value32(~__reduce_max_sync(ALL, keep ? ~value : 0u) & ~31u), other = value32(__reduce_max_sync(ALL, keep ? 0u : value) & ~31u);
-      sure = sure && least - other > most * 3.0517578e-5f;         // 2^-15: 2^-17 for the bits cut off of a sum of two, half as much for scores
+      sure = sure && least - other > most * 3.0517578e-5f + spread;         // 2^-15: 2^-17 for the bits cut off of a sum of two, half as much for scores
       if (in_lanes) whole_lane = keep;
       else kept = __ballot_sync(ALL, keep);
     }
@@ -429,7 +453,7 @@ __global__ void __launch_bounds__(MOST_WARPS<N> * 32, N <= 8 ? 2 : 1) route_kern
             if (i >= from && i < from + size) key[i] = 0u;
         }
     }
-    const float off = far * ((N + 8) * 2.3841858e-7f);     // (N + 8) 2^-22: N 2^-23 for the bits cut off, the rest for scores and sums
+    const float off = far * ((N + 8) * 2.3841858e-7f) + (biased ? spread : 0.f);      // (N + 8) 2^-22: N 2^-23 for the bits cut off, the rest for scores and sums
     sort_down<N>(key);
     uint32_t head = key[0], behind = N > 1 ? key[N > 1] : 0u, mine = 0u, last = 0u;
 #pragma unroll

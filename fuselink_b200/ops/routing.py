@@ -6,7 +6,8 @@ experts are ordered by their logits.  The weights are the scores of those chosen
 neighbouring values are told apart the same way wherever it is computed.
 
 ``balance`` is E / (T k) sum_e load_e mean_t p_te / sum_e' p_te': 1 where experts are chosen evenly.  The gradient is that of weights and balance;
-choice and loads are constants of it.
+choice and loads are constants of it.  On the GPU choice and weights are those of logits and offset added exactly; the balance term, and what every expert's gradient
+has from it or from weights that are not renormalised, go by the sum as fp32 has it, 2^-24 of the logit off.
 """
 from __future__ import annotations
 
