@@ -95,3 +95,55 @@ def test_what_resuming_takes_and_refuses():
     assert new[1].param_groups[0]["lr"] == 0.5 and int(new[1].state[new[0].embed]["step"]) == 1
     with pytest.raises(SystemExit, match="8 bits"):
         command.go_on_from(state, *_training("adamw"))
+
+
+def _gated_rank(rank, world, port, out):
+    import datetime
+
+    import torch
+    import torch.distributed as dist
+
+    torch.set_num_threads(2)
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=world, timeout=datetime.timedelta(seconds=120))
+    import dataclasses
+
+    from fuselink_b200.models.moe import Gate
+    from fuselink_b200.models.moe_transformer import MOE_ZOO, MoETransformer
+    from fuselink_b200.ops.adamw import AdamW
+    cfg = dataclasses.replace(MOE_ZOO["tiny_moe"], embed_scale=2.0, gate=Gate(groups=2, topk_groups=1, balance_bias=True), balance_rate=0.25)
+    net = MoETransformer(cfg, 2 * 8, None, rank, world, device="cpu", seed=3)
+    opt = AdamW(net.parameters(), lr=1e-2, state_bits=8, master=True)
+    loads = []
+    for k in range(3):
+        tokens = torch.randint(0, cfg.vocab, (2, 8), generator=torch.Generator().manual_seed(10 * k + rank))
+        old = net.token_logprobs(tokens)
+        net.policy_step(tokens, old, torch.ones(2, 1) * (1 - 2 * rank), opt)
+        loads.append([b.moe.last_load.clone() for b in net.blocks])
+    state = {n: [opt.state[p][n] for p in net.dense_parameters()] for n in ("exp_avg", "root_avg_sq", "master")}
+    torch.save({"loads": loads, "bias": [b.moe.balance_bias for b in net.blocks], "dense": [p.detach() for p in net.dense_parameters()], "state": state}, f"{out}.{rank}")
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_gates_and_policy_steps_on_two_ranks(tmp_path):
+    """Replicated parameters, their 8-bit moments and fp32 copies, and the balance biases are equal on both ranks; the biases moved by the loads of both."""
+    import socket
+
+    import torch
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    torch.multiprocessing.spawn(_gated_rank, args=(2, port, str(tmp_path / "out")), nprocs=2)
+    a, b = (torch.load(tmp_path / f"out.{r}") for r in (0, 1))
+    for x, y in zip(a["dense"], b["dense"]):
+        assert torch.equal(x, y)
+    for name in a["state"]:
+        for x, y in zip(a["state"][name], b["state"][name]):
+            assert (x is None and y is None) or torch.equal(x.float(), y.float()), name
+    assert any(not torch.equal(x, y) for k in range(3) for x, y in zip(a["loads"][k], b["loads"][k]))
+    for layer, bias in enumerate(a["bias"]):
+        want = torch.zeros_like(bias)
+        for k in range(3):
+            load = (a["loads"][k][layer] + b["loads"][k][layer]).float()
+            want += 0.25 * (load.mean() - load).sign()
+        assert torch.equal(bias, want) and torch.equal(bias, b["bias"][layer]) and bias.any()
