@@ -8,12 +8,12 @@
 // as NaN.  The step itself uses m and v as they are before they become codes.  The roundings of m, v and the root are each IEEE's, without fused
 // multiply-adds between them, so that the codes are the same wherever they are computed.
 //
-// A value becomes one of the two codes around it, the upper one with a chance equal to its place between them.  Codes lie 6 to 12% of a value apart, while a step
-// changes a root by 0.05% with b2 = 0.999: to the nearest code, all but the largest changes would be rounded away at every step, for good.  The chance goes by a hash of the
-// value's place and of the step's number: adding its bits below those of the code carries into the code where it has to.
+// Over many steps a value has to become one of the two codes around it, the upper one with a chance equal to its place between them.  Codes lie 6 to 12% of a value
+// apart, while a step changes a root by 0.05% with b2 = 0.999: to the nearest code, which a call without a seed takes, all but the largest changes are rounded away at every step,
+// for good.  The chance goes by a hash of the value's place, of the step's number and of the seed: adding its bits below those of the code carries into the code where it has to.
 //
 // Bound by memory in fp32: 22 bytes per bf16 weight, 28 with an fp32 copy of the weight as well (698 M weights: 2981 us, the measured copy rate).  With codes 10
-// bytes, and by instructions (657 M weights: 1490 us, 0.67 of the copy rate; to the nearest code, which does not train, it was 1370).  A CTA takes 8192
+// bytes, and by instructions (657 M weights: 1490 us at random, 0.67 of the copy rate, 1370 to the nearest code).  A CTA takes 8192
 // or 32768 values of one tensor; the tensors' addresses are kernel arguments, 400 tensors a launch, so that a captured step needs no copy of a table.
 // The number of steps is on the device: every CTA of a tensor adds 2^40 to it when it has read it, and the last one puts the next number.
 #include "adamw.cuh"
@@ -30,6 +30,7 @@ constexpr int BLOCK = FL_ADAMW_BLOCK, LEAST_CHUNK = 8192, MOST_CHUNK = 32768;
 constexpr int MOST = 400, FEW = 32;              // tensors of a launch: 32 KB of arguments, or 2.5
 constexpr unsigned ALL = 0xffffffffu;
 constexpr long long ARRIVED = 1ll << 40;
+enum Codes { NONE, NEAREST, RANDOM };              // how moments become codes
 
 template <int CAP>
 struct Launch {
@@ -37,6 +38,7 @@ struct Launch {
   int first[CAP];                                // chunks before the tensor's
   int count, chunk;                              // chunk: values of a CTA
   float b1, c1, b2, c2, eps, one;
+  uint32_t seed;                                 // mixed
   double lr, decay, log_b1, log_b2;
   const float* lr_on_device;
 };
@@ -74,7 +76,14 @@ __device__ __forceinline__ float any_rounded_by(float x, uint32_t bits) {
   const float size = fabsf(x), small = size < 0.015625f ? 0.015625f : 0.f;
   return x != x ? x : copysignf(__fsub_rn(rounded_by(__fadd_rn(size, small), bits), small), x);
 }
-// Codes of four values and roots, as far as scaled by powers of two already
+// Codes of four values and roots, scaled by powers of two already.  No root above 0 becomes 0 by that: one is 2^-75 at least, its scale 2^56 at most.
+__device__ __forceinline__ uint32_t not_lost(uint32_t rc, const float* root) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (root[i] > 0.f && (rc >> 8 * i & 0xffu) == 0u) rc |= 1u << 8 * i;         // the smallest in the place of 0, where the root is none
+  return rc;
+}
+__device__ __forceinline__ uint32_t nearest_codes(const float* x) { return codes_of2(x[2], x[3]) << 16 | codes_of2(x[0], x[1]); }
 __device__ __forceinline__ void any_codes(uint32_t& mc, uint32_t& rc, const float* m, const float* root, uint32_t u) {
   uint32_t x[2], y[2];
 #pragma unroll
@@ -85,10 +94,7 @@ __device__ __forceinline__ void any_codes(uint32_t& mc, uint32_t& rc, const floa
     u = next_draw(v);
   }
   mc = x[1] << 16 | x[0];
-  rc = y[1] << 16 | y[0];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (root[i] > 0.f && (rc >> 8 * i & 0xffu) == 0u) rc |= 1u << 8 * i;         // the smallest in the place of 0, where the root is none
+  rc = not_lost(y[1] << 16 | y[0], root);
 }
 __device__ __forceinline__ void values_of(float* x, uint32_t codes, float scale) {
 #pragma unroll
@@ -208,7 +214,7 @@ __device__ __forceinline__ void prefetch(const FlAdamwTensor& t, long long b) {
 }
 // Instructions go two values at a time where the hardware has that; the largest magnitudes are taken over numbers (a NaN is left out by itself), and
 // infinities looked for only in them.
-template <typename T, bool MASTER, typename L>
+template <typename T, Codes CODES, bool MASTER, typename L>
 __device__ __forceinline__ void step_codes(const Loaded<T, MASTER>& in, const FlAdamwTensor& t, const L& a, long long b, float first, float second, float keep, uint32_t salt) {
   constexpr bool APART = Loaded<T, MASTER>::APART;
   float g[8], w[8], m[8], root[8];
@@ -265,7 +271,6 @@ __device__ __forceinline__ void step_codes(const Loaded<T, MASTER>& in, const Fl
   uint32_t mo[2], ro[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint32_t drawn = draw(Eight<uint8_t, APART>::place(b) + h * (APART ? BLOCK / 2 : 4), salt);
     float p[4], q[4];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -273,6 +278,13 @@ __device__ __forceinline__ void step_codes(const Loaded<T, MASTER>& in, const Fl
       (F2(m[k], m[k + 1]) * m_inv2).get(p[2 * j], p[2 * j + 1]);
       (F2(root[k], root[k + 1]) * r_inv2).get(q[2 * j], q[2 * j + 1]);
     }
+    if (CODES == NEAREST) {
+      mo[h] = nearest_codes(p);
+      ro[h] = nearest_codes(q);
+      if ((ro[h] - 0x01010101u) & ~ro[h] & 0x80808080u) ro[h] = not_lost(ro[h], q);          // a code of 0 among the four
+      continue;
+    }
+    const uint32_t drawn = draw(Eight<uint8_t, APART>::place(b) + h * (APART ? BLOCK / 2 : 4), salt);
     uint32_t x[2], y[2], u = drawn;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -295,7 +307,7 @@ __device__ __forceinline__ void step_codes(const Loaded<T, MASTER>& in, const Fl
   }
 }
 
-template <typename T, bool CODES, bool MASTER, int CAP>
+template <typename T, Codes CODES, bool MASTER, int CAP>
 __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant__ Launch<CAP> a) {
   __shared__ float shared[3];
   __shared__ uint32_t shared_salt;
@@ -313,20 +325,20 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
     shared[0] = (float)(lr / -expm1((double)(step + 1) * a.log_b1));
     shared[1] = (float)(1.0 / sqrt(-expm1((double)(step + 1) * a.log_b2)));
     shared[2] = (float)(1.0 - lr * a.decay);
-    if (CODES) shared_salt = mix((uint32_t)(step + 1));
+    if (CODES == RANDOM) shared_salt = mix((uint32_t)(step + 1) ^ a.seed);
     const unsigned long long before = atomicAdd(reinterpret_cast<unsigned long long*>(t.step), (unsigned long long)ARRIVED);
     if ((int)(before >> 40) == chunks - 1) atomicExch(reinterpret_cast<unsigned long long*>(t.step), (unsigned long long)(step + 1));
   }
   __syncthreads();
   const float first = shared[0], second = shared[1], keep = shared[2];
-  const uint32_t salt = CODES ? shared_salt : 0u;
+  const uint32_t salt = CODES == RANDOM ? shared_salt : 0u;
   uintptr_t bits = (uintptr_t)t.param | (uintptr_t)t.grad;
   bool wide = (bits & (4 * sizeof(T) - 1)) == 0;
   bits = (uintptr_t)t.m | (uintptr_t)t.v;
   wide = wide && (bits & (CODES ? 3 : 15)) == 0 && (!MASTER || ((uintptr_t)t.master & 15) == 0);
   const long long begin = (long long)chunk * a.chunk, end = min(t.n, begin + a.chunk);
   long long b = begin + warp * BLOCK;
-  if constexpr (CODES) {
+  if constexpr (CODES != NONE) {
     const bool eights = (((uintptr_t)t.param | (uintptr_t)t.grad | (uintptr_t)t.master) & 15) == 0 && (((uintptr_t)t.m | (uintptr_t)t.v) & 7) == 0;
     // The next block's loads are on their way while one is computed.  Where weights are fp32 (or have a copy that is) the block behind it is asked into L2 as well: 285 M
     // weights 906 -> 770 us, with copies 979 -> 796; of 16-bit ones alone 588 -> 599, so there it is not.
@@ -339,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
         const bool more = to + BLOCK <= end;
         if (more) next.load(t, to);
         if (far && to + WARPS * BLOCK + BLOCK <= end) prefetch<T, MASTER>(t, to + WARPS * BLOCK);
-        step_codes<T, MASTER>(now, t, a, b, first, second, keep, salt);
+        step_codes<T, CODES, MASTER>(now, t, a, b, first, second, keep, salt);
         b = to;
         if (!more) break;
         now = next;
@@ -401,7 +413,12 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
           m[h][i] = no_inf(m[h][i]) * m_inv;
           root[h][i] = no_inf(root[h][i]) * r_inv;
         }
-        any_codes(mc, rc, m[h], root[h], draw(at, salt));
+        if (CODES == NEAREST) {
+          mc = nearest_codes(m[h]);
+          rc = not_lost(nearest_codes(root[h]), root[h]);
+        } else {
+          any_codes(mc, rc, m[h], root[h], draw(at, salt));
+        }
         store4<uint8_t>(t.m, at, t.n, wide, Pack<uint8_t, 4>{mc});
         store4<uint8_t>(t.v, at, t.n, wide, Pack<uint8_t, 4>{rc});
       }
@@ -413,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
   }
 }
 
-template <typename T, bool CODES, bool MASTER, int CAP>
+template <typename T, Codes CODES, bool MASTER, int CAP>
 static int launch(const FlAdamwTensor* t, int count, const FlAdamwArgs* a, cudaStream_t stream) {
   static thread_local Launch<CAP> l;
   long long all = 0, chunks = 0;
@@ -433,11 +450,12 @@ static int launch(const FlAdamwTensor* t, int count, const FlAdamwArgs* a, cudaS
   l.one = 1.f; l.eps = (float)a->eps; l.lr = a->lr; l.decay = a->weight_decay;
   l.log_b1 = log(a->beta1); l.log_b2 = log(a->beta2);
   l.lr_on_device = a->lr_on_device;
+  l.seed = mix(a->seed);
   adamw_kernel<T, CODES, MASTER, CAP><<<(unsigned)chunks, THREADS, 0, stream>>>(l);
   return (int)cudaGetLastError();
 }
 
-template <typename T, bool CODES, bool MASTER>
+template <typename T, Codes CODES, bool MASTER>
 static int run(const FlAdamwTensor* t, long long count, const FlAdamwArgs* a, cudaStream_t stream) {
   for (long long i = 0; i < count;) {
     const int n = (int)(count - i < MOST ? count - i : MOST);
@@ -458,10 +476,13 @@ extern "C" int fl_adamw(int dtype, const FlAdamwTensor* t, long long count, cons
     if (t[i].n < 0 || t[i].n > (long long)LEAST_CHUNK * (1 << 22) || t[i].step == nullptr) return -1;
   return fl_by_dtype(dtype, [&](auto type) {
     using T = decltype(type);
-    if (a->master) {
-      if constexpr (sizeof(T) == 2) return a->codes ? run<T, true, true>(t, count, a, stream) : run<T, false, true>(t, count, a, stream);
+    auto by_copies = [&](auto codes) {
+      constexpr Codes CODES = decltype(codes)::value;
+      if (!a->master) return run<T, CODES, false>(t, count, a, stream);
+      if constexpr (sizeof(T) == 2) return run<T, CODES, true>(t, count, a, stream);
       else return -1;
-    }
-    return a->codes ? run<T, true, false>(t, count, a, stream) : run<T, false, false>(t, count, a, stream);
+    };
+    if (!a->codes) return by_copies(std::integral_constant<Codes, NONE>{});
+    return a->random ? by_copies(std::integral_constant<Codes, RANDOM>{}) : by_copies(std::integral_constant<Codes, NEAREST>{});
   });
 }

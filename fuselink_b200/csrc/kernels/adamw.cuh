@@ -25,6 +25,8 @@ typedef struct {
   const float* lr_on_device;                     // in place of lr, or null
   int codes;                                     // moments as codes
   int master;                                    // every tensor has an fp32 copy
+  int random;                                    // codes: one of the two around a value, by place, step and seed; else the nearest, for single steps
+  uint32_t seed;
 } FlAdamwArgs;
 
 // dtype: FlDtype of parameters and gradients.  -1: sizes that the kernels do not take

@@ -441,7 +441,7 @@ struct Tensors {
 };
 void adamw_step(const pybind11::object& params_, const pybind11::object& grads_, const pybind11::object& m_, const pybind11::object& v_, const pybind11::object& steps_,
                 const pybind11::object& m_scales_, const pybind11::object& v_scales_, const pybind11::object& masters_, double lr, OptTensor lr_on_device, double beta1, double beta2, double eps,
-                double weight_decay, bool codes) {
+                double weight_decay, bool codes, c10::optional<int64_t> seed) {
   const Tensors params(params_), grads(grads_), m(m_), v(v_), steps(steps_), m_scales(m_scales_), v_scales(v_scales_), masters(masters_);
   const size_t n = params.size();
   TORCH_CHECK(grads.size() == n && m.size() == n && v.size() == n && steps.size() == n && (!codes || (m_scales.size() == n && v_scales.size() == n)) &&
@@ -453,6 +453,7 @@ void adamw_step(const pybind11::object& params_, const pybind11::object& grads_,
   FlAdamwArgs a;
   memset(&a, 0, sizeof a);
   a.lr = lr; a.beta1 = beta1; a.beta2 = beta2; a.eps = eps; a.weight_decay = weight_decay; a.codes = codes; a.master = !masters.empty();
+  a.random = seed.has_value(); a.seed = (uint32_t)seed.value_or(0);
   if (lr_on_device.has_value()) {
     TORCH_CHECK(lr_on_device->device() == device && lr_on_device->scalar_type() == torch::kFloat32 && lr_on_device->numel() == 1, "adamw: lr, one fp32 value on the parameters' device");
     a.lr_on_device = lr_on_device->const_data_ptr<float>();

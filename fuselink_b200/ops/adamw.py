@@ -3,10 +3,12 @@
     m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2      w = w (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
 Codes are e4m3 of m and of sqrt(v) with a scale for each 256 values of a tensor, as they lie in memory: the smallest power of two, 2^-100 at least, that keeps their
-largest finite magnitude within 448.  A step rounds to one of the two codes around a value, to the upper one with a chance equal to the value's place between them: a
-code's step is 6 to 12% of its value, a step of the optimizer changes a moment by less (its root by 0.05% with b2 = 0.999), and the nearest code would for the most part be
-the old one for good.  What decides is a hash of the place in the tensor and of the count of steps (:func:`draws`), so that a step can be done again, and tensors that
-several ranks hold stay equal.  A root above 0 keeps the smallest code at least; values that are not finite are kept as NaN.  The step itself uses the moments before
+largest finite magnitude within 448.  A root above 0 keeps the smallest code at least; values that are not finite are kept as NaN.
+
+A step with a ``seed`` rounds to one of the two codes around a value, to the upper one with a chance equal to the value's place between them.  That is what training takes, and
+what :class:`AdamW` does: a code's step is 6 to 12% of its value, a step of the optimizer changes a moment by less (its root by 0.05% with b2 = 0.999), and the nearest code
+would for the most part be the old one for good.  What decides is a hash of the place in the tensor, of the count of steps and of the seed (:func:`draws`), so that a step can
+be done again, and tensors that several ranks hold stay equal.  Without a seed codes are the nearest ones, for single steps.  The step itself uses the moments before
 they become codes.  The roundings of m, v and the root are IEEE's, one by one, so that the codes are the same on the CPU and on the GPU.
 
 The number of steps is a tensor's own and lives on its device, and the learning rate may: a captured step counts on when it is replayed.
@@ -34,9 +36,11 @@ def _settings(lr, betas, eps, weight_decay):
 
 def step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m: Sequence[torch.Tensor], v: Sequence[torch.Tensor], steps: Sequence[torch.Tensor], *,
          lr: Union[float, torch.Tensor], betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
-         scales: Optional[Tuple[Sequence[torch.Tensor], Sequence[torch.Tensor]]] = None, master: Optional[Sequence[torch.Tensor]] = None) -> None:
+         scales: Optional[Tuple[Sequence[torch.Tensor], Sequence[torch.Tensor]]] = None, master: Optional[Sequence[torch.Tensor]] = None,
+         seed: Optional[int] = None) -> None:
     """One step on ``params`` in place, each with its gradient, moments and count of steps (one int64 value, which the call raises by one).  m, v: fp32, laid out as
-    their parameter; with ``scales`` (of m, of the root) e4m3 codes, and scales fp32 [ceil(n / 256)].  ``master``: fp32 copies of bf16 or fp16 parameters; the
+    their parameter; with ``scales`` (of m, of the root) e4m3 codes, and scales fp32 [ceil(n / 256)], rounded at random by ``seed`` (32 bits of it), which many steps
+    need, or without one to the nearest.  ``master``: fp32 copies of bf16 or fp16 parameters; the
     step works on these and rounds them to the parameters.  ``lr``: a number, or one fp32 value on the device.  On the GPU bf16, fp16 and fp32, all on one device,
     parameters without gaps, each one once; gradients of their parameter's type."""
     _settings(lr, betas, eps, weight_decay)
@@ -44,20 +48,20 @@ def step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m: Seque
     if len(params) > 0 and params[0].is_cuda:
         on_device = isinstance(lr, torch.Tensor)
         require_native().adamw_step(params, grads, m, v, steps, m_scales, v_scales, master or (), 0.0 if on_device else lr, lr if on_device else None,
-                                    betas[0], betas[1], eps, weight_decay, scales is not None)
+                                    betas[0], betas[1], eps, weight_decay, scales is not None, seed)
         return
-    _plain(params, grads, m, v, steps, lr, betas, eps, weight_decay, scales, master)
+    _plain(params, grads, m, v, steps, lr, betas, eps, weight_decay, scales, master, seed)
 
 
 @torch.no_grad()
-def _plain(params, grads, m, v, steps, lr, betas, eps, weight_decay, scales, master):
+def _plain(params, grads, m, v, steps, lr, betas, eps, weight_decay, scales, master, seed):
     if any(len(x) != len(params) for x in [grads, m, v, steps, *(scales or ()), *([master] if master else ())]):
         raise RuntimeError("adamw: one of each for every parameter")
     for i, p in enumerate(params):
         if grads[i].layout != torch.strided or grads[i].shape != p.shape or grads[i].dtype != p.dtype:
             raise RuntimeError("adamw: a dense gradient of its parameter's type, shape and device")
         _plain_step(p, grads[i], m[i], v[i], steps[i], lr, betas, eps, weight_decay, (scales[0][i], scales[1][i]) if scales is not None else None,
-                    master[i] if master else None)
+                    master[i] if master else None, seed)
 
 
 def _in_memory(t: torch.Tensor) -> torch.Tensor:
@@ -74,10 +78,10 @@ def _mix(x: torch.Tensor) -> torch.Tensor:
     return x ^ x >> 16
 
 
-def draws(n: int, step: int, device=None) -> torch.Tensor:
-    """The 32 bits, as int64, by which the ``n`` values of a tensor are rounded in its step number ``step``, the first being 1: a hash of each four values' place and
-    of the step, and numbers that follow it.  Roots go by the upper 20 of them, means by the lower 20."""
-    x = _mix(_mix(torch.tensor(step & _WORD, device=device)) ^ torch.arange((n + 3) // 4, device=device) & _WORD)
+def draws(n: int, step: int, seed: int = 0, device=None) -> torch.Tensor:
+    """The 32 bits, as int64, by which the ``n`` values of a tensor are rounded in its step number ``step``, the first being 1: a hash of each four values' place,
+    of the step and of the seed, and numbers that follow it.  Roots go by the upper 20 of them, means by the lower 20."""
+    x = _mix(_mix(_mix(torch.tensor(seed & _WORD, device=device)) ^ step & _WORD) ^ torch.arange((n + 3) // 4, device=device) & _WORD)
     four = [x]
     for _ in range(3):
         four.append(four[-1] * _BY + _AND & _WORD)
@@ -125,7 +129,7 @@ def scale_of(amax: torch.Tensor) -> torch.Tensor:
     return torch.where(amax > 0, s, torch.zeros_like(s)).clamp(min=LEAST_SCALE)
 
 
-def _plain_step(p, grad, m, v, steps, lr, betas, eps, weight_decay, scales, master):
+def _plain_step(p, grad, m, v, steps, lr, betas, eps, weight_decay, scales, master, seed):
     b1, b2 = betas
     lr = float(lr)
     steps += 1
@@ -145,7 +149,7 @@ def _plain_step(p, grad, m, v, steps, lr, betas, eps, weight_decay, scales, mast
         v.copy_(new_v)
         return
     like = torch.empty_like(m, dtype=torch.float32)         # laid out as the parameter, whatever the gradient's strides
-    bits = draws(p.numel(), t, p.device)
+    bits = None if seed is None else draws(p.numel(), t, seed, p.device)
     for codes, scale, x, is_root in ((m, scales[0], new_m, False), (v, scales[1], root, True)):
         c, s = encode(like.copy_(x), is_root, bits)
         codes.view(torch.uint8).copy_(c.view(torch.uint8))
@@ -153,16 +157,21 @@ def _plain_step(p, grad, m, v, steps, lr, betas, eps, weight_decay, scales, mast
 
 
 class AdamW(torch.optim.Optimizer):
-    """The optimizer around :func:`step`: ``state_bits`` 32 or 8, ``master`` keeps fp32 copies of bf16 and fp16 parameters, from which the next step starts:
+    """The optimizer around :func:`step`: ``state_bits`` 32 or 8, the latter rounded at random by ``seed`` (the same on ranks that hold the same parameters), ``master`` keeps fp32 copies of bf16 and fp16 parameters, from which the next step starts:
     parameters that are written otherwise (loaded, broadcast) call for ``refresh_masters``.  Parameters without a gradient are left out of a step, their counts too.  ``lr`` of a group may be one fp32 value on the device, which a schedule writes between replays of a captured step; the first
     step, which makes the state, is not captured.  Sparse gradients are refused."""
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, *,
-                 state_bits: int = 32, master: bool = False):
+                 state_bits: int = 32, master: bool = False, seed: int = 0):
         _settings(lr, betas, eps, weight_decay)
         if state_bits not in (8, 32):
             raise ValueError(f"adamw: moments in 8 or 32 bits, not {state_bits}")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master=master))
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master=master, seed=seed))
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:
+            group.setdefault("seed", 0)                      # saved before there was one
 
     def _new_state(self, p: torch.Tensor, group: dict) -> dict:
         if not p.is_floating_point() or p.layout != torch.strided:
@@ -203,7 +212,7 @@ class AdamW(torch.optim.Optimizer):
                     to.append(x)
             for (_, has_master), (ps, gs, ms, vs, steps, m_scales, v_scales, masters) in calls.items():
                 step(ps, gs, ms, vs, steps, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                     scales=(m_scales, v_scales) if group["state_bits"] == 8 else None, master=masters if has_master else None)
+                     scales=(m_scales, v_scales) if group["state_bits"] == 8 else None, master=masters if has_master else None, seed=group["seed"])
         return loss
 
     @torch.no_grad()

@@ -72,7 +72,7 @@ def test_rounding_at_random_has_the_value_as_its_mean():
 
 
 def test_draws_are_even_and_unlike_from_step_to_step():
-    d = [adamw.draws(40000, t).double() / 2 ** 32 - 0.5 for t in (1, 2, 3, 1000000)]
+    d = [adamw.draws(40000, t, seed).double() / 2 ** 32 - 0.5 for t, seed in ((1, 0), (2, 0), (3, 0), (1000000, 0), (1, 1), (2, 1), (1, -7))]
     six = 6 / 40000 ** 0.5
     for i, x in enumerate(d):
         assert abs(x.mean()) <= six * 12 ** -0.5 and abs(12 * x.square().mean() - 1) <= six
@@ -95,3 +95,22 @@ def test_what_is_held_twice_stays_the_same():
             o.step()
     a, b = opts[0].state[ps[0]], opts[1].state[ps[2]]
     assert torch.equal(ps[0], ps[2]) and all(torch.equal(a[n].float(), b[n].float()) for n in a)
+
+
+def test_a_step_without_a_seed_takes_the_nearest_codes():
+    """As it did before there was one; and a state that was saved then goes on with a seed of 0."""
+    p, grad = torch.ones(600), torch.randn(600, generator=_gen(4))
+    out = []
+    for seed in (None, 0, 0, 1):
+        (m, ms), (v, vs) = adamw.encode(torch.zeros(600)), adamw.encode(torch.zeros(600), root=True)
+        adamw.step([p.clone()], [grad], [m], [v], [torch.tensor(0)], lr=0.1, scales=([ms], [vs]), seed=seed)
+        out.append((m.float(), v.float(), ms, vs))
+    near = adamw.encode(grad * (1 - 0.9))[0], adamw.encode((grad * grad * (1 - 0.999)).sqrt(), root=True)[0]
+    assert torch.equal(out[0][0], near[0].float()) and torch.equal(out[0][1], near[1].float())
+    assert all(torch.equal(a, b) for a, b in zip(out[1], out[2])) and not torch.equal(out[1][0], out[0][0]) and not torch.equal(out[1][0], out[3][0])
+    q = torch.nn.Parameter(p.clone())
+    opt = adamw.AdamW([q], state_bits=8, seed=3)
+    old = opt.state_dict()
+    del old["param_groups"][0]["seed"]
+    opt.load_state_dict(old)
+    assert opt.param_groups[0]["seed"] == 0

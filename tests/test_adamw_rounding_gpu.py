@@ -1,11 +1,11 @@
-"""AdamW's 8-bit moments, rounded at random by place and step (csrc/kernels/adamw.cu), against the same on the CPU bit by bit over many steps."""
+"""AdamW's 8-bit moments, rounded at random by place, step and seed or to the nearest code (csrc/kernels/adamw.cu), against the same on the CPU bit by bit over many steps."""
 import math
 
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
-HOW = dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0)
+HOW = dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, seed=5)
 
 
 def _same(a, b):
@@ -31,8 +31,9 @@ def _on_gpu(s):
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("seed", [0, 12345, -1, None])
 @pytest.mark.parametrize("kind", ["even", "wide", "none", "odd"])
-def test_many_steps(dt, kind):
+def test_many_steps(dt, kind, seed):
     """Gradients of one size, over the whole range of a code and below it, mostly zeros, and with infinities and NaN: whole blocks, ends of tensors, and no block at all."""
     shapes = [(4096,), (33, 257), (7,), (256,), (1300,)]
     want = _state(shapes, dt)
@@ -49,7 +50,7 @@ def test_many_steps(dt, kind):
             if kind == "odd" and k == 20:
                 g.view(-1)[[0, -1]] = torch.tensor([math.nan, -math.inf])
             grads.append(g.to(dt))
-        _step(want, grads), _step(got, [g.cuda() for g in grads])
+        _step(want, grads, seed=seed), _step(got, [g.cuda() for g in grads], seed=seed)
         for name in ("m", "v", "m_scale", "v_scale"):
             assert all(_same(a, b) for a, b in zip(got[name], want[name])), (k, name)
         if kind == "odd" and k >= 20:
