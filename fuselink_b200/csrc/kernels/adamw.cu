@@ -13,7 +13,8 @@
 // for good.  The chance goes by a hash of the value's place, of the step's number and of the seed: adding its bits below those of the code carries into the code where it has to.
 //
 // Bound by memory in fp32: 22 bytes per bf16 weight, 28 with an fp32 copy of the weight as well (698 M weights: 2981 us, the measured copy rate).  With codes 10
-// bytes, and by instructions (657 M weights: 1490 us at random, 0.67 of the copy rate, 1370 to the nearest code).  A CTA takes 8192
+// bytes, and by instructions (657 M weights: 59 a weight and 1480 us at random, 0.68 of the copy rate; 47 and 1370 to the nearest code;
+// fp32 weights, or with copies, 0.9 in both).  A CTA takes 8192
 // or 32768 values of one tensor; the tensors' addresses are kernel arguments, 400 tensors a launch, so that a captured step needs no copy of a table.
 // The number of steps is on the device: every CTA of a tensor adds 2^40 to it when it has read it, and the last one puts the next number.
 #include "adamw.cuh"
