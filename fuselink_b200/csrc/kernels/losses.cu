@@ -86,9 +86,9 @@ __device__ __forceinline__ Running merge(const Running& a, const Running& b, flo
   return {top, a.sum * ex2(below(a.top, top, unit)) + b.sum * ex2(below(b.top, top, unit))};
 }
 // Exponents are unit x - base, one instruction for two, with base = unit top rounded.  While a row is summed, threads joined and maxima rise, sums are ones of 2^(unit x - base),
-// which fall by the difference of two bases; the rounding's error comes in once, behind all that.  Where base is so large that it would matter (logits beyond `far`: 7e5 times
-// the temperature) exponents are taken one by one, as unit (x - top).
-constexpr float LARGE = 1048576.f;                 // of a base; the error is 1/32 at most
+// which fall by the difference of two bases; the rounding's error comes in once, behind all that.  Where base is so large that it would matter (logits beyond `far`: 5.8e6
+// times the temperature) exponents are taken one by one, as unit (x - top).
+constexpr float LARGE = 8388608.f;                 // of a base; the error is 1/4 at most, of a thread without a value 1/2
 __device__ __forceinline__ float far_of(double temperature) { return fminf((float)temperature * (0.69314718f * LARGE), 3.402823466e38f); }
 __device__ __forceinline__ bool is_far(float top, float far) { return !(fabsf(top) < far); }
 __device__ __forceinline__ Running merge_based(const Running& a, const Running& b, float unit) {

@@ -129,7 +129,7 @@ def test_logits_at_the_ends_of_their_type():
             assert ((lp - want).abs() <= _off(vocab) + 2 * HALF * want.abs() + 6e38 * 2.0 ** -150 * 2).all()
 
 
-@pytest.mark.parametrize("shift", [0.0, 1e3, -1e4, 1e5, -1e6, 1e7])
+@pytest.mark.parametrize("shift", [0.0, 1e3, -1e4, 1e5, -1e6, 5e6, 1e7])
 @pytest.mark.parametrize("n,vocab,temperature", [(388, 2048, 1.0), (1300, 1999, 0.7), (700, 5003, 1.3), (5, 32768, 1.0)])
 def test_logits_far_from_zero(n, vocab, temperature, shift):
     """A common offset changes nothing but which logits fp32 has: sums stay as exact as without it while a thread's maximum rises."""
